@@ -474,6 +474,102 @@ int zkb_witness_residual_stream(zkb_ctx* ctx, const zkb_rs_program* prog, const 
                                 uint32_t log_rows, uint32_t* const* cols, uint32_t n_cols, uint32_t* out_pat, int32_t* out_nat, int32_t* in_nat,
                                 const zkb_rs_mults* mults, uint32_t* counts);
 
+/* ---- The values of a decode step: what the witness generators above are made from ------------------
+ * A proof whose trace never leaves the device needs the model's own values there: the embedding's rows, the queries, keys
+ * and values of a block of tokens (zkb_witness_dequant leaves them as bf16 patterns in want_out), the cache that they
+ * fill, and the attention over it, which zkb_witness_residual_stream reads as leaves. These three calls make them. Values
+ * are bf16 numbers, held either two bytes apiece or, as everywhere above, as patterns in the low halves of 32-bit words;
+ * sums, norms and softmax statistics are 32-bit floats, and each output is rounded once, to nearest even.
+ *
+ * All pointers are device pointers of the context's device unless named h_; strides count elements (not bytes) and may be
+ * negative: row 0, head 0 is where the pointer points (want_out's tokens and channel blocks descend). Outputs overlap
+ * neither one another nor the inputs, save that q_out may be q itself with q's strides (16-bit values). Nothing is
+ * synchronised, nothing is allocated, no workspace is shared between calls: a call can be captured into a graph from the
+ * context's stream, and graphs replayed side by side. The device arrays of a batch (first, kv_len, ids) are read when the
+ * kernels run, so a captured call serves other batches of at most its n_rows. */
+#define ZKB_VALUE_BF16 0 /* 16 bits */
+#define ZKB_VALUE_WORD 1 /* a bf16 pattern in the low half of a 32-bit word (written with a zero high half; the high half is ignored when read) */
+#define ZKB_VALUE_INT8 2 /* an 8-bit code, with a float scale beside it: code * scale */
+
+/* Embedding rows: out[t][i] = bf16(table[ids[t]][i] * (row_scale[ids[t]] * scale)), element (t, i) at
+ * t * out_stride + (i / segment) * segment_stride + i % segment (segment 0: the whole row in one piece), so that rows can be
+ * written straight into a residual-stream component's `wit` (a segment per row of leaves). A token whose id lies outside
+ * [0, vocab) gets a row of zeros and adds 1 to *off_table (may be NULL). The table is BF16 (row_scale NULL) or INT8 (a scale a
+ * row); rows are `width` values, table_stride apart. */
+typedef struct zkb_step_embed_args {
+    const int32_t* ids; /* n_tokens */
+    const void* table;
+    const float* row_scale; /* vocab, INT8 tables only */
+    void* out;
+    uint64_t* off_table;
+    int64_t table_stride, out_stride, segment_stride;
+    uint32_t n_tokens, vocab, width, segment, table_type, out_type; /* out: BF16 or WORD */
+    float scale;
+} zkb_step_embed_args;
+int zkb_step_embed(zkb_ctx* ctx, const zkb_step_embed_args* args);
+
+/* A key-value cache: token p of kv head h of sequence b at b * seq_stride + h * head_stride + p * token_stride of k and of v,
+ * head_dim values in a row. INT8 caches keep one scale a token and head: k_scale and v_scale at
+ * b * scale_seq_stride + h * scale_head_stride + p. head_dim is 32, 64 or 128. */
+typedef struct zkb_kv_cache {
+    void* k;
+    void* v;
+    float* k_scale; /* NULL for BF16 */
+    float* v_scale;
+    int64_t seq_stride, head_stride, token_stride, scale_seq_stride, scale_head_stride;
+    uint32_t type, n_seqs, n_heads, head_dim, capacity; /* BF16 or INT8 */
+} zkb_kv_cache;
+/* Which rows of a step belong to which sequence: sequence b has rows first[b] .. first[b + 1] (ascending, at most n_rows) and
+ * kv_len[b] tokens in all, the step's own among them: its rows are the tokens at positions kv_len[b] - rows .. kv_len[b] - 1.
+ * Rows from first[n_seqs] on are left as they were. Positions below zero or from the capacity on are not in the cache: they are
+ * neither written nor seen. max_rows and max_len are the most rows and tokens of any sequence as the host knows them (0: it does
+ * not); they decide how the work is laid out, never what is computed. */
+typedef struct zkb_step_rows {
+    const int32_t* first;  /* n_seqs + 1 */
+    const int32_t* kv_len; /* n_seqs */
+    uint32_t n_rows, max_rows, max_len;
+} zkb_step_rows;
+
+/* Norms of each query and key head, the position rotation and the cache's new tokens, in one pass. For a head x of a row at
+ * position p: y = x * rsqrt(mean(x^2) + eps) * weight where the weight is given (q_weight, k_weight: head_dim bf16 values; NULL
+ * leaves the head as it is); then each pair (i, j) of the first rotary_dim values turns by a = p * h_inv_freq[i']:
+ * y_i cos a - y_j sin a, y_j cos a + y_i sin a, with j = i + rotary_dim / 2 (interleaved: j = i + 1). Angles are reduced to a turn in
+ * 64 bits. Queries go to q_out (BF16); keys and, unchanged, values go to the cache at position p. INT8 caches get
+ * scale = max|y| / 127 and code = y / scale rounded to nearest even (scale 0: codes 0). Rows without a position in the cache
+ * (below) still have their queries written. rotary_dim: a multiple of 16 up to head_dim, or 0; h_inv_freq: rotary_dim / 2 values
+ * on the host, read before the call returns. */
+typedef struct zkb_step_norm_rope_args {
+    zkb_kv_cache cache;
+    zkb_step_rows rows;
+    const void* q; /* n_rows x q_heads, rows q_stride apart, heads head_stride apart; k and v: n_heads of the cache */
+    const void* k;
+    const void* v;
+    const uint16_t* q_weight;
+    const uint16_t* k_weight;
+    const double* h_inv_freq;
+    void* q_out;
+    int64_t q_stride, k_stride, v_stride, head_stride, q_out_stride, q_out_head_stride;
+    uint32_t type, q_heads, rotary_dim, interleaved; /* type of q, k and v: BF16 or WORD */
+    float eps;
+} zkb_step_norm_rope_args;
+int zkb_step_norm_rope(zkb_ctx* ctx, const zkb_step_norm_rope_args* args);
+
+/* Attention of a step's rows over the cache (which holds the step's own tokens already). The row at position p sees key j when
+ * 0 <= j <= p and (window == 0 or p - j < window or j < sinks): out = sum_j softmax_j(scale * q . k_j) v_j for each query head, kv head
+ * h serving the q_heads / n_heads query heads from h * (q_heads / n_heads) on. A row that sees no key, or whose scores are all -inf, gets
+ * zeros. What a row does not see does not reach it, whatever it holds (NaN and infinities among it). q is BF16; out is BF16 or WORD.
+ * Scores, statistics and sums are 32-bit floats; the softmax's weights are rounded to bf16 for the product with v. */
+typedef struct zkb_step_attention_args {
+    zkb_kv_cache cache;
+    zkb_step_rows rows;
+    const void* q;
+    void* out;
+    int64_t q_stride, q_head_stride, out_stride, out_head_stride;
+    uint32_t q_heads, out_type, window, sinks;
+    float scale;
+} zkb_step_attention_args;
+int zkb_step_attention(zkb_ctx* ctx, const zkb_step_attention_args* args);
+
 #ifdef __cplusplus
 }
 #endif

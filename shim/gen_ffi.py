@@ -10,8 +10,9 @@ OPAQUE = {"zkb_ctx": "ZkbCtx", "zkb_air_program": "ZkbAirProgram", "zkb_shard_pc
 STRUCTS = {"zkb_grid": "ZkbGrid", "zkb_dequant_cfg": "ZkbDequantCfg", "zkb_pcs_config": "ZkbPcsConfig",
            "zkb_stark_component": "ZkbStarkComponent", "zkb_air_op": "ZkbAirOp", "zkb_air_stats": "ZkbAirStats", "zkb_rs_group": "ZkbRsGroup",
            "zkb_rs_slot": "ZkbRsSlot", "zkb_rs_program": "ZkbRsProgram", "zkb_rs_tables": "ZkbRsTables", "zkb_rs_mult": "ZkbRsMult",
-           "zkb_rs_mults": "ZkbRsMults"}
-SCALARS = {"int": "i32", "unsigned": "u32", "unsigned int": "u32", "uint32_t": "u32", "int32_t": "i32", "uint64_t": "u64",
+           "zkb_rs_mults": "ZkbRsMults", "zkb_step_embed_args": "ZkbStepEmbedArgs", "zkb_kv_cache": "ZkbKvCache", "zkb_step_rows": "ZkbStepRows",
+           "zkb_step_norm_rope_args": "ZkbStepNormRopeArgs", "zkb_step_attention_args": "ZkbStepAttentionArgs"}
+SCALARS = {"int": "i32", "unsigned": "u32", "unsigned int": "u32", "uint32_t": "u32", "int32_t": "i32", "uint64_t": "u64", "int64_t": "i64",
            "unsigned long long": "u64", "size_t": "usize", "float": "f32", "double": "f64", "int8_t": "i8", "uint8_t": "u8",
            "uint16_t": "u16", "unsigned char": "u8", "char": "std::os::raw::c_char", "void": "std::ffi::c_void"}
 
@@ -48,6 +49,9 @@ def rust_type(ctype):
     return t
 
 
+RENAMED = {"in": "inp", "type": "ty", "ref": "r", "fn": "f", "loop": "lp", "box": "bx"}  # Rust's own words
+
+
 def parse_param(p):
     p = p.strip()
     if p == "void":
@@ -56,7 +60,7 @@ def parse_param(p):
     ctype, name, arr = m.group(1).strip(), m.group(2), m.group(3)
     if arr:  # `T x[4]` is `T* x`; a leading const stays with the element
         ctype = ctype + "*"
-    name = {"in": "inp", "type": "ty", "ref": "r", "fn": "f", "loop": "lp", "box": "bx"}.get(name, name)
+    name = RENAMED.get(name, name)
     return name, rust_type(ctype)
 
 
@@ -76,7 +80,8 @@ def parse_struct(name, body):
                 fields.append((am.group(1), f"[{rust_type(ctype)}; {am.group(2)}]"))
             else:
                 stars = nm.count("*")
-                fields.append((nm.replace("*", "").strip(), rust_type(ctype + "*" * stars)))
+                nm = nm.replace("*", "").strip()
+                fields.append((RENAMED.get(nm, nm), rust_type(ctype + "*" * stars)))
     return fields
 
 

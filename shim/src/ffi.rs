@@ -108,6 +108,93 @@ pub struct ZkbRsMults {
     pub un: *const ZkbRsMult,
 }
 
+#[repr(C)] #[derive(Copy, Clone, Debug)]
+pub struct ZkbStepEmbedArgs {
+    pub ids: *const i32,
+    pub table: *const std::ffi::c_void,
+    pub row_scale: *const f32,
+    pub out: *mut std::ffi::c_void,
+    pub off_table: *mut u64,
+    pub table_stride: i64,
+    pub out_stride: i64,
+    pub segment_stride: i64,
+    pub n_tokens: u32,
+    pub vocab: u32,
+    pub width: u32,
+    pub segment: u32,
+    pub table_type: u32,
+    pub out_type: u32,
+    pub scale: f32,
+}
+
+#[repr(C)] #[derive(Copy, Clone, Debug)]
+pub struct ZkbKvCache {
+    pub k: *mut std::ffi::c_void,
+    pub v: *mut std::ffi::c_void,
+    pub k_scale: *mut f32,
+    pub v_scale: *mut f32,
+    pub seq_stride: i64,
+    pub head_stride: i64,
+    pub token_stride: i64,
+    pub scale_seq_stride: i64,
+    pub scale_head_stride: i64,
+    pub ty: u32,
+    pub n_seqs: u32,
+    pub n_heads: u32,
+    pub head_dim: u32,
+    pub capacity: u32,
+}
+
+#[repr(C)] #[derive(Copy, Clone, Debug)]
+pub struct ZkbStepRows {
+    pub first: *const i32,
+    pub kv_len: *const i32,
+    pub n_rows: u32,
+    pub max_rows: u32,
+    pub max_len: u32,
+}
+
+#[repr(C)] #[derive(Copy, Clone, Debug)]
+pub struct ZkbStepNormRopeArgs {
+    pub cache: ZkbKvCache,
+    pub rows: ZkbStepRows,
+    pub q: *const std::ffi::c_void,
+    pub k: *const std::ffi::c_void,
+    pub v: *const std::ffi::c_void,
+    pub q_weight: *const u16,
+    pub k_weight: *const u16,
+    pub h_inv_freq: *const f64,
+    pub q_out: *mut std::ffi::c_void,
+    pub q_stride: i64,
+    pub k_stride: i64,
+    pub v_stride: i64,
+    pub head_stride: i64,
+    pub q_out_stride: i64,
+    pub q_out_head_stride: i64,
+    pub ty: u32,
+    pub q_heads: u32,
+    pub rotary_dim: u32,
+    pub interleaved: u32,
+    pub eps: f32,
+}
+
+#[repr(C)] #[derive(Copy, Clone, Debug)]
+pub struct ZkbStepAttentionArgs {
+    pub cache: ZkbKvCache,
+    pub rows: ZkbStepRows,
+    pub q: *const std::ffi::c_void,
+    pub out: *mut std::ffi::c_void,
+    pub q_stride: i64,
+    pub q_head_stride: i64,
+    pub out_stride: i64,
+    pub out_head_stride: i64,
+    pub q_heads: u32,
+    pub out_type: u32,
+    pub window: u32,
+    pub sinks: u32,
+    pub scale: f32,
+}
+
 #[repr(C)] #[derive(Copy, Clone, Debug, Default)]
 pub struct ZkbAirOp {
     pub op: u32,
@@ -229,6 +316,9 @@ extern "C" {
     pub fn zkb_key_tile_flags(ctx: *mut ZkbCtx, shape: u32, log_rows: u32, groups: u32, chunks: u32, lead: u32, descending: u32, modulus: u32, rw: u32, flags: *mut u32) -> i32;
     pub fn zkb_witness_selectors(ctx: *mut ZkbCtx, shape: u32, log_rows: u32, groups: u32, chunks: u32, lead: u32, descending: u32, flags: *const u32, scale: *const u32, ctx_len: u32, n_insts: u32, with_scale: i32, cols: *const *mut u32, n_cols: u32) -> i32;
     pub fn zkb_witness_residual_stream(ctx: *mut ZkbCtx, prog: *const ZkbRsProgram, tables: *const ZkbRsTables, wit: *const u32, live_rows: u32, log_rows: u32, cols: *const *mut u32, n_cols: u32, out_pat: *mut u32, out_nat: *mut i32, in_nat: *mut i32, mults: *const ZkbRsMults, counts: *mut u32) -> i32;
+    pub fn zkb_step_embed(ctx: *mut ZkbCtx, args: *const ZkbStepEmbedArgs) -> i32;
+    pub fn zkb_step_norm_rope(ctx: *mut ZkbCtx, args: *const ZkbStepNormRopeArgs) -> i32;
+    pub fn zkb_step_attention(ctx: *mut ZkbCtx, args: *const ZkbStepAttentionArgs) -> i32;
     pub fn zkb_air_compile(ctx: *mut ZkbCtx, ops: *const ZkbAirOp, n_ops: usize, constraints: *const u32, n_constraints: usize, tree_cols: *const u32, n_trees: i32, n_scalars: usize, out: *mut *mut ZkbAirProgram) -> i32;
     pub fn zkb_air_free(prog: *mut ZkbAirProgram) -> i32;
     pub fn zkb_air_specialize(ctx: *mut ZkbCtx, prog: *mut ZkbAirProgram) -> i32;

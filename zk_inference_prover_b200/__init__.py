@@ -22,5 +22,13 @@ from .capi import (  # noqa: F401
     air_analyze,
     constraint_denom_inv,
     PCS_PHASES,
+    VALUE_BF16,
+    VALUE_WORD,
+    VALUE_INT8,
+    KvCache,
+    StepRows,
+    StepEmbed,
+    StepNormRope,
+    StepAttention,
 )
 from . import air, capi  # noqa: F401,E402

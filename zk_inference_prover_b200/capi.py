@@ -21,7 +21,7 @@ EXPORTED_SYMBOLS = [
     "zkb_accumulate", "zkb_lift_accumulate", "zkb_secure_powers", "zkb_gkr_eq_evals", "zkb_gkr_next_layer",
     "zkb_gkr_sum", "zkb_gkr_fix_and_sum", "zkb_mle_fix_qm31", "zkb_mle_fix_m31", "zkb_grind", "zkb_gkr_sum_noalloc", "zkb_gkr_sum_noalloc_error",
     "zkb_freivalds_scatter", "zkb_freivalds_acc", "zkb_witness_tables", "zkb_witness_dequant", "zkb_witness_pre_table", "zkb_key_tile_flags",
-    "zkb_witness_selectors", "zkb_witness_residual_stream",
+    "zkb_witness_selectors", "zkb_witness_residual_stream", "zkb_step_embed", "zkb_step_norm_rope", "zkb_step_attention",
 ]
 # Every symbol include/zkb200_prover.h declares.
 PROVER_SYMBOLS = ["zkb_pcs_prove_device", "zkb_pcs_prove_host", "zkb_stark_prove_device", "zkb_stark_prove_host", "zkb_stark_prove_multi_device", "zkb_stark_prove_multi_host", "zkb_gkr_prove_device",
@@ -62,6 +62,39 @@ class RsMult(C.Structure):  # zkb_rs_mult
 
 class RsMults(C.Structure):  # zkb_rs_mults
     _fields_ = [("pow", RsMult), ("norm", RsMult), ("val", RsMult), ("frac", RsMult), ("smul", RsMult), ("un", C.c_void_p)]
+
+
+VALUE_BF16, VALUE_WORD, VALUE_INT8 = 0, 1, 2  # how values are held: ZKB_VALUE_*
+
+
+class StepEmbed(C.Structure):
+    """zkb_step_embed_args: build one with the buffers' addresses, keep it, pass it to Context.step_embed."""
+    _fields_ = [(k, C.c_void_p) for k in ("ids", "table", "row_scale", "out", "off_table")] + \
+               [(k, C.c_int64) for k in ("table_stride", "out_stride", "segment_stride")] + \
+               [(k, C.c_uint32) for k in ("n_tokens", "vocab", "width", "segment", "table_type", "out_type")] + [("scale", C.c_float)]
+
+
+class KvCache(C.Structure):  # zkb_kv_cache
+    _fields_ = [(k, C.c_void_p) for k in ("k", "v", "k_scale", "v_scale")] + \
+               [(k, C.c_int64) for k in ("seq_stride", "head_stride", "token_stride", "scale_seq_stride", "scale_head_stride")] + \
+               [(k, C.c_uint32) for k in ("type", "n_seqs", "n_heads", "head_dim", "capacity")]
+
+
+class StepRows(C.Structure):  # zkb_step_rows
+    _fields_ = [("first", C.c_void_p), ("kv_len", C.c_void_p), ("n_rows", C.c_uint32), ("max_rows", C.c_uint32), ("max_len", C.c_uint32)]
+
+
+class StepNormRope(C.Structure):
+    """zkb_step_norm_rope_args; h_inv_freq is the address of rotary_dim / 2 doubles on the host, which the caller keeps."""
+    _fields_ = [("cache", KvCache), ("rows", StepRows)] + [(k, C.c_void_p) for k in ("q", "k", "v", "q_weight", "k_weight", "h_inv_freq", "q_out")] + \
+               [(k, C.c_int64) for k in ("q_stride", "k_stride", "v_stride", "head_stride", "q_out_stride", "q_out_head_stride")] + \
+               [(k, C.c_uint32) for k in ("type", "q_heads", "rotary_dim", "interleaved")] + [("eps", C.c_float)]
+
+
+class StepAttention(C.Structure):  # zkb_step_attention_args
+    _fields_ = [("cache", KvCache), ("rows", StepRows), ("q", C.c_void_p), ("out", C.c_void_p)] + \
+               [(k, C.c_int64) for k in ("q_stride", "q_head_stride", "out_stride", "out_head_stride")] + \
+               [(k, C.c_uint32) for k in ("q_heads", "out_type", "window", "sinks")] + [("scale", C.c_float)]
 
 
 class PcsConfig(C.Structure):
@@ -114,6 +147,8 @@ def load_library():
         _lib.zkb_merkle_layer.argtypes = [p, i, p, p, i, i, p]
         _lib.zkb_fold_line.argtypes = [p, p, p, i, p]
         _lib.zkb_d2d.argtypes = [p, p, p, C.c_size_t]
+        for name, args in (("zkb_step_embed", StepEmbed), ("zkb_step_norm_rope", StepNormRope), ("zkb_step_attention", StepAttention)):
+            getattr(_lib, name).argtypes = [p, C.POINTER(args)]
     return _lib
 
 
@@ -699,6 +734,19 @@ class Context:
                                                          C.c_uint32(log_rows), _ptr_array(col_ptrs), C.c_uint32(len(col_ptrs)),
                                                          C.c_void_p(out_pat_ptr), C.c_void_p(out_nat_ptr), C.c_void_p(in_nat_ptr), C.byref(m),
                                                          C.c_void_p(counts_ptr)))
+
+    # ---- the values of a decode step
+    def step_embed(self, args):
+        """args: a StepEmbed."""
+        self._check(self.lib.zkb_step_embed(self.h, args))
+
+    def step_norm_rope(self, args):
+        """args: a StepNormRope."""
+        self._check(self.lib.zkb_step_norm_rope(self.h, args))
+
+    def step_attention(self, args):
+        """args: a StepAttention."""
+        self._check(self.lib.zkb_step_attention(self.h, args))
 
     # ---- constraint quotients of a lowered AIR (include/zkb200_air.h)
     def air_compile(self, source):
