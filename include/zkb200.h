@@ -509,7 +509,7 @@ typedef struct zkb_step_embed_args {
 int zkb_step_embed(zkb_ctx* ctx, const zkb_step_embed_args* args);
 
 /* A key-value cache: token p of kv head h of sequence b at b * seq_stride + h * head_stride + p * token_stride of k and of v,
- * head_dim values in a row. INT8 caches keep one scale a token and head: k_scale and v_scale at
+ * head_dim values in a row, token_stride at most 2^29 either way. INT8 caches keep one scale a token and head: k_scale and v_scale at
  * b * scale_seq_stride + h * scale_head_stride + p. head_dim is 32, 64 or 128. */
 typedef struct zkb_kv_cache {
     void* k;

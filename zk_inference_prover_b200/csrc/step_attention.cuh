@@ -1,40 +1,85 @@
 // Attention over the key-value cache: what its kernels share.
 #pragma once
+#include <cuda.h>
+
 #include "step_values.cuh"
 
 namespace zk {
 
 __device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
 __device__ __forceinline__ uint32_t cluster_ranks() { uint32_t r; asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r)); return r; }
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+__device__ __forceinline__ void cluster_arrive() {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
 }
-// A word at this thread block's place in the shared memory of another one of the cluster.
-__device__ __forceinline__ uint32_t peer_word(const void* p, int rank) {
-    uint32_t at = (uint32_t)__cvta_generic_to_shared(p), there, w;
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// To this thread block's place in the shared memory of another one of the cluster.
+__device__ __forceinline__ void peer_store_word(const void* p, int rank, uint32_t w) {
+    const uint32_t at = (uint32_t)__cvta_generic_to_shared(p);
+    uint32_t there;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(rank));
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(w) : "r"(there) : "memory");
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(there), "r"(w) : "memory");
+}
+__device__ __forceinline__ void peer_store(float* p, int rank, float x) { peer_store_word(p, rank, __float_as_uint(x)); }
+__device__ __forceinline__ void peer_store(int* p, int rank, int x) { peer_store_word(p, rank, (uint32_t)x); }
+__device__ __forceinline__ uint32_t ld_shared(uint32_t p) {
+    uint32_t w;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(p) : "memory");
     return w;
 }
-__device__ __forceinline__ float peer_load(const float* p, int rank) { return __uint_as_float(peer_word(p, rank)); }
-__device__ __forceinline__ int peer_load(const int* p, int rank) { return (int)peer_word(p, rank); }
+__device__ __forceinline__ void ld_shared2(uint32_t p, uint32_t& a, uint32_t& b) { asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(a), "=r"(b) : "r"(p) : "memory"); }
+__device__ __forceinline__ void ld_shared4(uint32_t p, uint32_t& a, uint32_t& b, uint32_t& c, uint32_t& d) {
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(a), "=r"(b), "=r"(c), "=r"(d) : "r"(p) : "memory");
+}
+__device__ __forceinline__ void st_shared(uint32_t p, uint32_t w) { asm volatile("st.shared.u32 [%0], %1;" ::"r"(p), "r"(w) : "memory"); }
 
-// What is read once: past L1.
-__device__ __forceinline__ uint4 ld_stream(const uint4* p) {
-    uint4 a;
-    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w) : "l"(p));
-    return a;
+// ---- copies by the tensor memory unit --------------------------------------------------------------------------------------------------
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory"); }
+__device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) { asm volatile("mbarrier.arrive.expect_tx.shared.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory"); }
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared.b64 _, [%0];" ::"r"(bar) : "memory"); }
+// Waits for the phase of this parity to end; false when the limit of tries (seconds) ran out.
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
+    for (int tries = 0; tries < (1 << 20); tries++) {
+        uint32_t done;
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+        if (done) return true;
+    }
+    return false;
+}
+// The box of a cache's map from (value, token, head, sequence) on.
+__device__ __forceinline__ void tma_load(uint32_t to, const CUtensorMap* map, int value, int token, int head, int seq, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(to), "l"(map), "r"(value), "r"(token), "r"(head), "r"(seq), "r"(bar)
+                 : "memory");
+}
+constexpr unsigned WAIT_RAN_OUT = 0x57e9;  // what zkb_sync reports
+
+// Maps of a cache's K and V (boxes of `tokens` tokens by up to 128 bytes, swizzled by their own width), or false where the layout has none: the unit wants
+// 16-byte boundaries and strides that ascend.
+struct CacheMaps {
+    CUtensorMap k, v;
+};
+bool cache_maps(CacheMaps& maps, const zkb_kv_cache& c, uint32_t tokens);
+
+// 2^x, to 2^-22 of it; below 2^-126 it is 0.
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
 // c += a b, sixteen rows of a and eight columns of b, over sixteen.
 __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 // An 8 x 8 matrix of 16-bit values, row g's values 2t and 2t + 1 in lane 4g + t, transposed.
 __device__ __forceinline__ uint32_t transpose8(uint32_t a) {
     uint32_t b;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(b) : "r"(a));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(b) : "r"(a));
     return b;
 }
 
@@ -42,18 +87,42 @@ __device__ __forceinline__ uint32_t bf16_sub2(uint32_t a, uint32_t b) {
     const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
     return *reinterpret_cast<const uint32_t*>(&r);
 }
+// (w & mask) | bits in one instruction: `bits` in a register that the compiler does not know the value of, or it would write two constants anew each time.
+template <uint32_t MASK>
+__device__ __forceinline__ uint32_t mask_or(uint32_t w, uint32_t bits) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "n"(MASK), "r"(bits));
+    return r;
+}
+__device__ __forceinline__ uint32_t bf16_128() {
+    uint32_t c;
+    asm volatile("mov.u32 %0, 0x43004300;" : "=r"(c));
+    return c;
+}
 // Two 8-bit codes, in the low bytes of the halves of w, as bf16 (exactly): the low seven bits under 2^7's exponent are 128 + those bits, the sign bit
-// in that pattern's last exponent bit makes 256 of 128, and the code is their difference.
-__device__ __forceinline__ uint32_t code_halves(uint32_t w) { return bf16_sub2((w & 0x007f007fu) | 0x43004300u, (w & 0x00800080u) | 0x43004300u); }
-// Four adjacent codes: the first two, the last two.
-__device__ __forceinline__ void codes_to_bf16(uint32_t w, uint32_t& lo, uint32_t& hi) {
-    lo = code_halves(__byte_perm(w, 0, 0x4140));
-    hi = code_halves(__byte_perm(w, 0, 0x4342));
+// in that pattern's last exponent bit makes 256 of 128, and the code is their difference. c128: bf16_128().
+__device__ __forceinline__ uint32_t code_halves(uint32_t w, uint32_t c128) { return bf16_sub2(mask_or<0x007f007fu>(w, c128), mask_or<0x00800080u>(w, c128)); }
+// Four adjacent codes as fp16 (exactly): the first and the third, the second and the fourth. A code's byte with its sign bit turned is code + 128; under 2^10's
+// exponent it is 1152 + code. c1152: f16_1152(). An instruction a pair less than in bf16, whose seven bits do not hold eight.
+__device__ __forceinline__ uint32_t f16_1152() {
+    uint32_t c;
+    asm volatile("mov.u32 %0, 0x64806480;" : "=r"(c));
+    return c;
+}
+__device__ __forceinline__ uint32_t code_halves_f16(uint32_t w, uint32_t c1152) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, 0x00ff00ff, %2, 0x6a;\n\tsub.f16x2 %0, %0, %2;" : "=&r"(r) : "r"(w), "r"(c1152));
+    return r;
+}
+__device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t c1152, uint32_t& even, uint32_t& odd) {
+    even = code_halves_f16(w, c1152);
+    odd = code_halves_f16(w >> 8, c1152);
 }
 // Two keys' codes of adjacent dimensions, bytes 2 * upper and 2 * upper + 1 of a word apiece: the keys' pair for the one, and for the other.
-__device__ __forceinline__ void pair_codes_to_bf16(uint32_t a, uint32_t b, int upper, uint32_t& first, uint32_t& second) {
-    first = code_halves(__byte_perm(a, b, upper ? 0x0602 : 0x0400));
-    second = code_halves(__byte_perm(a, b, upper ? 0x0703 : 0x0501));
+__device__ __forceinline__ void pair_codes_to_bf16(uint32_t a, uint32_t b, int upper, uint32_t c128, uint32_t& first, uint32_t& second) {
+    const uint32_t pair = __byte_perm(a, b, upper ? 0x7632 : 0x5410);  // a's two bytes, b's two bytes
+    first = code_halves(pair, c128);
+    second = code_halves(pair >> 8, c128);
 }
 
 // 0 * x + test in both halves: stays zero while all values are numbers.

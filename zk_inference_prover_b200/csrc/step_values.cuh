@@ -1,6 +1,7 @@
 // The values of a decode step (zkb_step_*): what its three operators share.
 #pragma once
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 
 #include <cmath>
 
@@ -13,6 +14,10 @@ __device__ __forceinline__ float bf16_high(uint32_t w) { return __uint_as_float(
 // Two values rounded to bf16, to nearest even, the first in the low half.
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+    const __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 __device__ __forceinline__ uint16_t round_bf16(float x) { return __bfloat16_as_ushort(__float2bfloat16_rn(x)); }
@@ -88,10 +93,12 @@ inline const char* step_problem(const zkb_kv_cache& c, const zkb_step_rows& r, u
     if (!c.k || !c.v) return "cache.k or cache.v is NULL";
     if (c.type == ZKB_VALUE_INT8 && (!c.k_scale || !c.v_scale)) return "an INT8 cache needs k_scale and v_scale";
     if (c.type == ZKB_VALUE_BF16 && (!aligned_to(c.k, 2) || !aligned_to(c.v, 2))) return "cache.k or cache.v is not on a 2-byte boundary";
+    if (c.type == ZKB_VALUE_INT8 && (!aligned_to(c.k_scale, 4) || !aligned_to(c.v_scale, 4))) return "k_scale or v_scale is not on a 4-byte boundary";
     if (c.n_seqs < 1 || c.n_seqs > 65535) return "cache.n_seqs is not in 1 .. 65535";
     if (c.n_heads < 1 || c.n_heads > 1024) return "cache.n_heads is not in 1 .. 1024";
     if (c.capacity < 1 || c.capacity > (1u << 30)) return "cache.capacity is not in 1 .. 2^30";
     if (c.capacity > 1 && std::llabs(c.token_stride) < (long long)c.head_dim) return "cache.token_stride is shorter than a row";
+    if (std::llabs(c.token_stride) > (1ll << 29)) return "cache.token_stride exceeds 2^29";
     if (!r.first || !r.kv_len) return "rows.first or rows.kv_len is NULL";
     if (r.n_rows > (1u << 30)) return "rows.n_rows exceeds 2^30";
     if (q_heads < 1 || q_heads % c.n_heads != 0 || q_heads / c.n_heads > 64) return "q_heads is not 1 to 64 times cache.n_heads";
