@@ -57,11 +57,6 @@ struct Few {
     static constexpr int SMEM = 1024 + (RING > JOIN ? RING : JOIN);  // boxes start on 1024 bytes
 };
 
-// Where byte `at` of a box's row lies.
-template <int BOX>
-__device__ __forceinline__ uint32_t box_place(int row, int at) {
-    return row * BOX + (BOX == 128 ? at ^ ((row & 7) << 4) : BOX == 64 ? at ^ (((row >> 1) & 3) << 4) : at);
-}
 // WORDS words from byte `at` of a row on.
 template <int BOX, int WORDS>
 __device__ __forceinline__ void read_row(uint32_t box, int row, int at, uint32_t* w) {
@@ -415,7 +410,9 @@ static cudaError_t launch_few(zkb_ctx* ctx, const zkb_step_attention_args& a) {
 template <int D>
 static cudaError_t launch_attention(zkb_ctx* ctx, const zkb_step_attention_args& a) {
     const zkb_kv_cache& c = a.cache;
-    return c.type == ZKB_VALUE_INT8 ? launch_few<D, true>(ctx, a) : launch_few<D, false>(ctx, a);
+    const uint64_t most = (uint64_t)(a.rows.max_rows ? std::min(a.rows.max_rows, a.rows.n_rows) : a.rows.n_rows) * (a.q_heads / c.n_heads);
+    const bool few = most <= 8;
+    return c.type == ZKB_VALUE_INT8 ? (few ? launch_few<D, true>(ctx, a) : launch_many<D, true>(ctx, a)) : (few ? launch_few<D, false>(ctx, a) : launch_many<D, false>(ctx, a));
 }
 
 }  // namespace zk

@@ -22,6 +22,14 @@ __device__ __forceinline__ void peer_store_word(const void* p, int rank, uint32_
 }
 __device__ __forceinline__ void peer_store(float* p, int rank, float x) { peer_store_word(p, rank, __float_as_uint(x)); }
 __device__ __forceinline__ void peer_store(int* p, int rank, int x) { peer_store_word(p, rank, (uint32_t)x); }
+__device__ __forceinline__ void peer_store4(uint32_t at, int rank, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    uint32_t there;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(rank));
+    asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(there), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+// A barrier of some of the thread block's warps.
+__device__ __forceinline__ void named_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+__device__ __forceinline__ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 __device__ __forceinline__ uint32_t ld_shared(uint32_t p) {
     uint32_t w;
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(p) : "memory");
@@ -31,6 +39,7 @@ __device__ __forceinline__ void ld_shared2(uint32_t p, uint32_t& a, uint32_t& b)
 __device__ __forceinline__ void ld_shared4(uint32_t p, uint32_t& a, uint32_t& b, uint32_t& c, uint32_t& d) {
     asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(a), "=r"(b), "=r"(c), "=r"(d) : "r"(p) : "memory");
 }
+__device__ __forceinline__ void st_shared4(uint32_t p, uint32_t a, uint32_t b, uint32_t c, uint32_t d) { asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(p), "r"(a), "r"(b), "r"(c), "r"(d) : "memory"); }
 __device__ __forceinline__ void st_shared(uint32_t p, uint32_t w) { asm volatile("st.shared.u32 [%0], %1;" ::"r"(p), "r"(w) : "memory"); }
 
 // ---- copies by the tensor memory unit --------------------------------------------------------------------------------------------------
@@ -51,6 +60,11 @@ __device__ __forceinline__ void tma_load(uint32_t to, const CUtensorMap* map, in
     asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(to), "l"(map), "r"(value), "r"(token), "r"(head), "r"(seq), "r"(bar)
                  : "memory");
 }
+// Where byte `at` of a box's row lies, boxes as wide as BOX bytes.
+template <int BOX>
+__device__ __forceinline__ uint32_t box_place(int row, int at) {
+    return row * BOX + (BOX == 128 ? at ^ ((row & 7) << 4) : BOX == 64 ? at ^ (((row >> 1) & 3) << 4) : at);
+}
 constexpr unsigned WAIT_RAN_OUT = 0x57e9;  // what zkb_sync reports
 
 // Maps of a cache's K and V (boxes of `tokens` tokens by up to 128 bytes, swizzled by their own width), or false where the layout has none: the unit wants
@@ -59,6 +73,9 @@ struct CacheMaps {
     CUtensorMap k, v;
 };
 bool cache_maps(CacheMaps& maps, const zkb_kv_cache& c, uint32_t tokens);
+
+template <int D, bool INT8>
+cudaError_t launch_many(zkb_ctx* ctx, const zkb_step_attention_args& a);  // step_attention_many.cu
 
 // 2^x, to 2^-22 of it; below 2^-126 it is 0.
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -138,7 +155,7 @@ __device__ __forceinline__ uint32_t numbers_only(uint32_t x) {
 }
 // The sum of what is no number among the values of dimension d that the row at position p sees (bf16 caches): the products are made without
 // those values, because a matrix product has no way to keep 0 * NaN from the rows that do not see the key. Slow, and only for caches that hold such values.
-__device__ __noinline__ float what_is_no_number(const char* v, int64_t row_bytes, int d, int64_t p, uint32_t capacity, uint32_t window, uint32_t sinks) {
+static __device__ __noinline__ float what_is_no_number(const char* v, int64_t row_bytes, int d, int64_t p, uint32_t capacity, uint32_t window, uint32_t sinks) {
     float y = 0.f;
     const int64_t end = min(p + 1, (int64_t)capacity), near = window ? max((int64_t)0, p - (int64_t)window + 1) : 0;
     for (int64_t j = 0; j < end; j++) {
