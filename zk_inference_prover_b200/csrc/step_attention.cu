@@ -387,7 +387,7 @@ static cudaError_t launch_few(zkb_ctx* ctx, const zkb_step_attention_args& a) {
     // bf16 tokens take 14.6 us in 128 thread blocks and 22.8 in 256, one of 2,048 int8 tokens 23.2 in 8 and 10.6 in 64.
     const uint64_t units = (uint64_t)c.n_seqs * c.n_heads * tiles;
     uint32_t ranks = 1;
-    while (ranks < FEW_RANKS && units * ranks * 2 <= 148 * Few<D, INT8>::THREAD_BLOCKS && len > (uint64_t)ranks * FEW_WARPS * 16 * 2) ranks *= 2;
+    while (ranks < FEW_RANKS && units <= clusters_at_once(2 * ranks) * Few<D, INT8>::THREAD_BLOCKS && len > (uint64_t)ranks * FEW_WARPS * 16 * 2) ranks *= 2;
     CacheMaps maps;
     const bool tma = cache_maps(maps, c, 16);
     auto kernel = tma ? attention_few_kernel<D, INT8, true> : attention_few_kernel<D, INT8, false>;
