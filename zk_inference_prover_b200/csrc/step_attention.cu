@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, Few<D, INT8>::THREAD_BLOCKS)
             asm volatile("cp.async.commit_group;" ::: "memory");
             asm volatile("cp.async.wait_group %0;" ::"n"(F::STAGES - 1) : "memory");
             __syncwarp();
-            if (TMA && !failed) failed = !mbar_wait(bars + 8 * stage, parity);
+            if (TMA) failed = __any_sync(0xffffffffu, failed || !mbar_wait(bars + 8 * stage, parity));
             if (++stage == F::STAGES) stage = 0, parity ^= 1;
             float sc[4] = {0.f, 0.f, 0.f, 0.f}, sc2[4] = {0.f, 0.f, 0.f, 0.f};
             {
