@@ -6,13 +6,13 @@
 namespace zk {
 
 // Two tiles of 128 query rows (the heads of a kv head's group, token after token) share each block of 128 keys: S = Q K^T and O += P V are tcgen05
-// products whose sums lie in tensor memory, P in bf16 where S was. A tile's rows have two threads each, 64 keys apiece, that agree on the row's maximum and
-// need no one else. While one tile's rows are in the softmax the other's products run: per block and pair, 128 x 128 head dimensions take the tensor cores 2,048 cycles
-// (2,600 as it is: a product of 128 x 128 x 16 whose operands both come from shared memory is bound by that) and the exponentials, 16 a clock, 2,048.
-// Warps: 0-7 and 8-15 the tiles' rows, 16 the copies, 17 the products, 18 and on what has to be done to keys and values before a product may read them: 8-bit codes become
+// products whose sums lie in tensor memory, P in bf16 where S was. A thread has a row: its maximum, sum and weights need no other thread. The keys are taken
+// 64 at a time with two places for S a tile, so that a tile's next scores are there when its rows are done with the last ones: with one place of 128 keys each tile went
+// softmax, P V, Q K^T, softmax, 3,800 cycles a block and pair, where the tensor cores need 2,048 and the exponentials, 16 a clock, as many.
+// Warps: 0-3 and 4-7 the tiles' rows, 8 the copies, 9 the products, 10 and on what has to be done to keys and values before a product may read them: 8-bit codes become
 // fp16 (K) and bf16 (V), exactly; bf16 values behind the last token or that are no numbers are zeroed where some row does not see them.
 // A thread block takes one pair of tiles after the other; with too few of them for the GPU the keys are spread over a cluster's thread blocks, which add up through
-// each other's shared memory.
+// each other's shared memory, and one tile alone is two, of each block's two halves.
 constexpr int MANY_KEYS = 128, MANY_RANKS = 16;
 
 template <int D, bool INT8>
@@ -21,7 +21,7 @@ struct Many {
     static constexpr int BOX = D * 2 < 128 ? D * 2 : 128, PANELS = D * 2 / BOX;  // bytes of a panel's row of 16-bit values
     static constexpr int TILE = 128 * D * 2;  // bytes of 128 rows of 16-bit values
     static constexpr int RAW_BOX = D * SIZE < 128 ? D * SIZE : 128, RAW_BOXES = D * SIZE / RAW_BOX, RAW = 128 * D * SIZE;  // as the cache has them
-    static constexpr int READIERS = INT8 ? 192 : 64, THREADS = 576 + READIERS;  // threads that make ready, all
+    static constexpr int READIERS = INT8 ? 192 : 64, THREADS = 320 + READIERS;  // threads that make ready, all
     static constexpr int STAGES = INT8 ? 3 : 4, RAWS = INT8 ? 3 : 0;
     static constexpr int RING = STAGES * TILE, RAW_RING = RAWS * RAW;
     static_assert(256 * (D + 2) * 4 <= 2 * TILE + RING + RAW_RING, "the cluster's sums lie where Q and the keys were");
@@ -35,14 +35,24 @@ struct Many {
 // its swizzle (2: 128 bytes, 4: 64) in the upper.
 // kind::f16, sums in 32-bit floats, 128 rows: B type and A type 0 fp16, 1 bf16; b_along_n: B's rows run along N.
 __host__ __device__ constexpr uint32_t product_desc(int type, int n, bool b_along_n) { return 1u << 4 | (uint32_t)type << 7 | (uint32_t)type << 10 | (uint32_t)b_along_n << 16 | (uint32_t)(n / 8) << 17 | (128u / 16) << 24; }
-__device__ __forceinline__ void product_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t desc, bool add) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(desc), "r"((uint32_t)add) : "memory");
+// (Called by a whole warp; one lane issues. What the lanes have in common is then in uniform registers, where the instruction wants it.)
+__device__ __forceinline__ void product_ss(bool one, uint32_t d, uint64_t a, uint64_t b, uint32_t desc, bool add) {
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(desc), "r"((uint32_t)add),
+                 "r"((uint32_t)one)
+                 : "memory");
 }
-__device__ __forceinline__ void product_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t desc, bool add) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(desc), "r"((uint32_t)add) : "memory");
+__device__ __forceinline__ void product_ts(bool one, uint32_t d, uint32_t a, uint64_t b, uint32_t desc, bool add) {
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(desc), "r"((uint32_t)add),
+                 "r"((uint32_t)one)
+                 : "memory");
 }
 // The barrier gets an arrival when the products issued so far are done.
 __device__ __forceinline__ void products_done(uint32_t bar) { asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one;
+}
 __device__ __forceinline__ void tmem_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tmem_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -58,8 +68,9 @@ __device__ __forceinline__ void tmem_load32(uint32_t at, uint32_t* x) {
                  : R8(x, 0), R8(x, 8), R8(x, 16), R8(x, 24) : "r"(at));
 }
 __device__ __forceinline__ void tmem_load8(uint32_t at, uint32_t* x) { asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];" : R8(x, 0) : "r"(at)); }
-__device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t* x) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(at), W8(x, 0), W8(x, 8) : "memory");
+__device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t* x) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(at),
+                 W8(x, 0), W8(x, 8), W8(x, 16), W8(x, 24) : "memory");
 }
 __device__ __forceinline__ void tmem_store8(uint32_t at, const uint32_t* x) { asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(at), W8(x, 0) : "memory"); }
 #undef R8
@@ -76,6 +87,11 @@ __device__ __forceinline__ uint64_t two_floats(float a, float b) { return two_wo
 __device__ __forceinline__ void mul2(uint32_t& x, uint32_t& y, float a, float b) {
     asm("{\n\t.reg .b64 p;\n\tmul.rn.f32x2 p, %2, %3;\n\tmov.b64 {%0, %1}, p;\n\t}" : "=r"(x), "=r"(y) : "l"(two_words(x, y)), "l"(two_floats(a, b)));
 }
+__device__ __forceinline__ void scale2(float& x, float& y, float a, float b) {
+    uint32_t u = __float_as_uint(x), v = __float_as_uint(y);
+    mul2(u, v, a, b);
+    x = __uint_as_float(u), y = __uint_as_float(v);
+}
 __device__ __forceinline__ void fma2(uint32_t& x, uint32_t& y, float by, float plus) {
     asm("{\n\t.reg .b64 p;\n\tfma.rn.f32x2 p, %2, %3, %4;\n\tmov.b64 {%0, %1}, p;\n\t}" : "=r"(x), "=r"(y) : "l"(two_words(x, y)), "l"(two_floats(by, by)), "l"(two_floats(plus, plus)));
 }
@@ -83,11 +99,15 @@ __device__ __forceinline__ void add2(uint32_t& x, uint32_t& y, float a, float b)
     asm("{\n\t.reg .b64 p;\n\tadd.rn.f32x2 p, %2, %3;\n\tmov.b64 {%0, %1}, p;\n\t}" : "=r"(x), "=r"(y) : "l"(two_words(x, y)), "l"(two_floats(a, b)));
 }
 
+// 32 bytes, on a 32-byte boundary: a whole sector at once.
+__device__ __forceinline__ void store32(void* to, const uint32_t (&x)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7]) : "memory");
+}
 // The lowest n bits.
 __device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 
 struct ManyBars {
-    unsigned long long full[5], ready[5], empty[5], raw_full[4], raw_empty[4], s_ready[2], p_ready[2], o_ready[2], q_ready;
+    unsigned long long full[5], ready[5], empty[5], raw_full[4], raw_empty[4], s_ready[4], p_ready[4], o_ready[2], q_ready;  // s, p: of a tile's two places in turn
 };
 __device__ __forceinline__ uint32_t bar_of(const unsigned long long& b) { return (uint32_t)__cvta_generic_to_shared(&b); }
 
@@ -98,13 +118,12 @@ __device__ __forceinline__ uint32_t tile_place(int row, int at) {
     return at / M::BOX * (128 * M::BOX) + box_place<M::BOX>(row, at % M::BOX);
 }
 
-// Two tiles of one sequence's rows and one kv head, and the blocks of keys that this thread block has for them. With one tile only, both work on it, each on every
-// other block (split): their sums are joined as those of a cluster's thread blocks are.
+// Two tiles of one sequence's rows and one kv head, and the blocks of keys that this thread block has for them. With one tile only, both can work on it, each on a
+// half of every block (split): their sums are joined as those of a cluster's thread blocks are.
 struct Unit {
     StepSequence s;
     KeyBlocks blocks;
-    int64_t n_m, m0;
-    int seq, kv_head, last, n, whole_from, whole_to;
+    int seq, kv_head, n_m, m0, last, n, whole_from, whole_to;
     bool two, split;
 };
 // All units of a thread block, the ones with the most keys first: pair after pair from the last tokens on, in each all sequences and heads.
@@ -128,22 +147,22 @@ struct Units {
             const uint32_t one = at % (c.n_seqs * c.n_heads), z = at / (c.n_seqs * c.n_heads);
             u.seq = (int)(one / c.n_heads), u.kv_head = (int)(one % c.n_heads);
             u.s = step_sequence(a.rows, u.seq);
-            u.n_m = (int64_t)u.s.rows * group;
-            pair = (int)((u.n_m + 255) / 256) - 1 - (int)z;
+            u.n_m = u.s.rows * group;
+            pair = (u.n_m + 255) / 256 - 1 - (int)z;
         }
-        u.m0 = (int64_t)pair * 256;
+        u.m0 = pair * 256;
         u.two = u.m0 + 128 < u.n_m;
-        const int64_t low = u.s.pos + u.m0 / group, high = u.s.pos + (min(u.m0 + 256, u.n_m) - 1) / group;
+        const int64_t low = u.s.pos + (uint32_t)u.m0 / (uint32_t)group, high = u.s.pos + (uint32_t)(min(u.m0 + 256, u.n_m) - 1) / (uint32_t)group;
         u.blocks = key_blocks<MANY_KEYS>(low, high, c.capacity, a.window, a.sinks);
         u.last = u.blocks.end - 1;
         u.n = u.blocks.n > rank ? (u.blocks.n - rank + ranks - 1) / ranks : 0;
-        u.split = !u.two && u.blocks.n > ranks;
-        // blocks of which every row sees every key
-        u.whole_to = (int)min(low, (int64_t)u.last) - (MANY_KEYS - 1), u.whole_from = a.window ? (int)max((int64_t)0, high - (int64_t)a.window + 1) : 0;
+        u.split = !u.two && (ranks > 1 || u.blocks.n > 2);
+        // keys that every row sees
+        u.whole_to = (int)min(low, (int64_t)u.last), u.whole_from = a.window ? (int)max((int64_t)0, high - (int64_t)a.window + 1) : 0;
         return true;
     }
     __device__ __forceinline__ int base(const Unit& u, int j) const { return u.blocks.base(rank + j * ranks); }
-    __device__ __forceinline__ bool whole(const Unit& u, int base) const { return base >= u.whole_from && base <= u.whole_to; }
+    __device__ __forceinline__ bool whole(const Unit& u, int base, int keys) const { return base >= u.whole_from && base + keys - 1 <= u.whole_to; }
     __device__ __forceinline__ bool joined(const Unit& u) const { return ranks > 1 || u.split; }
 };
 
@@ -158,7 +177,6 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
     __shared__ int in_odd[MANY_RANKS];
     __shared__ int odd_sm[8];  // some value was no number: of the units in turn (what makes ready runs a few units ahead)
     __shared__ uint32_t tmem_sm;
-    __shared__ float row_sm[2][2][2][128];  // [block in turn][tile][half]: what the two threads of a row tell each other
     unsigned char* const sm = many_sm + (-(uint32_t)__cvta_generic_to_shared(many_sm) & 1023);
     float *const in_top = reinterpret_cast<float*>(sm + 256 * D * 4), *const in_sum = in_top + 256;  // behind the sums that are joined, where Q and the keys were
     const uint32_t q_at = (uint32_t)__cvta_generic_to_shared(sm), ring = q_at + 2 * M::TILE, raw_ring = ring + M::RING;
@@ -170,8 +188,9 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
     } else if (warp == 1 && lane == 0) {
         for (int i = 0; i < 5; i++) mbar_init(bar_of(bars.full[i]), 1), mbar_init(bar_of(bars.ready[i]), M::READIERS), mbar_init(bar_of(bars.empty[i]), 1);
         for (int i = 0; i < 4; i++) mbar_init(bar_of(bars.raw_full[i]), 1), mbar_init(bar_of(bars.raw_empty[i]), M::READIERS);
-        for (int i = 0; i < 2; i++) mbar_init(bar_of(bars.s_ready[i]), 2), mbar_init(bar_of(bars.p_ready[i]), 256), mbar_init(bar_of(bars.o_ready[i]), 1);
-        mbar_init(bar_of(bars.q_ready), 512);
+        for (int i = 0; i < 4; i++) mbar_init(bar_of(bars.s_ready[i]), 2), mbar_init(bar_of(bars.p_ready[i]), 128);
+        for (int i = 0; i < 2; i++) mbar_init(bar_of(bars.o_ready[i]), 1);
+        mbar_init(bar_of(bars.q_ready), 256);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -198,17 +217,22 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
     Unit u, after;
     bool more = units.next(u);
 
-    if (warp < 16) {  // ---- the rows: softmax
-        const int tile = warp >> 3, half = warp >> 2 & 1, row = threadIdx.x & 127;
-        const uint32_t lanes = (uint32_t)(warp & 3) << 21, s_at = tmem + tile * 128 + half * 64 + lanes, o_at = tmem + 256 + tile * D + half * (D / 2) + lanes;
+    if (warp < 8) {  // ---- the rows: softmax
+        const int tile = warp >> 2, row = threadIdx.x & 127;
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21, s_at = tmem + tile * 128 + lanes, o_at = tmem + 256 + tile * D + lanes;
         const float by = fmaxf(fabsf(a.scale) * 1.44269504f, 1.2e-38f);  // not zero: what is hidden is -inf times this
-        uint32_t done = 0, passed = 0, odd_at = 0;  // blocks of this tile, of all, units with blocks: what the barriers' phases, the scales' places and the flags go by
-        // This thread's half of a row of Q into shared memory, its sign that of the scale; for fp16 each row times the power of two that brings its largest value
+        uint32_t done = 0, passed = 0, odd_at = 0;  // steps of this tile, blocks, units with blocks: what the barriers' phases, the scales' places and the flags go by
+        auto row_of = [&](const Unit& n) { return n.m0 + (n.split ? row : tile * 128 + row); };
+        auto q_of = [&](const Unit& n, int m) {
+            const uint32_t i = (uint32_t)m / (uint32_t)group;
+            return static_cast<const uint16_t*>(a.q) + (n.s.first + (int)i) * a.q_stride + (n.kv_head * group + m - (int)i * group) * a.q_head_stride;
+        };
+        // This thread's row of Q into shared memory, its sign that of the scale; for fp16 each row times the power of two that brings its largest value
         // to 2^13: exact down to 2^-27 of that value, and below it off by 2^-38 of it. The factor that is left for the row's scores.
         auto load_q = [&](const Unit& n) {
-            const int64_t m = n.m0 + (n.split ? row : tile * 128 + row);
+            const int m = row_of(n);
             const bool live = m < n.n_m;
-            const uint16_t* from = static_cast<const uint16_t*>(a.q) + (live ? (n.s.first + m / group) * a.q_stride + (n.kv_head * group + m % group) * a.q_head_stride : 0);
+            const uint16_t* from = q_of(n, live ? m : 0);
             const bool vec = aligned16(from);
             auto eight = [&](int at) {
                 uint4 x = make_uint4(0u, 0u, 0u, 0u);
@@ -221,7 +245,7 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
             float f = 1.f, left = by;
             if constexpr (INT8) {
                 float most = 0.f;
-#pragma unroll 4
+#pragma unroll 8
                 for (int i = 0; i < D; i += 8) {
                     const uint4 x = eight(i);
                     for (uint32_t w : {x.x, x.y, x.z, x.w}) most = fmaxf(most, fmaxf(fabsf(bf16_low(w)), fabsf(bf16_high(w))));
@@ -232,8 +256,8 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
             }
             const uint32_t turn = a.scale < 0.f ? 0x80008000u : 0u;
             auto word = [&](uint32_t w) { return (INT8 ? pack_f16(bf16_low(w) * f, bf16_high(w) * f) : w) ^ turn; };
-#pragma unroll 4
-            for (int i = half * (D / 2); i < (half + 1) * (D / 2); i += 8) {
+#pragma unroll 8
+            for (int i = 0; i < D; i += 8) {
                 const uint4 x = eight(i);
                 st_shared4(q_at + tile * M::TILE + tile_place<D, INT8>(row, i * 2), word(x.x), word(x.y), word(x.z), word(x.w));
             }
@@ -243,60 +267,64 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
         };
         float by_row = more ? load_q(u) : 0.f;
         while (more) {
-            const int64_t m = u.m0 + (u.split ? row : tile * 128 + row);  // this thread's row
+            const int m = row_of(u);  // this thread's row
             const bool live = m < u.n_m;
-            const int p = live ? (int)(u.s.pos + m / group) : -1;
+            const int p = live ? (int)u.s.pos + (int)((uint32_t)m / (uint32_t)group) : -1;
             const int low = a.window ? max(0, p - (int)min(a.window, 1u << 30) + 1) : 0, high = min(p, u.last), sinks = a.window ? (int)min(a.sinks, c.capacity) : 0;
+            {  // the next unit's Q comes nearer
+                Units ahead = units;
+                Unit n;
+                if (ahead.next(n)) {
+                    const int mm = row_of(n);
+                    if (mm < n.n_m)
+                        for (int i = 0; i < D; i += 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(q_of(n, mm) + i));
+                }
+            }
             float top = -INFINITY, less = 0.f, sum = 0.f;
-            const int j0 = u.split ? tile : tile == 0 || u.two ? 0 : u.n, j_step = u.split ? 2 : 1;
-            for (int j = j0; j < u.n; j += j_step, done++) {
-                const int base = units.base(u, j);
-                const bool whole = units.whole(u, base);
-                const int slot = (passed + j) & 1;
-                wait(bars.s_ready[tile], done);
+            const int steps = u.split ? u.n : tile == 0 || u.two ? 2 * u.n : 0;
+            for (int j = 0; j < steps; j++, done++) {
+                const int block = u.split ? j : j >> 1, half = u.split ? tile : j & 1, base = units.base(u, block) + 64 * half, slot = (passed + block) & 1;
+                const bool whole = units.whole(u, base, 64);
+                const uint32_t place = s_at + (done & 1) * 64;
+                wait(bars.s_ready[2 * tile + (done & 1)], done >> 1);
                 tmem_fence_after();
-                // 32 of this thread's 64 scores, still without the factor by_row; bits of those that the row sees
-                auto scores = [&](int i, uint32_t (&x)[32]) {
-                    if constexpr (INT8) {
+                uint32_t x[64];  // the row's scores, still without the factor by_row
+                uint32_t(&x0)[32] = *reinterpret_cast<uint32_t(*)[32]>(&x[0]), (&x1)[32] = *reinterpret_cast<uint32_t(*)[32]>(&x[32]);
+                tmem_load32(place, x0);
+                tmem_load32(place + 32, x1);
+                tmem_loaded(x0);
+                tmem_loaded(x1);
+                if constexpr (INT8) {
 #pragma unroll
-                        for (int y = 0; y < 32; y += 4) {
-                            const float4 ks = *reinterpret_cast<const float4*>(&k_scale_sm[slot][half * 64 + i + y]);
-                            mul2(x[y], x[y + 1], ks.x, ks.y), mul2(x[y + 2], x[y + 3], ks.z, ks.w);
-                        }
+                    for (int y = 0; y < 64; y += 4) {
+                        const float4 ks = *reinterpret_cast<const float4*>(&k_scale_sm[slot][half * 64 + y]);
+                        mul2(x[y], x[y + 1], ks.x, ks.y), mul2(x[y + 2], x[y + 3], ks.z, ks.w);
                     }
-                    uint32_t seen = 0xffffffffu;
-                    if (!whole) {
-                        const int at = base + half * 64 + i;
-                        seen = bits_below(high + 1 - at) & (~bits_below(low - at) | bits_below(sinks - at));
+                }
+                uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
+                if (!whole) {
 #pragma unroll
-                        for (int y = 0; y < 32; y++) x[y] = seen >> y & 1 ? x[y] : 0xff800000u;  // -inf
+                    for (int i = 0; i < 2; i++) {
+                        const int at = base + 32 * i;
+                        seen[i] = bits_below(high + 1 - at) & (~bits_below(low - at) | bits_below(sinks - at));
+#pragma unroll
+                        for (int y = 0; y < 32; y++) x[32 * i + y] = seen[i] >> y & 1 ? x[32 * i + y] : 0xff800000u;  // -inf
                     }
-                    return seen;
-                };
+                }
                 float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int i = 0; i < 64; i += 32) {
-                    uint32_t x[32];
-                    tmem_load32(s_at + i, x);
-                    tmem_loaded(x);
-                    scores(i, x);
-#pragma unroll
-                    for (int z = 0; z < 32; z++) most[z & 3] = fmaxf(most[z & 3], __uint_as_float(x[z]));
-                }
-                float higher = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
-                row_sm[done & 1][tile][half][row] = higher;
-                named_sync(1 + tile, 256);
-                higher = fmaxf(higher, row_sm[done & 1][tile][half ^ 1][row]) * by_row;
+                for (int z = 0; z < 64; z++) most[z & 3] = fmaxf(most[z & 3], __uint_as_float(x[z]));
+                const float higher = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * by_row;
                 // The weights' common factor is 2^-top. It need not be the largest score's, only within 2^8 of it, so O is seldom read back for it.
                 const bool need = higher > top + 8.f;
                 if (__any_sync(0xffffffffu, need)) {
                     const float keep = need ? exp2_fast(top - higher) : 1.f;
                     if (need) top = higher, less = higher, sum *= keep;
-                    if (j > j0) {
+                    if (j > 0) {
                         wait(bars.o_ready[tile], done - 1);
                         tmem_fence_after();
 #pragma unroll 1
-                        for (int i = 0; i < D / 2; i += 8) {  // few at a time: the scores keep their registers
+                        for (int i = 0; i < D; i += 8) {  // few at a time: the scores keep their registers
                             uint32_t o[8];
                             tmem_load8(o_at + i, o);
                             tmem_loaded(o);
@@ -308,45 +336,34 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
                 }
                 uint32_t part[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
-                for (int i = 0; i < 64; i += 32) {  // the weights of this thread's scores go to the first half of where those were; read again, the scores need no registers between
-                    uint32_t y[32];
-                    tmem_load32(s_at + i, y);
-                    tmem_loaded(y);
-                    const uint32_t seen = scores(i, y);
+                for (int z = 0; z < 64; z += 4) {
+                    float w[4];
 #pragma unroll
-                    for (int z = 0; z < 32; z += 4) {
-                        float w[4];
-#pragma unroll
-                        for (int e = 0; e < 4; e += 2) {
-                            uint32_t f0 = y[z + e], f1 = y[z + e + 1];
-                            fma2(f0, f1, by_row, -less);
-                            w[e] = exp2_fast(__uint_as_float(f0)), w[e + 1] = exp2_fast(__uint_as_float(f1));
-                            add2(part[e], part[e + 1], w[e], w[e + 1]);
-                        }
-                        if constexpr (INT8) {
-                            const float4 vs = *reinterpret_cast<const float4*>(&v_scale_sm[slot][half * 64 + i + z]);
-                            w[0] *= vs.x, w[1] *= vs.y, w[2] *= vs.z, w[3] *= vs.w;
-                            if (!whole)
-#pragma unroll
-                                for (int e = 0; e < 4; e++) w[e] = seen >> (z + e) & 1 ? w[e] : 0.f;  // a hidden token's scale may be anything
-                        }
-                        y[z / 2] = pack_bf16(w[0], w[1]), y[z / 2 + 1] = pack_bf16(w[2], w[3]);
+                    for (int e = 0; e < 4; e += 2) {
+                        uint32_t f0 = x[z + e], f1 = x[z + e + 1];
+                        fma2(f0, f1, by_row, -less);
+                        w[e] = exp2_fast(__uint_as_float(f0)), w[e + 1] = exp2_fast(__uint_as_float(f1));
+                        add2(part[e], part[e + 1], w[e], w[e + 1]);
                     }
-                    tmem_store16(s_at + i / 2, y);
+                    if constexpr (INT8) {
+                        const float4 vs = *reinterpret_cast<const float4*>(&v_scale_sm[slot][half * 64 + z]);
+                        scale2(w[0], w[1], vs.x, vs.y), scale2(w[2], w[3], vs.z, vs.w);
+                        if (!whole)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) w[e] = seen[z / 32] >> (z % 32 + e) & 1 ? w[e] : 0.f;  // a hidden token's scale may be anything
+                    }
+                    x[z / 2] = pack_bf16(w[0], w[1]), x[z / 2 + 1] = pack_bf16(w[2], w[3]);
                 }
+                tmem_store32(place, x0);  // the weights go to the first half of where the scores were
                 sum += (__uint_as_float(part[0]) + __uint_as_float(part[1])) + (__uint_as_float(part[2]) + __uint_as_float(part[3]));
                 tmem_stored();
                 tmem_fence_before();
-                mbar_arrive(bar_of(bars.p_ready[tile]));
+                mbar_arrive(bar_of(bars.p_ready[2 * tile + (done & 1)]));
             }
-            const bool any = j0 < u.n, join = units.joined(u), again = units.next(after);
+            const bool any = steps > 0, join = units.joined(u), again = units.next(after);
             float by_next = by_row;
             if (again && !join) by_next = load_q(after);  // its products begin while this unit's rows are written
-            if (any) {  // the row's sum is both halves'
-                row_sm[done & 1][tile][half][row] = sum;
-                named_sync(1 + tile, 256);
-                sum += row_sm[done & 1][tile][half ^ 1][row];
-                named_sync(1 + tile, 256);
+            if (any) {
                 wait(bars.o_ready[tile], done - 1);
                 tmem_fence_after();
             }
@@ -356,23 +373,42 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
                 const int odd = odd_values();
                 if (tile == 0 || u.two) {
                     const float inverse = sum == 0.f ? 0.f : 1.f / sum;
-                    const int64_t to = live ? (u.s.first + m / group) * a.out_stride + (u.kv_head * group + m % group) * a.out_head_stride : 0;
-                    const bool word = a.out_type == ZKB_VALUE_WORD, vec = aligned16(static_cast<char*>(a.out) + to * (word ? 4 : 2));
+                    const int i0 = (int)((uint32_t)m / (uint32_t)group);
+                    const int64_t to = live ? (u.s.first + i0) * a.out_stride + (u.kv_head * group + m - i0 * group) * a.out_head_stride : 0;
+                    const bool word = a.out_type == ZKB_VALUE_WORD, vec = ((uintptr_t)(static_cast<char*>(a.out) + to * (word ? 4 : 2)) & 31) == 0;
 #pragma unroll 1
-                    for (int i = 0; i < D / 2; i += 16) {
+                    for (int i = 0; i < D; i += 16) {
                         uint32_t o[2][8];
                         if (any) tmem_load8(o_at + i, o[0]), tmem_load8(o_at + i + 8, o[1]), tmem_loaded(o[0]), tmem_loaded(o[1]);
                         if (!live) continue;
+                        const int d = i;
+                        float z[16];
 #pragma unroll
-                        for (int y = 0; y < 2; y++) {
-                            const int d = half * (D / 2) + i + 8 * y;
-                            float z[8];
+                        for (int e = 0; e < 16; e++) z[e] = sum == 0.f || !any ? 0.f : __uint_as_float(o[e / 8][e & 7]) * inverse;
+                        if (odd)
 #pragma unroll
-                            for (int e = 0; e < 8; e++) z[e] = sum == 0.f || !any ? 0.f : __uint_as_float(o[y][e]) * inverse;
-                            if (odd)
-                                for (int e = 0; e < 8; e++) z[e] += what_is_no_number(v, row_bytes, d + e, p, c.capacity, a.window, a.sinks);
-                            if (word) vec ? store8<true, true>(a.out, to + d, z) : store8<true, false>(a.out, to + d, z);
-                            else vec ? store8<false, true>(a.out, to + d, z) : store8<false, false>(a.out, to + d, z);
+                            for (int e = 0; e < 16; e++) z[e] += what_is_no_number(v, row_bytes, d + e, p, c.capacity, a.window, a.sinks);
+                        uint32_t w[8];
+#pragma unroll
+                        for (int e = 0; e < 8; e++) w[e] = pack_bf16(z[2 * e], z[2 * e + 1]);
+                        if (word) {
+                            uint32_t* const at = static_cast<uint32_t*>(a.out) + to + d;
+#pragma unroll
+                            for (int y = 0; y < 2; y++) {
+                                uint32_t x[8];
+#pragma unroll
+                                for (int e = 0; e < 8; e++) x[e] = w[4 * y + e / 2] >> 16 * (e & 1) & 0xffffu;
+                                if (vec) store32(at + 8 * y, x);
+                                else
+#pragma unroll
+                                    for (int e = 0; e < 8; e++) at[8 * y + e] = x[e];
+                            }
+                        } else {
+                            uint16_t* const at = static_cast<uint16_t*>(a.out) + to + d;
+                            if (vec) store32(at, w);
+                            else
+#pragma unroll
+                                for (int e = 0; e < 16; e++) at[e] = (uint16_t)(w[e / 2] >> 16 * (e & 1));
                         }
                     }
                 }
@@ -384,25 +420,23 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
                 const int whose = u.split ? 2 * units.rank + tile : units.rank, of = u.split ? 2 * units.ranks : units.ranks;
                 if (one < rows_here) {
                     const int owner = one / part, at = one % part;
-                    if (half == 0) {
-                        peer_store(&in_top[whose * part + at], owner, top);
-                        peer_store(&in_sum[whose * part + at], owner, sum);
-                        if (at == 0 && tile == 0) peer_store(&in_odd[units.rank], owner, odd);
-                    }
+                    peer_store(&in_top[whose * part + at], owner, top);
+                    peer_store(&in_sum[whose * part + at], owner, sum);
+                    if (at == 0 && tile == 0) peer_store(&in_odd[units.rank], owner, odd);
 #pragma unroll 1
-                    for (int i = 0; i < D / 2; i += 8) {
+                    for (int i = 0; i < D; i += 8) {
                         uint32_t o[8];
                         if (any) tmem_load8(o_at + i, o), tmem_loaded(o);
 #pragma unroll
                         for (int y = 0; y < 8; y += 4)
-                            peer_store4(q_at + ((whose * (D / 4) + (half * (D / 2) + i + y) / 4) * part + at) * 16, owner, any ? o[y] : 0u, any ? o[y + 1] : 0u, any ? o[y + 2] : 0u, any ? o[y + 3] : 0u);
+                            peer_store4(q_at + ((whose * (D / 4) + (i + y) / 4) * part + at) * 16, owner, any ? o[y] : 0u, any ? o[y + 1] : 0u, any ? o[y + 2] : 0u, any ? o[y + 3] : 0u);
                     }
                 }
                 meet();
 #pragma unroll 1
-                for (int i = threadIdx.x; i < part * (D / 4); i += 512) {
+                for (int i = threadIdx.x; i < part * (D / 4); i += 256) {
                     const int at = i % part, d = i / part * 4;
-                    const int64_t mm = u.m0 + units.rank * part + at;
+                    const int mm = u.m0 + units.rank * part + at;
                     if (mm >= u.n_m) continue;
                     float most = -INFINITY, all = 0.f, z[4] = {0.f, 0.f, 0.f, 0.f};
                     int set_aside = 0;
@@ -418,11 +452,12 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
                     }
                     if (!INT8)
                         for (int x = 0; x < units.ranks; x++) set_aside |= in_odd[x];
-                    const int64_t to = (u.s.first + mm / group) * a.out_stride + (u.kv_head * group + mm % group) * a.out_head_stride + d;
+                    const int i0 = (int)((uint32_t)mm / (uint32_t)group);
+                    const int64_t to = (u.s.first + i0) * a.out_stride + (u.kv_head * group + mm - i0 * group) * a.out_head_stride + d;
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         z[e] = all == 0.f ? 0.f : z[e] / all;
-                        if (set_aside) z[e] += what_is_no_number(v, row_bytes, d + e, u.s.pos + mm / group, c.capacity, a.window, a.sinks);
+                        if (set_aside) z[e] += what_is_no_number(v, row_bytes, d + e, u.s.pos + i0, c.capacity, a.window, a.sinks);
                         if (a.out_type == ZKB_VALUE_WORD) static_cast<uint32_t*>(a.out)[to + e] = round_bf16(z[e]);
                         else static_cast<uint16_t*>(a.out)[to + e] = round_bf16(z[e]);
                     }
@@ -440,11 +475,12 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
         }
     } else {
         uint32_t items = 0, units_done = 0, odd_at = 0, tile_done[2] = {0, 0};
+        int tiles = 1;
         bool odd = false;
-        const int th = threadIdx.x - 576;
+        const int th = threadIdx.x - 320;
         const uint32_t c128 = bf16_128(), c1152 = f16_1152();
         for (; more; units_done++) {
-            if (warp == 16) {  // ---- the copies
+            if (warp == 8) {  // ---- the copies
                 if (TMA && lane == 0) {
                     for (int i = 0; i < 2 * u.n; i++) {
                         const uint32_t item = items + i;
@@ -467,68 +503,71 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
                         }
                     }
                 }
-            } else if (warp == 17) {  // ---- the products
-                // One tile's after the other's, so that one tile's rows are in the softmax while the other's products run. (Each tile's from a warp of its
-                // own, both were in the softmax and then in their products at the same time: 6,100 cycles a block and pair.) The whole warp goes along, so that
-                // what it works out is the same for all lanes and needs no vector registers; one lane issues.
-                constexpr uint32_t qk = product_desc(INT8 ? 0 : 1, MANY_KEYS, false), pv = product_desc(1, D, true);
+            } else if (warp == 9) {  // ---- the products
+                // The whole warp goes along, so that what it works out is the same for all lanes and needs no vector registers; one lane issues. (As one lane's own work
+                // it took longer than the products.)
+                constexpr uint32_t qk = product_desc(INT8 ? 0 : 1, 64, false), pv = product_desc(1, D, true);
                 constexpr uint32_t high = (uint32_t)(M::GROUP >> 4) | 1u << 14 | (uint32_t)M::SWIZZLE_KIND << 29;  // the upper half of every matrix's description
                 // (an address in shared memory names the thread block of the cluster in bits that have no place there)
                 const uint32_t q_low = (q_at >> 4 & 0x3fff) | 1u << 16, k_low = (ring >> 4 & 0x3fff) | 1u << 16, v_low = (ring >> 4 & 0x3fff) | (uint32_t)(128 * M::BOX >> 4) << 16;
                 auto desc = [](uint32_t low) { return two_words(low, high); };
-                auto scores = [&](int tile, int j, bool release) {
-                    const uint32_t item = items + 2 * j, st = item % M::STAGES;
-                    wait(bars.ready[st], item / M::STAGES);
-                    if (tile_done[tile]) wait(bars.o_ready[tile], tile_done[tile] - 1);  // P has been read where S goes
+                const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
+                const bool one = elect_one();
+                // Step j of a tile: 64 keys of block j / 2 (split: a tile's half of block j).
+                auto scores = [&](int tile, int j, uint32_t count) {  // count: the tile's steps before this one
+                    const int block = u.split ? j : j >> 1, half = u.split ? tile : j & 1;
+                    const uint32_t item = items + 2 * block, st = item % M::STAGES;
+                    if (tile == 0 && (u.split || half == 0)) wait(bars.ready[st], item / M::STAGES);
+                    // P has been read where S goes: two steps ago, or, before a unit's first step, by all that came before (the barrier is not asked for a phase that lies two back)
+                    if (j == 0 ? count >= 1 : count >= 2) wait(bars.o_ready[tile], count - (j == 0 ? 1 : 2));
                     if (failed) return;
                     tmem_fence_after();
-                    if (lane == 0) {
-                        const uint32_t to = tmem + tile * 128, from_q = q_low + tile * (M::TILE >> 4), from_k = k_low + st * (M::TILE >> 4);
+                    const uint32_t to = tmem_u + tile * 128 + (count & 1) * 64, from_q = q_low + tile * (M::TILE >> 4), from_k = k_low + st * (M::TILE >> 4) + half * (64 * M::BOX >> 4);
+                    const uint32_t told = bar_of(bars.s_ready[2 * tile + (count & 1)]);
 #pragma unroll
-                        for (int i = 0; i < D / 16; i++) {
-                            const uint32_t at = (i / (M::BOX / 32) * (128 * M::BOX) + i % (M::BOX / 32) * 32) >> 4;
-                            product_ss(to, desc(from_q + at), desc(from_k + at), qk, i > 0);
-                        }
-                        products_done(bar_of(bars.s_ready[tile]));
-                        if (release) products_done(bar_of(bars.empty[st]));
-                        mbar_arrive(bar_of(bars.s_ready[tile]));
+                    for (int i = 0; i < D / 16; i++) {
+                        const uint32_t at = (i / (M::BOX / 32) * (128 * M::BOX) + i % (M::BOX / 32) * 32) >> 4;
+                        product_ss(one, to, desc(from_q + at), desc(from_k + at), qk, i > 0);
+                    }
+                    if (one) {
+                        products_done(told);
+                        if (tile == tiles - 1 && (u.split || half == 1)) products_done(bar_of(bars.empty[st]));
+                        mbar_arrive(told);
                     }
                     __syncwarp();
                 };
-                auto values = [&](int tile, int j, bool add, bool release) {
-                    const uint32_t item = items + 2 * j + 1, st = item % M::STAGES;
-                    wait(bars.ready[st], item / M::STAGES);
-                    wait(bars.p_ready[tile], tile_done[tile]);
+                auto values = [&](int tile, int j, uint32_t count) {
+                    const int block = u.split ? j : j >> 1, half = u.split ? tile : j & 1;
+                    const uint32_t item = items + 2 * block + 1, st = item % M::STAGES;
+                    if (tile == 0 && (u.split || half == 0)) wait(bars.ready[st], item / M::STAGES);
+                    wait(bars.p_ready[2 * tile + (count & 1)], count >> 1);
                     if (failed) return;
                     tmem_fence_after();
-                    if (lane == 0) {
-                        const uint32_t to = tmem + 256 + tile * D, from_p = tmem + tile * 128, from_v = v_low + st * (M::TILE >> 4);
+                    const uint32_t to = tmem_u + 256 + tile * D, from_p = tmem_u + tile * 128 + (count & 1) * 64, from_v = v_low + st * (M::TILE >> 4) + half * (64 * M::BOX >> 4);
 #pragma unroll
-                        for (int i = 0; i < MANY_KEYS / 16; i++)  // the weights of keys 64 and on are where their scores were
-                            product_ts(to, from_p + (i < 4 ? 8 * i : 32 + 8 * i), desc(from_v + i * (2 * M::GROUP >> 4)), pv, add || i > 0);
+                    for (int i = 0; i < 4; i++) product_ts(one, to, from_p + 8 * i, desc(from_v + i * (2 * M::GROUP >> 4)), pv, j > 0 || i > 0);
+                    if (one) {
                         products_done(bar_of(bars.o_ready[tile]));
-                        if (release) products_done(bar_of(bars.empty[st]));
+                        if (tile == tiles - 1 && (u.split || half == 1)) products_done(bar_of(bars.empty[st]));
                     }
                     __syncwarp();
-                    tile_done[tile]++;
                 };
+                tiles = u.two || u.split ? 2 : 1;
+                const int steps = u.split ? u.n : 2 * u.n;
                 wait(bars.q_ready, units_done);
-                if (u.split) {
-                    for (int j = 0; j < min(2, u.n); j++) scores(j, j, true);
-                    for (int j = 0; j < u.n; j++) {
-                        values(j & 1, j, j >= 2, true);
-                        if (j + 2 < u.n) scores(j & 1, j + 2, true);
-                    }
-                } else {
 #pragma unroll 1
-                    for (int j = -1; j < u.n; j++)
-#pragma unroll
-                        for (int tile = 0; tile < 2; tile++)
-                            if (tile == 0 || u.two) {
-                                if (j >= 0) values(tile, j, j > 0, tile == (int)u.two);
-                                if (j + 1 < u.n) scores(tile, j + 1, tile == (int)u.two);
-                            }
+                for (int j = -2; j < steps; j++) {
+                    if (j >= 0) {
+                        values(0, j, tile_done[0] + j);
+                        if (tiles == 2) values(1, j, tile_done[1] + j);
+                    }
+                    if (j + 2 < steps) {
+                        scores(0, j + 2, tile_done[0] + j + 2);
+                        if (tiles == 2) scores(1, j + 2, tile_done[1] + j + 2);
+                    }
                 }
+                tile_done[0] += steps;
+                if (tiles == 2) tile_done[1] += steps;
             } else {  // ---- what the products read is made ready
                 const char* const k = static_cast<const char*>(c.k) + (u.seq * c.seq_stride + u.kv_head * c.head_stride) * M::SIZE;
                 const char* const v = static_cast<const char*>(c.v) + (u.seq * c.seq_stride + u.kv_head * c.head_stride) * M::SIZE;
@@ -540,7 +579,7 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
                 for (int i = 0; i < 2 * u.n; i++) {
                     const uint32_t item = items + i, st = item % M::STAGES, to = ring + st * M::TILE;
                     const int base = units.base(u, i >> 1), kv = i & 1, last = u.last;
-                    const bool whole = units.whole(u, base);
+                    const bool whole = units.whole(u, base, MANY_KEYS);
                     if constexpr (INT8) {
                         wait(bars.empty[st], item / M::STAGES + 1);
                         if (kv == 0 && th < 128) {  // both of the block's scales: of the block before the last, nothing is needed any more when this place is free
