@@ -6,9 +6,8 @@
 namespace zk {
 
 // Two tiles of 128 query rows (the heads of a kv head's group, token after token) share each block of 128 keys: S = Q K^T and O += P V are tcgen05
-// products whose sums lie in tensor memory, P in bf16 where S was. A thread has a row: its maximum, sum and weights need no other thread. The keys are taken
-// 64 at a time with two places for S a tile, so that a tile's next scores are there when its rows are done with the last ones: with one place of 128 keys each tile went
-// softmax, P V, Q K^T, softmax, 3,800 cycles a block and pair, where the tensor cores need 2,048 and the exponentials, 16 a clock, as many.
+// products whose sums lie in tensor memory, P in bf16 where S was. A thread has a row: its maximum, sum and weights need no other thread. While one tile's
+// rows are in the softmax the other's products run: per block and pair the tensor cores need 2,048 cycles for 128 head dimensions and the exponentials, 16 a clock, as many.
 // Warps: 0-3 and 4-7 the tiles' rows, 8 the copies, 9 the products, 10 and on what has to be done to keys and values before a product may read them: 8-bit codes become
 // fp16 (K) and bf16 (V), exactly; bf16 values behind the last token or that are no numbers are zeroed where some row does not see them.
 // A thread block takes one pair of tiles after the other; with too few of them for the GPU the keys are spread over a cluster's thread blocks, which add up through
@@ -68,9 +67,8 @@ __device__ __forceinline__ void tmem_load32(uint32_t at, uint32_t* x) {
                  : R8(x, 0), R8(x, 8), R8(x, 16), R8(x, 24) : "r"(at));
 }
 __device__ __forceinline__ void tmem_load8(uint32_t at, uint32_t* x) { asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];" : R8(x, 0) : "r"(at)); }
-__device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t* x) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(at),
-                 W8(x, 0), W8(x, 8), W8(x, 16), W8(x, 24) : "memory");
+__device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t* x) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(at), W8(x, 0), W8(x, 8) : "memory");
 }
 __device__ __forceinline__ void tmem_store8(uint32_t at, const uint32_t* x) { asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(at), W8(x, 0) : "memory"); }
 #undef R8
@@ -107,7 +105,7 @@ __device__ __forceinline__ void store32(void* to, const uint32_t (&x)[8]) {
 __device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 
 struct ManyBars {
-    unsigned long long full[5], ready[5], empty[5], raw_full[4], raw_empty[4], s_ready[4], p_ready[4], o_ready[2], q_ready;  // s, p: of a tile's two places in turn
+    unsigned long long full[5], ready[5], empty[5], raw_full[4], raw_empty[4], s_ready[2], p_ready[2], o_ready[2], q_ready;
 };
 __device__ __forceinline__ uint32_t bar_of(const unsigned long long& b) { return (uint32_t)__cvta_generic_to_shared(&b); }
 
@@ -188,8 +186,7 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
     } else if (warp == 1 && lane == 0) {
         for (int i = 0; i < 5; i++) mbar_init(bar_of(bars.full[i]), 1), mbar_init(bar_of(bars.ready[i]), M::READIERS), mbar_init(bar_of(bars.empty[i]), 1);
         for (int i = 0; i < 4; i++) mbar_init(bar_of(bars.raw_full[i]), 1), mbar_init(bar_of(bars.raw_empty[i]), M::READIERS);
-        for (int i = 0; i < 4; i++) mbar_init(bar_of(bars.s_ready[i]), 2), mbar_init(bar_of(bars.p_ready[i]), 128);
-        for (int i = 0; i < 2; i++) mbar_init(bar_of(bars.o_ready[i]), 1);
+        for (int i = 0; i < 2; i++) mbar_init(bar_of(bars.s_ready[i]), 2), mbar_init(bar_of(bars.p_ready[i]), 128), mbar_init(bar_of(bars.o_ready[i]), 1);
         mbar_init(bar_of(bars.q_ready), 256);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -281,84 +278,100 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
                 }
             }
             float top = -INFINITY, less = 0.f, sum = 0.f;
-            const int steps = u.split ? u.n : tile == 0 || u.two ? 2 * u.n : 0;
+            const int steps = u.split || tile == 0 || u.two ? u.n : 0, half = u.split ? 64 * tile : 0, keys = u.split ? 64 : 128;
             for (int j = 0; j < steps; j++, done++) {
-                const int block = u.split ? j : j >> 1, half = u.split ? tile : j & 1, base = units.base(u, block) + 64 * half, slot = (passed + block) & 1;
-                const bool whole = units.whole(u, base, 64);
-                const uint32_t place = s_at + (done & 1) * 64;
-                wait(bars.s_ready[2 * tile + (done & 1)], done >> 1);
+                const int base = units.base(u, j) + half, slot = (passed + j) & 1;
+                const bool whole = units.whole(u, base, keys);
+                wait(bars.s_ready[tile], done);
                 tmem_fence_after();
-                uint32_t x[64];  // the row's scores, still without the factor by_row
-                uint32_t(&x0)[32] = *reinterpret_cast<uint32_t(*)[32]>(&x[0]), (&x1)[32] = *reinterpret_cast<uint32_t(*)[32]>(&x[32]);
-                tmem_load32(place, x0);
-                tmem_load32(place + 32, x1);
-                tmem_loaded(x0);
-                tmem_loaded(x1);
-                if constexpr (INT8) {
+                uint32_t part[4] = {0u, 0u, 0u, 0u};
+                // 32 scores at a time, read while the 32 before them are worked on, become weights that go where scores were that have been read. The weights' common factor is
+                // 2^-top, which need not be the largest score's: it is left as it is until a score exceeds it by 2^8, so that one pass over the scores will do.
+                auto weights = [&](int at, uint32_t (&x)[32]) {
+                    if constexpr (INT8) {
 #pragma unroll
-                    for (int y = 0; y < 64; y += 4) {
-                        const float4 ks = *reinterpret_cast<const float4*>(&k_scale_sm[slot][half * 64 + y]);
-                        mul2(x[y], x[y + 1], ks.x, ks.y), mul2(x[y + 2], x[y + 3], ks.z, ks.w);
-                    }
-                }
-                uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
-                if (!whole) {
-#pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        const int at = base + 32 * i;
-                        seen[i] = bits_below(high + 1 - at) & (~bits_below(low - at) | bits_below(sinks - at));
-#pragma unroll
-                        for (int y = 0; y < 32; y++) x[32 * i + y] = seen[i] >> y & 1 ? x[32 * i + y] : 0xff800000u;  // -inf
-                    }
-                }
-                float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int z = 0; z < 64; z++) most[z & 3] = fmaxf(most[z & 3], __uint_as_float(x[z]));
-                const float higher = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * by_row;
-                // The weights' common factor is 2^-top. It need not be the largest score's, only within 2^8 of it, so O is seldom read back for it.
-                const bool need = higher > top + 8.f;
-                if (__any_sync(0xffffffffu, need)) {
-                    const float keep = need ? exp2_fast(top - higher) : 1.f;
-                    if (need) top = higher, less = higher, sum *= keep;
-                    if (j > 0) {
-                        wait(bars.o_ready[tile], done - 1);
-                        tmem_fence_after();
-#pragma unroll 1
-                        for (int i = 0; i < D; i += 8) {  // few at a time: the scores keep their registers
-                            uint32_t o[8];
-                            tmem_load8(o_at + i, o);
-                            tmem_loaded(o);
-#pragma unroll
-                            for (int y = 0; y < 8; y++) o[y] = __float_as_uint(__uint_as_float(o[y]) * keep);
-                            tmem_store8(o_at + i, o);
+                        for (int y = 0; y < 32; y += 4) {
+                            const float4 ks = *reinterpret_cast<const float4*>(&k_scale_sm[slot][half + at + y]);
+                            mul2(x[y], x[y + 1], ks.x, ks.y), mul2(x[y + 2], x[y + 3], ks.z, ks.w);
                         }
                     }
-                }
-                uint32_t part[4] = {0u, 0u, 0u, 0u};
+                    uint32_t seen = 0xffffffffu;
+                    if (!whole) {
+                        const int first = base + at;
+                        seen = bits_below(high + 1 - first) & (~bits_below(low - first) | bits_below(sinks - first));
 #pragma unroll
-                for (int z = 0; z < 64; z += 4) {
-                    float w[4];
-#pragma unroll
-                    for (int e = 0; e < 4; e += 2) {
-                        uint32_t f0 = x[z + e], f1 = x[z + e + 1];
-                        fma2(f0, f1, by_row, -less);
-                        w[e] = exp2_fast(__uint_as_float(f0)), w[e + 1] = exp2_fast(__uint_as_float(f1));
-                        add2(part[e], part[e + 1], w[e], w[e + 1]);
+                        for (int y = 0; y < 32; y++) x[y] = seen >> y & 1 ? x[y] : 0xff800000u;  // -inf
                     }
-                    if constexpr (INT8) {
-                        const float4 vs = *reinterpret_cast<const float4*>(&v_scale_sm[slot][half * 64 + z]);
-                        scale2(w[0], w[1], vs.x, vs.y), scale2(w[2], w[3], vs.z, vs.w);
-                        if (!whole)
+                    float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                            for (int e = 0; e < 4; e++) w[e] = seen[z / 32] >> (z % 32 + e) & 1 ? w[e] : 0.f;  // a hidden token's scale may be anything
+                    for (int z = 0; z < 32; z++) most[z & 3] = fmaxf(most[z & 3], __uint_as_float(x[z]));
+                    const float higher = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * by_row;
+                    const bool need = higher > top + 8.f;
+                    if (__any_sync(0xffffffffu, need)) {
+                        const float keep = need ? exp2_fast(top - higher) : 1.f;
+                        if (need) top = higher, less = higher, sum *= keep;
+#pragma unroll
+                        for (int e = 0; e < 4; e++) part[e] = __float_as_uint(__uint_as_float(part[e]) * keep);
+                        tmem_stored();
+#pragma unroll 1
+                        for (int i = 0; i < at / 2; i += 8) {  // this block's weights so far
+                            uint32_t w[8];
+                            tmem_load8(s_at + i, w);
+                            tmem_loaded(w);
+#pragma unroll
+                            for (int y = 0; y < 8; y++) w[y] = pack_bf16(bf16_low(w[y]) * keep, bf16_high(w[y]) * keep);
+                            tmem_store8(s_at + i, w);
+                        }
+                        if (j > 0) {
+                            wait(bars.o_ready[tile], done - 1);
+                            tmem_fence_after();
+#pragma unroll 1
+                            for (int i = 0; i < D; i += 8) {
+                                uint32_t o[8];
+                                tmem_load8(o_at + i, o);
+                                tmem_loaded(o);
+#pragma unroll
+                                for (int y = 0; y < 8; y++) o[y] = __float_as_uint(__uint_as_float(o[y]) * keep);
+                                tmem_store8(o_at + i, o);
+                            }
+                        }
                     }
-                    x[z / 2] = pack_bf16(w[0], w[1]), x[z / 2 + 1] = pack_bf16(w[2], w[3]);
+#pragma unroll
+                    for (int z = 0; z < 32; z += 4) {
+                        float w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; e += 2) {
+                            uint32_t f0 = x[z + e], f1 = x[z + e + 1];
+                            fma2(f0, f1, by_row, -less);
+                            w[e] = exp2_fast(__uint_as_float(f0)), w[e + 1] = exp2_fast(__uint_as_float(f1));
+                            add2(part[e], part[e + 1], w[e], w[e + 1]);
+                        }
+                        if constexpr (INT8) {
+                            const float4 vs = *reinterpret_cast<const float4*>(&v_scale_sm[slot][half + at + z]);
+                            scale2(w[0], w[1], vs.x, vs.y), scale2(w[2], w[3], vs.z, vs.w);
+                            if (!whole)
+#pragma unroll
+                                for (int e = 0; e < 4; e++) w[e] = seen >> (z + e) & 1 ? w[e] : 0.f;  // a hidden token's scale may be anything
+                        }
+                        x[z / 2] = pack_bf16(w[0], w[1]), x[z / 2 + 1] = pack_bf16(w[2], w[3]);
+                    }
+                    tmem_store16(s_at + at / 2, x);
+                };
+                uint32_t x0[32], x1[32];
+                tmem_load32(s_at, x0);
+#pragma unroll 1
+                for (int at = 0; at < keys; at += 64) {
+                    tmem_loaded(x0);
+                    tmem_load32(s_at + at + 32, x1);
+                    weights(at, x0);
+                    tmem_loaded(x1);
+                    if (at + 64 < keys) tmem_load32(s_at + at + 64, x0);
+                    weights(at + 32, x1);
                 }
-                tmem_store32(place, x0);  // the weights go to the first half of where the scores were
                 sum += (__uint_as_float(part[0]) + __uint_as_float(part[1])) + (__uint_as_float(part[2]) + __uint_as_float(part[3]));
                 tmem_stored();
                 tmem_fence_before();
-                mbar_arrive(bar_of(bars.p_ready[2 * tile + (done & 1)]));
+                mbar_arrive(bar_of(bars.p_ready[tile]));
             }
             const bool any = steps > 0, join = units.joined(u), again = units.next(after);
             float by_next = by_row;
@@ -422,7 +435,7 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
                     const int owner = one / part, at = one % part;
                     peer_store(&in_top[whose * part + at], owner, top);
                     peer_store(&in_sum[whose * part + at], owner, sum);
-                    if (at == 0 && tile == 0) peer_store(&in_odd[units.rank], owner, odd);
+                    if (at == 0 && !(u.split && tile)) peer_store(&in_odd[units.rank], owner, odd);
 #pragma unroll 1
                     for (int i = 0; i < D; i += 8) {
                         uint32_t o[8];
@@ -475,7 +488,6 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
         }
     } else {
         uint32_t items = 0, units_done = 0, odd_at = 0, tile_done[2] = {0, 0};
-        int tiles = 1;
         bool odd = false;
         const int th = threadIdx.x - 320;
         const uint32_t c128 = bf16_128(), c1152 = f16_1152();
@@ -506,68 +518,62 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
             } else if (warp == 9) {  // ---- the products
                 // The whole warp goes along, so that what it works out is the same for all lanes and needs no vector registers; one lane issues. (As one lane's own work
                 // it took longer than the products.)
-                constexpr uint32_t qk = product_desc(INT8 ? 0 : 1, 64, false), pv = product_desc(1, D, true);
+                constexpr uint32_t qk = product_desc(INT8 ? 0 : 1, MANY_KEYS, false), qk_half = product_desc(INT8 ? 0 : 1, 64, false), pv = product_desc(1, D, true);
                 constexpr uint32_t high = (uint32_t)(M::GROUP >> 4) | 1u << 14 | (uint32_t)M::SWIZZLE_KIND << 29;  // the upper half of every matrix's description
                 // (an address in shared memory names the thread block of the cluster in bits that have no place there)
                 const uint32_t q_low = (q_at >> 4 & 0x3fff) | 1u << 16, k_low = (ring >> 4 & 0x3fff) | 1u << 16, v_low = (ring >> 4 & 0x3fff) | (uint32_t)(128 * M::BOX >> 4) << 16;
                 auto desc = [](uint32_t low) { return two_words(low, high); };
                 const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
                 const bool one = elect_one();
-                // Step j of a tile: 64 keys of block j / 2 (split: a tile's half of block j).
+                const int tiles = u.two || u.split ? 2 : 1;
                 auto scores = [&](int tile, int j, uint32_t count) {  // count: the tile's steps before this one
-                    const int block = u.split ? j : j >> 1, half = u.split ? tile : j & 1;
-                    const uint32_t item = items + 2 * block, st = item % M::STAGES;
-                    if (tile == 0 && (u.split || half == 0)) wait(bars.ready[st], item / M::STAGES);
-                    // P has been read where S goes: two steps ago, or, before a unit's first step, by all that came before (the barrier is not asked for a phase that lies two back)
-                    if (j == 0 ? count >= 1 : count >= 2) wait(bars.o_ready[tile], count - (j == 0 ? 1 : 2));
+                    const uint32_t item = items + 2 * j, st = item % M::STAGES;
+                    if (tile == 0) wait(bars.ready[st], item / M::STAGES);
+                    if (count) wait(bars.o_ready[tile], count - 1);  // P has been read where S goes
                     if (failed) return;
                     tmem_fence_after();
-                    const uint32_t to = tmem_u + tile * 128 + (count & 1) * 64, from_q = q_low + tile * (M::TILE >> 4), from_k = k_low + st * (M::TILE >> 4) + half * (64 * M::BOX >> 4);
-                    const uint32_t told = bar_of(bars.s_ready[2 * tile + (count & 1)]);
+                    const uint32_t to = tmem_u + tile * 128, from_q = q_low + tile * (M::TILE >> 4), from_k = k_low + st * (M::TILE >> 4) + (u.split ? tile * (64 * M::BOX >> 4) : 0);
 #pragma unroll
                     for (int i = 0; i < D / 16; i++) {
                         const uint32_t at = (i / (M::BOX / 32) * (128 * M::BOX) + i % (M::BOX / 32) * 32) >> 4;
-                        product_ss(one, to, desc(from_q + at), desc(from_k + at), qk, i > 0);
+                        product_ss(one, to, desc(from_q + at), desc(from_k + at), u.split ? qk_half : qk, i > 0);
                     }
                     if (one) {
-                        products_done(told);
-                        if (tile == tiles - 1 && (u.split || half == 1)) products_done(bar_of(bars.empty[st]));
-                        mbar_arrive(told);
+                        products_done(bar_of(bars.s_ready[tile]));
+                        if (tile == tiles - 1) products_done(bar_of(bars.empty[st]));
+                        mbar_arrive(bar_of(bars.s_ready[tile]));
                     }
                     __syncwarp();
                 };
                 auto values = [&](int tile, int j, uint32_t count) {
-                    const int block = u.split ? j : j >> 1, half = u.split ? tile : j & 1;
-                    const uint32_t item = items + 2 * block + 1, st = item % M::STAGES;
-                    if (tile == 0 && (u.split || half == 0)) wait(bars.ready[st], item / M::STAGES);
-                    wait(bars.p_ready[2 * tile + (count & 1)], count >> 1);
+                    const uint32_t item = items + 2 * j + 1, st = item % M::STAGES;
+                    if (tile == 0) wait(bars.ready[st], item / M::STAGES);
+                    wait(bars.p_ready[tile], count);
                     if (failed) return;
                     tmem_fence_after();
-                    const uint32_t to = tmem_u + 256 + tile * D, from_p = tmem_u + tile * 128 + (count & 1) * 64, from_v = v_low + st * (M::TILE >> 4) + half * (64 * M::BOX >> 4);
+                    const uint32_t to = tmem_u + 256 + tile * D, from_p = tmem_u + tile * 128, from_v = v_low + st * (M::TILE >> 4) + (u.split ? tile * (64 * M::BOX >> 4) : 0);
 #pragma unroll
                     for (int i = 0; i < 4; i++) product_ts(one, to, from_p + 8 * i, desc(from_v + i * (2 * M::GROUP >> 4)), pv, j > 0 || i > 0);
+                    if (!u.split)
+#pragma unroll
+                        for (int i = 4; i < 8; i++) product_ts(one, to, from_p + 8 * i, desc(from_v + i * (2 * M::GROUP >> 4)), pv, true);
                     if (one) {
                         products_done(bar_of(bars.o_ready[tile]));
-                        if (tile == tiles - 1 && (u.split || half == 1)) products_done(bar_of(bars.empty[st]));
+                        if (tile == tiles - 1) products_done(bar_of(bars.empty[st]));
                     }
                     __syncwarp();
                 };
-                tiles = u.two || u.split ? 2 : 1;
-                const int steps = u.split ? u.n : 2 * u.n;
                 wait(bars.q_ready, units_done);
 #pragma unroll 1
-                for (int j = -2; j < steps; j++) {
-                    if (j >= 0) {
-                        values(0, j, tile_done[0] + j);
-                        if (tiles == 2) values(1, j, tile_done[1] + j);
-                    }
-                    if (j + 2 < steps) {
-                        scores(0, j + 2, tile_done[0] + j + 2);
-                        if (tiles == 2) scores(1, j + 2, tile_done[1] + j + 2);
-                    }
-                }
-                tile_done[0] += steps;
-                if (tiles == 2) tile_done[1] += steps;
+                for (int j = -1; j < u.n; j++)
+#pragma unroll
+                    for (int tile = 0; tile < 2; tile++)
+                        if (tile < tiles) {
+                            if (j >= 0) values(tile, j, tile_done[tile] + j);
+                            if (j + 1 < u.n) scores(tile, j + 1, tile_done[tile] + j + 1);
+                        }
+                tile_done[0] += u.n;
+                if (tiles == 2) tile_done[1] += u.n;
             } else {  // ---- what the products read is made ready
                 const char* const k = static_cast<const char*>(c.k) + (u.seq * c.seq_stride + u.kv_head * c.head_stride) * M::SIZE;
                 const char* const v = static_cast<const char*>(c.v) + (u.seq * c.seq_stride + u.kv_head * c.head_stride) * M::SIZE;
