@@ -67,8 +67,9 @@ __device__ __forceinline__ void tmem_load32(uint32_t at, uint32_t* x) {
                  : R8(x, 0), R8(x, 8), R8(x, 16), R8(x, 24) : "r"(at));
 }
 __device__ __forceinline__ void tmem_load8(uint32_t at, uint32_t* x) { asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];" : R8(x, 0) : "r"(at)); }
-__device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t* x) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(at), W8(x, 0), W8(x, 8) : "memory");
+__device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t* x) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(at),
+                 W8(x, 0), W8(x, 8), W8(x, 16), W8(x, 24) : "memory");
 }
 __device__ __forceinline__ void tmem_store8(uint32_t at, const uint32_t* x) { asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(at), W8(x, 0) : "memory"); }
 #undef R8
@@ -268,14 +269,11 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
             const bool live = m < u.n_m;
             const int p = live ? (int)u.s.pos + (int)((uint32_t)m / (uint32_t)group) : -1;
             const int low = a.window ? max(0, p - (int)min(a.window, 1u << 30) + 1) : 0, high = min(p, u.last), sinks = a.window ? (int)min(a.sinks, c.capacity) : 0;
-            {  // the next unit's Q comes nearer
-                Units ahead = units;
-                Unit n;
-                if (ahead.next(n)) {
-                    const int mm = row_of(n);
-                    if (mm < n.n_m)
-                        for (int i = 0; i < D; i += 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(q_of(n, mm) + i));
-                }
+            const bool again = units.next(after);
+            if (again) {  // the next unit's Q comes nearer
+                const int mm = row_of(after);
+                if (mm < after.n_m)
+                    for (int i = 0; i < D; i += 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(q_of(after, mm) + i));
             }
             float top = -INFINITY, less = 0.f, sum = 0.f;
             const int steps = u.split || tile == 0 || u.two ? u.n : 0, half = u.split ? 64 * tile : 0, keys = u.split ? 64 : 128;
@@ -285,26 +283,36 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
                 wait(bars.s_ready[tile], done);
                 tmem_fence_after();
                 uint32_t part[4] = {0u, 0u, 0u, 0u};
-                // 32 scores at a time, read while the 32 before them are worked on, become weights that go where scores were that have been read. The weights' common factor is
-                // 2^-top, which need not be the largest score's: it is left as it is until a score exceeds it by 2^8, so that one pass over the scores will do.
-                auto weights = [&](int at, uint32_t (&x)[32]) {
+                // 64 scores at a time become weights that go where scores were that have been read. The weights' common factor is 2^-top, which need not be the largest
+                // score's: it is left as it is until a score exceeds it by 2^8, so that one pass over the scores will do.
+#pragma unroll 1
+                for (int at = 0; at < keys; at += 64) {
+                    uint32_t x[64];
+                    uint32_t(&x0)[32] = *reinterpret_cast<uint32_t(*)[32]>(&x[0]), (&x1)[32] = *reinterpret_cast<uint32_t(*)[32]>(&x[32]);
+                    tmem_load32(s_at + at, x0);
+                    tmem_load32(s_at + at + 32, x1);
+                    tmem_loaded(x0);
+                    tmem_loaded(x1);
                     if constexpr (INT8) {
 #pragma unroll
-                        for (int y = 0; y < 32; y += 4) {
+                        for (int y = 0; y < 64; y += 4) {
                             const float4 ks = *reinterpret_cast<const float4*>(&k_scale_sm[slot][half + at + y]);
                             mul2(x[y], x[y + 1], ks.x, ks.y), mul2(x[y + 2], x[y + 3], ks.z, ks.w);
                         }
                     }
-                    uint32_t seen = 0xffffffffu;
+                    uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
                     if (!whole) {
-                        const int first = base + at;
-                        seen = bits_below(high + 1 - first) & (~bits_below(low - first) | bits_below(sinks - first));
 #pragma unroll
-                        for (int y = 0; y < 32; y++) x[y] = seen >> y & 1 ? x[y] : 0xff800000u;  // -inf
+                        for (int i = 0; i < 2; i++) {
+                            const int first = base + at + 32 * i;
+                            seen[i] = bits_below(high + 1 - first) & (~bits_below(low - first) | bits_below(sinks - first));
+#pragma unroll
+                            for (int y = 0; y < 32; y++) x[32 * i + y] = seen[i] >> y & 1 ? x[32 * i + y] : 0xff800000u;  // -inf
+                        }
                     }
                     float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int z = 0; z < 32; z++) most[z & 3] = fmaxf(most[z & 3], __uint_as_float(x[z]));
+                    for (int z = 0; z < 64; z++) most[z & 3] = fmaxf(most[z & 3], __uint_as_float(x[z]));
                     const float higher = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * by_row;
                     const bool need = higher > top + 8.f;
                     if (__any_sync(0xffffffffu, need)) {
@@ -337,7 +345,7 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
                         }
                     }
 #pragma unroll
-                    for (int z = 0; z < 32; z += 4) {
+                    for (int z = 0; z < 64; z += 4) {
                         float w[4];
 #pragma unroll
                         for (int e = 0; e < 4; e += 2) {
@@ -351,29 +359,18 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
                             scale2(w[0], w[1], vs.x, vs.y), scale2(w[2], w[3], vs.z, vs.w);
                             if (!whole)
 #pragma unroll
-                                for (int e = 0; e < 4; e++) w[e] = seen >> (z + e) & 1 ? w[e] : 0.f;  // a hidden token's scale may be anything
+                                for (int e = 0; e < 4; e++) w[e] = seen[z / 32] >> (z % 32 + e) & 1 ? w[e] : 0.f;  // a hidden token's scale may be anything
                         }
                         x[z / 2] = pack_bf16(w[0], w[1]), x[z / 2 + 1] = pack_bf16(w[2], w[3]);
                     }
-                    tmem_store16(s_at + at / 2, x);
-                };
-                uint32_t x0[32], x1[32];
-                tmem_load32(s_at, x0);
-#pragma unroll 1
-                for (int at = 0; at < keys; at += 64) {
-                    tmem_loaded(x0);
-                    tmem_load32(s_at + at + 32, x1);
-                    weights(at, x0);
-                    tmem_loaded(x1);
-                    if (at + 64 < keys) tmem_load32(s_at + at + 64, x0);
-                    weights(at + 32, x1);
+                    tmem_store32(s_at + at / 2, x);
                 }
                 sum += (__uint_as_float(part[0]) + __uint_as_float(part[1])) + (__uint_as_float(part[2]) + __uint_as_float(part[3]));
                 tmem_stored();
                 tmem_fence_before();
                 mbar_arrive(bar_of(bars.p_ready[tile]));
             }
-            const bool any = steps > 0, join = units.joined(u), again = units.next(after);
+            const bool any = steps > 0, join = units.joined(u);
             float by_next = by_row;
             if (again && !join) by_next = load_q(after);  // its products begin while this unit's rows are written
             if (any) {
