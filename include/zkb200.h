@@ -535,7 +535,7 @@ typedef struct zkb_step_rows {
  * leaves the head as it is); then each pair (i, j) of the first rotary_dim values turns by a = p * h_inv_freq[i']:
  * y_i cos a - y_j sin a, y_j cos a + y_i sin a, with j = i + rotary_dim / 2 (interleaved: j = i + 1). Angles are reduced to a turn in
  * 64 bits. Queries go to q_out (BF16); keys and, unchanged, values go to the cache at position p. INT8 caches get
- * scale = max|y| / 127 and code = y / scale rounded to nearest even (scale 0: codes 0). Rows without a position in the cache
+ * scale = max|y| / 127 and code = y * (127 / max|y|) rounded to nearest even (scale 0: codes 0). Rows without a position in the cache
  * (below) still have their queries written. rotary_dim: a multiple of 16 up to head_dim, or 0; h_inv_freq: rotary_dim / 2 values
  * on the host, read before the call returns. */
 typedef struct zkb_step_norm_rope_args {

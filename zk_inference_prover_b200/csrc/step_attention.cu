@@ -76,7 +76,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, Few<D, INT8>::THREAD_BLOCKS)
     using F = Few<D, INT8>;
     constexpr int STEPS = D / 16, STRIDE = D + 4;
     extern __shared__ unsigned char few_sm[];
-    __shared__ float top_sm[FEW_WARPS][8], sum_sm[FEW_WARPS][8];
+    __shared__ float top_sm[FEW_WARPS][8], sum_sm[FEW_WARPS][8], all_top[8], all_sum[8];
     __shared__ float in_o[8 * D], in_top[FEW_RANKS][8], in_sum[FEW_RANKS][8];  // what the cluster's thread blocks write here: [rank][this one's part]
     __shared__ int in_odd[FEW_RANKS];  // some value of V was no number
     __shared__ __align__(8) unsigned long long full[FEW_WARPS][F::STAGES];
@@ -101,7 +101,8 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, Few<D, INT8>::THREAD_BLOCKS)
     const char* const v = static_cast<const char*>(c.v) + (seq * c.seq_stride + kv_head * c.head_stride) * F::SIZE;
     const float* const scales = INT8 ? (lane < 16 ? c.k_scale : c.v_scale) + seq * c.scale_seq_stride + kv_head * c.scale_head_stride : nullptr;
     const int row_bytes = (int)c.token_stride * F::SIZE;
-    const int64_t n_m = (int64_t)s.rows * group, m_step = (int64_t)(gridDim.x / ranks) * 8;
+    const int64_t n_m = (int64_t)s.rows * group, m_step = (int64_t)(gridDim.x / ranks) * 8;  // below 2^31, so that rows are found by 32-bit divisions
+    auto token = [&](int64_t m) { return (int)((uint32_t)m / (uint32_t)group); };
     const float by = a.scale * 1.44269504f;
     const uint32_t c128 = bf16_128(), c1152 = f16_1152();
     int stage = 0;
@@ -130,7 +131,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, Few<D, INT8>::THREAD_BLOCKS)
     };
     bool begun = ranks == 1;
     for (int64_t m0 = (int64_t)(blockIdx.x / ranks) * 8; m0 < n_m; m0 += m_step) {
-        const int64_t pos_low = s.pos + m0 / group, pos_high = s.pos + (min(m0 + 8, n_m) - 1) / group;
+        const int64_t pos_low = s.pos + token(m0), pos_high = s.pos + token(min(m0 + 8, n_m) - 1);
         const KeyBlocks blocks = key_blocks<16>(pos_low, pos_high, c.capacity, a.window, a.sinks);
         const int stride = ranks * FEW_WARPS, last = (int)blocks.end - 1;
         const int at0 = rank * FEW_WARPS + warp;
@@ -144,7 +145,8 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, Few<D, INT8>::THREAD_BLOCKS)
         {
             constexpr int BOX_DIMS = F::BOX / F::SIZE, LANE_DIMS = BOX_DIMS / 4;
             const int64_t m = m0 + g;
-            const uint16_t* from = static_cast<const uint16_t*>(a.q) + (m < n_m ? (s.first + m / group) * a.q_stride + (kv_head * group + m % group) * a.q_head_stride : 0);
+            const int i0 = m < n_m ? token(m) : 0;
+            const uint16_t* from = static_cast<const uint16_t*>(a.q) + (m < n_m ? (s.first + i0) * a.q_stride + (kv_head * group + (int)m - i0 * group) * a.q_head_stride : 0);
             const bool quads = ((uintptr_t)from & 7) == 0;
 #pragma unroll
             for (int i = 0; i < STEPS; i++) {
@@ -173,13 +175,13 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, Few<D, INT8>::THREAD_BLOCKS)
 #pragma unroll
             for (int i = 0; i < 2 * STEPS; i++) q[i / 2][i & 1] = pack_f16(bf16_low(q[i / 2][i & 1]) * f, bf16_high(q[i / 2][i & 1]) * f);
 #pragma unroll
-            for (int r = 0; r < 2; r++) by_row[r] = ldexpf(by, -__shfl_sync(0xffffffffu, up, (2 * t + r) * 4));
+            for (int r = 0; r < 2; r++) by_row[r] = by * __uint_as_float((uint32_t)(127 - __shfl_sync(0xffffffffu, up, (2 * t + r) * 4)) << 23);
         }
         // rows 2t and 2t + 1: their positions, running maxima and this lane's part of their sums
         int p[2];
         float top[2] = {-INFINITY, -INFINITY}, less[2] = {0.f, 0.f}, sum[2] = {0.f, 0.f}, o[STEPS][4];
 #pragma unroll
-        for (int r = 0; r < 2; r++) p[r] = m0 + 2 * t + r < n_m ? (int)s.pos + (int)((m0 + 2 * t + r) / group) : -1;
+        for (int r = 0; r < 2; r++) p[r] = m0 + 2 * t + r < n_m ? (int)s.pos + token(m0 + 2 * t + r) : -1;
 #pragma unroll
         for (int i = 0; i < STEPS; i++)
 #pragma unroll
@@ -321,28 +323,36 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, Few<D, INT8>::THREAD_BLOCKS)
             cluster_wait();
             begun = true;
         }
-        // this thread block's sums to whoever finishes them: outputs part, part + 1, ... of 8 D go to the thread block of that rank
-        const int part = 8 * D / ranks;
-        for (int i = threadIdx.x; i < 8 * D; i += FEW_WARPS * 32) {
-            const int r = i / D, d = i % D;
-            float most = top_sm[0][r], y = 0.f;
+        // the warps' factors, and the row's sum
+        if (threadIdx.x < 8) {
+            const int r = threadIdx.x;
+            float most = top_sm[0][r], all = 0.f, f[FEW_WARPS];
 #pragma unroll
             for (int w = 1; w < FEW_WARPS; w++) most = fmaxf(most, top_sm[w][r]);
             const float base = most == -INFINITY ? 0.f : most;
 #pragma unroll
-            for (int w = 0; w < FEW_WARPS; w++) y += o_sm[(w * 8 + r) * STRIDE + d] * exp2_fast(top_sm[w][r] - base);
-            float* const to = &in_o[rank * part + i % part];
-            if (ranks > 1) peer_store(to, i / part, y);
+            for (int w = 0; w < FEW_WARPS; w++) f[w] = exp2_fast(top_sm[w][r] - base), all += sum_sm[w][r] * f[w];
+#pragma unroll
+            for (int w = 0; w < FEW_WARPS; w++) sum_sm[w][r] = f[w];
+            all_top[r] = most, all_sum[r] = all;
+        }
+        __syncthreads();
+        // this thread block's sums to whoever finishes them: outputs part, part + 1, ... of 8 D go to the thread block of that rank (ranks: a power of two)
+        const int part_log = 31 - __clz(8 * D / ranks), part = 1 << part_log;
+#pragma unroll
+        for (int x = 0; x < 8 * D; x += FEW_WARPS * 32) {
+            const int i = x + threadIdx.x, r = i / D, d = i % D;
+            float y = 0.f;
+#pragma unroll
+            for (int w = 0; w < FEW_WARPS; w++) y += o_sm[(w * 8 + r) * STRIDE + d] * sum_sm[w][r];
+            float* const to = &in_o[rank * part + (i & (part - 1))];
+            if (ranks > 1) peer_store(to, i >> part_log, y);
             else *to = y;
         }
         for (int i = threadIdx.x; i < 8 * ranks; i += FEW_WARPS * 32) {
             const int r = i & 7;
-            float most = top_sm[0][r], all = 0.f;
-            for (int w = 1; w < FEW_WARPS; w++) most = fmaxf(most, top_sm[w][r]);
-            const float base = most == -INFINITY ? 0.f : most;
-            for (int w = 0; w < FEW_WARPS; w++) all += sum_sm[w][r] * exp2_fast(top_sm[w][r] - base);
-            peer_store(&in_top[rank][r], i >> 3, most);
-            peer_store(&in_sum[rank][r], i >> 3, all);
+            peer_store(&in_top[rank][r], i >> 3, all_top[r]);
+            peer_store(&in_sum[rank][r], i >> 3, all_sum[r]);
             if (r == 0) peer_store(&in_odd[rank], i >> 3, any_odd);
         }
         if (TMA) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the next rows' copies go where the warps' sums are
@@ -363,8 +373,9 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, Few<D, INT8>::THREAD_BLOCKS)
                 set_aside |= in_odd[x];
             }
             y = all == 0.f ? 0.f : y / all;
-            if (!INT8 && set_aside) y += what_is_no_number(v, row_bytes, d, s.pos + m / group, c.capacity, a.window, a.sinks);
-            const int64_t to = (s.first + m / group) * a.out_stride + (kv_head * group + m % group) * a.out_head_stride + d;
+            const int i0 = token(m);
+            if (!INT8 && set_aside) y += what_is_no_number(v, row_bytes, d, s.pos + i0, c.capacity, a.window, a.sinks);
+            const int64_t to = (s.first + i0) * a.out_stride + (kv_head * group + (int)m - i0 * group) * a.out_head_stride + d;
             if (a.out_type == ZKB_VALUE_WORD) static_cast<uint32_t*>(a.out)[to] = round_bf16(y);
             else static_cast<uint16_t*>(a.out)[to] = round_bf16(y);
         }
@@ -410,8 +421,13 @@ static cudaError_t launch_few(zkb_ctx* ctx, const zkb_step_attention_args& a) {
 template <int D>
 static cudaError_t launch_attention(zkb_ctx* ctx, const zkb_step_attention_args& a) {
     const zkb_kv_cache& c = a.cache;
-    const uint64_t most = (uint64_t)(a.rows.max_rows ? std::min(a.rows.max_rows, a.rows.n_rows) : a.rows.n_rows) * (a.q_heads / c.n_heads);
-    const bool few = most <= 8;
+    // Eight rows a product or 128. The first kernel takes some 9 us and 0.052 ns for each eight rows, kv head and key, the second some 20 us and 0.2 ns (bf16 caches: 0.12) for each 256: one sequence of
+    // 2,048 tokens and eight kv heads against 12 rows a head 14.6 us and 25, against 128 rows 23 and 27, 16 sequences against 32 rows 63 and 76, 64 rows of 8,192 tokens (256 a head) 12,000 and 1,300.
+    const uint64_t rows = (uint64_t)(a.rows.max_rows ? std::min(a.rows.max_rows, a.rows.n_rows) : a.rows.n_rows) * (a.q_heads / c.n_heads);
+    uint64_t len = a.rows.max_len ? std::min(a.rows.max_len, c.capacity) : c.capacity;
+    if (a.window) len = std::min<uint64_t>(len, (uint64_t)a.window + a.sinks + rows);
+    const double keys = (double)c.n_seqs * c.n_heads * (double)len;
+    const bool few = (0.052 * (double)((rows + 7) / 8) - (c.type == ZKB_VALUE_INT8 ? 0.2 : 0.12) * (double)((rows + 255) / 256)) * keys < 11000.;
     return c.type == ZKB_VALUE_INT8 ? (few ? launch_few<D, true>(ctx, a) : launch_many<D, true>(ctx, a)) : (few ? launch_few<D, false>(ctx, a) : launch_many<D, false>(ctx, a));
 }
 

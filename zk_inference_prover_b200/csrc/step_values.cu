@@ -2,6 +2,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdlib>
+#include <type_traits>
 
 #include "step_values.cuh"
 
@@ -73,106 +74,171 @@ __global__ void __launch_bounds__(256) embed_ragged_kernel(const __grid_constant
 // ---- norms, rotation, the cache's new tokens -------------------------------------------------------------------------------------------
 struct NormRopeArgs {
     zkb_step_norm_rope_args a;
-    uint32_t parts;   // thread blocks a row
+    uint32_t parts;   // warps a row
     double turns[64]; // h_inv_freq / (2 pi): turns a position
 };
 
-// A thread block takes the heads of one row (or one part of them); D / 8 lanes take a head, eight values each. The row's angles are worked
-// out once, by half a rotary dimension's threads, and read by all: position times turns in 64 bits, what is left of whole turns in 32.
+// Four adjacent values. VEC: the address is a multiple of their size.
+template <bool WORD, bool VEC>
+__device__ __forceinline__ void load4(const void* p, int64_t at, float* x) {
+    if constexpr (WORD) {
+        const uint32_t* w = static_cast<const uint32_t*>(p) + at;
+        if constexpr (VEC) {
+            const uint4 v = *reinterpret_cast<const uint4*>(w);
+            x[0] = bf16_low(v.x), x[1] = bf16_low(v.y), x[2] = bf16_low(v.z), x[3] = bf16_low(v.w);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) x[i] = bf16_low(w[i]);
+        }
+    } else {
+        const uint16_t* h = static_cast<const uint16_t*>(p) + at;
+        if constexpr (VEC) {
+            const uint2 v = *reinterpret_cast<const uint2*>(h);
+            x[0] = bf16_low(v.x), x[1] = bf16_high(v.x), x[2] = bf16_low(v.y), x[3] = bf16_high(v.y);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) x[i] = bf16_low(h[i]);
+        }
+    }
+}
+template <bool VEC>
+__device__ __forceinline__ void store4(void* p, int64_t at, const float* x) {
+    uint16_t* h = static_cast<uint16_t*>(p) + at;
+    if constexpr (VEC) *reinterpret_cast<uint2*>(h) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
+    else
+#pragma unroll
+        for (int i = 0; i < 4; i++) h[i] = round_bf16(x[i]);
+}
+
+// A warp takes the heads of one row (or one part of them), D / 8 lanes a head, four heads' loads on their way at a time. A lane has the values that turn together: four of the
+// first half of the rotary dimensions and the four they are paired with (interleaved, and behind the rotary dimensions: eight adjacent ones), so nothing of the rotation crosses
+// lanes. The row's angles are worked out once, two a lane: position times turns in 64 bits, what is left of whole turns in 32. Bound by the bytes: a value is read and written once.
 template <int D, bool WORD, bool INT8, bool VEC>
 __global__ void __launch_bounds__(128) norm_rope_kernel(const __grid_constant__ NormRopeArgs n) {
-    constexpr int LANES = D / 8, HEADS = 32 / LANES;  // lanes a head, heads a warp
-    __shared__ float cos_sm[64], sin_sm[64];
+    constexpr int LANES = D / 8, HEADS = 32 / LANES, AHEAD = 4;  // lanes a head, heads a warp, heads' loads at a time
+    __shared__ float2 turn_sm[4][64];
     const zkb_step_norm_rope_args& a = n.a;
-    const int t = (int)(blockIdx.x / n.parts), part = (int)(blockIdx.x % n.parts);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint64_t unit = (uint64_t)blockIdx.x * 4 + warp;
+    const int t = (int)(unit / n.parts), part = (int)(unit % n.parts);
+    if ((uint32_t)t >= a.rows.n_rows) return;
     const int seq = sequence_of(a.rows.first, (int)a.cache.n_seqs, t);
     if (seq < 0) return;
     const int64_t first = a.rows.first[seq];
     const int64_t pos = (int64_t)a.rows.kv_len[seq] - ((int64_t)a.rows.first[seq + 1] - first) + (t - first);
-    const int half = (int)a.rotary_dim / 2;
-    if ((int)threadIdx.x < half) {
-        const double turn = (double)pos * n.turns[threadIdx.x];
-        sincospif(2.f * (float)(turn - rint(turn)), &sin_sm[threadIdx.x], &cos_sm[threadIdx.x]);
+    const int rotary = (int)a.rotary_dim, half = rotary / 2;
+    for (int i = lane; i < half; i += 32) {
+        const double turn = (double)pos * n.turns[i];
+        float2 v;
+        sincospif(2.f * (float)(turn - rint(turn)), &v.y, &v.x);
+        turn_sm[warp][i] = v;
     }
-    __syncthreads();
+    __syncwarp();
     const bool cached = pos >= 0 && pos < (int64_t)a.cache.capacity;
-    const int lane = threadIdx.x & 31, l = lane % LANES, d0 = 8 * l;
-    const int heads = (int)(a.q_heads + 2 * a.cache.n_heads), q_heads = (int)a.q_heads, kv_heads = (int)a.cache.n_heads;
-    for (int h0 = (part * 4 + (int)(threadIdx.x >> 5)) * HEADS; h0 < heads; h0 += (int)n.parts * 4 * HEADS) {
-        const int hh = h0 + lane / LANES;
-        const bool live = hh < heads, is_q = hh < q_heads, is_v = hh >= q_heads + kv_heads;
-        const int h = is_q ? hh : is_v ? hh - q_heads - kv_heads : hh - q_heads;
-        float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        if (live) {
-            const void* from = is_q ? a.q : is_v ? a.v : a.k;
-            load8<WORD, VEC>(from, t * (is_q ? a.q_stride : is_v ? a.v_stride : a.k_stride) + h * a.head_stride + d0, x);
-        }
-        float ss = 0.f;
+    const int l = lane % LANES, mine = lane / LANES;
+    const bool turned = 8 * l < rotary, pairs = turned && !a.interleaved;
+    const int d0 = pairs ? 4 * l : 8 * l, d1 = pairs ? half + 4 * l : 8 * l + 4;
+    float c[4], s[4];
 #pragma unroll
-        for (int i = 0; i < 8; i++) ss = fmaf(x[i], x[i], ss);
+    for (int i = 0; i < 4; i++) {
+        const float2 v = turned ? turn_sm[warp][4 * l + i] : make_float2(1.f, 0.f);
+        c[i] = v.x, s[i] = v.y;
+    }
+    auto weight_of = [&](const uint16_t* w, uint32_t (&v)[4]) {
+        if (!w) return;
+        v[0] = w[d0] | (uint32_t)w[d0 + 1] << 16, v[1] = w[d0 + 2] | (uint32_t)w[d0 + 3] << 16, v[2] = w[d1] | (uint32_t)w[d1 + 1] << 16, v[3] = w[d1 + 2] | (uint32_t)w[d1 + 3] << 16;
+    };
+    // Heads part * HEADS + mine, ... of queries (0), keys (1) or values (2).
+    auto heads = [&](auto kind, const void* from, int64_t row, int count, const uint16_t* weight) {
+        constexpr int KIND = decltype(kind)::value;
+        uint32_t w[4] = {0, 0, 0, 0};
+        if (KIND < 2) weight_of(weight, w);
+        for (int h0 = part * HEADS; h0 < count; h0 += (int)n.parts * HEADS * AHEAD) {
+            float xs[AHEAD][8];
 #pragma unroll
-        for (int o = LANES / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        const uint16_t* weight = is_v ? nullptr : is_q ? a.q_weight : a.k_weight;
-        if (weight) {
-            const float by = rsqrtf(ss * (1.f / D) + a.eps);
+            for (int i = 0; i < AHEAD; i++) {
+                const int h = h0 + i * (int)n.parts * HEADS + mine;
+                if (h < count) {
+                    const int64_t at = row + h * a.head_stride;
+                    load4<WORD, VEC>(from, at + d0, xs[i]), load4<WORD, VEC>(from, at + d1, xs[i] + 4);
+                } else {
 #pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = x[i] * by * bf16_low(weight[d0 + i]);
-        }
-        if (half) {
-            if (a.interleaved) {
-                if (d0 < 2 * half && !is_v) {
+                    for (int y = 0; y < 8; y++) xs[i][y] = 0.f;
+                }
+            }
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const float c = cos_sm[d0 / 2 + i], s = sin_sm[d0 / 2 + i], u = x[2 * i], v = x[2 * i + 1];
-                        x[2 * i] = u * c - v * s;
-                        x[2 * i + 1] = v * c + u * s;
+            for (int i = 0; i < AHEAD; i++) {
+                const int h = h0 + i * (int)n.parts * HEADS + mine;
+                if (h0 + i * (int)n.parts * HEADS >= count) break;  // the same for the whole warp
+                float(&x)[8] = xs[i];
+                if (KIND < 2 && weight) {
+                    float ss = 0.f;
+#pragma unroll
+                    for (int y = 0; y < 8; y++) ss = fmaf(x[y], x[y], ss);
+#pragma unroll
+                    for (int o = LANES / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                    const float by = rsqrtf(ss * (1.f / D) + a.eps);
+#pragma unroll
+                    for (int y = 0; y < 4; y++) x[2 * y] *= by * bf16_low(w[y]), x[2 * y + 1] *= by * bf16_high(w[y]);
+                }
+                if (KIND < 2) {
+                    if (a.interleaved) {
+#pragma unroll
+                        for (int y = 0; y < 4; y++) {
+                            const float u = x[2 * y], v = x[2 * y + 1];
+                            x[2 * y] = u * c[y] - v * s[y], x[2 * y + 1] = v * c[y] + u * s[y];
+                        }
+                    } else {
+#pragma unroll
+                        for (int y = 0; y < 4; y++) {
+                            const float u = x[y], v = x[y + 4];
+                            x[y] = u * c[y] - v * s[y], x[y + 4] = v * c[y] + u * s[y];
+                        }
                     }
                 }
-            } else {
-                // half is a multiple of eight: the other value of each pair lies with one lane
-                const bool low = d0 < half, turned = d0 < 2 * half && !is_v;
-                const int other = lane + (d0 >= 2 * half ? 0 : low ? half / 8 : -(half / 8)), at = low ? d0 : d0 - half;
+                if (KIND == 0) {
+                    if (h < count) {
+                        const int64_t to = t * a.q_out_stride + h * a.q_out_head_stride;
+                        store4<VEC>(a.q_out, to + d0, x), store4<VEC>(a.q_out, to + d1, x + 4);
+                    }
+                } else if (INT8) {
+                    float most = 0.f;
+                    bool nan = false;
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float y = __shfl_sync(0xffffffffu, x[i], other);
-                    if (turned) x[i] = fmaf(x[i], cos_sm[at + i], (low ? -y : y) * sin_sm[at + i]);
+                    for (int y = 0; y < 8; y++) most = fmaxf(most, fabsf(x[y])), nan |= x[y] != x[y];
+#pragma unroll
+                    for (int o = LANES / 2; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                    if (__ballot_sync(0xffffffffu, nan) >> (mine * LANES) & (LANES == 32 ? 0xffffffffu : (1u << LANES % 32) - 1u)) most = __int_as_float(0x7fc00000);
+                    if (h < count && cached) {
+                        const float up = most > 0.f ? 127.f / most : 0.f;  // zeros' codes are 0, a NaN's and those of an infinite scale likewise
+                        uint32_t q[2] = {0, 0};
+#pragma unroll
+                        for (int y = 0; y < 8; y++) q[y / 4] |= (uint32_t)(max(-127, min(127, __float2int_rn(x[y] * up))) & 255) << (8 * (y % 4));
+                        int8_t* to = static_cast<int8_t*>(KIND == 2 ? a.cache.v : a.cache.k) + seq * a.cache.seq_stride + h * a.cache.head_stride + pos * a.cache.token_stride;
+                        if constexpr (VEC) {
+                            *reinterpret_cast<uint32_t*>(to + d0) = q[0], *reinterpret_cast<uint32_t*>(to + d1) = q[1];
+                        } else {
+#pragma unroll
+                            for (int y = 0; y < 4; y++) to[d0 + y] = (int8_t)(q[0] >> (8 * y)), to[d1 + y] = (int8_t)(q[1] >> (8 * y));
+                        }
+                        if (l == 0) (KIND == 2 ? a.cache.v_scale : a.cache.k_scale)[seq * a.cache.scale_seq_stride + h * a.cache.scale_head_stride + pos] = most / 127.f;
+                    }
+                } else if (h < count && cached) {
+                    void* const to = KIND == 2 ? a.cache.v : a.cache.k;
+                    const int64_t at = seq * a.cache.seq_stride + h * a.cache.head_stride + pos * a.cache.token_stride;
+                    store4<VEC>(to, at + d0, x), store4<VEC>(to, at + d1, x + 4);
                 }
             }
         }
-        if (is_q && live) store8<false, VEC>(a.q_out, t * a.q_out_stride + h * a.q_out_head_stride + d0, x);
-        if constexpr (INT8) {
-            float most = 0.f;
-            bool nan = false;
-#pragma unroll
-            for (int i = 0; i < 8; i++) most = fmaxf(most, fabsf(x[i])), nan |= x[i] != x[i];
-            if (nan) most = __int_as_float(0x7fc00000);
-#pragma unroll
-            for (int o = LANES / 2; o; o >>= 1) {
-                const float m = __shfl_xor_sync(0xffffffffu, most, o);
-                most = m != m || most != most ? m + most : fmaxf(most, m);
-            }
-            if (!is_q && live && cached) {
-                const float scale = __fdiv_rn(most, 127.f);
-                uint32_t w[2] = {0, 0};
-                if (scale > 0.f)
-#pragma unroll
-                    for (int i = 0; i < 8; i++) w[i / 4] |= (uint32_t)(max(-127, min(127, __float2int_rn(__fdiv_rn(x[i], scale)))) & 255) << (8 * (i % 4));
-                int8_t* to = static_cast<int8_t*>(is_v ? a.cache.v : a.cache.k) + seq * a.cache.seq_stride + h * a.cache.head_stride + pos * a.cache.token_stride + d0;
-                if constexpr (VEC) *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
-                else
-#pragma unroll
-                    for (int i = 0; i < 8; i++) to[i] = (int8_t)(w[i / 4] >> (8 * (i % 4)));
-                if (l == 0) (is_v ? a.cache.v_scale : a.cache.k_scale)[seq * a.cache.scale_seq_stride + h * a.cache.scale_head_stride + pos] = scale;
-            }
-        } else if (!is_q && live && cached) {
-            store8<false, VEC>(is_v ? a.cache.v : a.cache.k, seq * a.cache.seq_stride + h * a.cache.head_stride + pos * a.cache.token_stride + d0, x);
-        }
-    }
+    };
+    heads(std::integral_constant<int, 0>(), a.q, t * a.q_stride, (int)a.q_heads, a.q_weight);
+    heads(std::integral_constant<int, 1>(), a.k, t * a.k_stride, (int)a.cache.n_heads, a.k_weight);
+    heads(std::integral_constant<int, 2>(), a.v, t * a.v_stride, (int)a.cache.n_heads, nullptr);
 }
 
 template <int D, bool WORD, bool INT8>
 static cudaError_t launch_norm_rope(zkb_ctx* ctx, const NormRopeArgs& n, bool vec) {
-    const unsigned grid = n.a.rows.n_rows * n.parts;
+    const unsigned grid = (unsigned)(((uint64_t)n.a.rows.n_rows * n.parts + 3) / 4);
     if (vec) norm_rope_kernel<D, WORD, INT8, true><<<grid, 128, 0, ctx->stream>>>(n);
     else norm_rope_kernel<D, WORD, INT8, false><<<grid, 128, 0, ctx->stream>>>(n);
     return cudaGetLastError();
@@ -242,14 +308,13 @@ int zkb_step_norm_rope(zkb_ctx* ctx, const zkb_step_norm_rope_args* args) {
         n.turns[i] = a.h_inv_freq[i] / 6.283185307179586476925;
     }
     n.a.h_inv_freq = nullptr;
-    // a head's rows are read and written 16 bytes (INT8 caches: 8) at a time where every row starts on such a boundary
-    const int64_t in_step = 16 / (int64_t)in_size;
-    const bool vec = aligned_to(a.q, 16) && aligned_to(a.k, 16) && aligned_to(a.v, 16) && aligned_to(a.q_out, 16) && aligned_to(c.k, 8 * kv_size) && aligned_to(c.v, 8 * kv_size) &&
-                     a.q_stride % in_step == 0 && a.k_stride % in_step == 0 && a.v_stride % in_step == 0 && a.head_stride % in_step == 0 && a.q_out_stride % 8 == 0 && a.q_out_head_stride % 8 == 0 &&
-                     c.seq_stride % 8 == 0 && c.head_stride % 8 == 0 && c.token_stride % 8 == 0;
-    // Few rows are spread over the SMs, a pass of four warps each.
-    const uint32_t heads = a.q_heads + 2 * c.n_heads, a_pass = 4 * 32 / (c.head_dim / 8), passes = (heads + a_pass - 1) / a_pass;
-    n.parts = std::max(1u, std::min(passes, 148u * 4u / a.rows.n_rows));
+    // four values at a time where all rows start on such a boundary
+    const bool vec = aligned_to(a.q, 4 * in_size) && aligned_to(a.k, 4 * in_size) && aligned_to(a.v, 4 * in_size) && aligned_to(a.q_out, 8) && aligned_to(c.k, 4 * kv_size) && aligned_to(c.v, 4 * kv_size) &&
+                     a.q_stride % 4 == 0 && a.k_stride % 4 == 0 && a.v_stride % 4 == 0 && a.head_stride % 4 == 0 && a.q_out_stride % 4 == 0 && a.q_out_head_stride % 4 == 0 && c.seq_stride % 4 == 0 &&
+                     c.head_stride % 4 == 0 && c.token_stride % 4 == 0;
+    // A warp a row; few rows are spread over more, down to a warp for each of its passes over the query heads.
+    const uint32_t passes = (a.q_heads + 256 / c.head_dim - 1) / (256 / c.head_dim);
+    n.parts = std::max(1u, std::min(passes, 148u * 16u / a.rows.n_rows));
     DeviceGuard g(ctx);
     ProfScope prof(ctx, "step_norm_rope_kernel");
     ZKB_CUDA(ctx, c.head_dim == 128 ? launch_norm_rope<128>(ctx, n, vec) : c.head_dim == 64 ? launch_norm_rope<64>(ctx, n, vec) : launch_norm_rope<32>(ctx, n, vec));
