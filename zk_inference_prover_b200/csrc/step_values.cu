@@ -9,12 +9,14 @@
 namespace zk {
 
 // ---- embedding rows ------------------------------------------------------------------------------------------------------------------
+// A row of the table is scaled, rounded and written: bound by its bytes. Eight values a thread; blockIdx.y names the run of the row, blockIdx.x the tokens, whose ids and then
+// whose values are asked for together: EMBED_TOKENS loads on their way, where a load at a time left the memory waiting (16384 tokens of 4096 bf16: 40 us -> 35 us, 5.7 TB/s).
+constexpr int EMBED_TOKENS = 4;
 struct EmbedArgs {
     zkb_step_embed_args a;
-    uint32_t tokens_a_block;
+    uint32_t tokens_a_block;  // <= EMBED_TOKENS
 };
 
-// Eight values a thread; blockIdx.y names the run of the row, blockIdx.x the tokens.
 template <bool INT8, bool WORD>
 __global__ void __launch_bounds__(256) embed_kernel(const __grid_constant__ EmbedArgs e) {
     const zkb_step_embed_args& a = e.a;
@@ -22,28 +24,36 @@ __global__ void __launch_bounds__(256) embed_kernel(const __grid_constant__ Embe
     const uint32_t t0 = blockIdx.x * e.tokens_a_block, t1 = min(a.n_tokens, t0 + e.tokens_a_block);
     if (col >= a.width) return;
     const int64_t at = a.segment ? (int64_t)(col / a.segment) * a.segment_stride + col % a.segment : (int64_t)col;
-    for (uint32_t t = t0; t < t1; t++) {
-        const int32_t id = a.ids[t];
-        const bool inside = id >= 0 && (uint32_t)id < a.vocab;
-        if (!inside && col == 0 && a.off_table) atomicAdd(reinterpret_cast<unsigned long long*>(a.off_table), 1ull);
-        float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        if (inside) {
-            const int64_t from = (int64_t)id * a.table_stride + col;
-            if constexpr (INT8) {
-                const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const int8_t*>(a.table) + from);
-                const float by = a.row_scale[id] * a.scale;
+    int32_t id[EMBED_TOKENS];
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    x[i] = (float)(int8_t)(w.x >> (8 * i)) * by;
-                    x[4 + i] = (float)(int8_t)(w.y >> (8 * i)) * by;
-                }
-            } else {
-                load8<false, true>(a.table, from, x);
+    for (int i = 0; i < EMBED_TOKENS; i++) id[i] = t0 + i < t1 ? a.ids[t0 + i] : -1;
+    uint32_t raw[EMBED_TOKENS][INT8 ? 2 : 4];
+    float by[EMBED_TOKENS];
 #pragma unroll
-                for (int i = 0; i < 8; i++) x[i] *= a.scale;
-            }
+    for (int i = 0; i < EMBED_TOKENS; i++) {
+        const bool inside = id[i] >= 0 && (uint32_t)id[i] < a.vocab;
+        const int64_t from = (int64_t)id[i] * a.table_stride + col;
+        if constexpr (INT8) {
+            const uint2 w = inside ? *reinterpret_cast<const uint2*>(static_cast<const int8_t*>(a.table) + from) : make_uint2(0u, 0u);
+            raw[i][0] = w.x, raw[i][1] = w.y;
+            by[i] = inside ? a.row_scale[id[i]] * a.scale : 0.f;
+        } else {
+            const uint4 w = inside ? *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.table) + from) : make_uint4(0u, 0u, 0u, 0u);
+            raw[i][0] = w.x, raw[i][1] = w.y, raw[i][2] = w.z, raw[i][3] = w.w;
+            by[i] = inside ? a.scale : 0.f;
         }
-        store8<WORD, true>(a.out, (int64_t)t * a.out_stride + at, x);
+    }
+#pragma unroll
+    for (int i = 0; i < EMBED_TOKENS; i++) {
+        if (t0 + i >= t1) break;
+        if ((id[i] < 0 || (uint32_t)id[i] >= a.vocab) && col == 0 && a.off_table) atomicAdd(reinterpret_cast<unsigned long long*>(a.off_table), 1ull);
+        float x[8];
+#pragma unroll
+        for (int y = 0; y < 8; y++) {
+            if constexpr (INT8) x[y] = (float)(int8_t)(raw[i][y / 4] >> (8 * (y % 4))) * by[i];
+            else x[y] = (y % 2 ? bf16_high(raw[i][y / 2]) : bf16_low(raw[i][y / 2])) * by[i];
+        }
+        store8<WORD>(a.out, (int64_t)(t0 + i) * a.out_stride + at, x);
     }
 }
 
@@ -78,27 +88,41 @@ struct NormRopeArgs {
     double turns[64]; // h_inv_freq / (2 pi): turns a position
 };
 
-// Four adjacent values. VEC: the address is a multiple of their size.
+// The value n values of SIZE bytes behind p.
+template <int SIZE>
+__device__ __forceinline__ void* value_at(const void* p, int64_t n) {
+    return static_cast<char*>(const_cast<void*>(p)) + n * SIZE;
+}
+
+// Four adjacent values as they lie in memory, and as floats. VEC: the address is a multiple of their size.
 template <bool WORD, bool VEC>
-__device__ __forceinline__ void load4(const void* p, int64_t at, float* x) {
+__device__ __forceinline__ void load4(const void* p, int64_t at, uint32_t* x) {
     if constexpr (WORD) {
         const uint32_t* w = static_cast<const uint32_t*>(p) + at;
         if constexpr (VEC) {
             const uint4 v = *reinterpret_cast<const uint4*>(w);
-            x[0] = bf16_low(v.x), x[1] = bf16_low(v.y), x[2] = bf16_low(v.z), x[3] = bf16_low(v.w);
+            x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
         } else {
 #pragma unroll
-            for (int i = 0; i < 4; i++) x[i] = bf16_low(w[i]);
+            for (int i = 0; i < 4; i++) x[i] = w[i];
         }
     } else {
         const uint16_t* h = static_cast<const uint16_t*>(p) + at;
         if constexpr (VEC) {
             const uint2 v = *reinterpret_cast<const uint2*>(h);
-            x[0] = bf16_low(v.x), x[1] = bf16_high(v.x), x[2] = bf16_low(v.y), x[3] = bf16_high(v.y);
+            x[0] = v.x, x[1] = v.y;
         } else {
-#pragma unroll
-            for (int i = 0; i < 4; i++) x[i] = bf16_low(h[i]);
+            x[0] = h[0] | (uint32_t)h[1] << 16, x[1] = h[2] | (uint32_t)h[3] << 16;
         }
+    }
+}
+template <bool WORD>
+__device__ __forceinline__ void floats4(const uint32_t* w, float* x) {
+    if constexpr (WORD) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = bf16_low(w[i]);
+    } else {
+        x[0] = bf16_low(w[0]), x[1] = bf16_high(w[0]), x[2] = bf16_low(w[1]), x[3] = bf16_high(w[1]);
     }
 }
 template <bool VEC>
@@ -110,23 +134,28 @@ __device__ __forceinline__ void store4(void* p, int64_t at, const float* x) {
         for (int i = 0; i < 4; i++) h[i] = round_bf16(x[i]);
 }
 
-// A warp takes the heads of one row (or one part of them), D / 8 lanes a head, four heads' loads on their way at a time. A lane has the values that turn together: four of the
-// first half of the rotary dimensions and the four they are paired with (interleaved, and behind the rotary dimensions: eight adjacent ones), so nothing of the rotation crosses
-// lanes. The row's angles are worked out once, two a lane: position times turns in 64 bits, what is left of whole turns in 32. Bound by the bytes: a value is read and written once.
+// A warp takes the heads of one row (or one part of them), D / 8 lanes a head, the loads of four passes over them (words: two) on their way at a time. A lane has the values that
+// turn together: four of the first half of the rotary dimensions and the four they are paired with (interleaved, and behind the rotary dimensions: eight adjacent ones), so nothing
+// of the rotation crosses lanes. The row's angles are worked out once, two a lane: position times turns in 64 bits, what is left of whole turns in 32. Bound by the bytes: a value
+// is read and written once. 4 x 2048 rows of 32 + 2 x 8 heads of 128 into a bf16 cache: 37 us, 4.6 TB/s; with registers for eight
+// blocks a multiprocessor instead of six, which spills a few, 42 us, with eight passes' loads at a time for four blocks, 49 us.
 template <int D, bool WORD, bool INT8, bool VEC>
-__global__ void __launch_bounds__(128) norm_rope_kernel(const __grid_constant__ NormRopeArgs n) {
-    constexpr int LANES = D / 8, HEADS = 32 / LANES, AHEAD = 4;  // lanes a head, heads a warp, heads' loads at a time
+__global__ void __launch_bounds__(128, 6) norm_rope_kernel(const __grid_constant__ NormRopeArgs n) {
+    constexpr int LANES = D / 8, HEADS = 32 / LANES, AHEAD = WORD ? 2 : 4, FOUR = WORD ? 4 : 2;  // lanes a head, heads a warp, their loads at a time, words of four values
     __shared__ float2 turn_sm[4][64];
     const zkb_step_norm_rope_args& a = n.a;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint64_t unit = (uint64_t)blockIdx.x * 4 + warp;
     const int t = (int)(unit / n.parts), part = (int)(unit % n.parts);
     if ((uint32_t)t >= a.rows.n_rows) return;
+    const int rotary = (int)a.rotary_dim, half = rotary / 2;
+    const int l = lane % LANES, mine = lane / LANES;
+    const bool turned = 8 * l < rotary, pairs = turned && !a.interleaved;
+    const int d0 = pairs ? 4 * l : 8 * l, d1 = pairs ? half + 4 * l : 8 * l + 4;
     const int seq = sequence_of(a.rows.first, (int)a.cache.n_seqs, t);
     if (seq < 0) return;
     const int64_t first = a.rows.first[seq];
     const int64_t pos = (int64_t)a.rows.kv_len[seq] - ((int64_t)a.rows.first[seq + 1] - first) + (t - first);
-    const int rotary = (int)a.rotary_dim, half = rotary / 2;
     for (int i = lane; i < half; i += 32) {
         const double turn = (double)pos * n.turns[i];
         float2 v;
@@ -135,9 +164,6 @@ __global__ void __launch_bounds__(128) norm_rope_kernel(const __grid_constant__ 
     }
     __syncwarp();
     const bool cached = pos >= 0 && pos < (int64_t)a.cache.capacity;
-    const int l = lane % LANES, mine = lane / LANES;
-    const bool turned = 8 * l < rotary, pairs = turned && !a.interleaved;
-    const int d0 = pairs ? 4 * l : 8 * l, d1 = pairs ? half + 4 * l : 8 * l + 4;
     float c[4], s[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
@@ -149,28 +175,32 @@ __global__ void __launch_bounds__(128) norm_rope_kernel(const __grid_constant__ 
         v[0] = w[d0] | (uint32_t)w[d0 + 1] << 16, v[1] = w[d0 + 2] | (uint32_t)w[d0 + 3] << 16, v[2] = w[d1] | (uint32_t)w[d1 + 1] << 16, v[3] = w[d1 + 2] | (uint32_t)w[d1 + 3] << 16;
     };
     // Heads part * HEADS + mine, ... of queries (0), keys (1) or values (2).
-    auto heads = [&](auto kind, const void* from, int64_t row, int count, const uint16_t* weight) {
+    auto heads = [&](auto kind, const void* from, int64_t at, int count, const uint16_t* weight) {
         constexpr int KIND = decltype(kind)::value;
-        uint32_t w[4] = {0, 0, 0, 0};
-        if (KIND < 2) weight_of(weight, w);
-        for (int h0 = part * HEADS; h0 < count; h0 += (int)n.parts * HEADS * AHEAD) {
-            float xs[AHEAD][8];
+        uint32_t w[4] = {};
+        weight_of(weight, w);
+        const int stride = (int)n.parts * HEADS, h_first = part * HEADS + mine;
+        // where this lane's next head is read and written: heads are `stride` apart
+        const void* in = value_at<WORD ? 4 : 2>(from, at + h_first * a.head_stride + d0);
+        const int64_t in_step = stride * a.head_stride;
+        void* out = KIND == 0 ? value_at<2>(a.q_out, t * a.q_out_stride + h_first * a.q_out_head_stride + d0)
+                              : value_at<INT8 ? 1 : 2>(KIND == 2 ? a.cache.v : a.cache.k, seq * a.cache.seq_stride + h_first * a.cache.head_stride + pos * a.cache.token_stride + d0);
+        const int64_t out_step = stride * (KIND == 0 ? a.q_out_head_stride : a.cache.head_stride);
+        float* scale = (KIND == 2 ? a.cache.v_scale : a.cache.k_scale) + (INT8 ? seq * a.cache.scale_seq_stride + h_first * a.cache.scale_head_stride + pos : 0);
+#pragma unroll 1
+        for (int h0 = part * HEADS; h0 < count; h0 += stride * AHEAD) {
+            uint32_t raw[AHEAD][2 * FOUR] = {};
 #pragma unroll
             for (int i = 0; i < AHEAD; i++) {
-                const int h = h0 + i * (int)n.parts * HEADS + mine;
-                if (h < count) {
-                    const int64_t at = row + h * a.head_stride;
-                    load4<WORD, VEC>(from, at + d0, xs[i]), load4<WORD, VEC>(from, at + d1, xs[i] + 4);
-                } else {
-#pragma unroll
-                    for (int y = 0; y < 8; y++) xs[i][y] = 0.f;
-                }
+                if (h0 + i * stride + mine < count) load4<WORD, VEC>(in, 0, raw[i]), load4<WORD, VEC>(in, d1 - d0, raw[i] + FOUR);
+                in = value_at<WORD ? 4 : 2>(in, in_step);
             }
 #pragma unroll
             for (int i = 0; i < AHEAD; i++) {
-                const int h = h0 + i * (int)n.parts * HEADS + mine;
-                if (h0 + i * (int)n.parts * HEADS >= count) break;  // the same for the whole warp
-                float(&x)[8] = xs[i];
+                if (h0 + i * stride >= count) break;  // the same for the whole warp
+                const bool has = h0 + i * stride + mine < count;
+                float x[8];
+                floats4<WORD>(raw[i], x), floats4<WORD>(raw[i] + FOUR, x + 4);
                 if (KIND < 2 && weight) {
                     float ss = 0.f;
 #pragma unroll
@@ -197,10 +227,7 @@ __global__ void __launch_bounds__(128) norm_rope_kernel(const __grid_constant__ 
                     }
                 }
                 if (KIND == 0) {
-                    if (h < count) {
-                        const int64_t to = t * a.q_out_stride + h * a.q_out_head_stride;
-                        store4<VEC>(a.q_out, to + d0, x), store4<VEC>(a.q_out, to + d1, x + 4);
-                    }
+                    if (has) store4<VEC>(out, 0, x), store4<VEC>(out, d1 - d0, x + 4);
                 } else if (INT8) {
                     float most = 0.f;
                     bool nan = false;
@@ -209,25 +236,25 @@ __global__ void __launch_bounds__(128) norm_rope_kernel(const __grid_constant__ 
 #pragma unroll
                     for (int o = LANES / 2; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
                     if (__ballot_sync(0xffffffffu, nan) >> (mine * LANES) & (LANES == 32 ? 0xffffffffu : (1u << LANES % 32) - 1u)) most = __int_as_float(0x7fc00000);
-                    if (h < count && cached) {
+                    if (has && cached) {
                         const float up = most > 0.f ? 127.f / most : 0.f;  // zeros' codes are 0, a NaN's and those of an infinite scale likewise
                         uint32_t q[2] = {0, 0};
 #pragma unroll
                         for (int y = 0; y < 8; y++) q[y / 4] |= (uint32_t)(max(-127, min(127, __float2int_rn(x[y] * up))) & 255) << (8 * (y % 4));
-                        int8_t* to = static_cast<int8_t*>(KIND == 2 ? a.cache.v : a.cache.k) + seq * a.cache.seq_stride + h * a.cache.head_stride + pos * a.cache.token_stride;
+                        int8_t* to = static_cast<int8_t*>(out);
                         if constexpr (VEC) {
-                            *reinterpret_cast<uint32_t*>(to + d0) = q[0], *reinterpret_cast<uint32_t*>(to + d1) = q[1];
+                            *reinterpret_cast<uint32_t*>(to) = q[0], *reinterpret_cast<uint32_t*>(to + d1 - d0) = q[1];
                         } else {
 #pragma unroll
-                            for (int y = 0; y < 4; y++) to[d0 + y] = (int8_t)(q[0] >> (8 * y)), to[d1 + y] = (int8_t)(q[1] >> (8 * y));
+                            for (int y = 0; y < 4; y++) to[y] = (int8_t)(q[0] >> (8 * y)), to[d1 - d0 + y] = (int8_t)(q[1] >> (8 * y));
                         }
-                        if (l == 0) (KIND == 2 ? a.cache.v_scale : a.cache.k_scale)[seq * a.cache.scale_seq_stride + h * a.cache.scale_head_stride + pos] = most / 127.f;
+                        if (l == 0) *scale = most / 127.f;
                     }
-                } else if (h < count && cached) {
-                    void* const to = KIND == 2 ? a.cache.v : a.cache.k;
-                    const int64_t at = seq * a.cache.seq_stride + h * a.cache.head_stride + pos * a.cache.token_stride;
-                    store4<VEC>(to, at + d0, x), store4<VEC>(to, at + d1, x + 4);
+                } else if (has && cached) {
+                    store4<VEC>(out, 0, x), store4<VEC>(out, d1 - d0, x + 4);
                 }
+                out = value_at<KIND && INT8 ? 1 : 2>(out, out_step);
+                if (KIND && INT8) scale += stride * a.cache.scale_head_stride;
             }
         }
     };
@@ -275,7 +302,7 @@ int zkb_step_embed(zkb_ctx* ctx, const zkb_step_embed_args* args) {
                      (a.segment == 0 || (a.segment % 8 == 0 && a.segment_stride * (int64_t)out_size % 16 == 0));
     const uint32_t per_block = vec ? 2048 : 256, runs = (a.width + per_block - 1) / per_block;
     EmbedArgs e{a, 1};
-    while (e.tokens_a_block < 4 && (uint64_t)a.n_tokens * runs / e.tokens_a_block > 148 * 16) e.tokens_a_block *= 2;
+    while (e.tokens_a_block < EMBED_TOKENS && (uint64_t)a.n_tokens * runs / e.tokens_a_block > 148 * 16) e.tokens_a_block *= 2;
     const dim3 grid((a.n_tokens + e.tokens_a_block - 1) / e.tokens_a_block, runs);
     ProfScope prof(ctx, "step_embed_kernel");
     auto launch = [&](auto kernel) { kernel<<<grid, 256, 0, ctx->stream>>>(e); };

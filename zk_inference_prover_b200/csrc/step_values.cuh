@@ -22,51 +22,18 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
 }
 __device__ __forceinline__ uint16_t round_bf16(float x) { return __bfloat16_as_ushort(__float2bfloat16_rn(x)); }
 
-// Eight adjacent values, WORD: bf16 patterns in words, else bf16. VEC: the address is a multiple of 16 bytes.
-template <bool WORD, bool VEC>
-__device__ __forceinline__ void load8(const void* p, int64_t at, float (&x)[8]) {
-    if constexpr (WORD) {
-        const uint32_t* w = static_cast<const uint32_t*>(p) + at;
-        if constexpr (VEC) {
-            const uint4 a = *reinterpret_cast<const uint4*>(w), b = *reinterpret_cast<const uint4*>(w + 4);
-            const uint32_t v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = bf16_low(v[i]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = bf16_low(w[i]);
-        }
-    } else {
-        const uint16_t* h = static_cast<const uint16_t*>(p) + at;
-        if constexpr (VEC) {
-            const uint4 a = *reinterpret_cast<const uint4*>(h);
-            const uint32_t v[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-            for (int i = 0; i < 4; i++) x[2 * i] = bf16_low(v[i]), x[2 * i + 1] = bf16_high(v[i]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = bf16_low(h[i]);
-        }
-    }
-}
-template <bool WORD, bool VEC>
+// Eight values rounded to bf16 at a multiple of 16 bytes, WORD: their patterns in words.
+template <bool WORD>
 __device__ __forceinline__ void store8(void* p, int64_t at, const float (&x)[8]) {
-    if constexpr (VEC) {
-        uint32_t v[4];
+    uint32_t v[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = pack_bf16(x[2 * i], x[2 * i + 1]);
-        if constexpr (WORD) {
-            uint4* w = reinterpret_cast<uint4*>(static_cast<uint32_t*>(p) + at);
-            w[0] = make_uint4(v[0] & 0xffffu, v[0] >> 16, v[1] & 0xffffu, v[1] >> 16);
-            w[1] = make_uint4(v[2] & 0xffffu, v[2] >> 16, v[3] & 0xffffu, v[3] >> 16);
-        } else {
-            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + at) = make_uint4(v[0], v[1], v[2], v[3]);
-        }
+    for (int i = 0; i < 4; i++) v[i] = pack_bf16(x[2 * i], x[2 * i + 1]);
+    if constexpr (WORD) {
+        uint4* w = reinterpret_cast<uint4*>(static_cast<uint32_t*>(p) + at);
+        w[0] = make_uint4(v[0] & 0xffffu, v[0] >> 16, v[1] & 0xffffu, v[1] >> 16);
+        w[1] = make_uint4(v[2] & 0xffffu, v[2] >> 16, v[3] & 0xffffu, v[3] >> 16);
     } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++)
-            if constexpr (WORD) static_cast<uint32_t*>(p)[at + i] = round_bf16(x[i]);
-            else static_cast<uint16_t*>(p)[at + i] = round_bf16(x[i]);
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + at) = make_uint4(v[0], v[1], v[2], v[3]);
     }
 }
 
