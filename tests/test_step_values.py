@@ -53,6 +53,23 @@ def _rope_args(zkb, cache={}, rows={}, **other):
     return a
 
 
+@pytest.mark.parametrize("other,want", [(dict(ids=66), "ids"), (dict(row_scale=70), "row_scale"), (dict(off_table=68), "off_table")])
+def test_embed_refuses_arrays_off_their_boundaries(zkb, refuse, other, want):
+    refuse("zkb_step_embed", _embed_args(zkb, **other), want)
+
+
+@pytest.mark.parametrize("cache,rows,want", [(dict(k_scale=66), {}, "k_scale"), (dict(v_scale=65), {}, "v_scale"), (dict(token_stride=(1 << 29) + 1), {}, "2^29"), (dict(token_stride=-(1 << 30)), {}, "2^29"),
+                                             (dict(capacity=(1 << 30) + 1), {}, "capacity"), (dict(n_heads=1025), {}, "n_heads"), (dict(n_seqs=65536), {}, "n_seqs"), ({}, dict(kv_len=0), "kv_len"),
+                                             ({}, dict(first=66), "boundary"), ({}, dict(kv_len=65), "boundary")])
+def test_caches_and_rows_past_their_limits_are_refused(zkb, refuse, cache, rows, want):
+    refuse("zkb_step_norm_rope", _rope_args(zkb, cache, rows), want)
+    refuse("zkb_step_attention", _attention_args(zkb, cache, rows), want)
+
+
+def test_attention_refuses_more_rows_of_heads_than_it_can_number(zkb, refuse):
+    refuse("zkb_step_attention", _attention_args(zkb, {}, dict(n_rows=1 << 29), q_heads=4), "q_heads")
+
+
 @pytest.mark.parametrize("cache,rows,want", CACHE_REFUSALS)
 def test_norm_rope_refuses_caches_and_rows(zkb, refuse, cache, rows, want):
     refuse("zkb_step_norm_rope", _rope_args(zkb, cache, rows), want)
@@ -323,3 +340,330 @@ def test_attention_scores_far_apart(ctx, zkb, kind, rows, length):
     check_attention(ctx, zkb, batch, cache, q, "bf16", 0, 0, scale=3.0)
     check_attention(ctx, zkb, batch, cache, q, "bf16", 0, 0, scale=-3.0)
     check_attention(ctx, zkb, batch, cache, q, "bf16", 0, 0, scale=0.0)
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+@pytest.mark.parametrize("rows,length,d,window,sinks", [(5000, 5000, 64, 0, 0), (4000, 4200, 128, 300, 40), (100, 3000, 128, 0, 0)])
+def test_attention_of_many_units(ctx, zkb, kind, rows, length, d, window, sinks):
+    """More pairs of tiles than thread blocks, and keys spread over many thread blocks; infinities in one token's values that the last rows see."""
+    g = gen(rows)
+    batch, cache = Batch([(rows, length)]), Cache(g, kind, 1, 4, length, d)
+    q = torch.randn(rows, 16, d, generator=g, device="cuda").bfloat16()
+    check_attention(ctx, zkb, batch, cache, q, "bf16", window, sinks)
+    if kind == "bf16":
+        cache.v[0, 1, length - 20, 5:9] = math.inf
+        cache.v[0, 2, length - 30, 7] = -math.inf
+        check_attention(ctx, zkb, batch, cache, q, "bf16", window, sinks)
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+@pytest.mark.parametrize("max_rows,max_len", [(1, 1), (0, 1), (1, 0), (1 << 31, 1 << 31), (7, 900)])
+def test_attention_hints_that_are_wrong_change_no_result(ctx, zkb, kind, max_rows, max_len):
+    """Fewer rows and tokens than there are, and more; both ways of laying out the work meet them."""
+    g = gen(max_rows % 100)
+    for shape in ([(300, 700), (2, 5)], [(1, 1500), (3, 40)]):
+        batch, d = Batch(shape, behind=1), 64
+        cache = Cache(g, kind, 2, 2, 1500, d)
+        q = torch.randn(batch.n_rows, 8, d, generator=g, device="cuda").bfloat16()
+        args = batch.args
+
+        def hinted(zkb, hints=True):
+            r = args(zkb, hints)
+            r.max_rows, r.max_len = max_rows, max_len
+            return r
+
+        batch.args = hinted
+        check_attention(ctx, zkb, batch, cache, q, "bf16", 0, 0)
+        check_attention(ctx, zkb, batch, cache, q, "words", 100, 4)
+
+
+@gpu
+@pytest.mark.parametrize("first,lens", [([0, 9, 4, 30], [20, 20, 20]), ([-5, 3, 60, 10], [50, -3, 7]), ([40, 30, 20, 10], [5, 5, 5]), ([0, 2 ** 31 - 1, -(2 ** 31), 24], [2 ** 31 - 1, -(2 ** 31), 40])])
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+@pytest.mark.parametrize("rows,heads", [(24, 4), (24, 64)])
+def test_arrays_that_describe_no_batch_stay_inside_the_buffers(ctx, zkb, first, lens, kind, rows, heads):
+    """Borders that descend, or lie outside the rows; lengths below zero and past the capacity: what the rows get is undefined, what lies around them is not touched."""
+    g, d, cap = gen(rows), 64, 50 if heads == 4 else 600  # few rows a product, and many
+    cache = Cache(g, kind, 5, 2, cap, d)
+    before = [x.clone() for x in (cache.k, cache.v)]
+    f, n = torch.tensor(first, dtype=torch.int32, device="cuda"), torch.tensor(lens, dtype=torch.int32, device="cuda")
+    c = cache.args(zkb)
+    size = cache.k.element_size()
+    c.n_seqs, c.k, c.v = 3, c.k + size * cache.k.stride(0), c.v + size * cache.k.stride(0)  # sequences 0 and 4 lie around it
+    if kind == "int8":
+        c.k_scale, c.v_scale = c.k_scale + 4 * cache.k_scale.stride(0), c.v_scale + 4 * cache.k_scale.stride(0)
+    batch = zkb.StepRows(first=f.data_ptr(), kv_len=n.data_ptr(), n_rows=rows)
+    x = torch.randn(rows, heads + 4, d, generator=g, device="cuda").bfloat16()
+    out = torch.full((rows + 2, heads, d), -3.0, device="cuda", dtype=torch.bfloat16)
+    freq = np.ones(16)
+    torch.cuda.synchronize()
+    ctx.step_norm_rope(zkb.StepNormRope(cache=c, rows=batch, q=x.data_ptr(), k=x[:, heads:].data_ptr(), v=x[:, heads + 2:].data_ptr(), h_inv_freq=freq.ctypes.data, q_out=out[1].data_ptr(),
+                                        q_stride=x.stride(0), k_stride=x.stride(0), v_stride=x.stride(0), head_stride=d, q_out_stride=out.stride(0), q_out_head_stride=d, q_heads=heads, rotary_dim=32, eps=1e-6))
+    ctx.step_attention(zkb.StepAttention(cache=c, rows=batch, q=x.data_ptr(), out=out[1].data_ptr(), q_stride=x.stride(0), q_head_stride=d, out_stride=out.stride(0), out_head_stride=d, q_heads=heads, scale=0.1))
+    done(ctx)
+    assert bool((out[0] == -3).all()) and bool((out[-1] == -3).all())
+    for x, y in zip((cache.k, cache.v), before):
+        assert torch.equal(x[0], y[0]) and torch.equal(x[4], y[4])
+
+
+@gpu
+@pytest.mark.parametrize("d,order,heads", [(128, "thsd", 8), (64, "hstd", 2), (64, "shtd", 2)])
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+def test_offsets_past_32_bits(ctx, zkb, kind, d, order, heads):
+    """Tokens, heads or sequences so far apart that the last ones lie more than 2^32 bytes into the cache: written by norm_rope, read by the attention, by one row and by many."""
+    size, cap = 1 if kind == "int8" else 2, 33
+    far = dict(t=(1 << 32) // 30 // size, s=(1 << 32) // size, h=(1 << 32) // size)[order[0]] // 64 * 64
+    stride = {"thsd": dict(t=far, h=2 * d, s=d), "hstd": dict(h=far, s=cap * d, t=d), "shtd": dict(s=far, h=cap * d, t=d)}[order]
+    seqs = 2
+    need = (seqs - 1) * stride["s"] + (heads - 1) * stride["h"] + (cap - 1) * stride["t"] + d
+    assert need * size > 1 << 32
+    g = gen(d)
+    cache = Cache(g, kind, seqs, heads, cap, d, blank=True)
+    rooms = [torch.zeros(need, device="cuda", dtype=cache.k.dtype) for _ in range(2)]
+    cache.k, cache.v = (r.as_strided((seqs, heads, cap, d), (stride["s"], stride["h"], stride["t"], 1)) for r in rooms)
+    for rows in (cap - 2, 1):
+        batch = Batch([(rows, cap), (rows, cap - 1)])
+        x = torch.randn(batch.n_rows, 4 * heads, d, generator=g, device="cuda").bfloat16()
+        q = x[:, :2 * heads]
+        freq = 1e4 ** (-np.arange(d // 2) / (d // 2))
+        out = torch.zeros(batch.n_rows, 2 * heads, d, device="cuda", dtype=torch.bfloat16)
+        torch.cuda.synchronize()
+        ctx.step_norm_rope(zkb.StepNormRope(cache=cache.args(zkb), rows=batch.args(zkb), q=x.data_ptr(), k=x[:, 2 * heads:].data_ptr(), v=x[:, 3 * heads:].data_ptr(), h_inv_freq=freq.ctypes.data,
+                                            q_out=out.data_ptr(), q_stride=x.stride(0), k_stride=x.stride(0), v_stride=x.stride(0), head_stride=d, q_out_stride=out.stride(0), q_out_head_stride=d,
+                                            q_heads=2 * heads, rotary_dim=d, eps=1e-6))
+        done(ctx)
+        k, v = cache.values()
+        for b, r0, r, p0 in batch.each():
+            want = x[r0:r0 + r, 3 * heads:].double().transpose(0, 1)
+            step = cache.v_scale[b, :, p0:p0 + r].double()[..., None] if kind == "int8" else 0
+            assert bool(((v[b, :, p0:p0 + r] - want).abs() <= step * (0.5 + 127 * 2.0 ** -22)).all())
+            assert bool((k[b, :, p0:p0 + r] != 0).any(-1).all())
+        check_attention(ctx, zkb, batch, cache, q, "bf16", 0, 0)
+    del rooms, cache
+    torch.cuda.empty_cache()
+
+
+@gpu
+@pytest.mark.parametrize("table", ["bf16", "int8"])
+def test_embedding_rows_past_32_bits(ctx, zkb, table):
+    g, vocab, width, stride = gen(3), 1100, 40, 1 << 22
+    dtype = torch.int8 if table == "int8" else torch.bfloat16
+    room = torch.zeros((vocab - 1) * stride + width, device="cuda", dtype=dtype)
+    tab = room.as_strided((vocab, width), (stride, 1))
+    tab.copy_(torch.randint(-100, 100, (vocab, width), generator=g, device="cuda"))
+    scales = torch.rand(vocab, generator=g, device="cuda")
+    ids = torch.tensor([vocab - 1, 0, 3, vocab - 1, 1024, vocab - 1], dtype=torch.int32, device="cuda")
+    out = torch.zeros(len(ids), width, device="cuda", dtype=torch.bfloat16)
+    torch.cuda.synchronize()
+    ctx.step_embed(zkb.StepEmbed(ids=ids.data_ptr(), table=tab.data_ptr(), row_scale=scales.data_ptr() if table == "int8" else 0, out=out.data_ptr(), table_stride=stride, out_stride=width,
+                                 n_tokens=len(ids), vocab=vocab, width=width, table_type=2 if table == "int8" else 0, out_type=0, scale=1.0))
+    done(ctx)
+    want = tab[ids.long()].float() * (scales[ids.long()][:, None] if table == "int8" else 1.0)
+    assert torch.equal(out, want.bfloat16())
+    del room, tab
+    torch.cuda.empty_cache()
+
+
+@gpu
+def test_queries_may_be_turned_where_they_are(ctx, zkb):
+    g, d, heads = gen(9), 64, 6
+    batch, cache = Batch([(50, 60), (1, 9)], behind=2), Cache(gen(1), "bf16", 2, 2, 64, 64, blank=True)
+    x = torch.randn(batch.n_rows, heads + 4, d, generator=g, device="cuda").bfloat16()
+    freq, results = 1e4 ** (-np.arange(16) / 16), []
+    for inside in (False, True):
+        rows = x.clone()
+        out = rows if inside else x.clone()
+        torch.cuda.synchronize()
+        ctx.step_norm_rope(zkb.StepNormRope(cache=cache.args(zkb), rows=batch.args(zkb), q=rows.data_ptr(), k=rows[:, heads:].data_ptr(), v=rows[:, heads + 2:].data_ptr(), h_inv_freq=freq.ctypes.data,
+                                            q_out=out.data_ptr(), q_stride=rows.stride(0), k_stride=rows.stride(0), v_stride=rows.stride(0), head_stride=d, q_out_stride=out.stride(0), q_out_head_stride=d,
+                                            q_heads=heads, rotary_dim=32, eps=1e-6))
+        done(ctx)
+        results.append(out)
+    assert torch.equal(*results) and not torch.equal(results[0], x)
+
+
+class Step:
+    """A whole step on buffers of its own: embedding rows, norms and rotation, attention."""
+
+    def __init__(self, zkb, seed, kind, rows, cap=300, seqs=3, d=64, hq=8, hk=2):
+        self.zkb, self.g, self.dims = zkb, gen(seed), (seqs, rows, cap, d, hq, hk)
+        self.cache = Cache(self.g, kind, seqs, hk, cap, d, blank=True)
+        self.table = torch.randn(50, (hq + 2 * hk) * d, generator=self.g, device="cuda").bfloat16()
+        n = seqs * rows
+        self.ids, self.first, self.lens = (torch.zeros(x, dtype=torch.int32, device="cuda") for x in (n, seqs + 1, seqs))
+        self.x = torch.zeros(n, hq + 2 * hk, d, device="cuda", dtype=torch.bfloat16)
+        self.q, self.out = (torch.zeros(n, hq, d, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+        self.freq = 1e4 ** (-np.arange(d // 2) / (d // 2))
+        self.weight = torch.randn(d, generator=self.g, device="cuda").bfloat16()
+        rows_ = zkb.StepRows(first=self.first.data_ptr(), kv_len=self.lens.data_ptr(), n_rows=n)
+        c, w, s = self.cache.args(zkb), self.x.stride(0), self.q.stride(0)
+        self.calls = (zkb.StepEmbed(ids=self.ids.data_ptr(), table=self.table.data_ptr(), out=self.x.data_ptr(), table_stride=w, out_stride=w, n_tokens=n, vocab=50, width=w, scale=1.0),
+                      zkb.StepNormRope(cache=c, rows=rows_, q=self.x.data_ptr(), k=self.x[:, hq:].data_ptr(), v=self.x[:, hq + hk:].data_ptr(), q_weight=self.weight.data_ptr(),
+                                       k_weight=self.weight.data_ptr(), h_inv_freq=self.freq.ctypes.data, q_out=self.q.data_ptr(), q_stride=w, k_stride=w, v_stride=w, head_stride=d, q_out_stride=s,
+                                       q_out_head_stride=d, q_heads=hq, rotary_dim=d, eps=1e-6),
+                      zkb.StepAttention(cache=c, rows=rows_, q=self.q.data_ptr(), out=self.out.data_ptr(), q_stride=s, q_head_stride=d, out_stride=s, out_head_stride=d, q_heads=hq, scale=d ** -0.5))
+
+    def batch(self, shape, seed):
+        """Other tokens of another batch into the arrays that the calls read."""
+        self.shape = shape
+        self.ids.copy_(torch.randint(0, 50, self.ids.shape, generator=gen(seed), device="cuda", dtype=torch.int32))
+        self.first.copy_(torch.tensor(np.concatenate([[0], np.cumsum([r for r, _ in shape])]), dtype=torch.int32))
+        self.lens.copy_(torch.tensor([n for _, n in shape], dtype=torch.int32))
+        self.out.fill_(-3)
+        torch.cuda.synchronize()
+
+    def run(self, ctx):
+        ctx.step_embed(self.calls[0])
+        ctx.step_norm_rope(self.calls[1])
+        ctx.step_attention(self.calls[2])
+
+    def check(self):
+        """The attention over what the cache holds now; the cache's new tokens against the table's."""
+        batch = Batch(self.shape)
+        seqs, rows, cap, d, hq, hk = self.dims
+        n = batch.n_rows
+        want, bound = attention_reference(batch, self.cache, self.q[:n], d ** -0.5, 0, 0)
+        assert bool(((self.out[:n].double() - want).abs() <= bound).all()) and bool((self.out[n:] == -3).all())
+        x = self.table[self.ids.long()].view(-1, hq + 2 * hk, d)
+        assert torch.equal(self.x, x)
+        _, v = self.cache.values()
+        for b, at, r, pos in batch.each():
+            step = self.cache.v_scale[b, :, pos:pos + r].double()[..., None] if self.cache.kind == "int8" else 0
+            assert bool(((v[b, :, pos:pos + r].transpose(0, 1) - x[at:at + r, hq + hk:].double()).abs() <= (step.transpose(0, 1) if self.cache.kind == "int8" else 0) * (0.5 + 127 * 2.0 ** -22)).all())
+
+
+SHAPES = {1: [[(1, 5), (1, 300), (1, 77)], [(1, 6), (0, 300), (1, 1)]], 90: [[(90, 90), (1, 250), (90, 300)], [(3, 3), (80, 200), (0, 0)]]}
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+@pytest.mark.parametrize("rows", [1, 90])
+def test_captured_steps_serve_other_batches_side_by_side(ctx, zkb, kind, rows):
+    """Two steps of two contexts captured into graphs, replayed on streams of their own at the same time, for batches that were not there when they were captured;
+    what a replay computes is what the same call computes."""
+    other = zkb.Context(device=0, max_log_size=10)
+    try:
+        steps = [Step(zkb, 1 + i, kind, rows) for i in range(2)]
+        graphs = []
+        for step, c in zip(steps, (ctx, other)):
+            step.batch([(0, 0)] * 3, 0)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=torch.cuda.ExternalStream(c.stream())):
+                step.run(c)
+            graphs.append(graph)
+        streams = [torch.cuda.Stream() for _ in steps]
+        for shape in SHAPES[rows]:
+            for i, step in enumerate(steps):
+                step.batch(shape, 5 + i)
+            for _ in range(3):
+                for graph, stream in zip(graphs, streams):
+                    with torch.cuda.stream(stream):
+                        graph.replay()
+            torch.cuda.synchronize()
+            for step, c in zip(steps, (ctx, other)):
+                step.check()
+                replayed = step.out.clone(), step.cache.k.clone()
+                step.batch(shape, 5 + steps.index(step))
+                step.run(c)
+                done(c)
+                assert torch.equal(step.out, replayed[0]) and torch.equal(step.cache.k, replayed[1])
+        del graphs
+    finally:
+        other.close()
+
+
+@gpu
+def test_contexts_on_threads_of_their_own(zkb):
+    """Steps of four contexts at once, each from a thread of its own: one token a sequence and many."""
+    import threading
+
+    contexts = [zkb.Context(device=0, max_log_size=10) for _ in range(4)]
+    steps, wrong = [Step(zkb, 20 + i, ("bf16", "int8")[i % 2], (1, 90)[i // 2]) for i in range(4)], []
+    for i, s in enumerate(steps):
+        s.batch(SHAPES[s.dims[1]][0], i)
+
+    def work(c, s):
+        try:
+            for _ in range(20):
+                s.run(c)
+            c.sync()
+        except Exception as e:  # noqa: BLE001
+            wrong.append(e)
+
+    threads = [threading.Thread(target=work, args=a) for a in zip(contexts, steps)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+    torch.cuda.synchronize()
+    for s in steps:
+        s.check()
+    for c in contexts:
+        c.close()
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+def test_a_step_between_the_witness_generators(ctx, zkb, oracle, kind):
+    """The run of all calls as a proof makes its values: zkb_witness_dequant leaves a block of tokens' queries, keys and values as words, descending; they are normed, turned
+    and cached; the attention over the cache and the embedding's rows go straight into the leaves of zkb_witness_residual_stream, which adds them. Nothing waits in between."""
+    from zk_inference_prover_b200 import witness_cases as wc
+
+    g, tokens, d, hq, hk, before = gen(4), 32, 32, 4, 2, 40
+    heads, n = hq + 2 * hk, hq * d
+    dq = wc.dequant_case(3, 1, tokens, heads, d, 13, 1, 1)
+    cfg, rows = dq["cfg"], dq["rows"]
+    rs = wc.residual_stream_case(5, "pairs", n, 5, tokens, kind=0, spread=6)
+    up, ml = ctx.upload, rs["m_len"]
+    acc, sx, sw = (ctx.upload_bytes(np.ascontiguousarray(dq[k])) for k in ("acc", "sx", "sw"))
+    norm3, mul2 = up(dq["norm3"].reshape(-1)), up(dq["mul2"].reshape(-1))
+    base, pre = [ctx.alloc(rows).zero() for _ in range(dq["n_base"])], [ctx.alloc(rows).zero() for _ in range(dq["n_pre"])]
+    ms = [ctx.alloc(cfg[k]).zero() for k in ("n_norm", "n_frac", "n_mul", "n_r8")]
+    counts, want = ctx.alloc(4).zero(), ctx.alloc(rows * d).zero()
+    table = torch.randint(-127, 128, (60, n), generator=g, device="cuda", dtype=torch.int8)
+    scales = (0.5 + torch.rand(60, generator=g, device="cuda")) / 50
+    ids = torch.randint(0, 60, (tokens,), generator=g, device="cuda", dtype=torch.int32)
+    batch, cache = Batch([(tokens, before + tokens)]), Cache(g, kind, 1, hk, before + tokens + 5, d)
+    wq, wk = ((1 + 0.3 * torch.randn(d, generator=g, device="cuda")).bfloat16() for _ in range(2))
+    freq = 1e4 ** (-np.arange(d // 2) / (d // 2))
+    q = torch.zeros(tokens, hq, d, device="cuda", dtype=torch.bfloat16)
+    wit = torch.full((tokens, 2 * n), -1, device="cuda", dtype=torch.int32)
+    r_norm, r_smul = up(rs["norm3"]), ctx.upload_bytes(np.ascontiguousarray(rs["smul3"], np.int32))
+    cols = [ctx.alloc(32).zero() for _ in range(rs["n_cols"])]
+    out_pat, out_nat, in_nat = ctx.alloc(32 * n).zero(), ctx.alloc(64 * n).zero(), ctx.alloc(128 * n).zero()
+    r_ms, r_counts = {k: ctx.alloc(ml[k]).zero() for k in ("pow", "norm", "val", "frac", "smul")}, ctx.alloc(4).zero()
+    torch.cuda.synchronize()
+    ctx.witness_dequant(cfg, acc.ptr, 0, 0, sx.ptr, sw.ptr, norm3.ptr, mul2.ptr, [b.ptr for b in base], [p.ptr for p in pre], *[m.ptr for m in ms], counts.ptr, want.ptr)
+    at = lambda h: want.ptr + 4 * d * ((tokens - 1) * heads + heads - 1 - h)  # noqa: E731  head h of token 0
+    ctx.step_norm_rope(zkb.StepNormRope(cache=cache.args(zkb), rows=batch.args(zkb), q=at(0), k=at(hq), v=at(hq + hk), q_weight=wq.data_ptr(), k_weight=wk.data_ptr(), h_inv_freq=freq.ctypes.data,
+                                        q_out=q.data_ptr(), q_stride=-heads * d, k_stride=-heads * d, v_stride=-heads * d, head_stride=-d, q_out_stride=n, q_out_head_stride=d, type=zkb.VALUE_WORD,
+                                        q_heads=hq, rotary_dim=d, eps=1e-6))
+    ctx.step_embed(zkb.StepEmbed(ids=ids.data_ptr(), table=table.data_ptr(), row_scale=scales.data_ptr(), out=wit.data_ptr(), table_stride=n, out_stride=2 * n, n_tokens=tokens, vocab=60, width=n,
+                                 table_type=zkb.VALUE_INT8, out_type=zkb.VALUE_WORD, scale=1.0))
+    ctx.step_attention(zkb.StepAttention(cache=cache.args(zkb), rows=batch.args(zkb), q=q.data_ptr(), out=wit.data_ptr() + 4 * n, q_stride=n, q_head_stride=d, out_stride=2 * n, out_head_stride=d,
+                                         q_heads=hq, out_type=zkb.VALUE_WORD, scale=d ** -0.5))
+    ctx.witness_residual_stream(rs["lowered_groups"], rs["lowered_slots"], rs["out_slot"], rs["kind"], rs["sticky"], rs["kmax"], r_norm.ptr, len(rs["norm3"]) // 3, r_smul.ptr, len(rs["smul3"]) // 3, [],
+                                rs["n_val"], wit.data_ptr(), tokens, 5, [c.ptr for c in cols], out_pat.ptr, out_nat.ptr, in_nat.ptr, {k: (v.ptr, ml[k]) for k, v in r_ms.items()}, [], r_counts.ptr)
+    done(ctx)
+    o = oracle.witness_dequant(dq["acc"], dq["jx"], dq["jw"], dq["sx"], dq["sw"], dq["norm3"], dq["mul2"], dq["n_base"], dq["n_pre"], cfg)
+    given = want.download()[:rows * d]
+    assert np.array_equal(given, np.asarray(o["want"]).reshape(-1))
+    x = torch.from_numpy(given.astype(np.int32)).cuda().view(tokens, heads, d).flip(0, 1)
+    x = (x << 16).view(torch.float32)
+    y, size = rope_reference(batch, x[:, :hq + hk], [wq] * hq + [wk] * hk, 1e-6, freq, 0)
+    assert bool(((q.double() - y[:, :hq]).abs() <= 2.0 ** -8 * y[:, :hq].abs() + 2.0 ** -18 * size[:, :hq]).all())
+    k, v = cache.values()
+    for got, ref, s, scale in ((k, y[:, hq:], size[:, hq:], cache.k_scale), (v, x[:, hq + hk:].double(), 0 * x[:, hq + hk:].double(), cache.v_scale)):
+        diff = (got[0, :, before:before + tokens].transpose(0, 1) - ref).abs()
+        if kind == "bf16":
+            assert bool((diff <= 2.0 ** -8 * ref.abs() + 2.0 ** -18 * s).all())
+        else:
+            assert bool((diff <= scale[0, :, before:before + tokens].T.double()[..., None] * (0.5 + 127 * 2.0 ** -22) + 2.0 ** -18 * s.amax(-1, keepdim=True)).all())
+    assert torch.equal(wit[:, :n], words((table[ids.long()].float() * scales[ids.long()][:, None]).bfloat16()))
+    ref, bound = attention_reference(batch, cache, q, d ** -0.5, 0, 0)
+    assert bool(((values_of(wit[:, n:].reshape(tokens, hq, d)) - ref).abs() <= bound).all())
+    summed = oracle.witness_residual_stream({**rs, "wit": wit.cpu().numpy().astype(np.uint32).reshape(-1)})
+    assert np.array_equal(out_pat.download()[:32 * n], summed["out_pat"])

@@ -182,7 +182,7 @@ struct StepSequence {
 };
 __device__ __forceinline__ StepSequence step_sequence(const zkb_step_rows& r, int seq) {
     const int from = r.first[seq], to = r.first[seq + 1], n = (int)r.n_rows;
-    const int first = min(max(from, 0), n), rows = max(0, min(to, n) - first);
+    const int first = min(max(from, 0), n), rows = max(min(to, n), first) - first;
     return {first, rows, (int64_t)r.kv_len[seq] - ((int64_t)to - from) + (first - (int64_t)from)};
 }
 

@@ -294,7 +294,7 @@ int zkb_step_embed(zkb_ctx* ctx, const zkb_step_embed_args* args) {
     const bool int8 = a.table_type == ZKB_VALUE_INT8, word = a.out_type == ZKB_VALUE_WORD;
     const size_t in_size = int8 ? 1 : 2, out_size = word ? 4 : 2;
     ZKB_CHECK_ARG(ctx, a.ids && a.out && (a.vocab == 0 || a.table) && (int8 ? (a.vocab == 0 || a.row_scale) : !a.row_scale));
-    ZKB_CHECK_ARG(ctx, aligned_to(a.table, in_size) && aligned_to(a.out, out_size));
+    ZKB_CHECK_ARG(ctx, aligned_to(a.table, in_size) && aligned_to(a.out, out_size) && aligned_to(a.ids, 4) && aligned_to(a.row_scale, 4) && aligned_to(a.off_table, 8));
     ZKB_CHECK_ARG(ctx, a.segment == 0 || a.segment >= a.width || std::llabs(a.segment_stride) >= (long long)a.segment);
     ZKB_CHECK_ARG(ctx, a.n_tokens == 1 || std::llabs(a.out_stride) >= (long long)(a.segment && a.segment < a.width ? a.segment : a.width));
     DeviceGuard g(ctx);

@@ -67,6 +67,7 @@ inline const char* step_problem(const zkb_kv_cache& c, const zkb_step_rows& r, u
     if (c.capacity > 1 && std::llabs(c.token_stride) < (long long)c.head_dim) return "cache.token_stride is shorter than a row";
     if (std::llabs(c.token_stride) > (1ll << 29)) return "cache.token_stride exceeds 2^29";
     if (!r.first || !r.kv_len) return "rows.first or rows.kv_len is NULL";
+    if (!aligned_to(r.first, 4) || !aligned_to(r.kv_len, 4)) return "rows.first or rows.kv_len is not on a 4-byte boundary";
     if (r.n_rows > (1u << 30)) return "rows.n_rows exceeds 2^30";
     if (q_heads < 1 || q_heads % c.n_heads != 0 || q_heads / c.n_heads > 64) return "q_heads is not 1 to 64 times cache.n_heads";
     return nullptr;
