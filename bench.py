@@ -1348,6 +1348,64 @@ def run_witness(args, rank):
     ctx.close()
 
 
+def run_step_values(args, rank):
+    """--mode step-values: the values that a layer segment's witness is made from, as the library makes them on the device: 32 tokens at the end of 2,048 (a row of
+    4,096 of an 8-bit embedding table each, 32 query heads and 8 key-value heads of 128, norms, rotation, an 8-bit cache), read from words in the order in which the dequantize
+    generator leaves them and written as words. Each call is timed by itself, with the 126 MB L2 overwritten before it, and the three together as they follow one another."""
+    if rank != 0:
+        return
+    import zk_inference_prover_b200 as z
+
+    peak, peak_kind = measured_hbm_peak()
+    ctx, rng = z.Context(device=0, max_log_size=10), np.random.default_rng(5)
+    tokens, length, hq, hk, d, width, vocab, cap = 32, 2048, 32, 8, 128, 4096, 32000, 4096
+    heads = hq + 2 * hk
+    raw = lambda a: ctx.upload_bytes(np.ascontiguousarray(a))  # noqa: E731
+    pattern = lambda *shape: (rng.standard_normal(shape).astype(np.float32).view(np.uint32) >> 16).astype(np.uint32)  # noqa: E731
+    codes = lambda n: raw(rng.integers(-127, 128, n, dtype=np.int8))  # noqa: E731
+    k, v, table = codes(hk * cap * d), codes(hk * cap * d), codes(vocab * width)
+    scales = lambda n: raw(((0.5 + rng.random(n)) / 64).astype(np.float32))  # noqa: E731
+    k_scale, v_scale, row_scale = scales(hk * cap), scales(hk * cap), scales(vocab)
+    ids, first, lens = (raw(np.asarray(x, np.int32)) for x in (rng.integers(0, vocab, tokens), [0, tokens], [length]))
+    qkv, q = ctx.upload(pattern(tokens * heads * d)), ctx.alloc(tokens * hq * d // 2)
+    weight = raw(((1 + 0.1 * rng.standard_normal(d)).astype(np.float32).view(np.uint32) >> 16).astype(np.uint16))
+    wit, flush = ctx.alloc(tokens * 2 * width).zero(), ctx.alloc(48 << 20)
+    freq = 500000.0 ** (-np.arange(d // 2) / (d // 2))
+    cache = z.KvCache(k=k.ptr, v=v.ptr, k_scale=k_scale.ptr, v_scale=v_scale.ptr, seq_stride=hk * cap * d, head_stride=cap * d, token_stride=d, scale_seq_stride=hk * cap, scale_head_stride=cap,
+                      type=z.VALUE_INT8, n_seqs=1, n_heads=hk, head_dim=d, capacity=cap)
+    rows = z.StepRows(first=first.ptr, kv_len=lens.ptr, n_rows=tokens, max_rows=tokens, max_len=length)
+    at = lambda h: qkv.ptr + 4 * d * (tokens * heads - 1 - h)  # noqa: E731  token 0, head h: both descend
+    embed = z.StepEmbed(ids=ids.ptr, table=table.ptr, row_scale=row_scale.ptr, out=wit.ptr, table_stride=width, out_stride=2 * width, n_tokens=tokens, vocab=vocab, width=width,
+                        table_type=z.VALUE_INT8, out_type=z.VALUE_WORD, scale=1.0)
+    rope = z.StepNormRope(cache=cache, rows=rows, q=at(0), k=at(hq), v=at(hq + hk), q_weight=weight.ptr, k_weight=weight.ptr, h_inv_freq=freq.ctypes.data, q_out=q.ptr, q_stride=-heads * d,
+                          k_stride=-heads * d, v_stride=-heads * d, head_stride=-d, q_out_stride=hq * d, q_out_head_stride=d, type=z.VALUE_WORD, q_heads=hq, rotary_dim=d, eps=1e-6)
+    attend = z.StepAttention(cache=cache, rows=rows, q=q.ptr, out=wit.ptr + 4 * width, q_stride=hq * d, q_head_stride=d, out_stride=2 * width, out_head_stride=d, q_heads=hq,
+                             out_type=z.VALUE_WORD, scale=d ** -0.5)
+    calls = [lambda: ctx.step_embed(embed), lambda: ctx.step_norm_rope(rope), lambda: ctx.step_attention(attend)]
+    times = [[], [], [], []]
+    for it in range(args.warmup + args.steps):
+        for i in range(4):
+            flush.zero()
+            ctx.sync()
+            ctx.event_record(0)
+            for call in calls if i == 3 else [calls[i]]:
+                call()
+            ctx.event_record(1)
+            ctx.sync()
+            if it >= args.warmup:
+                times[i].append(ctx.event_elapsed_ms(0, 1))
+    embed_ms, rope_ms, attend_ms, step_ms = (float(np.median(x)) for x in times)
+    n_bytes = [tokens * width * 5, tokens * (heads * d * 4 + hq * d * 2 + 2 * hk * (d + 4)), hk * length * (2 * d + 8) + tokens * hq * d * 6]
+    part = lambda ms, by: {"us": ms * 1e3, "algorithmic_bytes": by, "gbs": by / ms / 1e6}  # noqa: E731
+    print(json.dumps({
+        "metric": "step_values_tokens_per_s", "value": tokens / (step_ms * 1e-3), "unit": "tokens/s (one layer)", "n_gpus": 1, "steps": args.steps, "warmup": args.warmup, "ms_per_step": step_ms,
+        "higher_is_better": True, "dtype": "bf16 words, int8 cache", "data": "synthetic",
+        "config": {"workload": "32 tokens at 2048, 32 + 2 x 8 heads of 128, rows of 4096; L2 overwritten before each timed region"},
+        "embed": part(embed_ms, n_bytes[0]), "norm_rope": part(rope_ms, n_bytes[1]), "attention": part(attend_ms, n_bytes[2]), "peak_gbs": peak, "peak_kind": peak_kind,
+        "gpu_launches": 3 * args.steps}))
+    ctx.close()
+
+
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--gpus", type=int, default=1)
@@ -1366,7 +1424,7 @@ def main():
     ap.add_argument("--gkr-log", type=int, default=24)
     ap.add_argument("--streams", type=int, default=1, help="decode-step: proofs side by side on one GPU (host threads, one context each)")
     ap.add_argument("--segment", default="layer_8b_s32_c2048", help="segment-replay: a key of tests/golden/segment_shapes.json")
-    ap.add_argument("--mode", default="proof", choices=["proof", "sharded-commit", "gkr", "freivalds", "constraints", "stark", "segment-replay", "decode-step", "witness"],
+    ap.add_argument("--mode", default="proof", choices=["proof", "sharded-commit", "gkr", "freivalds", "constraints", "stark", "segment-replay", "decode-step", "witness", "step-values"],
                     help="proof: one whole PCS proof per rank (ranks are independent); sharded-commit: one commitment over all ranks")
     args = ap.parse_args()
     rank = int(os.environ.get("RANK", "0"))
@@ -1388,6 +1446,8 @@ def main():
         run_segment_replay(args, rank)
     elif args.mode == "witness":
         run_witness(args, rank)
+    elif args.mode == "step-values":
+        run_step_values(args, rank)
     elif args.mode == "decode-step":
         run_decode_step(args, rank, world, local_rank)
     else:

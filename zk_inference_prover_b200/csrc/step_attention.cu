@@ -256,7 +256,15 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, Few<D, INT8>::THREAD_BLOCKS)
                 sum[i & 1] += w;
                 sc[i] = INT8 ? (sc[i] == -INFINITY ? 0.f : w * (i < 2 ? v0 : v1)) : w;  // a hidden token's scale may be anything
             }
-            const uint32_t w0 = transpose8(pack_bf16(sc[0], sc[1])), w1 = transpose8(pack_bf16(sc[2], sc[3]));
+            // A weight is two bf16 numbers, its rounding and what that leaves: off by 2^-16 where the result's own rounding takes 2^-8. (One number alone: 64 sequences of 8,192
+            // int8 tokens in 164 us instead of 174, bf16 240 instead of 243, and results up to 1.6 times as far off.)
+            const uint32_t high[2] = {pack_bf16(sc[0], sc[1]), pack_bf16(sc[2], sc[3])};
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                sc[i] -= i & 1 ? bf16_high(high[i >> 1]) : bf16_low(high[i >> 1]);
+                if (INT8) sc[i] = sc[i] == sc[i] ? sc[i] : 0.f;  // an infinity leaves nothing
+            }
+            const uint32_t w0 = transpose8(high[0]), w1 = transpose8(high[1]), left0 = transpose8(pack_bf16(sc[0], sc[1])), left1 = transpose8(pack_bf16(sc[2], sc[3]));
             uint32_t vw[4][F::VW];
 #pragma unroll
             for (int i = 0; i < 4; i++)
@@ -294,6 +302,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, Few<D, INT8>::THREAD_BLOCKS)
                     f[2] = __byte_perm(vw[2][i], vw[3][i], 0x5410), f[3] = __byte_perm(vw[2][i], vw[3][i], 0x7632);
                 }
                 mma_bf16(o[i], f, w0, w1);
+                mma_bf16(o[i], f, left0, left1);
             }
             __syncwarp();  // all lanes have read the block that the next copies go to
         }
