@@ -235,37 +235,34 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
             const bool live = m < n.n_m;
             const uint16_t* from = q_of(n, live ? m : 0);
             const bool vec = aligned16(from);
-            auto eight = [&](int at) {
-                uint4 x = make_uint4(0u, 0u, 0u, 0u);
-                if (live && vec) x = *reinterpret_cast<const uint4*>(from + at);
-                else if (live)
-                    x = make_uint4((uint32_t)from[at] | (uint32_t)from[at + 1] << 16, (uint32_t)from[at + 2] | (uint32_t)from[at + 3] << 16, (uint32_t)from[at + 4] | (uint32_t)from[at + 5] << 16,
-                                   (uint32_t)from[at + 6] | (uint32_t)from[at + 7] << 16);
-                return x;
-            };
+            uint4 x[D / 8];  // all loads on their way at once
+#pragma unroll
+            for (int i = 0; i < D / 8; i++) {
+                x[i] = make_uint4(0u, 0u, 0u, 0u);
+                const uint16_t* const p = from + 8 * i;
+                if (live && vec) x[i] = *reinterpret_cast<const uint4*>(p);
+                else if (live) x[i] = make_uint4((uint32_t)p[0] | (uint32_t)p[1] << 16, (uint32_t)p[2] | (uint32_t)p[3] << 16, (uint32_t)p[4] | (uint32_t)p[5] << 16, (uint32_t)p[6] | (uint32_t)p[7] << 16);
+            }
             float f = 1.f, left = by;
             if constexpr (INT8) {
                 float most = 0.f;
-#pragma unroll 8
-                for (int i = 0; i < D; i += 8) {
-                    const uint4 x = eight(i);
-                    for (uint32_t w : {x.x, x.y, x.z, x.w}) most = fmaxf(most, fmaxf(fabsf(bf16_low(w)), fabsf(bf16_high(w))));
-                }
+#pragma unroll
+                for (int i = 0; i < D / 8; i++)
+                    for (uint32_t w : {x[i].x, x[i].y, x[i].z, x[i].w}) most = fmaxf(most, fmaxf(fabsf(bf16_low(w)), fabsf(bf16_high(w))));
                 const int e = (int)(__float_as_uint(most) >> 23), up = e == 0 || e == 255 ? 0 : min(13 + 127 - e, 126);
                 f = __uint_as_float((uint32_t)(up + 127) << 23);
                 left = fmaxf(ldexpf(by, -up), 1.2e-38f);
             }
             const uint32_t turn = a.scale < 0.f ? 0x80008000u : 0u;
             auto word = [&](uint32_t w) { return (INT8 ? pack_f16(bf16_low(w) * f, bf16_high(w) * f) : w) ^ turn; };
-#pragma unroll 8
-            for (int i = 0; i < D; i += 8) {
-                const uint4 x = eight(i);
-                st_shared4(q_at + tile * M::TILE + tile_place<D, INT8>(row, i * 2), word(x.x), word(x.y), word(x.z), word(x.w));
-            }
+#pragma unroll
+            for (int i = 0; i < D / 8; i++)
+                st_shared4(q_at + tile * M::TILE + tile_place<D, INT8>(row, i * 16), word(x[i].x), word(x[i].y), word(x[i].z), word(x[i].w));
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             mbar_arrive(bar_of(bars.q_ready));
             return left;
         };
+        auto sums_place = [](int row, int four) { return (row * (D / 4) + (four ^ (row & 7))) * 16; };
         float by_row = more ? load_q(u) : 0.f;
         while (more) {
             const int m = row_of(u);  // this thread's row
@@ -426,7 +423,8 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
                     }
                 }
             } else {
-                // Each thread block finishes `part` of the rows: their sums go to [whose][four dimensions][row] of its shared memory, where Q and the keys were.
+                // Each thread block finishes `part` of the rows: their sums go to [whose][row][four dimensions] of its shared memory, where Q and the keys were
+                // (turned by the row's number, so that a warp's stores, a row a lane, and loads, a row after the other, each meet all banks).
                 meet();
                 const int odd = odd_values();
                 const int rows_here = u.two ? 256 : 128, part = rows_here / units.ranks, one = u.split ? row : tile * 128 + row;
@@ -442,13 +440,13 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
                         if (any) tmem_load8(o_at + i, o), tmem_loaded(o);
 #pragma unroll
                         for (int y = 0; y < 8; y += 4)
-                            peer_store4(q_at + ((whose * (D / 4) + (i + y) / 4) * part + at) * 16, owner, any ? o[y] : 0u, any ? o[y + 1] : 0u, any ? o[y + 2] : 0u, any ? o[y + 3] : 0u);
+                            peer_store4(q_at + sums_place(whose * part + at, (i + y) / 4), owner, any ? o[y] : 0u, any ? o[y + 1] : 0u, any ? o[y + 2] : 0u, any ? o[y + 3] : 0u);
                     }
                 }
                 meet();
 #pragma unroll 1
                 for (int i = threadIdx.x; i < part * (D / 4); i += 256) {
-                    const int at = i % part, d = i / part * 4;
+                    const int at = i / (D / 4), d = i % (D / 4) * 4;
                     const int mm = u.m0 + units.rank * part + at;
                     if (mm >= u.n_m) continue;
                     float most = -INFINITY, all = 0.f, z[4] = {0.f, 0.f, 0.f, 0.f};
@@ -459,7 +457,7 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
 #pragma unroll 4
                     for (int x = 0; x < of; x++) {
                         const float f = exp2_fast(in_top[x * part + at] - least);
-                        const float4 o = *reinterpret_cast<const float4*>(sm + ((x * (D / 4) + d / 4) * part + at) * 16);
+                        const float4 o = *reinterpret_cast<const float4*>(sm + sums_place(x * part + at, d / 4));
                         z[0] += o.x * f, z[1] += o.y * f, z[2] += o.z * f, z[3] += o.w * f;
                         all += in_sum[x * part + at] * f;
                     }
@@ -467,12 +465,25 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
                         for (int x = 0; x < units.ranks; x++) set_aside |= in_odd[x];
                     const int i0 = (int)((uint32_t)mm / (uint32_t)group);
                     const int64_t to = (u.s.first + i0) * a.out_stride + (u.kv_head * group + mm - i0 * group) * a.out_head_stride + d;
+                    const float inverse = all == 0.f ? 0.f : 1.f / all;
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        z[e] = all == 0.f ? 0.f : z[e] / all;
+                        z[e] = all == 0.f ? 0.f : z[e] * inverse;
                         if (set_aside) z[e] += what_is_no_number(v, row_bytes, d + e, u.s.pos + i0, c.capacity, a.window, a.sinks);
-                        if (a.out_type == ZKB_VALUE_WORD) static_cast<uint32_t*>(a.out)[to + e] = round_bf16(z[e]);
-                        else static_cast<uint16_t*>(a.out)[to + e] = round_bf16(z[e]);
+                    }
+                    const bool word = a.out_type == ZKB_VALUE_WORD;
+                    char* const out = static_cast<char*>(a.out) + to * (word ? 4 : 2);
+                    const uint32_t w0 = pack_bf16(z[0], z[1]), w1 = pack_bf16(z[2], z[3]);
+                    if (((uintptr_t)out & (word ? 15 : 7)) == 0) {
+                        if (word) *reinterpret_cast<uint4*>(out) = make_uint4(w0 & 0xffffu, w0 >> 16, w1 & 0xffffu, w1 >> 16);
+                        else *reinterpret_cast<uint2*>(out) = make_uint2(w0, w1);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const uint32_t h = (e < 2 ? w0 : w1) >> 16 * (e & 1) & 0xffffu;
+                            if (word) reinterpret_cast<uint32_t*>(out)[e] = h;
+                            else reinterpret_cast<uint16_t*>(out)[e] = (uint16_t)h;
+                        }
                     }
                 }
                 if (again) {
