@@ -435,40 +435,51 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
                     peer_store(&in_sum[whose * part + at], owner, sum);
                     if (at == 0 && !(u.split && tile)) peer_store(&in_odd[units.rank], owner, odd);
 #pragma unroll 1
-                    for (int i = 0; i < D; i += 8) {
-                        uint32_t o[8];
-                        if (any) tmem_load8(o_at + i, o), tmem_loaded(o);
+                    for (int i = 0; i < D; i += 32) {
+                        uint32_t o[32];
+                        if (any) tmem_load32(o_at + i, o), tmem_loaded(o);
 #pragma unroll
-                        for (int y = 0; y < 8; y += 4)
+                        for (int y = 0; y < 32; y += 4)
                             peer_store4(q_at + sums_place(whose * part + at, (i + y) / 4), owner, any ? o[y] : 0u, any ? o[y + 1] : 0u, any ? o[y + 2] : 0u, any ? o[y + 3] : 0u);
                     }
                 }
                 meet();
-#pragma unroll 1
-                for (int i = threadIdx.x; i < part * (D / 4); i += 256) {
-                    const int at = i / (D / 4), d = i % (D / 4) * 4;
-                    const int mm = u.m0 + units.rank * part + at;
-                    if (mm >= u.n_m) continue;
-                    float most = -INFINITY, all = 0.f, z[4] = {0.f, 0.f, 0.f, 0.f};
-                    int set_aside = 0;
+                int set_aside = 0;
+                if (!INT8)
+                    for (int x = 0; x < units.ranks; x++) set_aside |= in_odd[x];
+                if ((int)threadIdx.x < part) {  // a row's factors, its sum among them, where its maxima were
+                    const int at = threadIdx.x;
+                    float most = -INFINITY, all = 0.f;
 #pragma unroll 4
                     for (int x = 0; x < of; x++) most = fmaxf(most, in_top[x * part + at]);
                     const float least = most == -INFINITY ? 0.f : most;
 #pragma unroll 4
                     for (int x = 0; x < of; x++) {
                         const float f = exp2_fast(in_top[x * part + at] - least);
+                        all += in_sum[x * part + at] * f;
+                        in_top[x * part + at] = f;
+                    }
+                    in_sum[at] = all == 0.f ? 0.f : 1.f / all;  // (this thread alone has read that place)
+                }
+                named_sync(4, 256);
+#pragma unroll 1
+                for (int i = threadIdx.x; i < part * (D / 4); i += 256) {
+                    const int at = i / (D / 4), d = i % (D / 4) * 4;
+                    const int mm = u.m0 + units.rank * part + at;
+                    if (mm >= u.n_m) continue;
+                    float z[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+                    for (int x = 0; x < of; x++) {
+                        const float f = in_top[x * part + at];
                         const float4 o = *reinterpret_cast<const float4*>(sm + sums_place(x * part + at, d / 4));
                         z[0] += o.x * f, z[1] += o.y * f, z[2] += o.z * f, z[3] += o.w * f;
-                        all += in_sum[x * part + at] * f;
                     }
-                    if (!INT8)
-                        for (int x = 0; x < units.ranks; x++) set_aside |= in_odd[x];
+                    const float inverse = in_sum[at];
                     const int i0 = (int)((uint32_t)mm / (uint32_t)group);
                     const int64_t to = (u.s.first + i0) * a.out_stride + (u.kv_head * group + mm - i0 * group) * a.out_head_stride + d;
-                    const float inverse = all == 0.f ? 0.f : 1.f / all;
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        z[e] = all == 0.f ? 0.f : z[e] * inverse;
+                        z[e] = inverse == 0.f ? 0.f : z[e] * inverse;
                         if (set_aside) z[e] += what_is_no_number(v, row_bytes, d + e, u.s.pos + i0, c.capacity, a.window, a.sinks);
                     }
                     const bool word = a.out_type == ZKB_VALUE_WORD;
