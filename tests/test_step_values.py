@@ -293,6 +293,21 @@ def test_attention(ctx, zkb, shape, hq, hk, d, kind, out, window, sinks, order, 
 
 @gpu
 @pytest.mark.parametrize("kind", ["bf16", "int8"])
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("order,pad", [("shtd", 0), ("tshd", 0), ("hstd", 3)])
+@pytest.mark.parametrize("shape,hq,hk,window,sinks", [([(129, 400), (40, 390), (0, 3), (1, 60), (86, 86)], 24, 8, 0, 0), ([(129, 400), (40, 390), (0, 3), (1, 60), (86, 86)], 24, 8, 33, 5),
+                                                      ([(100, 700), (90, 600)], 32, 4, 0, 0), ([(100, 700), (90, 600)], 32, 4, 300, 2)])
+def test_attention_of_many_rows(ctx, zkb, kind, d, order, pad, shape, hq, hk, window, sinks):
+    """Batches whose rows fill the large products, with and without their keys spread over thread blocks, in caches that can be copied by tiles and in one that cannot."""
+    g = gen(d + window)
+    batch = Batch(shape, behind=1, gap=1)
+    cache = Cache(g, kind, len(shape), hk, max(n for _, n in shape) + 1, d, order, pad)
+    q = torch.randn(batch.n_rows, hq, d, generator=g, device="cuda").bfloat16()
+    check_attention(ctx, zkb, batch, cache, q, "bf16" if window else "words", window, sinks)
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
 @pytest.mark.parametrize("rows", [1, 3, 40, 200])
 def test_attention_rows_before_the_cache_and_behind_it(ctx, zkb, kind, rows):
     """More rows than tokens: the first rows see nothing and get zeros; lengths past the capacity: what is there is seen."""

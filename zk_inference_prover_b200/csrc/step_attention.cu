@@ -430,13 +430,14 @@ static cudaError_t launch_few(zkb_ctx* ctx, const zkb_step_attention_args& a) {
 template <int D>
 static cudaError_t launch_attention(zkb_ctx* ctx, const zkb_step_attention_args& a) {
     const zkb_kv_cache& c = a.cache;
-    // Eight rows a product or 128. The first kernel takes some 9 us and 0.052 ns for each eight rows, kv head and key, the second some 20 us and 0.2 ns (bf16 caches: 0.12) for each 256: one sequence of
-    // 2,048 tokens and eight kv heads against 12 rows a head 14.6 us and 25, against 128 rows 23 and 27, 16 sequences against 32 rows 63 and 76, 64 rows of 8,192 tokens (256 a head) 12,000 and 1,300.
-    const uint64_t rows = (uint64_t)(a.rows.max_rows ? std::min(a.rows.max_rows, a.rows.n_rows) : a.rows.n_rows) * (a.q_heads / c.n_heads);
-    uint64_t len = a.rows.max_len ? std::min(a.rows.max_len, c.capacity) : c.capacity;
-    if (a.window) len = std::min<uint64_t>(len, (uint64_t)a.window + a.sinks + rows);
-    const double keys = (double)c.n_seqs * c.n_heads * (double)len;
-    const bool few = (0.052 * (double)((rows + 7) / 8) - (c.type == ZKB_VALUE_INT8 ? 0.2 : 0.12) * (double)((rows + 255) / 256)) * keys < 11000.;
+    // Eight rows a product or 128, by what each was measured to take: the first kernel 30 ns for each eight rows of a kv head and 0.04 ns for each key that they are shown, the second, which starts
+    // some 12 us later, 0.2 ns (bf16 caches: 0.12) a key for each 256. Eight kv heads of 128, one sequence of 1,032 int8 tokens against 32 rows a head: 12.6 us and 25.5, of 8,032 against 128
+    // rows: 60 and 46; 16 sequences of 32 bf16 tokens against 128 rows: 79 and 13; one of 8,064 int8 tokens, a window of 1,024, against 256 rows: 24 and 31.
+    const uint32_t group = a.q_heads / c.n_heads;
+    const uint64_t rows = (uint64_t)(a.rows.max_rows ? std::min(a.rows.max_rows, a.rows.n_rows) : a.rows.n_rows) * group, len = a.rows.max_len ? std::min(a.rows.max_len, c.capacity) : c.capacity;
+    auto shown = [&](uint32_t tile, uint32_t block) { return a.window ? (double)std::min<uint64_t>(len, (uint64_t)a.window + a.sinks + tile / group + block) : (double)len; };
+    const double of_8 = 0.04 * shown(8, 16) + 30., of_256 = (c.type == ZKB_VALUE_INT8 ? 0.2 : 0.12) * shown(256, 128);
+    const bool few = ((double)((rows + 7) / 8) * of_8 - (double)((rows + 255) / 256) * of_256) * c.n_seqs * c.n_heads < 12000.;
     return c.type == ZKB_VALUE_INT8 ? (few ? launch_few<D, true>(ctx, a) : launch_many<D, true>(ctx, a)) : (few ? launch_few<D, false>(ctx, a) : launch_many<D, false>(ctx, a));
 }
 
