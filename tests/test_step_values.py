@@ -374,6 +374,54 @@ def test_attention_of_many_units(ctx, zkb, kind, rows, length, d, window, sinks)
 
 @gpu
 @pytest.mark.parametrize("kind", ["bf16", "int8"])
+@pytest.mark.parametrize("most,length", [(30, 120), (30, 250), (120, 250), (1, 2)])
+def test_attention_of_many_short_sequences(ctx, zkb, kind, most, length):
+    """Several sequences a thread block, of one tile or two and of one block of keys or two; some without rows, some without tokens."""
+    g, rng = gen(most + length), np.random.default_rng(most)
+    shape = [(int(r), int(n)) for r, n in zip(rng.integers(0, most + 1, 300), rng.integers(0, length + 1, 300))] + [(most, length)]
+    batch, cache = Batch(shape, behind=1), Cache(g, kind, len(shape), 4, length, 64)
+    q = torch.randn(batch.n_rows, 16, 64, generator=g, device="cuda").bfloat16()
+    check_attention(ctx, zkb, batch, cache, q, "words", 0, 0)
+
+
+@gpu
+def test_attention_values_that_are_no_numbers_in_a_long_cache(ctx, zkb):
+    """Every row sees an infinity among 30,000 tokens, so that all outputs go the slow way, for longer than a wait within the kernel may take without a reason."""
+    g, rows, length, heads, d = gen(8), 300, 30000, 40, 128
+    batch, cache = Batch([(rows, length)]), Cache(g, "bf16", 1, heads, length, d)
+    cache.v[0, :, 11, 3::7] = math.inf
+    cache.v[0, :, length - rows, 4::7] = -math.inf
+    q = torch.randn(rows, heads, d, generator=g, device="cuda").bfloat16()
+    check_attention(ctx, zkb, batch, cache, q, "bf16", 0, 0)
+
+
+@gpu
+def test_as_many_sequences_as_there_may_be(ctx, zkb):
+    """65,535 sequences of a token: written, and seen, each by its own row."""
+    g, seqs, d, cap = gen(6), 65535, 32, 3
+    pos = torch.arange(seqs, device="cuda") % cap
+    first, lens = torch.arange(seqs + 1, device="cuda", dtype=torch.int32), (pos + 1).int()
+    k, v = (torch.randn(seqs, 1, cap, d, generator=g, device="cuda").bfloat16() for _ in range(2))
+    x = torch.randn(seqs, 3, d, generator=g, device="cuda").bfloat16()
+    q, out = x[:, :1].clone(), torch.zeros(seqs, 1, d, device="cuda", dtype=torch.bfloat16)
+    cache = zkb.KvCache(k=k.data_ptr(), v=v.data_ptr(), type=zkb.VALUE_BF16, n_seqs=seqs, n_heads=1, head_dim=d, capacity=cap, seq_stride=cap * d, head_stride=cap * d, token_stride=d)
+    rows = zkb.StepRows(first=first.data_ptr(), kv_len=lens.data_ptr(), n_rows=seqs, max_rows=1, max_len=cap)
+    torch.cuda.synchronize()
+    ctx.step_norm_rope(zkb.StepNormRope(cache=cache, rows=rows, q=x.data_ptr(), k=x[:, 1:].data_ptr(), v=x[:, 2:].data_ptr(), q_out=q.data_ptr(), q_stride=3 * d, k_stride=3 * d, v_stride=3 * d,
+                                        head_stride=d, q_out_stride=d, q_out_head_stride=d, q_heads=1, rotary_dim=0, eps=1e-6))
+    ctx.step_attention(zkb.StepAttention(cache=cache, rows=rows, q=q.data_ptr(), out=out.data_ptr(), q_stride=d, q_head_stride=d, out_stride=d, out_head_stride=d, q_heads=1, scale=0.2))
+    done(ctx)
+    each = torch.arange(seqs, device="cuda")
+    assert torch.equal(q, x[:, :1]) and torch.equal(k[each, 0, pos], x[:, 1]) and torch.equal(v[each, 0, pos], x[:, 2])
+    s = torch.einsum("sd,std->st", q[:, 0].double(), k[:, 0].double()) * 0.2
+    w = torch.softmax(s.masked_fill(torch.arange(cap, device="cuda") > pos[:, None], -math.inf), -1)
+    want, size = (torch.einsum("st,std->sd", w, y) for y in (v[:, 0].double(), v[:, 0].double().abs()))
+    # as attention_reference counts: weights off by 2^-8 and scores by 36 roundings of 2^-24 of magnitudes below 64, the result's own 2^-8
+    assert bool(((out[:, 0].double() - want).abs() <= (2.0 ** -8 + 2.0 ** -11) * (size + want.abs())).all())
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
 @pytest.mark.parametrize("max_rows,max_len", [(1, 1), (0, 1), (1, 0), (1 << 31, 1 << 31), (7, 900)])
 def test_attention_hints_that_are_wrong_change_no_result(ctx, zkb, kind, max_rows, max_len):
     """Fewer rows and tokens than there are, and more; both ways of laying out the work meet them."""

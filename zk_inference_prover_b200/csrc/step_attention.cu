@@ -432,13 +432,14 @@ static cudaError_t launch_few(zkb_ctx* ctx, const zkb_step_attention_args& a) {
 template <int D>
 static cudaError_t launch_attention(zkb_ctx* ctx, const zkb_step_attention_args& a) {
     const zkb_kv_cache& c = a.cache;
-    // Eight rows a product or 128, by what each was measured to take: the first kernel 30 ns for each eight rows of a kv head and 0.04 ns for each key that they are shown, the second, which starts
-    // some 12 us later, 0.2 ns (bf16 caches: 0.12) a key for each 256. Eight kv heads of 128, one sequence of 1,032 int8 tokens against 32 rows a head: 12.6 us and 25.5, of 8,032 against 128
-    // rows: 60 and 46; 16 sequences of 32 bf16 tokens against 128 rows: 79 and 13; one of 8,064 int8 tokens, a window of 1,024, against 256 rows: 24 and 31.
+    // Eight rows a product or 128, by what each was measured to take when the GPU is full: the first kernel 40 ns for each eight rows of a kv head and 0.04 ns for each key that they are
+    // shown, the second, which starts some 12 us later, 80 ns (bf16 caches: 40) for each 256 rows and 0.2 ns (0.12) a key; over 300 batches the rule's choice is within 1 % of the better one on the
+    // average, within 1.5 times at the worst. Eight kv heads of 128, one sequence of 1,032 int8 tokens against 32 rows a head: 12.6 us and 25.5, of 8,032 against 128
+    // rows: 60 and 46; 16 sequences of 32 bf16 tokens against 128 rows: 79 and 13; 1,024 sequences of 64 int8 tokens against 16 rows: 419 and 673.
     const uint32_t group = a.q_heads / c.n_heads;
     const uint64_t rows = (uint64_t)(a.rows.max_rows ? std::min(a.rows.max_rows, a.rows.n_rows) : a.rows.n_rows) * group, len = a.rows.max_len ? std::min(a.rows.max_len, c.capacity) : c.capacity;
     auto shown = [&](uint32_t tile, uint32_t block) { return a.window ? (double)std::min<uint64_t>(len, (uint64_t)a.window + a.sinks + tile / group + block) : (double)len; };
-    const double of_8 = 0.04 * shown(8, 16) + 30., of_256 = (c.type == ZKB_VALUE_INT8 ? 0.2 : 0.12) * shown(256, 128);
+    const double of_8 = 0.04 * shown(8, 16) + 40., of_256 = c.type == ZKB_VALUE_INT8 ? 0.2 * shown(256, 128) + 80. : 0.12 * shown(256, 128) + 40.;
     const bool few = ((double)((rows + 7) / 8) * of_8 - (double)((rows + 255) / 256) * of_256) * c.n_seqs * c.n_heads < 12000.;
     return c.type == ZKB_VALUE_INT8 ? (few ? launch_few<D, true>(ctx, a) : launch_many<D, true>(ctx, a)) : (few ? launch_few<D, false>(ctx, a) : launch_many<D, false>(ctx, a));
 }

@@ -178,6 +178,7 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
     __shared__ __align__(16) float v_scale_sm[2][INT8 ? 128 : 1];
     __shared__ int in_odd[MANY_RANKS];
     __shared__ int odd_sm[8];  // some value was no number: of the units in turn (what makes ready runs a few units ahead)
+    __shared__ int slow_sm;  // threads that add up what is no number, which takes as long as the cache is
     __shared__ uint32_t tmem_sm;
     unsigned char* const sm = many_sm + (-(uint32_t)__cvta_generic_to_shared(many_sm) & 1023);
     float *const in_top = reinterpret_cast<float*>(sm + 256 * D * 4), *const in_sum = in_top + 256;  // behind the sums that are joined, where Q and the keys were
@@ -192,13 +193,14 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
         for (int i = 0; i < 4; i++) mbar_init(bar_of(bars.raw_full[i]), 1), mbar_init(bar_of(bars.raw_empty[i]), M::READIERS);
         for (int i = 0; i < 2; i++) mbar_init(bar_of(bars.s_ready[i]), 2), mbar_init(bar_of(bars.p_ready[i]), 128), mbar_init(bar_of(bars.o_ready[i]), 1);
         mbar_init(bar_of(bars.q_ready), 256);
+        slow_sm = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     const int64_t row_bytes = c.token_stride * M::SIZE;
     bool failed = false;  // a wait ran out: what follows is not valid, and nothing more is waited for
     auto wait_one = [&](const unsigned long long& b, uint32_t parity) {
-        if (!failed) failed = !mbar_wait(bar_of(b), parity & 1);
+        if (!failed) failed = !mbar_wait(bar_of(b), parity & 1, [&] { return *static_cast<volatile int*>(&slow_sm) != 0; });
     };
     auto wait = [&](const unsigned long long& b, uint32_t parity) {  // a whole warp: what follows may be an instruction that wants its lanes together
         wait_one(b, parity);
@@ -266,7 +268,7 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
             return left;
         };
         auto sums_place = [](int row, int four) { return (row * (D / 4) + (four ^ (row & 7))) * 16; };
-        float by_row = more ? load_q(u) : 0.f;
+        float by_row = more && u.n ? load_q(u) : 0.f;
         while (more) {
             const int m = row_of(u);  // this thread's row
             const bool live = m < u.n_m;
@@ -375,7 +377,9 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
             }
             const bool any = steps > 0, join = units.joined(u);
             float by_next = by_row;
-            if (again && !join) by_next = load_q(after);  // its products begin while this unit's rows are written
+            // The tile without rows waits for nothing of its own, and must not announce the next unit's Q before the other has announced this one's. (A unit without blocks has no Q.)
+            if (!u.two && !u.split) named_sync(5, 256);
+            if (again && !join && after.n) by_next = load_q(after);  // its products begin while this unit's rows are written
             if (any) {
                 wait(bars.o_ready[tile], done - 1);
                 tmem_fence_after();
@@ -389,6 +393,7 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
                     const int i0 = (int)((uint32_t)m / (uint32_t)group);
                     const int64_t to = live ? (u.s.first + i0) * a.out_stride + (u.kv_head * group + m - i0 * group) * a.out_head_stride : 0;
                     const bool word = a.out_type == ZKB_VALUE_WORD, vec = ((uintptr_t)(static_cast<char*>(a.out) + to * (word ? 4 : 2)) & 31) == 0;
+                    if (odd) atomicAdd(&slow_sm, 1);
 #pragma unroll 1
                     for (int i = 0; i < D; i += 16) {
                         uint32_t o[2][8];
@@ -424,6 +429,7 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
                                 for (int e = 0; e < 16; e++) at[e] = (uint16_t)(w[e / 2] >> 16 * (e & 1));
                         }
                     }
+                    if (odd) atomicAdd(&slow_sm, -1);
                 }
             } else {
                 // Each thread block finishes `part` of the rows: their sums go to [whose][row][four dimensions] of its shared memory, where Q and the keys were
@@ -502,7 +508,7 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
                 }
                 if (again) {
                     meet();
-                    by_next = load_q(after);
+                    if (after.n) by_next = load_q(after);
                 }
             }
             passed += u.n;
@@ -517,7 +523,7 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
         const int th = threadIdx.x - 320;
         if constexpr (INT8) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         const uint32_t c128 = bf16_128(), c1152 = f16_1152();
-        for (; more; units_done++) {
+        while (more) {
             if (warp == 8) {  // ---- the copies
                 if (TMA && lane == 0) {
                     for (int i = 0; i < 2 * u.n; i++) {
@@ -589,7 +595,7 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
                     }
                     __syncwarp();
                 };
-                wait(bars.q_ready, units_done);
+                if (u.n) wait(bars.q_ready, units_done++);
 #pragma unroll 1
                 for (int j = -1; j < u.n; j++)
 #pragma unroll
