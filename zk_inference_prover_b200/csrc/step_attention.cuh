@@ -52,17 +52,12 @@ __device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
     asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
     return done;
 }
-// Gives up after 2^20 tries in a row for whose waiting there is no reason.
-template <class Reason>
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, Reason reason) {
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
     if (mbar_test(bar, parity)) return true;
 #pragma unroll 1
-    for (int tries = 0; tries < (1 << 20); tries = reason() ? 0 : tries + 1)
+    for (int tries = 0; tries < (1 << 20); tries++)
         if (mbar_test(bar, parity)) return true;
     return false;
-}
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
-    return mbar_wait(bar, parity, [] { return false; });
 }
 // The box of a cache's map from (value, token, head, sequence) on.
 __device__ __forceinline__ void tma_load(uint32_t to, const CUtensorMap* map, int value, int token, int head, int seq, uint32_t bar) {

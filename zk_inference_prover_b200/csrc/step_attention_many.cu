@@ -13,8 +13,8 @@ namespace zk {
 // A thread block takes one pair of tiles after the other; with too few of them for the GPU the keys are spread over a cluster's thread blocks, which add up through
 // each other's shared memory, and one tile alone is two, of each block's two halves.
 // The weights are rounded to bf16 for the product (2^-8, as the result's own rounding): a second bf16 number for what that leaves, as the few rows' kernel has it, took 15 to 28 % longer.
-// 32 heads on 8 of 128, causal: 8,192 rows of one sequence, bf16, 504 us, 1,090 TFLOP/s of visible pairs; 1,290 to 2,048 rows of four sequences 148 us, int8 245 us; 8,192 rows with a window
-// of 1,024, bf16 199 us, int8 322 us: a block's products and its softmax take turns, 1,500 and 2,200 cycles, int8 scales another 2,000 of shared memory's.
+// 32 heads on 8 of 128, causal: 8,192 rows of one sequence, bf16, 510 us, 1,080 TFLOP/s of visible pairs; 1,290 to 2,048 rows of four sequences 150 us, int8 252 us; 8,192 rows with a window
+// of 1,024, bf16 202 us, int8 322 us: a block's products and its softmax take turns, 1,500 and 2,200 cycles, int8 scales another 2,000 of shared memory's.
 constexpr int MANY_KEYS = 128, MANY_RANKS = 16;
 
 template <int D, bool INT8>
@@ -109,7 +109,7 @@ __device__ __forceinline__ void store32(void* to, const uint32_t (&x)[8]) {
 __device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 
 struct ManyBars {
-    unsigned long long full[5], ready[5], empty[5], raw_full[4], raw_empty[4], s_ready[2], p_ready[2], o_ready[2], q_ready;
+    unsigned long long full[5], ready[5], empty[5], raw_full[4], raw_empty[4], s_ready[2], p_ready[2], o_ready[2], q_ready[2];
 };
 __device__ __forceinline__ uint32_t bar_of(const unsigned long long& b) { return (uint32_t)__cvta_generic_to_shared(&b); }
 
@@ -191,8 +191,7 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
     } else if (warp == 1 && lane == 0) {
         for (int i = 0; i < 5; i++) mbar_init(bar_of(bars.full[i]), 1), mbar_init(bar_of(bars.ready[i]), M::READIERS), mbar_init(bar_of(bars.empty[i]), 1);
         for (int i = 0; i < 4; i++) mbar_init(bar_of(bars.raw_full[i]), 1), mbar_init(bar_of(bars.raw_empty[i]), M::READIERS);
-        for (int i = 0; i < 2; i++) mbar_init(bar_of(bars.s_ready[i]), 2), mbar_init(bar_of(bars.p_ready[i]), 128), mbar_init(bar_of(bars.o_ready[i]), 1);
-        mbar_init(bar_of(bars.q_ready), 256);
+        for (int i = 0; i < 2; i++) mbar_init(bar_of(bars.s_ready[i]), 2), mbar_init(bar_of(bars.p_ready[i]), 128), mbar_init(bar_of(bars.o_ready[i]), 1), mbar_init(bar_of(bars.q_ready[i]), 128);
         slow_sm = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -200,7 +199,13 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
     const int64_t row_bytes = c.token_stride * M::SIZE;
     bool failed = false;  // a wait ran out: what follows is not valid, and nothing more is waited for
     auto wait_one = [&](const unsigned long long& b, uint32_t parity) {
-        if (!failed) failed = !mbar_wait(bar_of(b), parity & 1, [&] { return *static_cast<volatile int*>(&slow_sm) != 0; });
+        if (!failed && !mbar_test(bar_of(b), parity & 1)) {
+            int tries = 0;
+#pragma unroll 1
+            do tries = *static_cast<volatile int*>(&slow_sm) ? 0 : tries + 1;  // counted while there is no reason to wait
+            while (!mbar_test(bar_of(b), parity & 1) && tries < (1 << 20));
+            failed = tries >= 1 << 20;
+        }
     };
     auto wait = [&](const unsigned long long& b, uint32_t parity) {  // a whole warp: what follows may be an instruction that wants its lanes together
         wait_one(b, parity);
@@ -264,11 +269,13 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
             for (int i = 0; i < D / 8; i++)
                 st_shared4(q_at + tile * M::TILE + tile_place<D, INT8>(row, i * 16), word(x[i].x), word(x[i].y), word(x[i].z), word(x[i].w));
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            mbar_arrive(bar_of(bars.q_ready));
+            mbar_arrive(bar_of(bars.q_ready[tile]));
             return left;
         };
         auto sums_place = [](int row, int four) { return (row * (D / 4) + (four ^ (row & 7))) * 16; };
-        float by_row = more && u.n ? load_q(u) : 0.f;
+        // Q of a unit that this tile has products in: no other keeps it from announcing the next one's too soon.
+        auto works = [&](const Unit& n) { return n.n > 0 && (tile == 0 || n.two || n.split); };
+        float by_row = more && works(u) ? load_q(u) : 0.f;
         while (more) {
             const int m = row_of(u);  // this thread's row
             const bool live = m < u.n_m;
@@ -377,9 +384,7 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
             }
             const bool any = steps > 0, join = units.joined(u);
             float by_next = by_row;
-            // The tile without rows waits for nothing of its own, and must not announce the next unit's Q before the other has announced this one's. (A unit without blocks has no Q.)
-            if (!u.two && !u.split) named_sync(5, 256);
-            if (again && !join && after.n) by_next = load_q(after);  // its products begin while this unit's rows are written
+            if (again && !join && works(after)) by_next = load_q(after);  // its products begin while this unit's rows are written
             if (any) {
                 wait(bars.o_ready[tile], done - 1);
                 tmem_fence_after();
@@ -508,7 +513,7 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
                 }
                 if (again) {
                     meet();
-                    if (after.n) by_next = load_q(after);
+                    if (works(after)) by_next = load_q(after);
                 }
             }
             passed += u.n;
@@ -518,7 +523,7 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
             u = after;
         }
     } else {
-        uint32_t items = 0, units_done = 0, odd_at = 0, tile_done[2] = {0, 0};
+        uint32_t items = 0, odd_at = 0, q_done[2] = {0, 0}, tile_done[2] = {0, 0};
         bool odd = false;
         const int th = threadIdx.x - 320;
         if constexpr (INT8) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
@@ -595,7 +600,10 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
                     }
                     __syncwarp();
                 };
-                if (u.n) wait(bars.q_ready, units_done++);
+                if (u.n) {
+                    wait(bars.q_ready[0], q_done[0]++);
+                    if (tiles == 2) wait(bars.q_ready[1], q_done[1]++);
+                }
 #pragma unroll 1
                 for (int j = -1; j < u.n; j++)
 #pragma unroll
