@@ -60,7 +60,7 @@ __device__ __forceinline__ void tmem_fence_after() { asm volatile("tcgen05.fence
 __device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 #define R8(x, o) "=r"(x[o]), "=r"(x[o + 1]), "=r"(x[o + 2]), "=r"(x[o + 3]), "=r"(x[o + 4]), "=r"(x[o + 5]), "=r"(x[o + 6]), "=r"(x[o + 7])
 #define W8(x, o) "r"(x[o]), "r"(x[o + 1]), "r"(x[o + 2]), "r"(x[o + 3]), "r"(x[o + 4]), "r"(x[o + 5]), "r"(x[o + 6]), "r"(x[o + 7])
-// 32 columns of this thread's row; they are there after tmem_loaded, which names them so that nothing that uses them is moved before it.
+// 32 or 8 columns of this thread's row; they are there after tmem_loaded, which names them so that nothing that uses them is moved before it.
 #define RW8(x, o) "+r"(x[o]), "+r"(x[o + 1]), "+r"(x[o + 2]), "+r"(x[o + 3]), "+r"(x[o + 4]), "+r"(x[o + 5]), "+r"(x[o + 6]), "+r"(x[o + 7])
 __device__ __forceinline__ void tmem_loaded(uint32_t (&x)[32]) { asm volatile("tcgen05.wait::ld.sync.aligned;" : RW8(x, 0), RW8(x, 8), RW8(x, 16), RW8(x, 24)::"memory"); }
 __device__ __forceinline__ void tmem_loaded(uint32_t (&x)[8]) { asm volatile("tcgen05.wait::ld.sync.aligned;" : RW8(x, 0)::"memory"); }
@@ -77,7 +77,6 @@ __device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t* x) {
 __device__ __forceinline__ void tmem_store8(uint32_t at, const uint32_t* x) { asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(at), W8(x, 0) : "memory"); }
 #undef R8
 #undef W8
-
 
 // Two 32-bit floats at once, kept as their words.
 __device__ __forceinline__ uint64_t two_words(uint32_t a, uint32_t b) {
@@ -512,6 +511,7 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
                     }
                 }
                 if (again) {
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the next unit's copies go where these sums are
                     meet();
                     if (works(after)) by_next = load_q(after);
                 }
