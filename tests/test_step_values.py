@@ -374,6 +374,20 @@ def test_attention_of_many_units(ctx, zkb, kind, rows, length, d, window, sinks)
 
 @gpu
 @pytest.mark.parametrize("kind", ["bf16", "int8"])
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("order,pad", [("shtd", 0), ("hstd", 3)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1600, 7)])
+def test_attention_of_several_rows_over_long_caches(ctx, zkb, kind, d, order, pad, window, sinks):
+    """Rows that fill one small product and part of the next, and a sequence of fewer."""
+    g = gen(d + window)
+    batch = Batch([(3, 2500), (0, 0), (5, 1801), (1, 2500), (4, 2)])
+    cache = Cache(g, kind, 5, 2, 2501, d, order, pad)
+    q = torch.randn(batch.n_rows, 14, d, generator=g, device="cuda").bfloat16()
+    check_attention(ctx, zkb, batch, cache, q, "words", window, sinks)
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
 @pytest.mark.parametrize("most,length", [(30, 120), (30, 250), (120, 250), (1, 2)])
 def test_attention_of_many_short_sequences(ctx, zkb, kind, most, length):
     """Several sequences a thread block, of one tile or two and of one block of keys or two; some without rows, some without tokens."""

@@ -46,15 +46,17 @@ bool cache_maps(CacheMaps& maps, const zkb_kv_cache& c, uint32_t tokens) {
 // products for a warp's sixteen keys waiting for it. One sequence of 2,048 int8 tokens: 9.4 us, most of it the launch and the joining.
 constexpr int FEW_WARPS = 8, FEW_RANKS = 16;
 
-template <int D, bool INT8>
+// T: how many times eight rows a thread block has for the keys that it reads.
+template <int D, bool INT8, int T>
 struct Few {
+    static constexpr int ROWS = 8 * T;
     static constexpr int SIZE = INT8 ? 1 : 2;
     static constexpr int ROW = D * SIZE, BOX = ROW < 128 ? ROW : 128, BOXES = ROW / BOX;  // bytes of a token and head, and of a box's row
     static constexpr int KW = ROW / 16, VW = ROW / 32, KB = KW / BOXES, VB = VW / BOXES;  // words a lane and key, in all and in a box
     static constexpr int TILE = 16 * ROW;  // bytes of sixteen keys of K or of V
-    static constexpr int THREAD_BLOCKS = TILE <= 2048 ? 2 : 1;  // an SM
+    static constexpr int THREAD_BLOCKS = TILE <= 2048 && T == 1 ? 2 : 1;  // an SM
     static constexpr int STAGES = 3;
-    static constexpr int JOIN = FEW_WARPS * 8 * (D + 4) * 4;  // the warps' sums, after the rings are done with
+    static constexpr int JOIN = FEW_WARPS * ROWS * (D + 4) * 4;  // the warps' sums, after the rings are done with
     static constexpr int RING = FEW_WARPS * STAGES * 2 * TILE;
     static constexpr int SMEM = 1024 + (RING > JOIN ? RING : JOIN);  // boxes start on 1024 bytes
 };
@@ -72,14 +74,14 @@ __device__ __forceinline__ void read_row(uint32_t box, int row, int at, uint32_t
     }
 }
 
-template <int D, bool INT8, bool TMA>
-__global__ void __launch_bounds__(FEW_WARPS * 32, Few<D, INT8>::THREAD_BLOCKS)
+template <int D, bool INT8, int T, bool TMA>
+__global__ void __launch_bounds__(FEW_WARPS * 32, (Few<D, INT8, T>::THREAD_BLOCKS))
     attention_few_kernel(const __grid_constant__ zkb_step_attention_args a, const __grid_constant__ CacheMaps maps, unsigned* dev_err) {
-    using F = Few<D, INT8>;
-    constexpr int STEPS = D / 16, STRIDE = D + 4;
+    using F = Few<D, INT8, T>;
+    constexpr int STEPS = D / 16, STRIDE = D + 4, ROWS = F::ROWS;
     extern __shared__ unsigned char few_sm[];
-    __shared__ float top_sm[FEW_WARPS][8], sum_sm[FEW_WARPS][8], all_top[8], all_sum[8];
-    __shared__ float in_o[8 * D], in_top[FEW_RANKS][8], in_sum[FEW_RANKS][8];  // what the cluster's thread blocks write here: [rank][this one's part]
+    __shared__ float top_sm[FEW_WARPS][ROWS], sum_sm[FEW_WARPS][ROWS], all_top[ROWS], all_sum[ROWS];
+    __shared__ float in_o[ROWS * D], in_top[FEW_RANKS][ROWS], in_sum[FEW_RANKS][ROWS];  // what the cluster's thread blocks write here: [rank][this one's part]
     __shared__ int in_odd[FEW_RANKS];  // some value of V was no number
     __shared__ __align__(8) unsigned long long full[FEW_WARPS][F::STAGES];
     __shared__ float scale_sm[INT8 ? FEW_WARPS * F::STAGES * 32 : 1];
@@ -103,7 +105,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, Few<D, INT8>::THREAD_BLOCKS)
     const char* const v = static_cast<const char*>(c.v) + (seq * c.seq_stride + kv_head * c.head_stride) * F::SIZE;
     const float* const scales = INT8 ? (lane < 16 ? c.k_scale : c.v_scale) + seq * c.scale_seq_stride + kv_head * c.scale_head_stride : nullptr;
     const int row_bytes = (int)c.token_stride * F::SIZE;
-    const int64_t n_m = (int64_t)s.rows * group, m_step = (int64_t)(gridDim.x / ranks) * 8;  // below 2^31, so that rows are found by 32-bit divisions
+    const int64_t n_m = (int64_t)s.rows * group, m_step = (int64_t)(gridDim.x / ranks) * ROWS;  // below 2^31, so that rows are found by 32-bit divisions
     auto token = [&](int64_t m) { return (int)((uint32_t)m / (uint32_t)group); };
     const float by = a.scale * 1.44269504f;
     const uint32_t c128 = bf16_128(), c1152 = f16_1152();
@@ -132,8 +134,8 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, Few<D, INT8>::THREAD_BLOCKS)
         if constexpr (INT8) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(scale_ring + st * 128 + 4 * lane), "l"(scales + min(base + (lane & 15), last)) : "memory");
     };
     bool begun = ranks == 1;
-    for (int64_t m0 = (int64_t)(blockIdx.x / ranks) * 8; m0 < n_m; m0 += m_step) {
-        const int64_t pos_low = s.pos + token(m0), pos_high = s.pos + token(min(m0 + 8, n_m) - 1);
+    for (int64_t m0 = (int64_t)(blockIdx.x / ranks) * ROWS; m0 < n_m; m0 += m_step) {
+        const int64_t pos_low = s.pos + token(m0), pos_high = s.pos + token(min(m0 + ROWS, n_m) - 1);
         const KeyBlocks blocks = key_blocks<16>(pos_low, pos_high, c.capacity, a.window, a.sinks);
         const int stride = ranks * FEW_WARPS, last = (int)blocks.end - 1;
         const int at0 = rank * FEW_WARPS + warp;
@@ -142,11 +144,13 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, Few<D, INT8>::THREAD_BLOCKS)
             if (at0 + i * stride < blocks.n) copy(stage + i < F::STAGES ? stage + i : stage + i - F::STAGES, blocks.base(at0 + i * stride), last);
             asm volatile("cp.async.commit_group;" ::: "memory");
         }
-        // Q: lane (g, t) has row g's dimensions in the order in which its K quarter comes
-        uint32_t q[STEPS][2];
-        {
+        // Q: lane (g, t) has row g's dimensions (of each eight rows) in the order in which its K quarter comes
+        uint32_t q[T][STEPS][2];
+        float by_row[T][2];
+#pragma unroll
+        for (int n = 0; n < T; n++) {
             constexpr int BOX_DIMS = F::BOX / F::SIZE, LANE_DIMS = BOX_DIMS / 4;
-            const int64_t m = m0 + g;
+            const int64_t m = m0 + 8 * n + g;
             const int i0 = m < n_m ? token(m) : 0;
             const uint16_t* from = static_cast<const uint16_t*>(a.q) + (m < n_m ? (s.first + i0) * a.q_stride + (kv_head * group + (int)m - i0 * group) * a.q_head_stride : 0);
             const bool quads = ((uintptr_t)from & 7) == 0;
@@ -158,36 +162,43 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, Few<D, INT8>::THREAD_BLOCKS)
                     if (quads) w = *reinterpret_cast<const uint2*>(from + d);
                     else w = make_uint2((uint32_t)from[d] | (uint32_t)from[d + 1] << 16, (uint32_t)from[d + 2] | (uint32_t)from[d + 3] << 16);
                 }
-                q[i][0] = INT8 ? __byte_perm(w.x, w.y, 0x5410) : w.x;  // codes_to_f16's order
-                q[i][1] = INT8 ? __byte_perm(w.x, w.y, 0x7632) : w.y;
+                q[n][i][0] = INT8 ? __byte_perm(w.x, w.y, 0x5410) : w.x;  // codes_to_f16's order
+                q[n][i][1] = INT8 ? __byte_perm(w.x, w.y, 0x7632) : w.y;
+            }
+            by_row[n][0] = by_row[n][1] = by;
+            if constexpr (INT8) {
+                // Codes are cheaper to have in fp16, so Q is taken there too, each row times the power of two that brings its largest value to 2^13: exact down to
+                // 2^-27 of that value, and below it off by 2^-38 of it.
+                float most = 0.f;
+#pragma unroll
+                for (int i = 0; i < 2 * STEPS; i++) most = fmaxf(most, fmaxf(fabsf(bf16_low(q[n][i / 2][i & 1])), fabsf(bf16_high(q[n][i / 2][i & 1]))));
+                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+                const int e = (int)(__float_as_uint(most) >> 23);  // 0: all zero or nearly; 255: an infinity, which stays one
+                const int up = e == 0 || e == 255 ? 0 : min(13 + 127 - e, 126);
+                const float f = __uint_as_float((uint32_t)(up + 127) << 23);
+#pragma unroll
+                for (int i = 0; i < 2 * STEPS; i++) q[n][i / 2][i & 1] = pack_f16(bf16_low(q[n][i / 2][i & 1]) * f, bf16_high(q[n][i / 2][i & 1]) * f);
+#pragma unroll
+                for (int r = 0; r < 2; r++) by_row[n][r] = by * __uint_as_float((uint32_t)(127 - __shfl_sync(0xffffffffu, up, (2 * t + r) * 4)) << 23);
             }
         }
-        float by_row[2] = {by, by};
-        if constexpr (INT8) {
-            // Codes are cheaper to have in fp16, so Q is taken there too, each row times the power of two that brings its largest value to 2^13: exact down to
-            // 2^-27 of that value, and below it off by 2^-38 of it.
-            float most = 0.f;
+        // rows 2t and 2t + 1 (of each eight): their positions, running maxima and this lane's part of their sums
+        int p[T][2];
+        float top[T][2], less[T][2], sum[T][2], o[T][STEPS][4];
 #pragma unroll
-            for (int i = 0; i < 2 * STEPS; i++) most = fmaxf(most, fmaxf(fabsf(bf16_low(q[i / 2][i & 1])), fabsf(bf16_high(q[i / 2][i & 1]))));
-            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-            const int e = (int)(__float_as_uint(most) >> 23);  // 0: all zero or nearly; 255: an infinity, which stays one
-            const int up = e == 0 || e == 255 ? 0 : min(13 + 127 - e, 126);
-            const float f = __uint_as_float((uint32_t)(up + 127) << 23);
+        for (int n = 0; n < T; n++) {
 #pragma unroll
-            for (int i = 0; i < 2 * STEPS; i++) q[i / 2][i & 1] = pack_f16(bf16_low(q[i / 2][i & 1]) * f, bf16_high(q[i / 2][i & 1]) * f);
+            for (int r = 0; r < 2; r++) {
+                const int64_t m = m0 + 8 * n + 2 * t + r;
+                p[n][r] = m < n_m ? (int)s.pos + token(m) : -1;
+                top[n][r] = -INFINITY, less[n][r] = 0.f, sum[n][r] = 0.f;
+            }
 #pragma unroll
-            for (int r = 0; r < 2; r++) by_row[r] = by * __uint_as_float((uint32_t)(127 - __shfl_sync(0xffffffffu, up, (2 * t + r) * 4)) << 23);
+            for (int i = 0; i < STEPS; i++)
+#pragma unroll
+                for (int x = 0; x < 4; x++) o[n][i][x] = 0.f;
         }
-        // rows 2t and 2t + 1: their positions, running maxima and this lane's part of their sums
-        int p[2];
-        float top[2] = {-INFINITY, -INFINITY}, less[2] = {0.f, 0.f}, sum[2] = {0.f, 0.f}, o[STEPS][4];
-#pragma unroll
-        for (int r = 0; r < 2; r++) p[r] = m0 + 2 * t + r < n_m ? (int)s.pos + token(m0 + 2 * t + r) : -1;
-#pragma unroll
-        for (int i = 0; i < STEPS; i++)
-#pragma unroll
-            for (int x = 0; x < 4; x++) o[i][x] = 0.f;
         bool odd = false;
         const int whole_to = (int)min(pos_low, (int64_t)last) - 15, whole_from = a.window ? (int)max((int64_t)0, pos_high - (int64_t)a.window + 1) : 0;  // blocks that all rows see
         for (int at = at0; at < blocks.n; at += stride) {
@@ -199,7 +210,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, Few<D, INT8>::THREAD_BLOCKS)
             __syncwarp();
             if (TMA) failed = __any_sync(0xffffffffu, failed || !mbar_wait(bars + 8 * stage, parity));
             if (++stage == F::STAGES) stage = 0, parity ^= 1;
-            float sc[4] = {0.f, 0.f, 0.f, 0.f}, sc2[4] = {0.f, 0.f, 0.f, 0.f};
+            float sc[T][4] = {}, sc2[T][4] = {};
             {
                 uint32_t k0[F::KW], k1[F::KW];
 #pragma unroll
@@ -213,60 +224,64 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, Few<D, INT8>::THREAD_BLOCKS)
                     if constexpr (INT8) {
                         codes_to_f16(k0[i], c1152, f[0], f[2]);
                         codes_to_f16(k1[i], c1152, f[1], f[3]);
-                        mma_f16(i & 1 ? sc2 : sc, f, q[i][0], q[i][1]);
+#pragma unroll
+                        for (int n = 0; n < T; n++) mma_f16(i & 1 ? sc2[n] : sc[n], f, q[n][i][0], q[n][i][1]);
                     } else {
                         f[0] = k0[2 * i], f[1] = k1[2 * i], f[2] = k0[2 * i + 1], f[3] = k1[2 * i + 1];
-                        mma_bf16(i & 1 ? sc2 : sc, f, q[i][0], q[i][1]);
+#pragma unroll
+                        for (int n = 0; n < T; n++) mma_bf16(i & 1 ? sc2[n] : sc[n], f, q[n][i][0], q[n][i][1]);
                     }
                 }
             }
-            // sc: key g with rows 2t, 2t + 1, then key g + 8
-#pragma unroll
-            for (int i = 0; i < 4; i++) sc[i] += sc2[i];
+            float k_by[2] = {1.f, 1.f}, v_by[2] = {1.f, 1.f};  // keys g and g + 8
             if constexpr (INT8) {
-                const float k0 = __uint_as_float(ld_shared(scales_here)), k1 = __uint_as_float(ld_shared(scales_here + 32));
-#pragma unroll
-                for (int i = 0; i < 4; i++) sc[i] *= by_row[i & 1] * (i < 2 ? k0 : k1);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; i++) sc[i] *= by;
+                k_by[0] = __uint_as_float(ld_shared(scales_here)), k_by[1] = __uint_as_float(ld_shared(scales_here + 32));
+                v_by[0] = __uint_as_float(ld_shared(scales_here + 64)), v_by[1] = __uint_as_float(ld_shared(scales_here + 96));
             }
-            if (base < whole_from || base > whole_to) {
+            uint32_t w[T][2], left[T][2];
+#pragma unroll
+            for (int n = 0; n < T; n++) {
+                // z: key g with rows 2t, 2t + 1, then key g + 8
+                float z[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) z[i] = (sc[n][i] + sc2[n][i]) * (INT8 ? by_row[n][i & 1] * k_by[i >> 1] : by);
+                if (base < whole_from || base > whole_to) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int key = base + g + 8 * (i >> 1), gap = p[n][i & 1] - key;
+                        if (gap < 0 || key > last || (a.window != 0 && (uint32_t)gap >= a.window && (uint32_t)key >= a.sinks)) z[i] = -INFINITY;
+                    }
+                }
+                // The weights' common factor is 2^-top. It need not be the largest score's, only within 2^8 of it, so it is seldom that it changes.
+                if (__any_sync(0xffffffffu, fmaxf(z[0], z[2]) > top[n][0] + 8.f || fmaxf(z[1], z[3]) > top[n][1] + 8.f)) {
+#pragma unroll
+                    for (int r = 0; r < 2; r++) {
+                        float higher = fmaxf(top[n][r], fmaxf(z[r], z[r + 2]));
+#pragma unroll
+                        for (int x = 4; x < 32; x <<= 1) higher = fmaxf(higher, __shfl_xor_sync(0xffffffffu, higher, x));
+                        const float keep = higher > top[n][r] ? exp2_fast(top[n][r] - higher) : 1.f;
+                        sum[n][r] *= keep, top[n][r] = higher, less[n][r] = higher == -INFINITY ? 0.f : higher;
+#pragma unroll
+                        for (int i = 0; i < STEPS; i++) o[n][i][r] *= keep, o[n][i][r + 2] *= keep;
+                    }
+                }
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const int key = base + g + 8 * (i >> 1), gap = p[i & 1] - key;
-                    if (gap < 0 || key > last || (a.window != 0 && (uint32_t)gap >= a.window && (uint32_t)key >= a.sinks)) sc[i] = -INFINITY;
+                    const float e = exp2_fast(z[i] - less[n][i & 1]);
+                    sum[n][i & 1] += e;
+                    z[i] = INT8 ? (z[i] == -INFINITY ? 0.f : e * v_by[i >> 1]) : e;  // a hidden token's scale may be anything
                 }
-            }
-            // The weights' common factor is 2^-top. It need not be the largest score's, only within 2^8 of it, so it is seldom that it changes.
-            if (__any_sync(0xffffffffu, fmaxf(sc[0], sc[2]) > top[0] + 8.f || fmaxf(sc[1], sc[3]) > top[1] + 8.f)) {
+                // A weight is two bf16 numbers, its rounding and what that leaves: off by 2^-16 where the result's own rounding takes 2^-8. (One number alone: 64 sequences of 8,192
+                // int8 tokens in 164 us instead of 174, bf16 240 instead of 243, and results up to 1.6 times as far off.)
+                const uint32_t high[2] = {pack_bf16(z[0], z[1]), pack_bf16(z[2], z[3])};
 #pragma unroll
-                for (int r = 0; r < 2; r++) {
-                    float higher = fmaxf(top[r], fmaxf(sc[r], sc[r + 2]));
-#pragma unroll
-                    for (int x = 4; x < 32; x <<= 1) higher = fmaxf(higher, __shfl_xor_sync(0xffffffffu, higher, x));
-                    const float keep = higher > top[r] ? exp2_fast(top[r] - higher) : 1.f;
-                    sum[r] *= keep, top[r] = higher, less[r] = higher == -INFINITY ? 0.f : higher;
-#pragma unroll
-                    for (int i = 0; i < STEPS; i++) o[i][r] *= keep, o[i][r + 2] *= keep;
+                for (int i = 0; i < 4; i++) {
+                    z[i] -= i & 1 ? bf16_high(high[i >> 1]) : bf16_low(high[i >> 1]);
+                    if (INT8) z[i] = z[i] == z[i] ? z[i] : 0.f;  // an infinity leaves nothing
                 }
-            }
-            const float v0 = INT8 ? __uint_as_float(ld_shared(scales_here + 64)) : 1.f, v1 = INT8 ? __uint_as_float(ld_shared(scales_here + 96)) : 1.f;
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float w = exp2_fast(sc[i] - less[i & 1]);
-                sum[i & 1] += w;
-                sc[i] = INT8 ? (sc[i] == -INFINITY ? 0.f : w * (i < 2 ? v0 : v1)) : w;  // a hidden token's scale may be anything
+                for (int i = 0; i < 2; i++) w[n][i] = transpose8(high[i]), left[n][i] = transpose8(pack_bf16(z[2 * i], z[2 * i + 1]));
             }
-            // A weight is two bf16 numbers, its rounding and what that leaves: off by 2^-16 where the result's own rounding takes 2^-8. (One number alone: 64 sequences of 8,192
-            // int8 tokens in 164 us instead of 174, bf16 240 instead of 243, and results up to 1.6 times as far off.)
-            const uint32_t high[2] = {pack_bf16(sc[0], sc[1]), pack_bf16(sc[2], sc[3])};
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                sc[i] -= i & 1 ? bf16_high(high[i >> 1]) : bf16_low(high[i >> 1]);
-                if (INT8) sc[i] = sc[i] == sc[i] ? sc[i] : 0.f;  // an infinity leaves nothing
-            }
-            const uint32_t w0 = transpose8(high[0]), w1 = transpose8(high[1]), left0 = transpose8(pack_bf16(sc[0], sc[1])), left1 = transpose8(pack_bf16(sc[2], sc[3]));
             uint32_t vw[4][F::VW];
 #pragma unroll
             for (int i = 0; i < 4; i++)
@@ -303,8 +318,8 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, Few<D, INT8>::THREAD_BLOCKS)
                     f[0] = __byte_perm(vw[0][i], vw[1][i], 0x5410), f[1] = __byte_perm(vw[0][i], vw[1][i], 0x7632);
                     f[2] = __byte_perm(vw[2][i], vw[3][i], 0x5410), f[3] = __byte_perm(vw[2][i], vw[3][i], 0x7632);
                 }
-                mma_bf16(o[i], f, w0, w1);
-                mma_bf16(o[i], f, left0, left1);
+#pragma unroll
+                for (int n = 0; n < T; n++) mma_bf16(o[n][i], f, w[n][0], w[n][1]), mma_bf16(o[n][i], f, left[n][0], left[n][1]);
             }
             __syncwarp();  // all lanes have read the block that the next copies go to
         }
@@ -313,19 +328,20 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, Few<D, INT8>::THREAD_BLOCKS)
         if (failed && lane == 0) *dev_err = WAIT_RAN_OUT;
         const int any_odd = __syncthreads_or(odd);  // and the rings are done with
 #pragma unroll
-        for (int r = 0; r < 2; r++) {
-#pragma unroll
-            for (int x = 4; x < 32; x <<= 1) sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], x);
-            if (g == 0) top_sm[warp][2 * t + r] = top[r], sum_sm[warp][2 * t + r] = sum[r];
-        }
-        {
+        for (int n = 0; n < T; n++) {
             constexpr int BOX_DIMS = F::BOX / F::SIZE, LANE_DIMS = BOX_DIMS / 8;
+#pragma unroll
+            for (int r = 0; r < 2; r++) {
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) sum[n][r] += __shfl_xor_sync(0xffffffffu, sum[n][r], x);
+                if (g == 0) top_sm[warp][8 * n + 2 * t + r] = top[n][r], sum_sm[warp][8 * n + 2 * t + r] = sum[n][r];
+            }
 #pragma unroll
             for (int i = 0; i < STEPS; i++)
 #pragma unroll
                 for (int x = 0; x < 4; x++) {
                     const int e = 2 * i + (x >> 1);
-                    o_sm[(warp * 8 + 2 * t + (x & 1)) * STRIDE + e / LANE_DIMS * BOX_DIMS + g * LANE_DIMS + e % LANE_DIMS] = o[i][x];
+                    o_sm[(warp * ROWS + 8 * n + 2 * t + (x & 1)) * STRIDE + e / LANE_DIMS * BOX_DIMS + g * LANE_DIMS + e % LANE_DIMS] = o[n][i][x];
                 }
         }
         __syncthreads();
@@ -335,7 +351,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, Few<D, INT8>::THREAD_BLOCKS)
             begun = true;
         }
         // the warps' factors, and the row's sum
-        if (threadIdx.x < 8) {
+        if (threadIdx.x < ROWS) {
             const int r = threadIdx.x;
             float most = top_sm[0][r], all = 0.f, f[FEW_WARPS];
 #pragma unroll
@@ -348,23 +364,23 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, Few<D, INT8>::THREAD_BLOCKS)
             all_top[r] = most, all_sum[r] = all;
         }
         __syncthreads();
-        // this thread block's sums to whoever finishes them: outputs part, part + 1, ... of 8 D go to the thread block of that rank (ranks: a power of two)
-        const int part_log = 31 - __clz(8 * D / ranks), part = 1 << part_log;
+        // this thread block's sums to whoever finishes them: outputs part, part + 1, ... of them all go to the thread block of that rank (ranks: a power of two)
+        const int part_log = 31 - __clz(ROWS * D / ranks), part = 1 << part_log;
 #pragma unroll
-        for (int x = 0; x < 8 * D; x += FEW_WARPS * 32) {
+        for (int x = 0; x < ROWS * D; x += FEW_WARPS * 32) {
             const int i = x + threadIdx.x, r = i / D, d = i % D;
             float y = 0.f;
 #pragma unroll
-            for (int w = 0; w < FEW_WARPS; w++) y += o_sm[(w * 8 + r) * STRIDE + d] * sum_sm[w][r];
+            for (int w = 0; w < FEW_WARPS; w++) y += o_sm[(w * ROWS + r) * STRIDE + d] * sum_sm[w][r];
             float* const to = &in_o[rank * part + (i & (part - 1))];
             if (ranks > 1) peer_store(to, i >> part_log, y);
             else *to = y;
         }
-        for (int i = threadIdx.x; i < 8 * ranks; i += FEW_WARPS * 32) {
-            const int r = i & 7;
-            peer_store(&in_top[rank][r], i >> 3, all_top[r]);
-            peer_store(&in_sum[rank][r], i >> 3, all_sum[r]);
-            if (r == 0) peer_store(&in_odd[rank], i >> 3, any_odd);
+        for (int i = threadIdx.x; i < ROWS * ranks; i += FEW_WARPS * 32) {
+            const int r = i % ROWS, to = i / ROWS;
+            peer_store(&in_top[rank][r], to, all_top[r]);
+            peer_store(&in_sum[rank][r], to, all_sum[r]);
+            if (r == 0) peer_store(&in_odd[rank], to, any_odd);
         }
         if (TMA) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the next rows' copies go where the warps' sums are
         if (ranks > 1) cluster_arrive(), cluster_wait();
@@ -398,23 +414,24 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, Few<D, INT8>::THREAD_BLOCKS)
     if (!begun) cluster_wait();
 }
 
-template <int D, bool INT8>
+template <int D, bool INT8, int T>
 static cudaError_t launch_few(zkb_ctx* ctx, const zkb_step_attention_args& a) {
     const zkb_kv_cache& c = a.cache;
     const uint32_t group = a.q_heads / c.n_heads, most = a.rows.max_rows ? std::min(a.rows.max_rows, a.rows.n_rows) : a.rows.n_rows;
-    const uint32_t tiles = (uint32_t)std::min<uint64_t>(((uint64_t)most * group + 7) / 8, 1u << 20);
+    using F = Few<D, INT8, T>;
+    const uint32_t tiles = (uint32_t)std::min<uint64_t>(((uint64_t)most * group + F::ROWS - 1) / F::ROWS, 1u << 20);
     uint64_t len = a.rows.max_len ? std::min(a.rows.max_len, c.capacity) : c.capacity;
     if (a.window) len = std::min<uint64_t>(len, (uint64_t)a.window + a.sinks + 32);
     // Split a sequence over more thread blocks while all of them are on the GPU at once and each warp keeps two blocks of keys: 16 sequences of 1,028 visible
     // bf16 tokens take 14.6 us in 128 thread blocks and 22.8 in 256, one of 2,048 int8 tokens 23.2 in 8 and 10.6 in 64.
     const uint64_t units = (uint64_t)c.n_seqs * c.n_heads * tiles;
     uint32_t ranks = 1;
-    while (ranks < FEW_RANKS && units <= clusters_at_once(2 * ranks) * Few<D, INT8>::THREAD_BLOCKS && len > (uint64_t)ranks * FEW_WARPS * 16 * 2) ranks *= 2;
+    while (ranks < FEW_RANKS && units <= clusters_at_once(2 * ranks) * F::THREAD_BLOCKS && len > (uint64_t)ranks * FEW_WARPS * 16 * 2) ranks *= 2;
     CacheMaps maps;
     const bool tma = cache_maps(maps, c, 16);
-    auto kernel = tma ? attention_few_kernel<D, INT8, true> : attention_few_kernel<D, INT8, false>;
+    auto kernel = tma ? attention_few_kernel<D, INT8, T, true> : attention_few_kernel<D, INT8, T, false>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Few<D, INT8>::SMEM);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, F::SMEM);
     if (e != cudaSuccess) return e;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -422,7 +439,7 @@ static cudaError_t launch_few(zkb_ctx* ctx, const zkb_step_attention_args& a) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(tiles * ranks, c.n_heads, c.n_seqs);
     cfg.blockDim = dim3(FEW_WARPS * 32);
-    cfg.dynamicSmemBytes = Few<D, INT8>::SMEM;
+    cfg.dynamicSmemBytes = F::SMEM;
     cfg.stream = ctx->stream;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
@@ -441,7 +458,11 @@ static cudaError_t launch_attention(zkb_ctx* ctx, const zkb_step_attention_args&
     auto shown = [&](uint32_t tile, uint32_t block) { return a.window ? (double)std::min<uint64_t>(len, (uint64_t)a.window + a.sinks + tile / group + block) : (double)len; };
     const double of_8 = 0.04 * shown(8, 16) + 40., of_256 = c.type == ZKB_VALUE_INT8 ? 0.2 * shown(256, 128) + 80. : 0.12 * shown(256, 128) + 40.;
     const bool few = ((double)((rows + 7) / 8) * of_8 - (double)((rows + 255) / 256) * of_256) * c.n_seqs * c.n_heads < 12000.;
-    return c.type == ZKB_VALUE_INT8 ? (few ? launch_few<D, true>(ctx, a) : launch_many<D, true>(ctx, a)) : (few ? launch_few<D, false>(ctx, a) : launch_many<D, false>(ctx, a));
+    if (!few) return c.type == ZKB_VALUE_INT8 ? launch_many<D, true>(ctx, a) : launch_many<D, false>(ctx, a);
+    if (c.type != ZKB_VALUE_INT8) return launch_few<D, false, 1>(ctx, a);
+    // Sixteen rows for each code that is turned into a 16-bit value instead of eight, with half the warps on an SM: 16 sequences of 8,008 tokens against 32 rows a head 164 us instead of 208, one of 2,048
+    // against 128 rows 20.7 instead of 22.5, but 16 of 1,040 against 64 rows 78 instead of 71.
+    return rows > 8 && shown(16, 16) >= 1500. ? launch_few<D, true, 2>(ctx, a) : launch_few<D, true, 1>(ctx, a);
 }
 
 }  // namespace zk
