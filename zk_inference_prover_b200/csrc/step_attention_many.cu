@@ -132,9 +132,10 @@ struct Units {
     const zkb_step_attention_args& a;
     uint32_t turn, all, depth;  // `depth`: pairs of a sequence that are units of their own
     int rank, ranks, pair;
+    uint32_t one;  // sequence and head whose pairs are in turn: the next unit may be another pair of the same
     __device__ Units(const zkb_step_attention_args& args, uint32_t pairs)
         : a(args), turn(0), all(pairs * args.cache.n_seqs * args.cache.n_heads), depth(pairs), rank((int)cluster_rank()),
-          ranks((int)cluster_ranks()), pair(-1) {}
+          ranks((int)cluster_ranks()), pair(-1), one(0) {}
     __device__ bool next(Unit& u) {
         const zkb_kv_cache& c = a.cache;
         const int group = (int)(a.q_heads / c.n_heads);
@@ -145,12 +146,12 @@ struct Units {
             if (turn * step >= all) return false;
             turn++;
             if (at >= all) continue;
-            const uint32_t one = at % (c.n_seqs * c.n_heads), z = at / (c.n_seqs * c.n_heads);
-            u.seq = (int)(one / c.n_heads), u.kv_head = (int)(one % c.n_heads);
-            u.s = step_sequence(a.rows, u.seq);
-            u.n_m = u.s.rows * group;
-            pair = (u.n_m + 255) / 256 - 1 - (int)z;
+            one = at % (c.n_seqs * c.n_heads);
+            pair = (step_sequence(a.rows, (int)(one / c.n_heads)).rows * group + 255) / 256 - 1 - (int)(at / (c.n_seqs * c.n_heads));
         }
+        u.seq = (int)(one / c.n_heads), u.kv_head = (int)(one % c.n_heads);
+        u.s = step_sequence(a.rows, u.seq);
+        u.n_m = u.s.rows * group;
         u.m0 = pair * 256;
         u.two = u.m0 + 128 < u.n_m;
         const int64_t low = u.s.pos + (uint32_t)u.m0 / (uint32_t)group, high = u.s.pos + (uint32_t)(min(u.m0 + 256, u.n_m) - 1) / (uint32_t)group;
