@@ -1,10 +1,12 @@
 """zkb_step_* where their definitions and their layouts have corners: hints that do not fit the batch, values that are no numbers, scales and windows at the ends of their
 ranges, launches that are refused. The references and bounds are those of tests/step_cases.py."""
+import math
+
 import pytest
 import torch
 
-from step_cases import Batch, Cache
-from test_step_values import check_attention, gen
+from step_cases import Batch, Cache, attention_reference, values_of
+from test_step_values import check_attention, done, gen
 
 gpu = pytest.mark.gpu
 
@@ -63,3 +65,42 @@ def test_a_captured_call_serves_a_batch_of_longer_sequences(ctx, zkb, kind):
         got = check_attention(ctx, zkb, other, cache, q, "bf16", 0, 0)
         assert torch.equal(got, replayed)
     del graph
+
+
+def attend(ctx, zkb, batch, cache, q, out, window=0, sinks=0, scale=None):
+    """The call, into `out` [row][head][dim] as it lies."""
+    torch.cuda.synchronize()
+    ctx.step_attention(zkb.StepAttention(cache=cache.args(zkb), rows=batch.args(zkb), q=q.data_ptr(), out=out.data_ptr(), q_stride=q.stride(0), q_head_stride=q.stride(1), out_stride=out.stride(0),
+                                         out_head_stride=out.stride(1), q_heads=q.shape[1], out_type=zkb.VALUE_WORD if out.dtype == torch.int32 else zkb.VALUE_BF16, window=window, sinks=sinks,
+                                         scale=q.shape[2] ** -0.5 if scale is None else scale))
+    done(ctx)
+    return out
+
+
+def same(got, want, bound):
+    """Infinities and NaN where the definition has them, the rest within the bound."""
+    x, fine = values_of(got), torch.isfinite(want)
+    assert torch.equal(torch.isnan(x), torch.isnan(want)) and torch.equal(x[~fine & ~torch.isnan(want)], want[~fine & ~torch.isnan(want)])
+    over = ((x - want).abs() - bound)[fine]
+    assert not over.numel() or float(over.max()) <= 0, (float(over.max()), int((over > 0).sum()), over.numel())
+
+
+# Rows of one warp that go different ways: of unlike alignment, with and without values that are no numbers, behind the last one.
+@gpu
+@pytest.mark.parametrize("kind,out", [("bf16", "bf16"), ("bf16", "words"), ("int8", "bf16")])
+@pytest.mark.parametrize("shape,hk,d,window", [([(201, 500)], 1, 64, 0), ([(201, 500)], 40, 128, 0), ([(77, 300), (130, 131), (50, 90)], 60, 32, 40)])
+def test_attention_rows_of_a_warp_go_different_ways(ctx, zkb, kind, out, shape, hk, d, window):
+    g, group = gen(d + hk), 3
+    batch, hq = Batch(shape, behind=1), group * hk
+    cache = Cache(g, kind, len(shape), hk, max(n for _, n in shape), d)
+    q = torch.randn(batch.n_rows, hq, d, generator=g, device="cuda").bfloat16()
+    if kind == "bf16":
+        for b, at, rows, pos in batch.each():
+            cache.v[b, :, pos + rows // 2, 3] = math.inf
+            cache.v[b, :, pos + rows - 3, ::7] = math.nan
+    room = torch.full((batch.n_rows * hq * (d + 1) + 1,), -3, device="cuda", dtype=torch.int32 if out == "words" else torch.bfloat16)
+    got = attend(ctx, zkb, batch, cache, q, room[1:].view(batch.n_rows, hq, d + 1)[..., :d], window, 2)
+    want, bound = attention_reference(batch, cache, q, d ** -0.5, window, 2)
+    last = sum(r for r, _ in shape)
+    same(got[:last], want[:last], bound[:last])
+    assert bool((got[last:] == -3).all()) and bool((room[1:].view(-1, d + 1)[:, d] == -3).all())

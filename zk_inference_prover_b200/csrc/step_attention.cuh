@@ -28,7 +28,10 @@ __device__ __forceinline__ void peer_store4(uint32_t at, int rank, uint32_t a, u
     asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(there), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 // A barrier of some of the thread block's warps.
-__device__ __forceinline__ void named_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+__device__ __forceinline__ void named_sync(int id, int threads) {
+    __syncwarp();
+    asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
 __device__ __forceinline__ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 __device__ __forceinline__ uint32_t ld_shared(uint32_t p) {
     uint32_t w;

@@ -332,6 +332,7 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
                         if (need) top = higher, less = higher, sum *= keep;
 #pragma unroll
                         for (int e = 0; e < 4; e++) part[e] = __float_as_uint(__uint_as_float(part[e]) * keep);
+                        __syncwarp();
                         tmem_stored();
 #pragma unroll 1
                         for (int i = 0; i < at / 2; i += 8) {  // this block's weights so far
@@ -402,36 +403,38 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
 #pragma unroll 1
                     for (int i = 0; i < D; i += 16) {
                         uint32_t o[2][8];
+                        __syncwarp();  // rows part ways below: not all are live, written alike or slow
                         if (any) tmem_load8(o_at + i, o[0]), tmem_load8(o_at + i + 8, o[1]), tmem_loaded(o[0]), tmem_loaded(o[1]);
-                        if (!live) continue;
-                        const int d = i;
-                        float z[16];
+                        if (live) {
+                            const int d = i;
+                            float z[16];
 #pragma unroll
-                        for (int e = 0; e < 16; e++) z[e] = sum == 0.f || !any ? 0.f : __uint_as_float(o[e / 8][e & 7]) * inverse;
-                        if (odd)
+                            for (int e = 0; e < 16; e++) z[e] = sum == 0.f || !any ? 0.f : __uint_as_float(o[e / 8][e & 7]) * inverse;
+                            if (odd)
 #pragma unroll
-                            for (int e = 0; e < 16; e++) z[e] += what_is_no_number(v, row_bytes, d + e, p, c.capacity, a.window, a.sinks);
-                        uint32_t w[8];
+                                for (int e = 0; e < 16; e++) z[e] += what_is_no_number(v, row_bytes, d + e, p, c.capacity, a.window, a.sinks);
+                            uint32_t w[8];
 #pragma unroll
-                        for (int e = 0; e < 8; e++) w[e] = pack_bf16(z[2 * e], z[2 * e + 1]);
-                        if (word) {
-                            uint32_t* const at = static_cast<uint32_t*>(a.out) + to + d;
+                            for (int e = 0; e < 8; e++) w[e] = pack_bf16(z[2 * e], z[2 * e + 1]);
+                            if (word) {
+                                uint32_t* const at = static_cast<uint32_t*>(a.out) + to + d;
 #pragma unroll
-                            for (int y = 0; y < 2; y++) {
-                                uint32_t x[8];
+                                for (int y = 0; y < 2; y++) {
+                                    uint32_t x[8];
 #pragma unroll
-                                for (int e = 0; e < 8; e++) x[e] = w[4 * y + e / 2] >> 16 * (e & 1) & 0xffffu;
-                                if (vec) store32(at + 8 * y, x);
+                                    for (int e = 0; e < 8; e++) x[e] = w[4 * y + e / 2] >> 16 * (e & 1) & 0xffffu;
+                                    if (vec) store32(at + 8 * y, x);
+                                    else
+#pragma unroll
+                                        for (int e = 0; e < 8; e++) at[8 * y + e] = x[e];
+                                }
+                            } else {
+                                uint16_t* const at = static_cast<uint16_t*>(a.out) + to + d;
+                                if (vec) store32(at, w);
                                 else
 #pragma unroll
-                                    for (int e = 0; e < 8; e++) at[8 * y + e] = x[e];
+                                    for (int e = 0; e < 16; e++) at[e] = (uint16_t)(w[e / 2] >> 16 * (e & 1));
                             }
-                        } else {
-                            uint16_t* const at = static_cast<uint16_t*>(a.out) + to + d;
-                            if (vec) store32(at, w);
-                            else
-#pragma unroll
-                                for (int e = 0; e < 16; e++) at[e] = (uint16_t)(w[e / 2] >> 16 * (e & 1));
                         }
                     }
                     if (odd) atomicAdd(&slow_sm, -1);
@@ -448,6 +451,7 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
                     peer_store(&in_top[whose * part + at], owner, top);
                     peer_store(&in_sum[whose * part + at], owner, sum);
                     if (at == 0 && !(u.split && tile)) peer_store(&in_odd[units.rank], owner, odd);
+                    __syncwarp();
 #pragma unroll 1
                     for (int i = 0; i < D; i += 32) {
                         uint32_t o[32];
