@@ -2,10 +2,11 @@
 ranges, launches that are refused. The references and bounds are those of tests/step_cases.py."""
 import math
 
+import numpy as np
 import pytest
 import torch
 
-from step_cases import Batch, Cache, attention_reference, values_of
+from step_cases import Batch, Cache, attention_reference, rope_reference, values_of, words
 from test_step_values import check_attention, done, gen
 
 gpu = pytest.mark.gpu
@@ -104,3 +105,50 @@ def test_attention_rows_of_a_warp_go_different_ways(ctx, zkb, kind, out, shape, 
     last = sum(r for r, _ in shape)
     same(got[:last], want[:last], bound[:last])
     assert bool((got[last:] == -3).all()) and bool((room[1:].view(-1, d + 1)[:, d] == -3).all())
+
+
+@gpu
+@pytest.mark.parametrize("source", ["bf16", "words"])
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+@pytest.mark.parametrize("d,rotary,interleaved", [(64, 0, 0), (64, 0, 1), (64, 16, 0), (128, 64, 1), (32, 16, 0), (128, 128, 0)])
+@pytest.mark.parametrize("norm", [False, True])
+def test_rotation_of_values_that_are_no_numbers(ctx, zkb, source, kind, d, rotary, interleaved, norm):
+    """What does not turn stays as it is, bit for bit, whatever lies beside it; what turns has infinities and NaN where the definition has them."""
+    g, hq, hk, rows = gen(d + rotary), 6, 3, 21
+    batch, cache = Batch([(rows, rows + 50)], behind=1), Cache(gen(0), kind, 1, hk, rows + 55, d, blank=True)
+    x = torch.randn(batch.n_rows, hq + 2 * hk, d, generator=g, device="cuda").bfloat16()
+    x[::2, :, rotary // 2::5] = -0.0
+    for i, (h, at) in enumerate([(0, d - 1), (1, rotary % d), (2, max(0, rotary - 1)), (hq, d - 3), (hq + 1, rotary // 2), (hq + hk, d // 2), (hq + hk + 1, 1)]):
+        x[3 + i, h, at] = [math.inf, -math.inf, math.nan][i % 3]
+        x[11 + i, h, at] = math.inf
+    weight = (1 + 0.3 * torch.randn(d, generator=g, device="cuda")).bfloat16()
+    freq = 10000.0 ** (-np.arange(rotary // 2) / max(1, rotary // 2))
+    laid, out = words(x) if source == "words" else x, torch.zeros(batch.n_rows, hq, d, device="cuda", dtype=torch.bfloat16)
+    at = lambda h: laid.data_ptr() + laid.element_size() * h * d  # noqa: E731
+    s, w = laid.stride(0), weight.data_ptr() if norm else 0
+    torch.cuda.synchronize()
+    ctx.step_norm_rope(zkb.StepNormRope(cache=cache.args(zkb), rows=batch.args(zkb), q=at(0), k=at(hq), v=at(hq + hk), q_weight=w, k_weight=w, h_inv_freq=freq.ctypes.data, q_out=out.data_ptr(),
+                                        q_stride=s, k_stride=s, v_stride=s, head_stride=d, q_out_stride=out.stride(0), q_out_head_stride=d, type=1 if source == "words" else 0, q_heads=hq,
+                                        rotary_dim=rotary, interleaved=interleaved, eps=1e-6))
+    done(ctx)
+    y, size = rope_reference(batch, x[:, :hq + hk], [weight if norm else None] * (hq + hk), 1e-6, freq, interleaved)
+    y, size, v = y[:rows], size[:rows], x[:rows, hq + hk:]
+    same(out[:rows], y[:, :hq], 2.0 ** -8 * y[:, :hq].abs() + 2.0 ** -18 * size[:, :hq])
+    bits = lambda t: t.contiguous().view(torch.int16)  # noqa: E731
+    alike = lambda a, b: bool(((bits(a) == bits(b)) | (a.isnan() & b.isnan())).all())  # noqa: E731
+    if not norm:
+        assert alike(out[:rows, :, rotary:], x[:rows, :hq, rotary:])
+    for part, scale, want, room in ((cache.k, cache.k_scale, y[:, hq:], size[:, hq:]), (cache.v, cache.v_scale, v.double(), 0 * v.double())):
+        got = part[0, :, 50:50 + rows].transpose(0, 1)
+        if kind == "bf16":
+            same(got, want, 2.0 ** -8 * want.abs() + 2.0 ** -18 * room)
+            if not norm:
+                old = x[:rows, hq:hq + hk] if part is cache.k else v
+                begin = rotary if part is cache.k else 0
+                assert alike(got[..., begin:], old[..., begin:])
+        else:  # one scale a head: an infinity's is infinite, a NaN's NaN
+            step, most = scale[0, :, 50:50 + rows].T.double(), want.abs().amax(-1)
+            same(step, most / 127, 2.0 ** -18 * (room.amax(-1) + most))
+            fine = torch.isfinite(most)
+            over = (got.double() * step[..., None] - want).abs() - step[..., None] * (0.5 + 127 * 2.0 ** -22) - 2.0 ** -18 * room.amax(-1, keepdim=True)
+            assert bool((over[fine] <= 0).all())
