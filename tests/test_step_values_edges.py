@@ -152,3 +152,28 @@ def test_rotation_of_values_that_are_no_numbers(ctx, zkb, source, kind, d, rotar
             fine = torch.isfinite(most)
             over = (got.double() * step[..., None] - want).abs() - step[..., None] * (0.5 + 127 * 2.0 ** -22) - 2.0 ** -18 * room.amax(-1, keepdim=True)
             assert bool((over[fine] <= 0).all())
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+@pytest.mark.parametrize("rows,hk", [(1, 2), (3, 2), (300, 2), (300, 40)])
+def test_attention_rows_whose_scores_are_all_minus_infinity_get_zeros(ctx, zkb, kind, rows, hk):
+    """Whatever the values are that they see, some of them no numbers."""
+    g, d, n = gen(rows), 64, rows + 150
+    batch, cache = Batch([(rows, n)]), Cache(g, kind, 1, hk, n, d)
+    q = torch.randn(rows, 4 * hk, d, generator=g, device="cuda").bfloat16()
+    q[..., 0] = q[..., 0].abs() + 0.25
+    if kind == "int8":
+        cache.k.zero_()
+        cache.k[..., 0] = -1
+        cache.k_scale.fill_(math.inf)
+        cache.v_scale[:, :, ::11] = math.nan
+    else:
+        cache.k[..., 0] = -math.inf
+        cache.v[:, :, ::11, ::3] = math.inf
+    q[rows // 2, 1, 0] = 0 if kind == "int8" else q[rows // 2, 1, 0]  # 0 times an infinity: NaN
+    got = attend(ctx, zkb, batch, cache, q, torch.full_like(q, 7))
+    if kind == "int8":
+        assert bool(got[rows // 2, 1].isnan().all())
+        got[rows // 2, 1] = 0
+    assert bool((got == 0).all())

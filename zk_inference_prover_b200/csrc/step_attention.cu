@@ -401,7 +401,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, (Few<D, INT8, T>::THREAD_BLOCK
             }
             y = all == 0.f ? 0.f : y / all;
             const int i0 = token(m);
-            if (!INT8 && set_aside) y += what_is_no_number(v, row_bytes, d, s.pos + i0, c.capacity, a.window, a.sinks);
+            if (!INT8 && set_aside && all != 0.f) y += what_is_no_number(v, row_bytes, d, s.pos + i0, c.capacity, a.window, a.sinks);
             const int64_t to = (s.first + i0) * a.out_stride + (kv_head * group + (int)m - i0 * group) * a.out_head_stride + d;
             if (a.out_type == ZKB_VALUE_WORD) static_cast<uint32_t*>(a.out)[to] = round_bf16(y);
             else static_cast<uint16_t*>(a.out)[to] = round_bf16(y);

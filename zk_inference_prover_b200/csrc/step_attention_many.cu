@@ -410,7 +410,7 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
                             float z[16];
 #pragma unroll
                             for (int e = 0; e < 16; e++) z[e] = sum == 0.f || !any ? 0.f : __uint_as_float(o[e / 8][e & 7]) * inverse;
-                            if (odd)
+                            if (odd && sum != 0.f)
 #pragma unroll
                                 for (int e = 0; e < 16; e++) z[e] += what_is_no_number(v, row_bytes, d + e, p, c.capacity, a.window, a.sinks);
                             uint32_t w[8];
@@ -498,7 +498,7 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         z[e] = inverse == 0.f ? 0.f : z[e] * inverse;
-                        if (set_aside) z[e] += what_is_no_number(v, row_bytes, d + e, u.s.pos + i0, c.capacity, a.window, a.sinks);
+                        if (set_aside && inverse != 0.f) z[e] += what_is_no_number(v, row_bytes, d + e, u.s.pos + i0, c.capacity, a.window, a.sinks);
                     }
                     const bool word = a.out_type == ZKB_VALUE_WORD;
                     char* const out = static_cast<char*>(a.out) + to * (word ? 4 : 2);
