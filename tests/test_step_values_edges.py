@@ -177,3 +177,31 @@ def test_attention_rows_whose_scores_are_all_minus_infinity_get_zeros(ctx, zkb, 
         assert bool(got[rows // 2, 1].isnan().all())
         got[rows // 2, 1] = 0
     assert bool((got == 0).all())
+
+
+def far_apart(g, shape, hq, d):
+    """Queries whose scores (by a scale of 3) lie so far apart that most weights are below the smallest float."""
+    return (6 * torch.randn(shape, hq, d, generator=g, device="cuda")).bfloat16()
+
+
+# A token's value that is no number reaches every row that sees the token, however small its weight: in blocks that all rows see and in others, with keys spread and not.
+@gpu
+@pytest.mark.parametrize("kind", ["bf16"])
+@pytest.mark.parametrize("shape,hk,d,window", [([(1, 1500)], 2, 128, 0), ([(3, 700), (2, 90)], 3, 64, 0), ([(300, 2000)], 1, 128, 0), ([(300, 1500)], 40, 64, 0), ([(200, 1200), (90, 90)], 30, 32, 400),
+                                               ([(100, 900)], 1, 64, 0)])
+def test_attention_values_that_are_no_numbers_under_weights_of_nothing(ctx, zkb, kind, shape, hk, d, window):
+    g, hq = gen(d + hk), 4 * hk
+    batch = Batch(shape)
+    cache = Cache(g, kind, len(shape), hk, max(n for _, n in shape), d)
+    for b, _, rows, pos in batch.each():
+        for i, j in enumerate([0, 5, 130, pos - 200, pos - 1]):
+            if 0 <= j < pos:
+                x = [math.inf, -math.inf, math.nan][(i + b) % 3]
+                if kind == "int8":
+                    cache.v[b, :, j][cache.v[b, :, j] == 0] = 1  # of a code of zero and an infinity the product is NaN: kept out of the comparison
+                    cache.v_scale[b, i % hk, j] = x
+                else:
+                    cache.v[b, i % hk, j, i::9] = x
+    q = far_apart(g, batch.n_rows, hq, d)
+    check_attention(ctx, zkb, batch, cache, q, "words" if window else "bf16", window, 4, scale=3.0)
+    check_attention(ctx, zkb, batch, cache, q, "bf16", window, 4, scale=-0.05)

@@ -165,8 +165,9 @@ __device__ __forceinline__ uint32_t numbers_only(uint32_t x) {
     if ((x & 0x7f800000u) == 0x7f800000u) x &= 0xffffu;
     return x;
 }
-// The sum of what is no number among the values of dimension d that the row at position p sees (bf16 caches): the products are made without
-// those values, because a matrix product has no way to keep 0 * NaN from the rows that do not see the key. Slow, and only for caches that hold such values.
+// The sum of what is no number among the values of dimension d that the row at position p sees (bf16 caches), which is that output where there is any. The products are
+// made without those values where a row does not see their key, because a matrix product has no way to keep 0 * NaN from it; where all rows do, what comes out is
+// no number either, though not always the same one (a weight too small for a float makes NaN of an infinity). Slow, and only for caches that hold such values.
 static __device__ __noinline__ float what_is_no_number(const char* v, int64_t row_bytes, int d, int64_t p, uint32_t capacity, uint32_t window, uint32_t sinks) {
     float y = 0.f;
     const int64_t end = min(p + 1, (int64_t)capacity), near = window ? max((int64_t)0, p - (int64_t)window + 1) : 0;

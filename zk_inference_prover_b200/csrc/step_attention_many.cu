@@ -104,6 +104,15 @@ __device__ __forceinline__ void add2(uint32_t& x, uint32_t& y, float a, float b)
 __device__ __forceinline__ void store32(void* to, const uint32_t (&x)[8]) {
     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7]) : "memory");
 }
+// An output again that is not what it should be where the row sees values that are no numbers: if it is no number either, or (`odd`) was made without some of them.
+static __device__ __noinline__ void put_what_is_no_number(const zkb_step_attention_args& a, int64_t at, bool odd, const char* v, int64_t row_bytes, int d, int64_t p) {
+    const uint32_t now = a.out_type == ZKB_VALUE_WORD ? static_cast<const uint32_t*>(a.out)[at] : static_cast<const uint16_t*>(a.out)[at];
+    if (!odd && (now & 0x7f80u) != 0x7f80u) return;
+    const float x = what_is_no_number(v, row_bytes, d, p, a.cache.capacity, a.window, a.sinks);
+    if (x == 0.f) return;
+    if (a.out_type == ZKB_VALUE_WORD) static_cast<uint32_t*>(a.out)[at] = round_bf16(x);
+    else static_cast<uint16_t*>(a.out)[at] = round_bf16(x);
+}
 // The lowest n bits.
 __device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 
@@ -399,7 +408,7 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
                     const int i0 = (int)((uint32_t)m / (uint32_t)group);
                     const int64_t to = live ? (u.s.first + i0) * a.out_stride + (u.kv_head * group + m - i0 * group) * a.out_head_stride : 0;
                     const bool word = a.out_type == ZKB_VALUE_WORD, vec = ((uintptr_t)(static_cast<char*>(a.out) + to * (word ? 4 : 2)) & 31) == 0;
-                    if (odd) atomicAdd(&slow_sm, 1);
+                    bool slow = odd;
 #pragma unroll 1
                     for (int i = 0; i < D; i += 16) {
                         uint32_t o[2][8];
@@ -410,12 +419,10 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
                             float z[16];
 #pragma unroll
                             for (int e = 0; e < 16; e++) z[e] = sum == 0.f || !any ? 0.f : __uint_as_float(o[e / 8][e & 7]) * inverse;
-                            if (odd && sum != 0.f)
+                            uint32_t w[8], test = 0;
 #pragma unroll
-                                for (int e = 0; e < 16; e++) z[e] += what_is_no_number(v, row_bytes, d + e, p, c.capacity, a.window, a.sinks);
-                            uint32_t w[8];
-#pragma unroll
-                            for (int e = 0; e < 8; e++) w[e] = pack_bf16(z[2 * e], z[2 * e + 1]);
+                            for (int e = 0; e < 8; e++) w[e] = pack_bf16(z[2 * e], z[2 * e + 1]), test = zero_or_nan(w[e], test);
+                            slow |= (test & 0x7fff7fffu) != 0;
                             if (word) {
                                 uint32_t* const at = static_cast<uint32_t*>(a.out) + to + d;
 #pragma unroll
@@ -437,7 +444,13 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
                             }
                         }
                     }
-                    if (odd) atomicAdd(&slow_sm, -1);
+                    // visible values that are no numbers: taken out where some row does not see their key, else lost where a weight or a factor of nothing met them
+                    if (!INT8 && slow && live && sum > 0.f) {
+                        atomicAdd(&slow_sm, 1);
+#pragma unroll 1
+                        for (int d = 0; d < D; d++) put_what_is_no_number(a, to + d, odd, v, row_bytes, d, p);
+                        atomicAdd(&slow_sm, -1);
+                    }
                 }
             } else {
                 // Each thread block finishes `part` of the rows: their sums go to [whose][row][four dimensions] of its shared memory, where Q and the keys were
@@ -480,6 +493,7 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
                     in_sum[at] = all == 0.f ? 0.f : 1.f / all;  // (this thread alone has read that place)
                 }
                 named_sync(4, 256);
+                bool slow = false;
 #pragma unroll 1
                 for (int i = threadIdx.x; i < part * (D / 4); i += 256) {
                     const int at = i / (D / 4), d = i % (D / 4) * 4;
@@ -496,13 +510,11 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
                     const int i0 = (int)((uint32_t)mm / (uint32_t)group);
                     const int64_t to = (u.s.first + i0) * a.out_stride + (u.kv_head * group + mm - i0 * group) * a.out_head_stride + d;
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        z[e] = inverse == 0.f ? 0.f : z[e] * inverse;
-                        if (set_aside && inverse != 0.f) z[e] += what_is_no_number(v, row_bytes, d + e, u.s.pos + i0, c.capacity, a.window, a.sinks);
-                    }
+                    for (int e = 0; e < 4; e++) z[e] = inverse == 0.f ? 0.f : z[e] * inverse;
                     const bool word = a.out_type == ZKB_VALUE_WORD;
                     char* const out = static_cast<char*>(a.out) + to * (word ? 4 : 2);
                     const uint32_t w0 = pack_bf16(z[0], z[1]), w1 = pack_bf16(z[2], z[3]);
+                    if (!INT8 && inverse > 0.f) slow |= set_aside || (zero_or_nan(w1, zero_or_nan(w0, 0)) & 0x7fff7fffu);
                     if (((uintptr_t)out & (word ? 15 : 7)) == 0) {
                         if (word) *reinterpret_cast<uint4*>(out) = make_uint4(w0 & 0xffffu, w0 >> 16, w1 & 0xffffu, w1 >> 16);
                         else *reinterpret_cast<uint2*>(out) = make_uint2(w0, w1);
@@ -513,6 +525,17 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
                             if (word) reinterpret_cast<uint32_t*>(out)[e] = h;
                             else reinterpret_cast<uint16_t*>(out)[e] = (uint16_t)h;
                         }
+                    }
+                }
+                if (!INT8 && slow) {  // as above
+#pragma unroll 1
+                    for (int i = threadIdx.x; i < part * (D / 4); i += 256) {
+                        const int at = i / (D / 4), d = i % (D / 4) * 4, mm = u.m0 + units.rank * part + at;
+                        if (mm >= u.n_m || !(in_sum[at] > 0.f)) continue;
+                        const int i0 = (int)((uint32_t)mm / (uint32_t)group);
+                        const int64_t to = (u.s.first + i0) * a.out_stride + (u.kv_head * group + mm - i0 * group) * a.out_head_stride + d;
+#pragma unroll 1
+                        for (int e = 0; e < 4; e++) put_what_is_no_number(a, to + e, set_aside, v, row_bytes, d + e, u.s.pos + i0);
                     }
                 }
                 if (again) {
