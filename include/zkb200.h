@@ -557,7 +557,8 @@ int zkb_step_norm_rope(zkb_ctx* ctx, const zkb_step_norm_rope_args* args);
 /* Attention of a step's rows over the cache (which holds the step's own tokens already). The row at position p sees key j when
  * 0 <= j <= p and (window == 0 or p - j < window or j < sinks): out = sum_j softmax_j(scale * q . k_j) v_j for each query head, kv head
  * h serving the q_heads / n_heads query heads from h * (q_heads / n_heads) on. A row that sees no key, or whose scores are all -inf, gets
- * zeros. What a row does not see does not reach it, whatever it holds (NaN and infinities among it). q is BF16; out is BF16 or WORD.
+ * zeros. What a row does not see does not reach it, whatever it holds (NaN and infinities among it); a value that is no number (of INT8 caches: a
+ * code times its scale) reaches every other row that sees its token, whatever the token's weight there. q is BF16; out is BF16 or WORD.
  * Scores, statistics and sums are 32-bit floats; the softmax's weights enter the product with v as bf16 numbers (for few
  * rows the sum of two). At most 64 query heads a kv head, and n_rows * q_heads below 2^31. */
 typedef struct zkb_step_attention_args {

@@ -186,7 +186,7 @@ def far_apart(g, shape, hq, d):
 
 # A token's value that is no number reaches every row that sees the token, however small its weight: in blocks that all rows see and in others, with keys spread and not.
 @gpu
-@pytest.mark.parametrize("kind", ["bf16"])
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
 @pytest.mark.parametrize("shape,hk,d,window", [([(1, 1500)], 2, 128, 0), ([(3, 700), (2, 90)], 3, 64, 0), ([(300, 2000)], 1, 128, 0), ([(300, 1500)], 40, 64, 0), ([(200, 1200), (90, 90)], 30, 32, 400),
                                                ([(100, 900)], 1, 64, 0)])
 def test_attention_values_that_are_no_numbers_under_weights_of_nothing(ctx, zkb, kind, shape, hk, d, window):
@@ -205,3 +205,41 @@ def test_attention_values_that_are_no_numbers_under_weights_of_nothing(ctx, zkb,
     q = far_apart(g, batch.n_rows, hq, d)
     check_attention(ctx, zkb, batch, cache, q, "words" if window else "bf16", window, 4, scale=3.0)
     check_attention(ctx, zkb, batch, cache, q, "bf16", window, 4, scale=-0.05)
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+@pytest.mark.parametrize("rows,hk", [(1, 2), (3, 2), (300, 2), (300, 40)])
+def test_attention_values_that_are_no_numbers_of_a_token_whose_score_is_minus_infinity(ctx, zkb, kind, rows, hk):
+    """They reach the rows that see it like any other's; the other tokens' weights are as without it."""
+    g, d, n = gen(rows), 64, rows + 300
+    batch, cache = Batch([(rows, n)]), Cache(g, kind, 1, hk, n, d)
+    q = torch.randn(rows, 4 * hk, d, generator=g, device="cuda").bfloat16()
+    q[..., 0] = q[..., 0].abs() + 0.25
+    for j in (7, 200, n - 3):
+        if kind == "int8":
+            cache.k[0, :, j] = 0
+            cache.k[0, :, j, 0] = -1
+            cache.k_scale[0, :, j] = math.inf
+        else:
+            cache.k[0, :, j] = 0.5
+            cache.k[0, :, j, 0] = -math.inf
+        if j == 200 and kind == "bf16":
+            cache.v[0, 0, j, 1::5] = math.inf
+        elif j == 200:
+            cache.v[0, 0, j] = 3
+            cache.v_scale[0, 0, j] = -math.inf
+    got = attend(ctx, zkb, batch, cache, q, torch.full_like(q, 7))
+    cache.k[0, :, [7, 200, n - 3]] = 0  # a definition without products of zero and infinity: those tokens' scores by hand
+    if kind == "int8":
+        cache.k_scale[0, :, [7, 200, n - 3]] = 1
+    k, v = cache.values()
+    p, j = torch.arange(n - rows, n, device="cuda")[:, None], torch.arange(n, device="cuda")
+    for h in range(4 * hk):
+        s = (q[:, h].double() @ k[0, h // 4].T * d ** -0.5).masked_fill(j > p, -math.inf)
+        s[:, [7, 200, n - 3]] = -math.inf
+        w, bad = torch.softmax(s, -1), ~torch.isfinite(v[0, h // 4])
+        want = w @ v[0, h // 4].masked_fill(bad, 0) + torch.where(bad[200], v[0, h // 4, 200], 0.0)
+        # as attention_reference counts: weights by 2^-8 and scores by 68 roundings of 2^-24 of magnitudes below 2^8, the result by 2^-8
+        bound = (2.0 ** -8 + 2.0 ** -9) * (w @ v[0, h // 4].masked_fill(bad, 0).abs() + want.abs())
+        same(got[:, h], want, bound)

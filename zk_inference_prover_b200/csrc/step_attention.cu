@@ -45,6 +45,7 @@ bool cache_maps(CacheMaps& maps, const zkb_kv_cache& c, uint32_t tokens) {
 // 64 sequences of 4,096 to 8,192 bf16 tokens, 32 heads on 8 of 128: 241 us, 6.7 TB/s; int8 tokens 174 us, 4.8 TB/s: their conversion keeps the warps' issue slots busy to 56 %, each of the two
 // products for a warp's sixteen keys waiting for it. One sequence of 2,048 int8 tokens: 9.4 us, most of it the launch and the joining.
 constexpr int FEW_WARPS = 8, FEW_RANKS = 16;
+constexpr float NO_SCORE = -3.40282346e38f;  // of a hidden key, the lowest number: a visible one's may be -inf; both weigh nothing
 
 // T: how many times eight rows a thread block has for the keys that it reads.
 template <int D, bool INT8, int T>
@@ -192,7 +193,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, (Few<D, INT8, T>::THREAD_BLOCK
             for (int r = 0; r < 2; r++) {
                 const int64_t m = m0 + 8 * n + 2 * t + r;
                 p[n][r] = m < n_m ? (int)s.pos + token(m) : -1;
-                top[n][r] = -INFINITY, less[n][r] = 0.f, sum[n][r] = 0.f;
+                top[n][r] = NO_SCORE, less[n][r] = 0.f, sum[n][r] = 0.f;
             }
 #pragma unroll
             for (int i = 0; i < STEPS; i++)
@@ -249,7 +250,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, (Few<D, INT8, T>::THREAD_BLOCK
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const int key = base + g + 8 * (i >> 1), gap = p[n][i & 1] - key;
-                        if (gap < 0 || key > last || (a.window != 0 && (uint32_t)gap >= a.window && (uint32_t)key >= a.sinks)) z[i] = -INFINITY;
+                        if (gap < 0 || key > last || (a.window != 0 && (uint32_t)gap >= a.window && (uint32_t)key >= a.sinks)) z[i] = NO_SCORE;
                     }
                 }
                 // The weights' common factor is 2^-top. It need not be the largest score's, only within 2^8 of it, so it is seldom that it changes.
@@ -260,7 +261,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, (Few<D, INT8, T>::THREAD_BLOCK
 #pragma unroll
                         for (int x = 4; x < 32; x <<= 1) higher = fmaxf(higher, __shfl_xor_sync(0xffffffffu, higher, x));
                         const float keep = higher > top[n][r] ? exp2_fast(top[n][r] - higher) : 1.f;
-                        sum[n][r] *= keep, top[n][r] = higher, less[n][r] = higher == -INFINITY ? 0.f : higher;
+                        sum[n][r] *= keep, top[n][r] = higher, less[n][r] = higher == NO_SCORE ? 0.f : higher;
 #pragma unroll
                         for (int i = 0; i < STEPS; i++) o[n][i][r] *= keep, o[n][i][r + 2] *= keep;
                     }
@@ -269,7 +270,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, (Few<D, INT8, T>::THREAD_BLOCK
                 for (int i = 0; i < 4; i++) {
                     const float e = exp2_fast(z[i] - less[n][i & 1]);
                     sum[n][i & 1] += e;
-                    z[i] = INT8 ? (z[i] == -INFINITY ? 0.f : e * v_by[i >> 1]) : e;  // a hidden token's scale may be anything
+                    z[i] = INT8 ? (z[i] == NO_SCORE ? 0.f : e * v_by[i >> 1]) : e;  // a hidden token's scale may be anything; a visible one's reaches the row whatever its score
                 }
                 // A weight is two bf16 numbers, its rounding and what that leaves: off by 2^-16 where the result's own rounding takes 2^-8. (One number alone: 64 sequences of 8,192
                 // int8 tokens in 164 us instead of 174, bf16 240 instead of 243, and results up to 1.6 times as far off.)
@@ -294,7 +295,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, (Few<D, INT8, T>::THREAD_BLOCK
 #pragma unroll
                         for (int x = 0; x < F::VW; x++) vw[i][x] = base + 2 * t + (i & 1) + 8 * (i >> 1) > last ? 0u : vw[i][x];
                 }
-                // a value that is no number would reach the rows that do not see its key: it is set aside (what_is_no_number)
+                // a value that is no number would reach the rows that do not see its key: it is set aside (put_what_is_no_number)
                 uint32_t test = 0;
 #pragma unroll
                 for (int i = 0; i < 4; i++)
@@ -356,7 +357,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, (Few<D, INT8, T>::THREAD_BLOCK
             float most = top_sm[0][r], all = 0.f, f[FEW_WARPS];
 #pragma unroll
             for (int w = 1; w < FEW_WARPS; w++) most = fmaxf(most, top_sm[w][r]);
-            const float base = most == -INFINITY ? 0.f : most;
+            const float base = most == NO_SCORE ? 0.f : most;
 #pragma unroll
             for (int w = 0; w < FEW_WARPS; w++) f[w] = exp2_fast(top_sm[w][r] - base), all += sum_sm[w][r] * f[w];
 #pragma unroll
@@ -389,10 +390,10 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, (Few<D, INT8, T>::THREAD_BLOCK
             const int r = (rank * part + i) / D, d = (rank * part + i) % D;
             const int64_t m = m0 + r;
             if (m >= n_m) continue;
-            float most = -INFINITY, y = 0.f, all = 0.f;
+            float most = NO_SCORE, y = 0.f, all = 0.f;
             int set_aside = 0;
             for (int x = 0; x < ranks; x++) most = fmaxf(most, in_top[x][r]);
-            const float base = most == -INFINITY ? 0.f : most;
+            const float base = most == NO_SCORE ? 0.f : most;
             for (int x = 0; x < ranks; x++) {
                 const float f = exp2_fast(in_top[x][r] - base);
                 y += in_o[x * part + i] * f;
@@ -401,10 +402,10 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, (Few<D, INT8, T>::THREAD_BLOCK
             }
             y = all == 0.f ? 0.f : y / all;
             const int i0 = token(m);
-            if (!INT8 && set_aside && all != 0.f) y += what_is_no_number(v, row_bytes, d, s.pos + i0, c.capacity, a.window, a.sinks);
             const int64_t to = (s.first + i0) * a.out_stride + (kv_head * group + (int)m - i0 * group) * a.out_head_stride + d;
             if (a.out_type == ZKB_VALUE_WORD) static_cast<uint32_t*>(a.out)[to] = round_bf16(y);
             else static_cast<uint16_t*>(a.out)[to] = round_bf16(y);
+            if ((INT8 ? !isfinite(y) : set_aside) && all > 0.f) put_what_is_no_number<INT8>(a, to, set_aside, seq, kv_head, d, s.pos + i0);
         }
         if (m0 + m_step < n_m) {  // the next rows' sums come to the same places
             if (ranks > 1) cluster_arrive(), cluster_wait();

@@ -165,19 +165,30 @@ __device__ __forceinline__ uint32_t numbers_only(uint32_t x) {
     if ((x & 0x7f800000u) == 0x7f800000u) x &= 0xffffu;
     return x;
 }
-// The sum of what is no number among the values of dimension d that the row at position p sees (bf16 caches), which is that output where there is any. The products are
-// made without those values where a row does not see their key, because a matrix product has no way to keep 0 * NaN from it; where all rows do, what comes out is
-// no number either, though not always the same one (a weight too small for a float makes NaN of an infinity). Slow, and only for caches that hold such values.
-static __device__ __noinline__ float what_is_no_number(const char* v, int64_t row_bytes, int d, int64_t p, uint32_t capacity, uint32_t window, uint32_t sinks) {
+// An output once more, of the row at position p, that is no number or (`odd`) was made without some that are none: where the row sees values of that dimension that are no numbers, it
+// is their sum. The products cannot have it right: 0 * NaN is not kept from the rows that do not see a key (bf16 values are taken out where there are such rows; 8-bit codes are
+// numbers, and their scales a part of each row's own weights), and a weight too small for a float makes NaN of an infinity. Slow, and only for caches that hold such values.
+template <bool INT8>
+static __device__ __noinline__ void put_what_is_no_number(const zkb_step_attention_args& a, int64_t at, bool odd, int seq, int kv_head, int d, int64_t p) {
+    const zkb_kv_cache& c = a.cache;
+    const bool word = a.out_type == ZKB_VALUE_WORD;
+    const uint32_t now = word ? static_cast<const uint32_t*>(a.out)[at] : static_cast<const uint16_t*>(a.out)[at];
+    if (!odd && (now & 0x7f80u) != 0x7f80u) return;
+    const int64_t from = seq * c.seq_stride + kv_head * c.head_stride + d, end = min(p + 1, (int64_t)c.capacity), near = a.window ? max((int64_t)0, p - (int64_t)a.window + 1) : 0;
+    const float* const scale = INT8 ? c.v_scale + seq * c.scale_seq_stride + kv_head * c.scale_head_stride : nullptr;
     float y = 0.f;
-    const int64_t end = min(p + 1, (int64_t)capacity), near = window ? max((int64_t)0, p - (int64_t)window + 1) : 0;
     for (int64_t j = 0; j < end; j++) {
-        if (j >= (int64_t)sinks && j < near) j = near;
+        if (j >= (int64_t)a.sinks && j < near) j = near;
         if (j >= end) break;
-        const float x = bf16_low(*reinterpret_cast<const uint16_t*>(v + j * row_bytes + 2 * d));
+        const int64_t place = from + j * c.token_stride;
+        float x;
+        if constexpr (INT8) x = (float)static_cast<const int8_t*>(c.v)[place] * scale[j];
+        else x = bf16_low(static_cast<const uint16_t*>(c.v)[place]);
         if (!isfinite(x)) y += x;
     }
-    return y;
+    if (y == 0.f) return;
+    if (word) static_cast<uint32_t*>(a.out)[at] = round_bf16(y);
+    else static_cast<uint16_t*>(a.out)[at] = round_bf16(y);
 }
 
 // The rows of a sequence: the first of them, how many, and the first one's position. Whatever the arrays hold, the rows are within n_rows.

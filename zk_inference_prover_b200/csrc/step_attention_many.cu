@@ -104,15 +104,6 @@ __device__ __forceinline__ void add2(uint32_t& x, uint32_t& y, float a, float b)
 __device__ __forceinline__ void store32(void* to, const uint32_t (&x)[8]) {
     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7]) : "memory");
 }
-// An output again that is not what it should be where the row sees values that are no numbers: if it is no number either, or (`odd`) was made without some of them.
-static __device__ __noinline__ void put_what_is_no_number(const zkb_step_attention_args& a, int64_t at, bool odd, const char* v, int64_t row_bytes, int d, int64_t p) {
-    const uint32_t now = a.out_type == ZKB_VALUE_WORD ? static_cast<const uint32_t*>(a.out)[at] : static_cast<const uint16_t*>(a.out)[at];
-    if (!odd && (now & 0x7f80u) != 0x7f80u) return;
-    const float x = what_is_no_number(v, row_bytes, d, p, a.cache.capacity, a.window, a.sinks);
-    if (x == 0.f) return;
-    if (a.out_type == ZKB_VALUE_WORD) static_cast<uint32_t*>(a.out)[at] = round_bf16(x);
-    else static_cast<uint16_t*>(a.out)[at] = round_bf16(x);
-}
 // The lowest n bits.
 __device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 
@@ -399,7 +390,6 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
                 wait(bars.o_ready[tile], done - 1);
                 tmem_fence_after();
             }
-            const char* const v = static_cast<const char*>(c.v) + (u.seq * c.seq_stride + u.kv_head * c.head_stride) * M::SIZE;
             auto odd_values = [&] { return !INT8 && u.n ? odd_sm[odd_at & 7] : 0; };
             if (!join) {
                 const int odd = odd_values();
@@ -444,11 +434,11 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
                             }
                         }
                     }
-                    // visible values that are no numbers: taken out where some row does not see their key, else lost where a weight or a factor of nothing met them
-                    if (!INT8 && slow && live && sum > 0.f) {
+                    // visible values that are no numbers: taken out (bf16) where some row does not see their key, else lost where a weight or a factor of nothing met them
+                    if (slow && live && sum > 0.f) {
                         atomicAdd(&slow_sm, 1);
 #pragma unroll 1
-                        for (int d = 0; d < D; d++) put_what_is_no_number(a, to + d, odd, v, row_bytes, d, p);
+                        for (int d = 0; d < D; d++) put_what_is_no_number<INT8>(a, to + d, odd, u.seq, u.kv_head, d, p);
                         atomicAdd(&slow_sm, -1);
                     }
                 }
@@ -514,7 +504,7 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
                     const bool word = a.out_type == ZKB_VALUE_WORD;
                     char* const out = static_cast<char*>(a.out) + to * (word ? 4 : 2);
                     const uint32_t w0 = pack_bf16(z[0], z[1]), w1 = pack_bf16(z[2], z[3]);
-                    if (!INT8 && inverse > 0.f) slow |= set_aside || (zero_or_nan(w1, zero_or_nan(w0, 0)) & 0x7fff7fffu);
+                    if (inverse > 0.f) slow |= set_aside || (zero_or_nan(w1, zero_or_nan(w0, 0)) & 0x7fff7fffu);
                     if (((uintptr_t)out & (word ? 15 : 7)) == 0) {
                         if (word) *reinterpret_cast<uint4*>(out) = make_uint4(w0 & 0xffffu, w0 >> 16, w1 & 0xffffu, w1 >> 16);
                         else *reinterpret_cast<uint2*>(out) = make_uint2(w0, w1);
@@ -527,7 +517,7 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
                         }
                     }
                 }
-                if (!INT8 && slow) {  // as above
+                if (slow) {  // as above
 #pragma unroll 1
                     for (int i = threadIdx.x; i < part * (D / 4); i += 256) {
                         const int at = i / (D / 4), d = i % (D / 4) * 4, mm = u.m0 + units.rank * part + at;
@@ -535,7 +525,7 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
                         const int i0 = (int)((uint32_t)mm / (uint32_t)group);
                         const int64_t to = (u.s.first + i0) * a.out_stride + (u.kv_head * group + mm - i0 * group) * a.out_head_stride + d;
 #pragma unroll 1
-                        for (int e = 0; e < 4; e++) put_what_is_no_number(a, to + e, set_aside, v, row_bytes, d + e, u.s.pos + i0);
+                        for (int e = 0; e < 4; e++) put_what_is_no_number<INT8>(a, to + e, set_aside, u.seq, u.kv_head, d + e, u.s.pos + i0);
                     }
                 }
                 if (again) {
@@ -706,7 +696,7 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
                                     }
 #pragma unroll
                                     for (int y = 0; y < 4; y++) test = zero_or_nan(w[y], test);
-                                    if (test & 0x7fff7fffu) {  // what is no number would reach the rows that do not see its key: it is set aside (what_is_no_number)
+                                    if (test & 0x7fff7fffu) {  // what is no number would reach the rows that do not see its key: it is set aside (put_what_is_no_number)
                                         odd = true;
 #pragma unroll
                                         for (int y = 0; y < 4; y++) w[y] = numbers_only(w[y]);
