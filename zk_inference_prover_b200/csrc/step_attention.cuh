@@ -177,14 +177,18 @@ static __device__ __noinline__ void put_what_is_no_number(const zkb_step_attenti
     const int64_t from = seq * c.seq_stride + kv_head * c.head_stride + d, end = min(p + 1, (int64_t)c.capacity), near = a.window ? max((int64_t)0, p - (int64_t)a.window + 1) : 0;
     const float* const scale = INT8 ? c.v_scale + seq * c.scale_seq_stride + kv_head * c.scale_head_stride : nullptr;
     float y = 0.f;
-    for (int64_t j = 0; j < end; j++) {
-        if (j >= (int64_t)a.sinks && j < near) j = near;
-        if (j >= end) break;
-        const int64_t place = from + j * c.token_stride;
-        float x;
-        if constexpr (INT8) x = (float)static_cast<const int8_t*>(c.v)[place] * scale[j];
-        else x = bf16_low(static_cast<const uint16_t*>(c.v)[place]);
-        if (!isfinite(x)) y += x;
+    for (int part = 0; part < 2; part++) {  // first tokens, window; several loads on their way; a NaN stays one
+        const int64_t to = part ? end : min(min((int64_t)a.sinks, near), end);
+        for (int64_t j0 = part ? near : 0; j0 < to && y == y; j0 += 64) {
+            const int64_t stop = min(j0 + 64, to);
+#pragma unroll 8
+            for (int64_t j = j0; j < stop; j++) {
+                float x;
+                if constexpr (INT8) x = (float)static_cast<const int8_t*>(c.v)[from + j * c.token_stride] * scale[j];
+                else x = bf16_low(static_cast<const uint16_t*>(c.v)[from + j * c.token_stride]);
+                y += isfinite(x) ? 0.f : x;
+            }
+        }
     }
     if (y == 0.f) return;
     if (word) static_cast<uint32_t*>(a.out)[at] = round_bf16(y);
