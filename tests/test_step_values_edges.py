@@ -243,3 +243,15 @@ def test_attention_values_that_are_no_numbers_of_a_token_whose_score_is_minus_in
         # as attention_reference counts: weights by 2^-8 and scores by 68 roundings of 2^-24 of magnitudes below 2^8, the result by 2^-8
         bound = (2.0 ** -8 + 2.0 ** -9) * (w @ v[0, h // 4].masked_fill(bad, 0).abs() + want.abs())
         same(got[:, h], want, bound)
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+@pytest.mark.parametrize("rows", [1, 3, 300])
+@pytest.mark.parametrize("window,sinks", [((1 << 31) - 10, 0), ((1 << 31) - 250, 3), ((1 << 31) + 5, 0), ((1 << 32) - 1, 7), ((1 << 30) + 3, 2)])
+def test_attention_windows_of_more_than_2_to_the_30(ctx, zkb, kind, rows, window, sinks):
+    """The rows of the last positions that there are, over the first tokens: what a window of about as many leaves of them."""
+    g, cap = gen(rows), 70
+    batch, cache = Batch([(rows, (1 << 31) - 1), (rows, 60)]), Cache(g, kind, 2, 4, cap, 64)
+    q = torch.randn(batch.n_rows, 16, 64, generator=g, device="cuda").bfloat16()
+    check_attention(ctx, zkb, batch, cache, q, "bf16", window, sinks)

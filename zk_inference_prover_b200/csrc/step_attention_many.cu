@@ -280,7 +280,7 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
             const int m = row_of(u);  // this thread's row
             const bool live = m < u.n_m;
             const int p = live ? (int)u.s.pos + (int)((uint32_t)m / (uint32_t)group) : -1;
-            const int low = a.window ? max(0, p - (int)min(a.window, 1u << 30) + 1) : 0, high = min(p, u.last), sinks = a.window ? (int)min(a.sinks, c.capacity) : 0;
+            const int low = a.window ? (int)max((int64_t)0, (int64_t)p - (int64_t)a.window + 1) : 0, high = min(p, u.last), sinks = a.window ? (int)min(a.sinks, c.capacity) : 0;
             const bool again = units.next(after);
             if (again) {  // the next unit's Q comes nearer
                 const int mm = row_of(after);
