@@ -560,7 +560,7 @@ int zkb_step_norm_rope(zkb_ctx* ctx, const zkb_step_norm_rope_args* args);
  * zeros. What a row does not see does not reach it, whatever it holds (NaN and infinities among it); a value that is no number (of INT8 caches: a
  * code times its scale) reaches every other row that sees its token, whatever the token's weight there. q is BF16; out is BF16 or WORD.
  * Scores, statistics and sums are 32-bit floats; the softmax's weights enter the product with v as bf16 numbers (for few
- * rows the sum of two). At most 64 query heads a kv head, and n_rows * q_heads below 2^31. */
+ * rows the sum of two). At most 64 query heads a kv head, n_rows * q_heads below 2^31 and, of one kv head, at most 2^31 - 256. */
 typedef struct zkb_step_attention_args {
     zkb_kv_cache cache;
     zkb_step_rows rows;

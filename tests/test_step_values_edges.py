@@ -7,9 +7,15 @@ import pytest
 import torch
 
 from step_cases import Batch, Cache, attention_reference, rope_reference, values_of, words
-from test_step_values import check_attention, done, gen
+from test_step_values import _attention_args, check_attention, done, gen, refuse  # noqa: F401
 
 gpu = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("n_rows,group,heads", [((1 << 30) - 1, 2, 1), ((1 << 30) - 127, 2, 1), (((1 << 31) - 254) // 3 + 1, 3, 1), ((1 << 30) - 1, 2, 3), (1 << 29, 2, 2)])
+def test_attention_refuses_more_rows_of_a_head_than_it_can_number(zkb, refuse, n_rows, group, heads):  # noqa: F811
+    """Up to 2^31 - 256 rows of a kv head: tiles are numbered by the row behind their last one."""
+    refuse("zkb_step_attention", _attention_args(zkb, dict(n_heads=heads), dict(n_rows=n_rows), q_heads=group * heads), "n_rows")
 
 
 def hinted(batch, max_rows, max_len):

@@ -477,7 +477,7 @@ extern "C" int zkb_step_attention(zkb_ctx* ctx, const zkb_step_attention_args* a
     const zkb_kv_cache& c = a.cache;
     if (const char* why = step_problem(c, a.rows, a.q_heads)) return set_error(ctx, ZKB_EINVAL, "zkb_step_attention: %s", why);
     ZKB_CHECK_ARG(ctx, a.out_type == ZKB_VALUE_BF16 || a.out_type == ZKB_VALUE_WORD);
-    ZKB_CHECK_ARG(ctx, std::isfinite(a.scale) && (uint64_t)a.rows.n_rows * a.q_heads <= 0x7fffffffu);
+    ZKB_CHECK_ARG(ctx, std::isfinite(a.scale) && (uint64_t)a.rows.n_rows * a.q_heads <= 0x7fffffffu && (uint64_t)a.rows.n_rows * (a.q_heads / c.n_heads) <= 0x7fffff00u);
     if (a.rows.n_rows == 0) return ZKB_OK;
     ZKB_CHECK_ARG(ctx, a.q && a.out && aligned_to(a.q, 2) && aligned_to(a.out, a.out_type == ZKB_VALUE_WORD ? 4 : 2));
     ZKB_CHECK_ARG(ctx, a.q_heads == 1 || std::llabs(a.out_head_stride) >= (long long)c.head_dim);
