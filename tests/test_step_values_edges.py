@@ -261,3 +261,29 @@ def test_attention_windows_of_more_than_2_to_the_30(ctx, zkb, kind, rows, window
     batch, cache = Batch([(rows, (1 << 31) - 1), (rows, 60)]), Cache(g, kind, 2, 4, cap, 64)
     q = torch.randn(batch.n_rows, 16, 64, generator=g, device="cuda").bfloat16()
     check_attention(ctx, zkb, batch, cache, q, "bf16", window, sinks)
+
+
+@gpu
+@pytest.mark.parametrize("source", ["bf16", "words"])
+@pytest.mark.parametrize("d", [32, 128])
+def test_int8_codes_of_the_smallest_heads(ctx, zkb, source, d):
+    """Heads down to the smallest bf16 number, 2^-133, whose scales are among the smallest floats (steps of 2^-149: a scale is off by up to 2^-150, a value of 127 of them by 2^-143)."""
+    g, hk, rows = gen(d), 2, 140
+    batch, cache = Batch([(rows, rows)]), Cache(gen(0), "int8", 1, hk, rows, d, blank=True)
+    x = torch.rand(rows, 3 * hk, d, generator=g, device="cuda", dtype=torch.float64) * 2 - 1
+    x = (x * torch.exp2(-torch.arange(rows, device="cuda", dtype=torch.float64))[:, None, None]).bfloat16()
+    x[7:] *= torch.randint(0, 2, (rows - 7, 3 * hk, 1), generator=g, device="cuda")  # heads of zeros among them
+    laid, out = words(x) if source == "words" else x, torch.zeros(rows, hk, d, device="cuda", dtype=torch.bfloat16)
+    at = lambda h: laid.data_ptr() + laid.element_size() * h * d  # noqa: E731
+    s = laid.stride(0)
+    torch.cuda.synchronize()
+    ctx.step_norm_rope(zkb.StepNormRope(cache=cache.args(zkb), rows=batch.args(zkb), q=at(0), k=at(hk), v=at(2 * hk), q_out=out.data_ptr(), q_stride=s, k_stride=s, v_stride=s, head_stride=d,
+                                        q_out_stride=out.stride(0), q_out_head_stride=d, type=1 if source == "words" else 0, q_heads=hk, rotary_dim=0, eps=1e-6))
+    done(ctx)
+    for part, scale, h in ((cache.k, cache.k_scale, hk), (cache.v, cache.v_scale, 2 * hk)):
+        y, codes, step = x[:, h:h + hk].double(), part[0].transpose(0, 1).double(), scale[0].T.double()
+        most = y.abs().amax(-1)
+        assert bool(((step - most / 127).abs() <= 2.0 ** -24 * most / 127 + 2.0 ** -150).all())
+        ideal = y * 127 / torch.where(most > 0, most, 1.0)[..., None]
+        assert bool(((codes - ideal).abs() <= 0.5 + 127 * 2.0 ** -22).all())
+        assert bool(((codes * step[..., None] - y).abs() <= step[..., None] * (0.5 + 127 * 2.0 ** -22) + 2.0 ** -142).all())

@@ -237,7 +237,13 @@ __global__ void __launch_bounds__(128, 6) norm_rope_kernel(const __grid_constant
                     for (int o = LANES / 2; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
                     if (__ballot_sync(0xffffffffu, nan) >> (mine * LANES) & (LANES == 32 ? 0xffffffffu : (1u << LANES % 32) - 1u)) most = __int_as_float(0x7fc00000);
                     if (has && cached) {
-                        const float up = most > 0.f ? 127.f / most : 0.f;  // zeros' codes are 0, a NaN's and those of an infinite scale likewise
+                        float top = most;
+                        if (most < 0x1p-64f) {  // (127 over less than 2^-121 is no float)
+                            top *= 0x1p64f;
+#pragma unroll
+                            for (int y = 0; y < 8; y++) x[y] *= 0x1p64f;
+                        }
+                        const float up = top > 0x1.fcp-80f ? 127.f / top : 0.f;  // codes are 0 where the scale is (up to 127 x 2^-150), and where it is NaN or infinite
                         uint32_t q[2] = {0, 0};
 #pragma unroll
                         for (int y = 0; y < 8; y++) q[y / 4] |= (uint32_t)(max(-127, min(127, __float2int_rn(x[y] * up))) & 255) << (8 * (y % 4));
