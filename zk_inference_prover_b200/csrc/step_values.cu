@@ -215,14 +215,14 @@ __global__ void __launch_bounds__(128, 6) norm_rope_kernel(const __grid_constant
                     if (a.interleaved) {
 #pragma unroll
                         for (int y = 0; y < 4; y++) {
-                            const float u = x[2 * y], v = x[2 * y + 1];
-                            x[2 * y] = turned ? u * c[y] - v * s[y] : u, x[2 * y + 1] = turned ? u * s[y] + v * c[y] : v;
+                            const float u = x[2 * y], v = x[2 * y + 1], r = u * c[y] - v * s[y], t = u * s[y] + v * c[y];
+                            x[2 * y] = turned ? r : u, x[2 * y + 1] = turned ? t : v;
                         }
                     } else {
 #pragma unroll
                         for (int y = 0; y < 4; y++) {
-                            const float u = x[y], v = x[y + 4];
-                            x[y] = turned ? u * c[y] - v * s[y] : u, x[y + 4] = turned ? u * s[y] + v * c[y] : v;
+                            const float u = x[y], v = x[y + 4], r = u * c[y] - v * s[y], t = u * s[y] + v * c[y];
+                            x[y] = turned ? r : u, x[y + 4] = turned ? t : v;
                         }
                     }
                 }
