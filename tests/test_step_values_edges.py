@@ -287,3 +287,19 @@ def test_int8_codes_of_the_smallest_heads(ctx, zkb, source, d):
         ideal = y * 127 / torch.where(most > 0, most, 1.0)[..., None]
         assert bool(((codes - ideal).abs() <= 0.5 + 127 * 2.0 ** -22).all())
         assert bool(((codes * step[..., None] - y).abs() <= step[..., None] * (0.5 + 127 * 2.0 ** -22) + 2.0 ** -142).all())
+
+
+@gpu
+def test_attention_weights_are_rounded_once(ctx, zkb):
+    """Weights of the first half of a block whose second half has a score more than 2^8 times above: 63 alike, so that their roundings add up, for 512 weights a row apiece and 64 later
+    scores. The bound has one rounding of a weight and the result's."""
+    rows, hq, d = 512, 64, 64
+    n = rows + 128
+    batch, cache = Batch([(rows, n)]), Cache(gen(0), "bf16", 1, 1, n, d, blank=True)
+    q = torch.zeros(rows, hq, d, device="cuda")
+    q[..., 0], q[..., 1] = torch.linspace(0.01, 3.9, rows, device="cuda")[:, None], torch.linspace(8.6, 14, hq, device="cuda")
+    cache.k[0, 0, :63, 0] = -1
+    cache.k[0, 0, 64, 1] = 1
+    cache.k[0, 0, 65:, 1] = -16
+    cache.v[0, 0, :63] = 1
+    check_attention(ctx, zkb, batch, cache, q.bfloat16(), "bf16", 0, 0, scale=math.log(2.0))
