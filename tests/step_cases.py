@@ -69,11 +69,11 @@ class Cache:
         return self.k.double(), self.v.double()
 
 
-def attention_reference(batch, cache, q, scale, window, sinks):
+def attention_reference(batch, cache, q, scale, window, sinks, weight=2.0 ** -8):
     """(out, bound): the definition in 64 bits, nan in rows of no sequence, and how far an output may be from it.
 
     Scores are sums of D products in 32 bits: off by D + 4 roundings of 2^-24 of the sum of their magnitudes B, and so the weights by that
-    much relatively, by 2^-20 for the exponential and the scores' own size in it, and by a bf16 rounding 2^-8; the sum of n weights in 32 bits adds n 2^-24.
+    much relatively, by 2^-20 for the exponential and the scores' own size in it, and by a bf16 rounding 2^-8 (`weight`; two bf16 numbers: 2^-16); the sum of n weights in 32 bits adds n 2^-24.
     The result takes another 2^-8. None of this is relative below 2^-126, where 32-bit floats and bf16 have a fixed step of at most 2^-133, or nothing:
     a weight is then off by up to 2^-126, n of them by n 2^-126 of the largest value, the result by another 2^-126."""
     n, hq, d = q.shape
@@ -102,7 +102,7 @@ def attention_reference(batch, cache, q, scale, window, sinks):
             for key in bad.any(-1).nonzero().flatten().tolist():
                 o = o + torch.where(seen[:, key, None] & bad[key], vv[key], torch.zeros_like(vv[key]))
             out[at:at + rows, h] = o
-            rel = 2.0 ** -8 + 2 * (d + 4) * 2.0 ** -24 * size.amax(-1, keepdim=True) + 2.0 ** -19 + seen.sum(-1, keepdim=True) * 2.0 ** -24
+            rel = weight + 2 * (d + 4) * 2.0 ** -24 * size.amax(-1, keepdim=True) + 2.0 ** -19 + seen.sum(-1, keepdim=True) * 2.0 ** -24
             least = 2.0 ** -126 * (1 + seen.sum(-1, keepdim=True) * clean.abs().amax(0))
             bound[at:at + rows, h] = (rel * a) * (1 + 2.0 ** -8) + 2.0 ** -8 * o.abs() + least
     return out, bound

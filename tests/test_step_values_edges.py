@@ -303,3 +303,20 @@ def test_attention_weights_are_rounded_once(ctx, zkb):
     cache.k[0, 0, 65:, 1] = -16
     cache.v[0, 0, :63] = 1
     check_attention(ctx, zkb, batch, cache, q.bfloat16(), "bf16", 0, 0, scale=math.log(2.0))
+
+
+# What the few rows' kernel says of its weights: two bf16 numbers, off by 2^-16. Means of a few hundred values of either sign are so far below them that one number's 2^-8
+# would show (worked out with one: 57 of 1,024 values of 300 tokens and 128 dimensions are out of the bound).
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+@pytest.mark.parametrize("shape,hq,hk,d,window,long", [([(1, 300)], 32, 8, 128, 0, False), ([(1, 200), (1, 64), (1, 333)], 8, 2, 128, 0, False), ([(3, 333), (2, 64)], 6, 3, 32, 0, False),
+                                                       ([(4, 250)], 16, 2, 64, 0, False), ([(1, 3000)] * 6, 16, 4, 64, 200, False), ([(8, 300)], 16, 4, 128, 0, True), ([(5, 250), (8, 200)], 16, 4, 64, 0, True)])
+def test_attention_weights_of_few_rows(ctx, zkb, kind, shape, hq, hk, d, window, long):
+    """`long`: caches that have room for 1,600 tokens and hints that say so, for which int8 caches have sixteen rows a product."""
+    g = gen(d + hq)
+    batch, cache = Batch(shape), Cache(g, kind, len(shape), hk, 1600 if long else max(n for _, n in shape), d)
+    if long:
+        hinted(batch, max(r for r, _ in shape), 1600)
+    q = torch.randn(batch.n_rows, hq, d, generator=g, device="cuda").bfloat16()
+    got = attend(ctx, zkb, batch, cache, q, torch.zeros_like(q), window, 4)
+    same(got, *attention_reference(batch, cache, q, d ** -0.5, window, 4, weight=2.0 ** -16))
