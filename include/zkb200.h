@@ -523,7 +523,8 @@ typedef struct zkb_kv_cache {
  * kv_len[b] tokens in all, the step's own among them: its rows are the tokens at positions kv_len[b] - rows .. kv_len[b] - 1.
  * Rows from first[n_seqs] on are left as they were. Positions below zero or from the capacity on are not in the cache: they are
  * neither written nor seen. max_rows and max_len are the most rows and tokens of any sequence as the host knows them (0: it does
- * not); they decide how the work is laid out, never what is computed. */
+ * not). They decide how the work is laid out, and with it the order of sums and which of the roundings named below an output
+ * has had; what rows see, and that every row is done, does not depend on them. */
 typedef struct zkb_step_rows {
     const int32_t* first;  /* n_seqs + 1 */
     const int32_t* kv_len; /* n_seqs */
@@ -559,8 +560,11 @@ int zkb_step_norm_rope(zkb_ctx* ctx, const zkb_step_norm_rope_args* args);
  * h serving the q_heads / n_heads query heads from h * (q_heads / n_heads) on. A row that sees no key, or whose scores are all -inf, gets
  * zeros. What a row does not see does not reach it, whatever it holds (NaN and infinities among it); a value that is no number (of INT8 caches: a
  * code times its scale) reaches every other row that sees its token, whatever the token's weight there. q is BF16; out is BF16 or WORD.
- * Scores, statistics and sums are 32-bit floats; the softmax's weights enter the product with v as bf16 numbers (for few
- * rows the sum of two). At most 64 query heads a kv head, n_rows * q_heads below 2^31 and, of one kv head, at most 2^31 - 256. */
+ * Scores, statistics and sums are 32-bit floats. The softmax's weights (INT8 caches: times the token's v_scale) enter the product with v
+ * as bf16 numbers, each rounded once, off by 2^-8; where the rows are few, by the batch's size and the hints, each is the sum of two, off by
+ * 2^-16. INT8 caches: queries enter theirs as fp16 numbers, each row scaled by a power of two, exact but for values below 2^-27 of the row's
+ * largest, which are off by up to 2^-38 of that. At most 64 query heads a kv head, n_rows * q_heads below 2^31 and, of one kv head, at most
+ * 2^31 - 256. */
 typedef struct zkb_step_attention_args {
     zkb_kv_cache cache;
     zkb_step_rows rows;
