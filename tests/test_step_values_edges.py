@@ -320,3 +320,16 @@ def test_attention_weights_of_few_rows(ctx, zkb, kind, shape, hq, hk, d, window,
     q = torch.randn(batch.n_rows, hq, d, generator=g, device="cuda").bfloat16()
     got = attend(ctx, zkb, batch, cache, q, torch.zeros_like(q), window, 4)
     same(got, *attention_reference(batch, cache, q, d ** -0.5, window, 4, weight=2.0 ** -16))
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+@pytest.mark.parametrize("most", [1, 2, 4, 8])
+def test_attention_whose_clusters_are_refused(ctx, zkb, monkeypatch, kind, most):
+    """Keys spread over fewer thread blocks than planned: a token of one sequence and several, few rows of a long cache, many rows."""
+    monkeypatch.setenv("ZKB_STEP_CLUSTERS", str(most))
+    for shape, hk, d, window in (([(1, 3000)], 2, 128, 0), ([(1, 900), (2, 2100)], 3, 64, 0), ([(8, 2500)], 1, 32, 0), ([(300, 2000)], 1, 128, 0), ([(90, 1700), (100, 1500)], 2, 64, 900)):
+        g = gen(d + hk)
+        batch, cache = Batch(shape), Cache(g, kind, len(shape), hk, max(n for _, n in shape), d)
+        q = torch.randn(batch.n_rows, 4 * hk, d, generator=g, device="cuda").bfloat16()
+        check_attention(ctx, zkb, batch, cache, q, "bf16", window, 5)

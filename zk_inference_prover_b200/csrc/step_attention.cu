@@ -434,17 +434,19 @@ static cudaError_t launch_few(zkb_ctx* ctx, const zkb_step_attention_args& a) {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, F::SMEM);
     if (e != cudaSuccess) return e;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim = {ranks, 1, 1};
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(tiles * ranks, c.n_heads, c.n_seqs);
-    cfg.blockDim = dim3(FEW_WARPS * 32);
-    cfg.dynamicSmemBytes = F::SMEM;
-    cfg.stream = ctx->stream;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, a, maps, ctx->dev_err);
+    return launch_clusters(ranks, [&](uint32_t n) {
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim = {n, 1, 1};
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(tiles * n, c.n_heads, c.n_seqs);
+        cfg.blockDim = dim3(FEW_WARPS * 32);
+        cfg.dynamicSmemBytes = F::SMEM;
+        cfg.stream = ctx->stream;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        return cudaLaunchKernelEx(&cfg, kernel, a, maps, ctx->dev_err);
+    });
 }
 
 template <int D>

@@ -2,6 +2,9 @@
 #pragma once
 #include <cuda.h>
 
+#include <algorithm>
+#include <cstdlib>
+
 #include "step_values.cuh"
 
 namespace zk {
@@ -85,6 +88,19 @@ bool cache_maps(CacheMaps& maps, const zkb_kv_cache& c, uint32_t tokens);
 // How many clusters of 1, 2, 4, 8 or 16 thread blocks the GPU holds at a time with one thread block an SM (cudaOccupancyMaxActiveClusters): a cluster lies in one of
 // the GPU's eight groups of 16 to 20 SMs. Clusters that have to wait for others double the time: eight of 16 take 38 us where eight of 8 take 25.
 inline uint32_t clusters_at_once(uint32_t ranks) { return ranks <= 1 ? 148 : ranks == 2 ? 74 : ranks == 4 ? 33 : ranks == 8 ? 15 : 7; }
+
+// Launches clusters of `ranks` (a power of two) thread blocks, or of fewer where the device, or the share of it that this process has, does not take as many.
+// ZKB_STEP_CLUSTERS: as though it took that many at most, to try these ways.
+template <class Launch>
+inline cudaError_t launch_clusters(uint32_t ranks, Launch launch) {
+    const char* const env = getenv("ZKB_STEP_CLUSTERS");
+    const uint32_t most = env ? (uint32_t)std::max(1, atoi(env)) : ranks;
+    for (;; ranks /= 2) {
+        const cudaError_t e = ranks <= most ? launch(ranks) : cudaErrorInvalidClusterSize;
+        if (ranks == 1 || (e != cudaErrorInvalidClusterSize && e != cudaErrorInvalidConfiguration && e != cudaErrorLaunchOutOfResources && e != cudaErrorNotSupported)) return e;
+        (void)cudaGetLastError();
+    }
+}
 
 template <int D, bool INT8>
 cudaError_t launch_many(zkb_ctx* ctx, const zkb_step_attention_args& a);  // step_attention_many.cu

@@ -757,17 +757,19 @@ cudaError_t launch_many(zkb_ctx* ctx, const zkb_step_attention_args& a) {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, M::SMEM);
     if (e != cudaSuccess) return e;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim = {ranks, 1, 1};
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((uint32_t)std::min<uint64_t>(units, clusters_at_once(ranks)) * ranks);
-    cfg.blockDim = dim3(M::THREADS);
-    cfg.dynamicSmemBytes = M::SMEM;
-    cfg.stream = ctx->stream;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, a, maps, pairs, ctx->dev_err);
+    return launch_clusters(ranks, [&](uint32_t n) {
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim = {n, 1, 1};
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((uint32_t)std::min<uint64_t>(units, clusters_at_once(n)) * n);
+        cfg.blockDim = dim3(M::THREADS);
+        cfg.dynamicSmemBytes = M::SMEM;
+        cfg.stream = ctx->stream;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        return cudaLaunchKernelEx(&cfg, kernel, a, maps, pairs, ctx->dev_err);
+    });
 }
 template cudaError_t launch_many<32, false>(zkb_ctx*, const zkb_step_attention_args&);
 template cudaError_t launch_many<64, false>(zkb_ctx*, const zkb_step_attention_args&);
