@@ -333,3 +333,11 @@ def test_attention_whose_clusters_are_refused(ctx, zkb, monkeypatch, kind, most)
         batch, cache = Batch(shape), Cache(g, kind, len(shape), hk, max(n for _, n in shape), d)
         q = torch.randn(batch.n_rows, 4 * hk, d, generator=g, device="cuda").bfloat16()
         check_attention(ctx, zkb, batch, cache, q, "bf16", window, 5)
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+@pytest.mark.parametrize("shape,d", [([(8, 300)], 128), ([(5, 250), (8, 200)], 64), ([(3, 290), (4, 150)], 32)])
+def test_attention_weights_of_few_rows_of_many_heads(ctx, zkb, kind, shape, d):
+    """As above where eight rows a product would have thread blocks share SMs."""
+    test_attention_weights_of_few_rows(ctx, zkb, kind, shape, 64, 16, d, 0, True)

@@ -415,31 +415,45 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, (Few<D, INT8, T>::THREAD_BLOCK
     if (!begun) cluster_wait();
 }
 
+// How a call is laid out: `tiles` of T times eight rows a kv head of the longest sequence, each spread over `ranks` thread blocks.
+struct FewPlan {
+    uint64_t len, units;
+    uint32_t tiles, ranks;
+};
 template <int D, bool INT8, int T>
-static cudaError_t launch_few(zkb_ctx* ctx, const zkb_step_attention_args& a) {
+static FewPlan plan_few(const zkb_step_attention_args& a) {
     const zkb_kv_cache& c = a.cache;
     const uint32_t group = a.q_heads / c.n_heads, most = a.rows.max_rows ? std::min(a.rows.max_rows, a.rows.n_rows) : a.rows.n_rows;
     using F = Few<D, INT8, T>;
-    const uint32_t tiles = (uint32_t)std::min<uint64_t>(((uint64_t)most * group + F::ROWS - 1) / F::ROWS, 1u << 20);
-    uint64_t len = a.rows.max_len ? std::min(a.rows.max_len, c.capacity) : c.capacity;
-    if (a.window) len = std::min<uint64_t>(len, (uint64_t)a.window + a.sinks + 32);
+    FewPlan p;
+    p.tiles = (uint32_t)std::min<uint64_t>(((uint64_t)most * group + F::ROWS - 1) / F::ROWS, 1u << 20);
+    p.len = a.rows.max_len ? std::min(a.rows.max_len, c.capacity) : c.capacity;
+    if (a.window) p.len = std::min<uint64_t>(p.len, (uint64_t)a.window + a.sinks + 32);
     // Split a sequence over more thread blocks while all of them are on the GPU at once and each warp keeps two blocks of keys: 16 sequences of 1,028 visible
     // bf16 tokens take 14.6 us in 128 thread blocks and 22.8 in 256, one of 2,048 int8 tokens 23.2 in 8 and 10.6 in 64.
-    const uint64_t units = (uint64_t)c.n_seqs * c.n_heads * tiles;
-    uint32_t ranks = 1;
-    while (ranks < FEW_RANKS && units <= clusters_at_once(2 * ranks) * F::THREAD_BLOCKS && len > (uint64_t)ranks * FEW_WARPS * 16 * 2) ranks *= 2;
+    p.units = (uint64_t)c.n_seqs * c.n_heads * p.tiles;
+    p.ranks = 1;
+    while (p.ranks < FEW_RANKS && p.units <= clusters_at_once(2 * p.ranks) * F::THREAD_BLOCKS && p.len > (uint64_t)p.ranks * FEW_WARPS * 16 * 2) p.ranks *= 2;
+    return p;
+}
+
+template <int D, bool INT8, int T>
+static cudaError_t launch_few(zkb_ctx* ctx, const zkb_step_attention_args& a) {
+    const zkb_kv_cache& c = a.cache;
+    using F = Few<D, INT8, T>;
+    const FewPlan plan = plan_few<D, INT8, T>(a);
     CacheMaps maps;
     const bool tma = cache_maps(maps, c, 16);
     auto kernel = tma ? attention_few_kernel<D, INT8, T, true> : attention_few_kernel<D, INT8, T, false>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, F::SMEM);
     if (e != cudaSuccess) return e;
-    return launch_clusters(ranks, [&](uint32_t n) {
+    return launch_clusters(plan.ranks, [&](uint32_t n) {
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeClusterDimension;
         attr[0].val.clusterDim = {n, 1, 1};
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(tiles * n, c.n_heads, c.n_seqs);
+        cfg.gridDim = dim3(plan.tiles * n, c.n_heads, c.n_seqs);
         cfg.blockDim = dim3(FEW_WARPS * 32);
         cfg.dynamicSmemBytes = F::SMEM;
         cfg.stream = ctx->stream;
@@ -453,8 +467,8 @@ template <int D>
 static cudaError_t launch_attention(zkb_ctx* ctx, const zkb_step_attention_args& a) {
     const zkb_kv_cache& c = a.cache;
     // Eight rows a product or 128, by what each was measured to take when the GPU is full: the first kernel 40 ns for each eight rows of a kv head and 0.04 ns for each key that they are
-    // shown, the second, which starts some 12 us later, 80 ns (bf16 caches: 40) for each 256 rows and 0.2 ns (0.12) a key; over 300 batches the rule's choice is within 1 % of the better one on the
-    // average, within 1.5 times at the worst. Eight kv heads of 128, one sequence of 1,032 int8 tokens against 32 rows a head: 12.6 us and 25.5, of 8,032 against 128
+    // shown, the second, which starts some 12 us later, 80 ns (bf16 caches: 40) for each 256 rows and 0.2 ns (0.12) a key. The figures are those of 128 head dimensions; with fewer both kernels get
+    // faster alike: over 306 batches of 128 and 153 each of 64 and 32 the rule's choice is within 1 % of the better one on the average, within 1.4 times at the worst. Eight kv heads of 128, one sequence of 1,032 int8 tokens against 32 rows a head: 12.6 us and 25.5, of 8,032 against 128
     // rows: 60 and 46; 16 sequences of 32 bf16 tokens against 128 rows: 79 and 13; 1,024 sequences of 64 int8 tokens against 16 rows: 419 and 673.
     const uint32_t group = a.q_heads / c.n_heads;
     const uint64_t rows = (uint64_t)(a.rows.max_rows ? std::min(a.rows.max_rows, a.rows.n_rows) : a.rows.n_rows) * group, len = a.rows.max_len ? std::min(a.rows.max_len, c.capacity) : c.capacity;
@@ -463,9 +477,14 @@ static cudaError_t launch_attention(zkb_ctx* ctx, const zkb_step_attention_args&
     const bool few = ((double)((rows + 7) / 8) * of_8 - (double)((rows + 255) / 256) * of_256) * c.n_seqs * c.n_heads < 12000.;
     if (!few) return c.type == ZKB_VALUE_INT8 ? launch_many<D, true>(ctx, a) : launch_many<D, false>(ctx, a);
     if (c.type != ZKB_VALUE_INT8) return launch_few<D, false, 1>(ctx, a);
-    // Sixteen rows for each code that is turned into a 16-bit value instead of eight, with half the warps on an SM: 16 sequences of 8,008 tokens against 32 rows a head 164 us instead of 208, one of 2,048
-    // against 128 rows 20.7 instead of 22.5, but 16 of 1,040 against 64 rows 78 instead of 71.
-    return rows > 8 && shown(16, 16) >= 1500. ? launch_few<D, true, 2>(ctx, a) : launch_few<D, true, 1>(ctx, a);
+    // Sixteen rows for each code that is turned into a 16-bit value instead of eight, with half the warps on an SM. That gains where eight rows would have thread blocks share SMs, over caches
+    // long enough, and loses where half as many units spread over no more thread blocks. Eight kv heads of 128: 16 sequences of 8,008 tokens against 32 rows a head 164 us instead of 206, one of
+    // 2,048 against 128 rows 20.9 instead of 23.2; but one of 8,008 against 32 rows 29.2 instead of 23.3, 48 of 1,600 against 24 rows 138 instead of 105. (675 batches of head dimensions 32 to 128:
+    // within 0.4 % of the better one on the average, within 13 % at the worst.)
+    const FewPlan of8 = plan_few<D, true, 1>(a), of16 = plan_few<D, true, 2>(a);
+    const bool sixteen = rows > 8 && of8.len >= std::max(1500u, 256 * of8.ranks) && of8.units > clusters_at_once(of8.ranks) && of16.ranks >= of8.ranks &&
+                         (of8.units <= 512 || (D == 128 && 8 * (uint64_t)of16.tiles < 5 * (uint64_t)of8.tiles));
+    return sixteen ? launch_few<D, true, 2>(ctx, a) : launch_few<D, true, 1>(ctx, a);
 }
 
 }  // namespace zk
