@@ -341,3 +341,22 @@ def test_attention_whose_clusters_are_refused(ctx, zkb, monkeypatch, kind, most)
 def test_attention_weights_of_few_rows_of_many_heads(ctx, zkb, kind, shape, d):
     """As above where eight rows a product would have thread blocks share SMs."""
     test_attention_weights_of_few_rows(ctx, zkb, kind, shape, 64, 16, d, 0, True)
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+@pytest.mark.parametrize("rows", [1, 3, 300])
+@pytest.mark.parametrize("scale", [0.0, 1e-39, -1e-38, 2e-38])
+def test_attention_scales_of_nothing_and_nearly(ctx, zkb, kind, rows, scale):
+    """Products of 10^38 and a scale that makes less than one, or nothing, of them: by nothing all keys that a row sees weigh alike."""
+    g, d, n = gen(rows), 64, rows + 200
+    batch, cache = Batch([(rows, n)]), Cache(g, kind, 1, 4, n, d)
+    q = torch.randn(rows, 16, d, generator=g, device="cuda").bfloat16()
+    q[..., 0] = 1e19
+    cache.k[..., 0] = 0
+    if kind == "int8":
+        cache.k[:, :, ::3, 0] = 100
+        cache.k_scale.fill_(1e17)
+    else:
+        cache.k[:, :, ::3, 0] = 1e19
+    check_attention(ctx, zkb, batch, cache, q, "bf16", 0, 0, scale=scale)

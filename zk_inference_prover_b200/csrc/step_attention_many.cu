@@ -233,7 +233,7 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
         if constexpr (INT8) asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
         const int tile = warp >> 2, row = threadIdx.x & 127;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21, s_at = tmem + tile * 128 + lanes, o_at = tmem + 256 + tile * D + lanes;
-        const float by = fmaxf(fabsf(a.scale) * 1.44269504f, 1.2e-38f);  // not zero: what is hidden is -inf times this
+        const float by = fmaxf(fabsf(a.scale) * 1.44269504f, 1.4e-45f);  // not zero, but the smallest float: what is hidden is -inf times this
         uint32_t done = 0, passed = 0, odd_at = 0;  // steps of this tile, blocks, units with blocks: what the barriers' phases, the scales' places and the flags go by
         auto row_of = [&](const Unit& n) { return n.m0 + (n.split ? row : tile * 128 + row); };
         auto q_of = [&](const Unit& n, int m) {
@@ -263,7 +263,7 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
                     for (uint32_t w : {x[i].x, x[i].y, x[i].z, x[i].w}) most = fmaxf(most, fmaxf(fabsf(bf16_low(w)), fabsf(bf16_high(w))));
                 const int e = (int)(__float_as_uint(most) >> 23), up = e == 0 || e == 255 ? 0 : min(13 + 127 - e, 126);
                 f = __uint_as_float((uint32_t)(up + 127) << 23);
-                left = fmaxf(ldexpf(by, -up), 1.2e-38f);
+                left = fmaxf(ldexpf(by, -up), 1.4e-45f);
             }
             const uint32_t turn = a.scale < 0.f ? 0x80008000u : 0u;
             auto word = [&](uint32_t w) { return (INT8 ? pack_f16(bf16_low(w) * f, bf16_high(w) * f) : w) ^ turn; };
