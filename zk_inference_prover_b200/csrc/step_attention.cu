@@ -138,11 +138,11 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, (Few<D, INT8, T>::THREAD_BLOCK
     for (int64_t m0 = (int64_t)(blockIdx.x / ranks) * ROWS; m0 < n_m; m0 += m_step) {
         const int64_t pos_low = s.pos + token(m0), pos_high = s.pos + token(min(m0 + ROWS, n_m) - 1);
         const KeyBlocks blocks = key_blocks<16>(pos_low, pos_high, c.capacity, a.window, a.sinks);
-        const int stride = ranks * FEW_WARPS, last = (int)blocks.end - 1;
+        const int stride = ranks * FEW_WARPS, last = (int)blocks.end - 1, n_blocks = failed ? 0 : blocks.n;
         const int at0 = rank * FEW_WARPS + warp;
 #pragma unroll
         for (int i = 0; i < F::STAGES - 1; i++) {
-            if (at0 + i * stride < blocks.n) copy(stage + i < F::STAGES ? stage + i : stage + i - F::STAGES, blocks.base(at0 + i * stride), last);
+            if (at0 + i * stride < n_blocks) copy(stage + i < F::STAGES ? stage + i : stage + i - F::STAGES, blocks.base(at0 + i * stride), last);
             asm volatile("cp.async.commit_group;" ::: "memory");
         }
         // Q: lane (g, t) has row g's dimensions (of each eight rows) in the order in which its K quarter comes
@@ -202,14 +202,18 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, (Few<D, INT8, T>::THREAD_BLOCK
         }
         bool odd = false;
         const int whole_to = (int)min(pos_low, (int64_t)last) - 15, whole_from = a.window ? (int)max((int64_t)0, pos_high - (int64_t)a.window + 1) : 0;  // blocks that all rows see
-        for (int at = at0; at < blocks.n; at += stride) {
+        for (int at = at0; at < n_blocks; at += stride) {
             const int base = blocks.base(at), ahead = at + (F::STAGES - 1) * stride;
             const uint32_t here = ring + stage * 2 * F::TILE, scales_here = scale_ring + stage * 128 + 4 * g;
-            if (ahead < blocks.n) copy(stage == 0 ? F::STAGES - 1 : stage - 1, blocks.base(ahead), last);
+            if (ahead < n_blocks) copy(stage == 0 ? F::STAGES - 1 : stage - 1, blocks.base(ahead), last);
             asm volatile("cp.async.commit_group;" ::: "memory");
             asm volatile("cp.async.wait_group %0;" ::"n"(F::STAGES - 1) : "memory");
             __syncwarp();
-            if (TMA) failed = __any_sync(0xffffffffu, failed || !mbar_wait(bars + 8 * stage, parity));
+            if (TMA && __any_sync(0xffffffffu, !mbar_wait(bars + 8 * stage, parity))) {
+                failed = true;  // the copies that are still on their way come first (a stage that has none takes the wait's limit)
+                for (int i = 0; i < F::STAGES; i++) mbar_wait(bars + 8 * i, i < stage ? parity ^ 1 : parity);
+                break;
+            }
             if (++stage == F::STAGES) stage = 0, parity ^= 1;
             float sc[T][4] = {}, sc2[T][4] = {};
             {

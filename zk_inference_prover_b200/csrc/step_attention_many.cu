@@ -551,9 +551,13 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
         const int th = threadIdx.x - 320;
         if constexpr (INT8) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         const uint32_t c128 = bf16_128(), c1152 = f16_1152();
+        auto landed = [&](uint32_t sent) {  // the last copies of that many
+            constexpr uint32_t RING = INT8 ? M::RAWS : M::STAGES;
+            for (uint32_t item = sent > RING ? sent - RING : 0; item < sent; item++) mbar_wait(bar_of(INT8 ? bars.raw_full[item % RING] : bars.full[item % RING]), item / RING & 1);
+        };
         while (more) {
             if (warp == 8) {  // ---- the copies
-                if (TMA && lane == 0) {
+                if (TMA && lane == 0 && !failed) {
                     for (int i = 0; i < 2 * u.n; i++) {
                         const uint32_t item = items + i;
                         const CUtensorMap* map = i & 1 ? &maps.v : &maps.k;
@@ -561,14 +565,20 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
                         if constexpr (INT8) {
                             const uint32_t st = item % M::RAWS, bar = bar_of(bars.raw_full[st]);
                             wait_one(bars.raw_empty[st], item / M::RAWS + 1);
-                            if (failed) break;
+                            if (failed) {
+                                landed(item);
+                                break;
+                            }
                             mbar_expect(bar, M::RAW);
 #pragma unroll
                             for (int x = 0; x < M::RAW_BOXES; x++) tma_load(raw_ring + st * M::RAW + x * 128 * M::RAW_BOX, map, x * M::RAW_BOX, base, u.kv_head, u.seq, bar);
                         } else {
                             const uint32_t st = item % M::STAGES, bar = bar_of(bars.full[st]);
                             wait_one(bars.empty[st], item / M::STAGES + 1);
-                            if (failed) break;
+                            if (failed) {
+                                landed(item);
+                                break;
+                            }
                             mbar_expect(bar, M::TILE);
 #pragma unroll
                             for (int x = 0; x < M::PANELS; x++) tma_load(ring + st * M::TILE + x * 128 * M::BOX, map, x * (M::BOX / 2), base, u.kv_head, u.seq, bar);
@@ -729,6 +739,14 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
             }
             u = after;
         }
+        // Nothing is on its way to shared memory or at work in tensor memory when the thread block gives them up, though a wait may have run out.
+        if (TMA && warp == 8 && lane == 0 && !failed) {
+            landed(items);
+        } else if (warp == 9) {
+            if (elect_one()) products_done(bar_of(bars.full[4]));  // (no stage has that one)
+            mbar_wait(bar_of(bars.full[4]), 0);
+        }
+        __syncwarp();
     }
     if (failed && lane == 0) *dev_err = WAIT_RAN_OUT;
     tmem_fence_before();
