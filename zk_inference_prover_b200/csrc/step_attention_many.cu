@@ -141,7 +141,13 @@ struct Units {
     __device__ bool next(Unit& u) {
         const zkb_kv_cache& c = a.cache;
         const int group = (int)(a.q_heads / c.n_heads);
-        pair -= (int)depth;  // sequences of more pairs than the host knew of
+        auto take = [&] {
+            u.seq = (int)(one / c.n_heads), u.kv_head = (int)(one % c.n_heads);
+            u.s = step_sequence(a.rows, u.seq);
+            u.n_m = u.s.rows * group;
+        };
+        pair -= (int)depth;
+        if (pair >= 0) take();  // sequences of more pairs than the host knew of
         while (pair < 0) {
             // there and back, so that all get as much
             const uint32_t who = blockIdx.x / ranks, step = gridDim.x / ranks, at = turn * step + (turn & 1 ? step - 1 - who : who);
@@ -149,11 +155,9 @@ struct Units {
             turn++;
             if (at >= all) continue;
             one = at % (c.n_seqs * c.n_heads);
-            pair = (step_sequence(a.rows, (int)(one / c.n_heads)).rows * group + 255) / 256 - 1 - (int)(at / (c.n_seqs * c.n_heads));
+            take();
+            pair = (u.n_m + 255) / 256 - 1 - (int)(at / (c.n_seqs * c.n_heads));
         }
-        u.seq = (int)(one / c.n_heads), u.kv_head = (int)(one % c.n_heads);
-        u.s = step_sequence(a.rows, u.seq);
-        u.n_m = u.s.rows * group;
         u.m0 = pair * 256;
         u.two = u.m0 + 128 < u.n_m;
         const int64_t low = u.s.pos + (uint32_t)u.m0 / (uint32_t)group, high = u.s.pos + (uint32_t)(min(u.m0 + 256, u.n_m) - 1) / (uint32_t)group;
