@@ -42,8 +42,8 @@ bool cache_maps(CacheMaps& maps, const zkb_kv_cache& c, uint32_t tokens) {
 // sum, and its own ring in shared memory that the tensor memory unit fills two blocks ahead (copies by the lanes themselves came to 26 bytes a clock
 // and SM): nothing waits for other warps. Warps join through shared memory, thread blocks of a cluster by writing into each other's, so that
 // a long sequence is spread over up to 16 SMs without a workspace or a second launch.
-// 64 sequences of 4,096 to 8,192 bf16 tokens, 32 heads on 8 of 128: 241 us, 6.7 TB/s; int8 tokens 174 us, 4.8 TB/s: their conversion keeps the warps' issue slots busy to 56 %, each of the two
-// products for a warp's sixteen keys waiting for it. One sequence of 2,048 int8 tokens: 9.4 us, most of it the launch and the joining.
+// 64 sequences of 4,096 to 8,192 bf16 tokens, 32 heads on 8 of 128, call after call: 243 us, 6.6 TB/s, a copy's rate; int8 tokens 171 us, 4.9 TB/s: each of the two products for a warp's sixteen keys
+// waits for the conversion of its codes, which take turns in one warp, and issue slots are busy to 57 %. One sequence of 2,048 int8 tokens: 8.9 us, most of it the launch and the joining.
 constexpr int FEW_WARPS = 8, FEW_RANKS = 16;
 constexpr float NO_SCORE = -3.40282346e38f;  // of a hidden key, the lowest number: a visible one's may be -inf; both weigh nothing
 
@@ -276,8 +276,8 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, (Few<D, INT8, T>::THREAD_BLOCK
                     sum[n][i & 1] += e;
                     z[i] = INT8 ? (z[i] == NO_SCORE ? 0.f : e * v_by[i >> 1]) : e;  // a hidden token's scale may be anything; a visible one's reaches the row whatever its score
                 }
-                // A weight is two bf16 numbers, its rounding and what that leaves: off by 2^-16 where the result's own rounding takes 2^-8. (One number alone: 64 sequences of 8,192
-                // int8 tokens in 164 us instead of 174, bf16 240 instead of 243, and results up to 1.6 times as far off.)
+                // A weight is two bf16 numbers, its rounding and what that leaves: off by 2^-16 where the result's own rounding takes 2^-8. (One number alone, when it was timed: 64 sequences of
+                // 8,192 int8 tokens in 164 us instead of 174, bf16 240 instead of 243, and results up to 1.6 times as far off.)
                 const uint32_t high[2] = {pack_bf16(z[0], z[1]), pack_bf16(z[2], z[3])};
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
@@ -472,8 +472,9 @@ static cudaError_t launch_attention(zkb_ctx* ctx, const zkb_step_attention_args&
     const zkb_kv_cache& c = a.cache;
     // Eight rows a product or 128, by what each was measured to take when the GPU is full: the first kernel 40 ns for each eight rows of a kv head and 0.04 ns for each key that they are
     // shown, the second, which starts some 12 us later, 80 ns (bf16 caches: 40) for each 256 rows and 0.2 ns (0.12) a key. The figures are those of 128 head dimensions; with fewer both kernels get
-    // faster alike: over 306 batches of 128 and 153 each of 64 and 32 the rule's choice is within 1 % of the better one on the average, within 1.4 times at the worst. Eight kv heads of 128, one sequence of 1,032 int8 tokens against 32 rows a head: 12.6 us and 25.5, of 8,032 against 128
-    // rows: 60 and 46; 16 sequences of 32 bf16 tokens against 128 rows: 79 and 13; 1,024 sequences of 64 int8 tokens against 16 rows: 419 and 673.
+    // faster alike: over 306 batches of 128 and 153 each of 64 and 32 the rule's choice is within 1 % of the better one on the average, within 1.4 times at the worst. Eight kv heads of 128, one
+    // sequence of 1,032 int8 tokens against 32 rows a head: 12.6 us and 25.5, of 8,032 against 128 rows: 60 and 46; 16 sequences of 32 bf16 tokens against 128 rows: 79 and 13; 1,024
+    // sequences of 64 int8 tokens against 16 rows: 419 and 673.
     const uint32_t group = a.q_heads / c.n_heads;
     const uint64_t rows = (uint64_t)(a.rows.max_rows ? std::min(a.rows.max_rows, a.rows.n_rows) : a.rows.n_rows) * group, len = a.rows.max_len ? std::min(a.rows.max_len, c.capacity) : c.capacity;
     auto shown = [&](uint32_t tile, uint32_t block) { return a.window ? (double)std::min<uint64_t>(len, (uint64_t)a.window + a.sinks + tile / group + block) : (double)len; };

@@ -13,8 +13,9 @@ namespace zk {
 // A thread block takes one pair of tiles after the other; with too few of them for the GPU the keys are spread over a cluster's thread blocks, which add up through
 // each other's shared memory, and one tile alone is two, of each block's two halves.
 // The weights are rounded to bf16 for the product (2^-8, as the result's own rounding): a second bf16 number for what that leaves, as the few rows' kernel has it, took 15 to 28 % longer.
-// 32 heads on 8 of 128, causal: 8,192 rows of one sequence, bf16, 510 us, 1,080 TFLOP/s of visible pairs; 1,290 to 2,048 rows of four sequences 150 us, int8 252 us; 8,192 rows with a window
-// of 1,024, bf16 202 us, int8 322 us: a block's products and its softmax take turns, 1,500 and 2,200 cycles, int8 scales another 2,000 of shared memory's.
+// 32 heads on 8 of 128, causal, call after call: 8,192 rows of one sequence, bf16, 513 us, 1,070 TFLOP/s of visible pairs; 1,290 to 2,048 rows of four sequences 150 us, int8 245 us; 8,192 rows
+// with a window of 1,024, bf16 200 us, int8 320 us: a block's products and its softmax take turns, 1,500 and 2,200 cycles, int8 scales another 2,000 of shared memory's. The three bf16 times
+// are 2 us for each block of 128 keys and pair of tiles, and some 10 us for each pair whatever its keys (its Q, the first scores, the rows written), which nothing hides: both tiles are at it at once.
 constexpr int MANY_KEYS = 128, MANY_RANKS = 16;
 
 template <int D, bool INT8>
@@ -233,7 +234,8 @@ __global__ void __launch_bounds__((Many<D, INT8>::THREADS), 1)
 
     if (warp < 8) {  // ---- the rows: softmax
         // An int8 cache takes more threads than leave a row the registers for 64 scores: they get some of those of the other warps (256 * 184 + 256 * 72 = 512 * 128, what the
-        // launch has). 8192 rows, window of 1024, int8: 367 -> 331 us.
+        // launch has). 8192 rows, window of 1024, int8: 367 -> 331 us when it was
+        // tried. -Xptxas -v: the int8 variants keep 72 to 88 bytes of stack and 288 to 354 of spill stores, the bf16 ones (168 registers) 32 to 40 and 42 to 56.
         if constexpr (INT8) asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
         const int tile = warp >> 2, row = threadIdx.x & 127;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21, s_at = tmem + tile * 128 + lanes, o_at = tmem + 256 + tile * D + lanes;

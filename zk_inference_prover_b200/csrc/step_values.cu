@@ -137,7 +137,7 @@ __device__ __forceinline__ void store4(void* p, int64_t at, const float* x) {
 // A warp takes the heads of one row (or one part of them), D / 8 lanes a head, the loads of four passes over them (words: two) on their way at a time. A lane has the values that
 // turn together: four of the first half of the rotary dimensions and the four they are paired with (interleaved, and behind the rotary dimensions: eight adjacent ones), so nothing
 // of the rotation crosses lanes. The row's angles are worked out once, two a lane: position times turns in 64 bits, what is left of whole turns in 32. Bound by the bytes: a value
-// is read and written once. 4 x 2048 rows of 32 + 2 x 8 heads of 128 into a bf16 cache: 37 us, 4.6 TB/s; with registers for eight
+// is read and written once. 4 x 2048 rows of 32 + 2 x 8 heads of 128 into a bf16 cache: 37 us, 4.6 TB/s; int8 42 us; with registers for eight
 // blocks a multiprocessor instead of six, which spills a few, 42 us, with eight passes' loads at a time for four blocks, 49 us.
 template <int D, bool WORD, bool INT8, bool VEC>
 __global__ void __launch_bounds__(128, 6) norm_rope_kernel(const __grid_constant__ NormRopeArgs n) {
