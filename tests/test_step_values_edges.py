@@ -360,3 +360,80 @@ def test_attention_scales_of_nothing_and_nearly(ctx, zkb, kind, rows, scale):
     else:
         cache.k[:, :, ::3, 0] = 1e19
     check_attention(ctx, zkb, batch, cache, q, "bf16", 0, 0, scale=scale)
+
+
+class Backwards(Cache):
+    """The same cache, laid out with its tokens, heads or sequences descending: the address is that of the first one, behind the others."""
+
+    def args(self, zkb):
+        c = super().args(zkb)
+        size, (s, h, t, _), k = self.k.element_size(), self.dims, self.k
+        self.room = [x.flip([dict(s=0, h=1, t=2)[y] for y in self.down]).contiguous() for x in (self.k, self.v)]
+        seq, head, token = h * t * k.shape[3], t * k.shape[3], k.shape[3]
+        off = (s - 1) * seq * ("s" in self.down) + (h - 1) * head * ("h" in self.down) + (t - 1) * token * ("t" in self.down)
+        c.k, c.v = (x.data_ptr() + size * off for x in self.room)
+        c.seq_stride, c.head_stride, c.token_stride = (-x if y in self.down else x for x, y in ((seq, "s"), (head, "h"), (token, "t")))
+        torch.cuda.synchronize()
+        return c
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+@pytest.mark.parametrize("down", ["t", "h", "s", "sht"])
+@pytest.mark.parametrize("shape,window", [([(1, 300), (2, 77)], 0), ([(200, 400), (90, 200)], 60)])
+def test_caches_laid_out_backwards(ctx, zkb, kind, down, shape, window):
+    g = gen(len(down))
+    batch, cache = Batch(shape), Backwards(g, kind, 2, 8, 400, 64)
+    cache.down = down
+    q = torch.randn(batch.n_rows, 32, 64, generator=g, device="cuda").bfloat16()
+    if kind == "bf16":
+        cache.v[0, 1, 9, 5] = math.inf
+    check_attention(ctx, zkb, batch, cache, q, "words", window, 3)
+    x = torch.randn(batch.n_rows, 32 + 16, 64, generator=g, device="cuda").bfloat16()
+    args, freq = cache.args(zkb), 1e4 ** (-np.arange(32) / 32)
+    torch.cuda.synchronize()
+    out = torch.zeros(batch.n_rows, 32, 64, device="cuda", dtype=torch.bfloat16)
+    ctx.step_norm_rope(zkb.StepNormRope(cache=args, rows=batch.args(zkb), q=x.data_ptr(), k=x[:, 32:].data_ptr(), v=x[:, 40:].data_ptr(), h_inv_freq=freq.ctypes.data, q_out=out.data_ptr(),
+                                        q_stride=x.stride(0), k_stride=x.stride(0), v_stride=x.stride(0), head_stride=64, q_out_stride=out.stride(0), q_out_head_stride=64, q_heads=32,
+                                        rotary_dim=64, eps=1e-6))
+    done(ctx)
+    cache.v = cache.room[1].flip([dict(s=0, h=1, t=2)[y] for y in down])
+    for b, at, rows, pos in batch.each():
+        got, want = cache.values()[1][b, :, pos:pos + rows].transpose(0, 1), x[at:at + rows, 40:].double()
+        step = cache.v_scale[b, :, pos:pos + rows].T.double()[..., None] if kind == "int8" else 0
+        assert bool(((got - want).abs() <= step * (0.5 + 127 * 2.0 ** -22)).all())
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+@pytest.mark.parametrize("rows,length", [(1, 500), (70, 400)])
+def test_sequences_that_share_a_cache(ctx, zkb, kind, rows, length):
+    """A sequence stride of zero: each sees its own first tokens of the same ones."""
+    g = gen(rows)
+    batch, cache = Batch([(rows, length), (rows, length - 100), (rows, length)]), Cache(g, kind, 3, 8, length, 64)
+    for x in (cache.k, cache.v, cache.k_scale, cache.v_scale):
+        if x is not None:
+            x[1:] = x[:1]
+    own = cache.args
+
+    def shared(zkb):
+        c = own(zkb)
+        c.seq_stride = c.scale_seq_stride = 0
+        return c
+
+    cache.args = shared
+    q = torch.randn(batch.n_rows, 32, 64, generator=g, device="cuda").bfloat16()
+    check_attention(ctx, zkb, batch, cache, q, "bf16", 0, 0)
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+@pytest.mark.parametrize("shape,hk,window", [([(1, 3000)], 8, 0), ([(32, 2048)], 8, 0), ([(500, 900), (3, 70), (300, 300)], 8, 0), ([(700, 1500)], 1, 200)])
+def test_attention_gives_the_same_bits_each_time(ctx, zkb, kind, shape, hk, window):
+    """Sums have one order, whichever thread blocks come first."""
+    g = gen(hk)
+    batch, cache = Batch(shape), Cache(g, kind, len(shape), hk, max(n for _, n in shape), 128)
+    q = torch.randn(batch.n_rows, 4 * hk, 128, generator=g, device="cuda").bfloat16()
+    first = attend(ctx, zkb, batch, cache, q, torch.zeros_like(q), window, 3)
+    for _ in range(10):
+        assert torch.equal(attend(ctx, zkb, batch, cache, q, torch.full_like(q, 5), window, 3), first)
