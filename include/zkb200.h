@@ -477,7 +477,7 @@ int zkb_witness_residual_stream(zkb_ctx* ctx, const zkb_rs_program* prog, const 
 /* ---- The values of a decode step: what the witness generators above are made from ------------------
  * A proof whose trace never leaves the device needs the model's own values there: the embedding's rows, the queries, keys
  * and values of a block of tokens (zkb_witness_dequant leaves them as bf16 patterns in want_out), the cache that they
- * fill, and the attention over it, which zkb_witness_residual_stream reads as leaves. These three calls make them. Values
+ * fill, and the attention over it, which zkb_witness_residual_stream reads as leaves. These calls make them. Values
  * are bf16 numbers, held either two bytes apiece or, as everywhere above, as patterns in the low halves of 32-bit words;
  * sums, norms and softmax statistics are 32-bit floats, and each output is rounded once, to nearest even.
  *
@@ -490,6 +490,9 @@ int zkb_witness_residual_stream(zkb_ctx* ctx, const zkb_rs_program* prog, const 
 #define ZKB_VALUE_BF16 0 /* 16 bits */
 #define ZKB_VALUE_WORD 1 /* a bf16 pattern in the low half of a 32-bit word (written with a zero high half; the high half is ignored when read) */
 #define ZKB_VALUE_INT8 2 /* an 8-bit code, with a float scale beside it: code * scale */
+#define ZKB_VALUE_F32 3   /* a 32-bit float */
+#define ZKB_VALUE_INT32 4 /* a 32-bit whole number */
+#define ZKB_VALUE_INT4 5  /* a 4-bit code of -8 .. 7, two a byte, the first in the low half, with a bf16 scale for each group of codes beside them */
 
 /* Embedding rows: out[t][i] = bf16(table[ids[t]][i] * (row_scale[ids[t]] * scale)), element (t, i) at
  * t * out_stride + (i / segment) * segment_stride + i % segment (segment 0: the whole row in one piece), so that rows can be
@@ -575,6 +578,80 @@ typedef struct zkb_step_attention_args {
     float scale;
 } zkb_step_attention_args;
 int zkb_step_attention(zkb_ctx* ctx, const zkb_step_attention_args* args);
+
+/* What lies between those calls and behind them, with the same conventions. zkb_step_residual_norm and zkb_step_gate leave rows of 8-bit
+ * codes with a scale a row, zkb_step_product multiplies them with weights held as codes (as INT32 its results are the accumulators that
+ * zkb_witness_dequant proves), and zkb_step_logprobs reads the output head's. Rows of codes: scale = max|y| / 127 and code =
+ * y * (127 / max|y|), rounded to nearest even (a scale of zero, NaN or infinity: codes 0), y the values before any rounding. */
+
+/* The residual stream's next rows and their norms: s = bf16(residual + x), or x itself where residual is NULL, and
+ * y = s * rsqrt(mean(s^2) + eps) * weight over a row's `width` values (weight: bf16, NULL: ones). s goes to sum_out where that is given; it
+ * may be residual itself, with its type and stride. y goes to out: BF16, WORD, or INT8 with a scale a row in out_scale. x, residual and
+ * sum_out are BF16 or WORD. Element i of row t of x is at t * x_stride + (i / x_segment) * x_segment_stride + i % x_segment (x_segment 0:
+ * the whole row in one piece), which reads want_out of zkb_witness_dequant where it lies. width is at most 32768. */
+typedef struct zkb_step_residual_norm_args {
+    const void* x;
+    const void* residual;
+    const uint16_t* weight;
+    void* sum_out;
+    void* out;
+    float* out_scale; /* n_rows, INT8 only */
+    int64_t x_stride, x_segment_stride, residual_stride, sum_stride, out_stride;
+    uint32_t n_rows, width, x_segment, x_type, residual_type, sum_type, out_type;
+    float eps;
+} zkb_step_residual_norm_args;
+int zkb_step_residual_norm(zkb_ctx* ctx, const zkb_step_residual_norm_args* args);
+
+/* The gate between a feed-forward layer's products: y = gate / (1 + exp(-gate)) * x, or x itself where gate is NULL (which turns rows of
+ * values, an attention's for one, into codes). Values are read as zkb_step_residual_norm reads x, gate with x's type and segments, and y goes to
+ * out as there. width is at most 32768. */
+typedef struct zkb_step_gate_args {
+    const void* gate;
+    const void* x;
+    void* out;
+    float* out_scale; /* n_rows, INT8 only */
+    int64_t gate_stride, x_stride, segment_stride, out_stride;
+    uint32_t n_rows, width, segment, x_type, out_type;
+} zkb_step_gate_args;
+int zkb_step_gate(zkb_ctx* ctx, const zkb_step_gate_args* args);
+
+/* Rows of codes times weights held as codes: acc[t][c] = sum over i < n_in of x[t][i] * w[c][i], exactly; x is INT8, w INT8 or INT4, w_stride (codes,
+ * for INT4 an even number) from one output's weights to the next. With INT8 weights, out is INT32: acc itself (x_scale and w_scale NULL), or BF16, WORD
+ * or F32: acc * (x_scale[t] * w_scale[c]), w_scale n_out floats. With INT4 weights each `group` (32, 64 or 128) of a row's codes has a bf16 scale,
+ * the scales of output c from w_scale + c * w_scale_stride on, and out is BF16, WORD or F32: x_scale[t] times the sum, in
+ * 32-bit floats, of scale * the exact sum of 32 or more codes of a group. out[t][c] is at t * out_stride + c. n_in is at most 131071, so that no sum leaves 32 bits; n_out at most 2^24, n_rows 2^18. Which
+ * kernel computes a sum of groups, and so its order, is decided by the sizes and the alignment alone. */
+typedef struct zkb_step_product_args {
+    const int8_t* x;
+    const float* x_scale; /* n_rows */
+    const void* w;
+    const void* w_scale;
+    void* out;
+    int64_t x_stride, w_stride, w_scale_stride, out_stride;
+    uint32_t n_rows, n_in, n_out, w_type, group, out_type; /* group: INT4 only, else 0 */
+} zkb_step_product_args;
+int zkb_step_product(zkb_ctx* ctx, const zkb_step_product_args* args);
+
+/* What a model answers with: of each row of `vocab` logits (BF16, WORD or F32), with z = scale * logit and lse = log(sum of exp(z)), the log
+ * probabilities z - lse of the n_given tokens ids[t * n_given ..], the entropy of all of them (entropy NULL: not asked for), and the n_top (at
+ * most 32) tokens of the largest logits with theirs, equal logits by ascending index. An id outside [0, vocab) gets 0 and adds 1 to *off_table (may be
+ * NULL). A logit of -infinity is a token that cannot be: it has a log probability of -infinity and is no alternative; where fewer than n_top are
+ * left, and in rows where none is, the other places get the index -1 and -infinity; a row where none is left has entropy 0. A row with a NaN
+ * or +infinity among its logits has NaN everywhere and the index -1. Probabilities, sums and results are 32-bit floats, logarithms are taken of
+ * what the largest logit leaves. vocab is at most 2^19. */
+typedef struct zkb_step_logprobs_args {
+    const void* logits;
+    const int32_t* ids;
+    float* logprobs; /* n_rows x n_given */
+    float* entropy;  /* n_rows */
+    int32_t* top_ids;    /* n_rows x n_top */
+    float* top_logprobs; /* n_rows x n_top */
+    uint64_t* off_table;
+    int64_t logits_stride;
+    uint32_t n_rows, vocab, n_given, n_top, type;
+    float scale; /* above 0: one over the temperature */
+} zkb_step_logprobs_args;
+int zkb_step_logprobs(zkb_ctx* ctx, const zkb_step_logprobs_args* args);
 
 #ifdef __cplusplus
 }

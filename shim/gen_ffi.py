@@ -11,7 +11,9 @@ STRUCTS = {"zkb_grid": "ZkbGrid", "zkb_dequant_cfg": "ZkbDequantCfg", "zkb_pcs_c
            "zkb_stark_component": "ZkbStarkComponent", "zkb_air_op": "ZkbAirOp", "zkb_air_stats": "ZkbAirStats", "zkb_rs_group": "ZkbRsGroup",
            "zkb_rs_slot": "ZkbRsSlot", "zkb_rs_program": "ZkbRsProgram", "zkb_rs_tables": "ZkbRsTables", "zkb_rs_mult": "ZkbRsMult",
            "zkb_rs_mults": "ZkbRsMults", "zkb_step_embed_args": "ZkbStepEmbedArgs", "zkb_kv_cache": "ZkbKvCache", "zkb_step_rows": "ZkbStepRows",
-           "zkb_step_norm_rope_args": "ZkbStepNormRopeArgs", "zkb_step_attention_args": "ZkbStepAttentionArgs"}
+           "zkb_step_norm_rope_args": "ZkbStepNormRopeArgs", "zkb_step_attention_args": "ZkbStepAttentionArgs",
+           "zkb_step_residual_norm_args": "ZkbStepResidualNormArgs", "zkb_step_gate_args": "ZkbStepGateArgs", "zkb_step_product_args": "ZkbStepProductArgs",
+           "zkb_step_logprobs_args": "ZkbStepLogprobsArgs"}
 SCALARS = {"int": "i32", "unsigned": "u32", "unsigned int": "u32", "uint32_t": "u32", "int32_t": "i32", "uint64_t": "u64", "int64_t": "i64",
            "unsigned long long": "u64", "size_t": "usize", "float": "f32", "double": "f64", "int8_t": "i8", "uint8_t": "u8",
            "uint16_t": "u16", "unsigned char": "u8", "char": "std::os::raw::c_char", "void": "std::ffi::c_void"}

@@ -195,6 +195,83 @@ pub struct ZkbStepAttentionArgs {
     pub scale: f32,
 }
 
+#[repr(C)] #[derive(Copy, Clone, Debug)]
+pub struct ZkbStepResidualNormArgs {
+    pub x: *const std::ffi::c_void,
+    pub residual: *const std::ffi::c_void,
+    pub weight: *const u16,
+    pub sum_out: *mut std::ffi::c_void,
+    pub out: *mut std::ffi::c_void,
+    pub out_scale: *mut f32,
+    pub x_stride: i64,
+    pub x_segment_stride: i64,
+    pub residual_stride: i64,
+    pub sum_stride: i64,
+    pub out_stride: i64,
+    pub n_rows: u32,
+    pub width: u32,
+    pub x_segment: u32,
+    pub x_type: u32,
+    pub residual_type: u32,
+    pub sum_type: u32,
+    pub out_type: u32,
+    pub eps: f32,
+}
+
+#[repr(C)] #[derive(Copy, Clone, Debug)]
+pub struct ZkbStepGateArgs {
+    pub gate: *const std::ffi::c_void,
+    pub x: *const std::ffi::c_void,
+    pub out: *mut std::ffi::c_void,
+    pub out_scale: *mut f32,
+    pub gate_stride: i64,
+    pub x_stride: i64,
+    pub segment_stride: i64,
+    pub out_stride: i64,
+    pub n_rows: u32,
+    pub width: u32,
+    pub segment: u32,
+    pub x_type: u32,
+    pub out_type: u32,
+}
+
+#[repr(C)] #[derive(Copy, Clone, Debug)]
+pub struct ZkbStepProductArgs {
+    pub x: *const i8,
+    pub x_scale: *const f32,
+    pub w: *const std::ffi::c_void,
+    pub w_scale: *const std::ffi::c_void,
+    pub out: *mut std::ffi::c_void,
+    pub x_stride: i64,
+    pub w_stride: i64,
+    pub w_scale_stride: i64,
+    pub out_stride: i64,
+    pub n_rows: u32,
+    pub n_in: u32,
+    pub n_out: u32,
+    pub w_type: u32,
+    pub group: u32,
+    pub out_type: u32,
+}
+
+#[repr(C)] #[derive(Copy, Clone, Debug)]
+pub struct ZkbStepLogprobsArgs {
+    pub logits: *const std::ffi::c_void,
+    pub ids: *const i32,
+    pub logprobs: *mut f32,
+    pub entropy: *mut f32,
+    pub top_ids: *mut i32,
+    pub top_logprobs: *mut f32,
+    pub off_table: *mut u64,
+    pub logits_stride: i64,
+    pub n_rows: u32,
+    pub vocab: u32,
+    pub n_given: u32,
+    pub n_top: u32,
+    pub ty: u32,
+    pub scale: f32,
+}
+
 #[repr(C)] #[derive(Copy, Clone, Debug, Default)]
 pub struct ZkbAirOp {
     pub op: u32,
@@ -319,6 +396,10 @@ extern "C" {
     pub fn zkb_step_embed(ctx: *mut ZkbCtx, args: *const ZkbStepEmbedArgs) -> i32;
     pub fn zkb_step_norm_rope(ctx: *mut ZkbCtx, args: *const ZkbStepNormRopeArgs) -> i32;
     pub fn zkb_step_attention(ctx: *mut ZkbCtx, args: *const ZkbStepAttentionArgs) -> i32;
+    pub fn zkb_step_residual_norm(ctx: *mut ZkbCtx, args: *const ZkbStepResidualNormArgs) -> i32;
+    pub fn zkb_step_gate(ctx: *mut ZkbCtx, args: *const ZkbStepGateArgs) -> i32;
+    pub fn zkb_step_product(ctx: *mut ZkbCtx, args: *const ZkbStepProductArgs) -> i32;
+    pub fn zkb_step_logprobs(ctx: *mut ZkbCtx, args: *const ZkbStepLogprobsArgs) -> i32;
     pub fn zkb_air_compile(ctx: *mut ZkbCtx, ops: *const ZkbAirOp, n_ops: usize, constraints: *const u32, n_constraints: usize, tree_cols: *const u32, n_trees: i32, n_scalars: usize, out: *mut *mut ZkbAirProgram) -> i32;
     pub fn zkb_air_free(prog: *mut ZkbAirProgram) -> i32;
     pub fn zkb_air_specialize(ctx: *mut ZkbCtx, prog: *mut ZkbAirProgram) -> i32;

@@ -25,10 +25,17 @@ from .capi import (  # noqa: F401
     VALUE_BF16,
     VALUE_WORD,
     VALUE_INT8,
+    VALUE_F32,
+    VALUE_INT32,
+    VALUE_INT4,
     KvCache,
     StepRows,
     StepEmbed,
     StepNormRope,
     StepAttention,
+    StepResidualNorm,
+    StepGate,
+    StepProduct,
+    StepLogprobs,
 )
 from . import air, capi  # noqa: F401,E402

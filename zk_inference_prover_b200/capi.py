@@ -22,6 +22,7 @@ EXPORTED_SYMBOLS = [
     "zkb_gkr_sum", "zkb_gkr_fix_and_sum", "zkb_mle_fix_qm31", "zkb_mle_fix_m31", "zkb_grind", "zkb_gkr_sum_noalloc", "zkb_gkr_sum_noalloc_error",
     "zkb_freivalds_scatter", "zkb_freivalds_acc", "zkb_witness_tables", "zkb_witness_dequant", "zkb_witness_pre_table", "zkb_key_tile_flags",
     "zkb_witness_selectors", "zkb_witness_residual_stream", "zkb_step_embed", "zkb_step_norm_rope", "zkb_step_attention",
+    "zkb_step_residual_norm", "zkb_step_gate", "zkb_step_product", "zkb_step_logprobs",
 ]
 # Every symbol include/zkb200_prover.h declares.
 PROVER_SYMBOLS = ["zkb_pcs_prove_device", "zkb_pcs_prove_host", "zkb_stark_prove_device", "zkb_stark_prove_host", "zkb_stark_prove_multi_device", "zkb_stark_prove_multi_host", "zkb_gkr_prove_device",
@@ -64,7 +65,7 @@ class RsMults(C.Structure):  # zkb_rs_mults
     _fields_ = [("pow", RsMult), ("norm", RsMult), ("val", RsMult), ("frac", RsMult), ("smul", RsMult), ("un", C.c_void_p)]
 
 
-VALUE_BF16, VALUE_WORD, VALUE_INT8 = 0, 1, 2  # how values are held: ZKB_VALUE_*
+VALUE_BF16, VALUE_WORD, VALUE_INT8, VALUE_F32, VALUE_INT32, VALUE_INT4 = 0, 1, 2, 3, 4, 5  # how values are held: ZKB_VALUE_*
 
 
 class StepEmbed(C.Structure):
@@ -95,6 +96,27 @@ class StepAttention(C.Structure):  # zkb_step_attention_args
     _fields_ = [("cache", KvCache), ("rows", StepRows), ("q", C.c_void_p), ("out", C.c_void_p)] + \
                [(k, C.c_int64) for k in ("q_stride", "q_head_stride", "out_stride", "out_head_stride")] + \
                [(k, C.c_uint32) for k in ("q_heads", "out_type", "window", "sinks")] + [("scale", C.c_float)]
+
+
+class StepResidualNorm(C.Structure):  # zkb_step_residual_norm_args
+    _fields_ = [(k, C.c_void_p) for k in ("x", "residual", "weight", "sum_out", "out", "out_scale")] + \
+               [(k, C.c_int64) for k in ("x_stride", "x_segment_stride", "residual_stride", "sum_stride", "out_stride")] + \
+               [(k, C.c_uint32) for k in ("n_rows", "width", "x_segment", "x_type", "residual_type", "sum_type", "out_type")] + [("eps", C.c_float)]
+
+
+class StepGate(C.Structure):  # zkb_step_gate_args
+    _fields_ = [(k, C.c_void_p) for k in ("gate", "x", "out", "out_scale")] + [(k, C.c_int64) for k in ("gate_stride", "x_stride", "segment_stride", "out_stride")] + \
+               [(k, C.c_uint32) for k in ("n_rows", "width", "segment", "x_type", "out_type")]
+
+
+class StepProduct(C.Structure):  # zkb_step_product_args
+    _fields_ = [(k, C.c_void_p) for k in ("x", "x_scale", "w", "w_scale", "out")] + [(k, C.c_int64) for k in ("x_stride", "w_stride", "w_scale_stride", "out_stride")] + \
+               [(k, C.c_uint32) for k in ("n_rows", "n_in", "n_out", "w_type", "group", "out_type")]
+
+
+class StepLogprobs(C.Structure):  # zkb_step_logprobs_args
+    _fields_ = [(k, C.c_void_p) for k in ("logits", "ids", "logprobs", "entropy", "top_ids", "top_logprobs", "off_table")] + [("logits_stride", C.c_int64)] + \
+               [(k, C.c_uint32) for k in ("n_rows", "vocab", "n_given", "n_top", "type")] + [("scale", C.c_float)]
 
 
 class PcsConfig(C.Structure):
@@ -147,7 +169,8 @@ def load_library():
         _lib.zkb_merkle_layer.argtypes = [p, i, p, p, i, i, p]
         _lib.zkb_fold_line.argtypes = [p, p, p, i, p]
         _lib.zkb_d2d.argtypes = [p, p, p, C.c_size_t]
-        for name, args in (("zkb_step_embed", StepEmbed), ("zkb_step_norm_rope", StepNormRope), ("zkb_step_attention", StepAttention)):
+        for name, args in (("zkb_step_embed", StepEmbed), ("zkb_step_norm_rope", StepNormRope), ("zkb_step_attention", StepAttention),
+                           ("zkb_step_residual_norm", StepResidualNorm), ("zkb_step_gate", StepGate), ("zkb_step_product", StepProduct), ("zkb_step_logprobs", StepLogprobs)):
             getattr(_lib, name).argtypes = [p, C.POINTER(args)]
     return _lib
 
@@ -747,6 +770,22 @@ class Context:
     def step_attention(self, args):
         """args: a StepAttention."""
         self._check(self.lib.zkb_step_attention(self.h, args))
+
+    def step_residual_norm(self, args):
+        """args: a StepResidualNorm."""
+        self._check(self.lib.zkb_step_residual_norm(self.h, args))
+
+    def step_gate(self, args):
+        """args: a StepGate."""
+        self._check(self.lib.zkb_step_gate(self.h, args))
+
+    def step_product(self, args):
+        """args: a StepProduct."""
+        self._check(self.lib.zkb_step_product(self.h, args))
+
+    def step_logprobs(self, args):
+        """args: a StepLogprobs."""
+        self._check(self.lib.zkb_step_logprobs(self.h, args))
 
     # ---- constraint quotients of a lowered AIR (include/zkb200_air.h)
     def air_compile(self, source):

@@ -1,0 +1,305 @@
+// Rows of the residual stream: its next values with their norms, and the gate between a feed-forward layer's products, as values or as 8-bit codes.
+#include <algorithm>
+#include <cmath>
+#include <cstdlib>
+
+#include "step_values.cuh"
+
+namespace zk {
+
+// Both calls are a pass over rows: values in, one number of the whole row (the mean of squares, the largest value), values out. A row stays in registers between
+// its reading and its writing, V times eight values a thread, so nothing is read twice: bound by the bytes.
+struct RowsArgs {
+    const void* x;
+    const void* other;  // the residual stream, or the gate
+    const uint16_t* weight;
+    void* sum;
+    void* out;
+    float* scale;
+    int64_t x_stride, segment_stride, other_stride, sum_stride, out_stride;
+    uint32_t n_rows, width, segment, out_type;
+    bool other_word, sum_word;
+    float eps;
+    uint32_t warps;  // a row's
+};
+
+// This thread's values of a row: VEC eight adjacent ones at a time, on 16-byte boundaries; else a value at a time, adjacent ones in adjacent lanes.
+template <bool VEC>
+__device__ __forceinline__ uint32_t column_of(uint32_t v, uint32_t y, uint32_t threads, uint32_t th) {
+    return VEC ? (v * threads + th) * 8 + y : (v * 8 + y) * threads + th;
+}
+template <int V, bool VEC>
+__device__ __forceinline__ void load_row(const void* p, int64_t row, uint32_t segment, int64_t segment_stride, bool word, uint32_t width, uint32_t threads, uint32_t th, float (&x)[V][8]) {
+    auto place = [&](uint32_t col) { return row + (segment ? (int64_t)(col / segment) * segment_stride + col % segment : (int64_t)col); };
+    if (word) {
+#pragma unroll
+        for (int v = 0; v < V; v++) {
+            if constexpr (VEC) {
+                const uint32_t col = column_of<VEC>(v, 0, threads, th);
+                uint4 a = make_uint4(0u, 0u, 0u, 0u), b = a;
+                if (col < width) {
+                    const uint4* w = reinterpret_cast<const uint4*>(static_cast<const uint32_t*>(p) + place(col));
+                    a = w[0], b = w[1];
+                }
+                x[v][0] = bf16_low(a.x), x[v][1] = bf16_low(a.y), x[v][2] = bf16_low(a.z), x[v][3] = bf16_low(a.w);
+                x[v][4] = bf16_low(b.x), x[v][5] = bf16_low(b.y), x[v][6] = bf16_low(b.z), x[v][7] = bf16_low(b.w);
+            } else {
+#pragma unroll
+                for (int y = 0; y < 8; y++) {
+                    const uint32_t col = column_of<VEC>(v, y, threads, th);
+                    x[v][y] = col < width ? bf16_low(static_cast<const uint32_t*>(p)[place(col)]) : 0.f;
+                }
+            }
+        }
+    } else {
+#pragma unroll
+        for (int v = 0; v < V; v++) {
+            if constexpr (VEC) {
+                const uint32_t col = column_of<VEC>(v, 0, threads, th);
+                uint4 a = make_uint4(0u, 0u, 0u, 0u);
+                if (col < width) a = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + place(col));
+                x[v][0] = bf16_low(a.x), x[v][1] = bf16_high(a.x), x[v][2] = bf16_low(a.y), x[v][3] = bf16_high(a.y);
+                x[v][4] = bf16_low(a.z), x[v][5] = bf16_high(a.z), x[v][6] = bf16_low(a.w), x[v][7] = bf16_high(a.w);
+            } else {
+#pragma unroll
+                for (int y = 0; y < 8; y++) {
+                    const uint32_t col = column_of<VEC>(v, y, threads, th);
+                    x[v][y] = col < width ? bf16_low(static_cast<const uint16_t*>(p)[place(col)]) : 0.f;
+                }
+            }
+        }
+    }
+}
+template <int V, bool VEC>
+__device__ __forceinline__ void store_row(void* p, int64_t row, bool word, uint32_t width, uint32_t threads, uint32_t th, const float (&x)[V][8]) {
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+        if constexpr (VEC) {
+            const uint32_t col = column_of<VEC>(v, 0, threads, th);
+            if (col < width) word ? store8<true>(p, row + col, x[v]) : store8<false>(p, row + col, x[v]);
+        } else {
+#pragma unroll
+            for (int y = 0; y < 8; y++) {
+                const uint32_t col = column_of<VEC>(v, y, threads, th);
+                if (col >= width) continue;
+                if (word) static_cast<uint32_t*>(p)[row + col] = round_bf16(x[v][y]);
+                else static_cast<uint16_t*>(p)[row + col] = round_bf16(x[v][y]);
+            }
+        }
+    }
+}
+
+// A sum and a largest word over a row's warps. `room`: the warps' own words, another one for each use within a row.
+struct RowRoom {
+    float sum[32];
+    uint32_t most[32];
+};
+__device__ __forceinline__ void over_row(RowRoom& room, uint32_t warps, float& sum, uint32_t& most) {
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    most = __reduce_max_sync(0xffffffffu, most);
+    if (warps == 1) return;
+    if (lane == 0) room.sum[warp] = sum, room.most[warp] = most;
+    __syncthreads();
+    sum = lane < warps ? room.sum[lane] : 0.f;
+    most = __reduce_max_sync(0xffffffffu, lane < warps ? room.most[lane] : 0u);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+}
+__device__ __forceinline__ uint32_t size_word(float x) { return __float_as_uint(x) & 0x7fffffffu; }  // ordered as |x|, NaN above all
+
+constexpr int ROW_GROUP = 4;  // rows a thread block has where a row is a warp's
+
+template <int V, bool GATE, bool VEC>
+__global__ void __launch_bounds__(V == 4 ? 512 : 1024) rows_kernel(const __grid_constant__ RowsArgs a, bool x_word) {
+    __shared__ RowRoom room[2];
+    const uint32_t threads = a.warps * 32, th = a.warps == 1 ? threadIdx.x & 31 : threadIdx.x;
+    const int64_t t = a.warps == 1 ? (int64_t)blockIdx.x * ROW_GROUP + (threadIdx.x >> 5) : (int64_t)blockIdx.x;
+    if (t >= a.n_rows) return;  // (a whole warp)
+    float x[V][8];
+    uint32_t most = 0;
+    float by = 1.f;
+    {
+        float y[V][8];
+        load_row<V, VEC>(a.x, t * a.x_stride, a.segment, a.segment_stride, x_word, a.width, threads, th, x);
+        if (a.other) load_row<V, VEC>(a.other, t * a.other_stride, GATE ? a.segment : 0u, a.segment_stride, GATE ? x_word : a.other_word, a.width, threads, th, y);
+        if (a.other) {
+#pragma unroll
+            for (int v = 0; v < V; v++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    if constexpr (GATE) {
+                        // 1 / (1 + exp(-g)) by way of e = exp(-|g|), which does not overflow
+                        const float e = __expf(-fabsf(y[v][i])), s = __fdividef(1.f, 1.f + e);
+                        x[v][i] *= y[v][i] * (y[v][i] < 0.f ? e * s : s);
+                    } else {
+                        x[v][i] = bf16_low(round_bf16(x[v][i] + y[v][i]));
+                    }
+                }
+        }
+    }
+    if constexpr (!GATE) {
+        if (a.sum) store_row<V, VEC>(a.sum, t * a.sum_stride, a.sum_word, a.width, threads, th, x);
+        float ss = 0.f;
+        float w[V][8];
+        if (a.weight) load_row<V, VEC>(a.weight, 0, 0, 0, false, a.width, threads, th, w);
+#pragma unroll
+        for (int v = 0; v < V; v++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                ss = fmaf(x[v][i], x[v][i], ss);
+                if (a.weight) w[v][i] *= x[v][i];
+                else w[v][i] = x[v][i];
+                most = max(most, size_word(w[v][i]));
+            }
+        over_row(room[0], a.warps, ss, most);
+        const float mean = ss / (float)a.width + a.eps;
+        if (mean > 0x1p-90f && mean < 0x1p120f && most < 0x7f800000u) {  // the same for the whole row
+            by = rsqrtf(mean);
+            most = __float_as_uint(__uint_as_float(most) * by);
+#pragma unroll
+            for (int v = 0; v < V; v++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) x[v][i] = w[v][i] * by;
+        } else {  // squares or products that 32 bits do not hold, or values that are no numbers
+            double wide = 0.;
+#pragma unroll
+            for (int v = 0; v < V; v++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) wide += (double)x[v][i] * x[v][i];
+#pragma unroll
+            for (int o = 16; o; o >>= 1) wide += __shfl_xor_sync(0xffffffffu, wide, o);
+            __shared__ double wide_sm[32];
+            if (a.warps > 1) {
+                if ((threadIdx.x & 31) == 0) wide_sm[threadIdx.x >> 5] = wide;
+                __syncthreads();
+                wide = 0.;
+                for (uint32_t i = 0; i < a.warps; i++) wide += wide_sm[i];
+            }
+            const double root = rsqrt(wide / a.width + (double)a.eps);
+            most = 0;
+            if (a.weight) load_row<V, VEC>(a.weight, 0, 0, 0, false, a.width, threads, th, w);
+#pragma unroll
+            for (int v = 0; v < V; v++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    x[v][i] = (float)((double)x[v][i] * (a.weight ? (double)w[v][i] : 1.) * root);
+                    if (column_of<VEC>(v, i, threads, th) < a.width) most = max(most, size_word(x[v][i]));
+                }
+            float none = 0.f;
+            over_row(room[1], a.warps, none, most);
+        }
+    } else if (a.out_type == ZKB_VALUE_INT8) {
+#pragma unroll
+        for (int v = 0; v < V; v++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) most = max(most, size_word(x[v][i]));
+        float none = 0.f;
+        over_row(room[0], a.warps, none, most);
+    }
+    if (a.out_type != ZKB_VALUE_INT8) {
+        store_row<V, VEC>(a.out, t * a.out_stride, a.out_type == ZKB_VALUE_WORD, a.width, threads, th, x);
+        return;
+    }
+    float top = __uint_as_float(most), up = 1.f;
+    if (th == 0) a.scale[t] = top / 127.f;
+    if (most < 0x1f800000u) top *= 0x1p64f, up = 0x1p64f;  // below 2^-64: 127 over less than 2^-121 is no float
+    const float to_code = top > 0x1.fcp-80f && most < 0x7f800000u ? 127.f / top : 0.f;  // codes are 0 where the scale is (up to 127 x 2^-150), and where it is NaN or infinite
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+        uint32_t q[2] = {0, 0};
+#pragma unroll
+        for (int i = 0; i < 8; i++) q[i / 4] |= (uint32_t)(max(-127, min(127, __float2int_rn(x[v][i] * up * to_code))) & 255) << (8 * (i % 4));
+        int8_t* to = static_cast<int8_t*>(a.out) + t * a.out_stride;
+        if constexpr (VEC) {
+            const uint32_t col = column_of<VEC>(v, 0, threads, th);
+            if (col < a.width) *reinterpret_cast<uint2*>(to + col) = make_uint2(q[0], q[1]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const uint32_t col = column_of<VEC>(v, i, threads, th);
+                if (col < a.width) to[col] = (int8_t)(q[i / 4] >> (8 * (i % 4)));
+            }
+        }
+    }
+}
+
+template <bool GATE>
+static cudaError_t launch_rows(zkb_ctx* ctx, RowsArgs a, bool x_word, bool vec) {
+    const uint32_t eights = (a.width + 7) / 8;
+    uint32_t v = 4;
+    if (eights <= 32 || (a.n_rows < 148 * 4 && eights <= 1024)) v = 1;
+    else if (eights <= 64 || (a.n_rows < 148 * 4 && eights <= 2048)) v = 2;
+    while (v < 4 && (eights + 32 * v - 1) / (32 * v) > 32) v *= 2;
+    a.warps = (eights + 32 * v - 1) / (32 * v);
+    if (v == 4 && a.warps > 16) v = 8, a.warps = (eights + 255) / 256;
+    const uint32_t block = a.warps == 1 ? 32 * ROW_GROUP : 32 * a.warps, grid = a.warps == 1 ? (a.n_rows + ROW_GROUP - 1) / ROW_GROUP : a.n_rows;
+    auto launch = [&](auto one, auto two, auto four, auto eight) {
+        if (v == 1) one<<<grid, block, 0, ctx->stream>>>(a, x_word);
+        else if (v == 2) two<<<grid, block, 0, ctx->stream>>>(a, x_word);
+        else if (v == 4) four<<<grid, block, 0, ctx->stream>>>(a, x_word);
+        else eight<<<grid, block, 0, ctx->stream>>>(a, x_word);
+    };
+    if (vec) launch(rows_kernel<1, GATE, true>, rows_kernel<2, GATE, true>, rows_kernel<4, GATE, true>, rows_kernel<8, GATE, true>);
+    else launch(rows_kernel<1, GATE, false>, rows_kernel<2, GATE, false>, rows_kernel<4, GATE, false>, rows_kernel<8, GATE, false>);
+    return cudaGetLastError();
+}
+
+static size_t value_size(uint32_t type) { return type == ZKB_VALUE_WORD ? 4 : type == ZKB_VALUE_INT8 ? 1 : 2; }
+static bool is_values(uint32_t type) { return type == ZKB_VALUE_BF16 || type == ZKB_VALUE_WORD; }
+
+}  // namespace zk
+
+using namespace zk;
+
+extern "C" {
+
+int zkb_step_residual_norm(zkb_ctx* ctx, const zkb_step_residual_norm_args* args) {
+    if (!ctx) return ZKB_EINVAL;
+    ZKB_CHECK_ARG(ctx, args);
+    const zkb_step_residual_norm_args& a = *args;
+    ZKB_CHECK_ARG(ctx, is_values(a.x_type) && is_values(a.residual_type) && is_values(a.sum_type) && (is_values(a.out_type) || a.out_type == ZKB_VALUE_INT8));
+    ZKB_CHECK_ARG(ctx, a.width >= 1 && a.width <= 32768 && a.n_rows <= 0x7fffffffu && std::isfinite(a.eps) && a.eps >= 0.f);
+    if (a.n_rows == 0) return ZKB_OK;
+    const size_t xs = value_size(a.x_type), rs = value_size(a.residual_type), ss = value_size(a.sum_type), os = value_size(a.out_type);
+    ZKB_CHECK_ARG(ctx, a.x && a.out && (a.out_type == ZKB_VALUE_INT8 ? a.out_scale != nullptr : !a.out_scale));
+    ZKB_CHECK_ARG(ctx, aligned_to(a.x, xs) && aligned_to(a.residual, rs) && aligned_to(a.weight, 2) && aligned_to(a.sum_out, ss) && aligned_to(a.out, os) && aligned_to(a.out_scale, 4));
+    ZKB_CHECK_ARG(ctx, a.n_rows == 1 || std::llabs(a.out_stride) >= (long long)a.width);
+    ZKB_CHECK_ARG(ctx, a.n_rows == 1 || !a.sum_out || std::llabs(a.sum_stride) >= (long long)a.width);
+    ZKB_CHECK_ARG(ctx, a.sum_out == nullptr || a.sum_out != a.residual || (a.sum_type == a.residual_type && (a.n_rows == 1 || a.sum_stride == a.residual_stride)));
+    const bool split = a.x_segment && a.x_segment < a.width;
+    auto wide = [](const void* p, size_t size, int64_t stride) { return aligned_to(p, size == 1 ? 8 : 16) && (size == 1 ? stride % 8 == 0 : stride * (int64_t)size % 16 == 0); };
+    const bool vec = a.width % 8 == 0 && wide(a.x, xs, a.x_stride) && wide(a.residual, rs, a.residual ? a.residual_stride : 0) && aligned_to(a.weight, 16) && wide(a.sum_out, ss, a.sum_out ? a.sum_stride : 0) &&
+                     wide(a.out, os, a.out_stride) && (!split || (a.x_segment % 8 == 0 && a.x_segment_stride * (int64_t)xs % 16 == 0));
+    DeviceGuard g(ctx);
+    ProfScope prof(ctx, "step_residual_norm_kernel");
+    const RowsArgs r{a.x, a.residual, a.weight, a.sum_out, a.out, a.out_scale, a.x_stride, a.x_segment_stride, a.residual_stride, a.sum_stride, a.out_stride, a.n_rows, a.width, split ? a.x_segment : 0u,
+                     a.out_type, a.residual_type == ZKB_VALUE_WORD, a.sum_type == ZKB_VALUE_WORD, a.eps, 0};
+    ZKB_CUDA(ctx, launch_rows<false>(ctx, r, a.x_type == ZKB_VALUE_WORD, vec));
+    return ZKB_OK;
+}
+
+int zkb_step_gate(zkb_ctx* ctx, const zkb_step_gate_args* args) {
+    if (!ctx) return ZKB_EINVAL;
+    ZKB_CHECK_ARG(ctx, args);
+    const zkb_step_gate_args& a = *args;
+    ZKB_CHECK_ARG(ctx, is_values(a.x_type) && (is_values(a.out_type) || a.out_type == ZKB_VALUE_INT8));
+    ZKB_CHECK_ARG(ctx, a.width >= 1 && a.width <= 32768 && a.n_rows <= 0x7fffffffu);
+    if (a.n_rows == 0) return ZKB_OK;
+    const size_t xs = value_size(a.x_type), os = value_size(a.out_type);
+    ZKB_CHECK_ARG(ctx, a.x && a.out && (a.out_type == ZKB_VALUE_INT8 ? a.out_scale != nullptr : !a.out_scale));
+    ZKB_CHECK_ARG(ctx, aligned_to(a.x, xs) && aligned_to(a.gate, xs) && aligned_to(a.out, os) && aligned_to(a.out_scale, 4));
+    ZKB_CHECK_ARG(ctx, a.n_rows == 1 || std::llabs(a.out_stride) >= (long long)a.width);
+    const bool split = a.segment && a.segment < a.width;
+    auto wide = [](const void* p, size_t size, int64_t stride) { return aligned_to(p, size == 1 ? 8 : 16) && (size == 1 ? stride % 8 == 0 : stride * (int64_t)size % 16 == 0); };
+    const bool vec = a.width % 8 == 0 && wide(a.x, xs, a.x_stride) && wide(a.gate, xs, a.gate ? a.gate_stride : 0) && wide(a.out, os, a.out_stride) &&
+                     (!split || (a.segment % 8 == 0 && a.segment_stride * (int64_t)xs % 16 == 0));
+    DeviceGuard g(ctx);
+    ProfScope prof(ctx, "step_gate_kernel");
+    const RowsArgs r{a.x, a.gate, nullptr, nullptr, a.out, a.out_scale, a.x_stride, a.segment_stride, a.gate_stride, 0, a.out_stride, a.n_rows, a.width, split ? a.segment : 0u, a.out_type, false, false, 0.f, 0};
+    ZKB_CUDA(ctx, launch_rows<true>(ctx, r, a.x_type == ZKB_VALUE_WORD, vec));
+    return ZKB_OK;
+}
+
+}  // extern "C"
