@@ -7,15 +7,18 @@
 
 namespace zk {
 
-bool cache_maps(CacheMaps& maps, const zkb_kv_cache& c, uint32_t tokens) {
-    typedef CUresult (*Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                               CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-    static const Encode encode = [] {
+TensorMapEncode tensor_map_encode() {
+    static const TensorMapEncode encode = [] {
         void* f = nullptr;
         cudaDriverEntryPointQueryResult found;
         if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) f = nullptr;
-        return (Encode)f;
+        return (TensorMapEncode)f;
     }();
+    return encode;
+}
+
+bool cache_maps(CacheMaps& maps, const zkb_kv_cache& c, uint32_t tokens) {
+    const TensorMapEncode encode = tensor_map_encode();
     const bool int8 = c.type == ZKB_VALUE_INT8;
     const int64_t size = int8 ? 1 : 2, row = c.head_dim * size, box = std::min<int64_t>(row, 128);
     // a dimension of one entry has no stride to speak of

@@ -78,6 +78,11 @@ __device__ __forceinline__ uint32_t box_place(int row, int at) {
 }
 constexpr unsigned WAIT_RAN_OUT = 0x57e9;  // what zkb_sync reports
 
+// The driver's call that makes a tensor's map, or NULL.
+typedef CUresult (*TensorMapEncode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                    CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+TensorMapEncode tensor_map_encode();
+
 // Maps of a cache's K and V (boxes of `tokens` tokens by up to 128 bytes, swizzled by their own width), or false where the layout has none: the unit wants
 // 16-byte boundaries and strides that ascend.
 struct CacheMaps {

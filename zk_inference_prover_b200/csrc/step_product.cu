@@ -13,27 +13,6 @@ namespace zk {
 // the even and the odd codes of x; 16 bytes are 32 codes of one group, whose sum is exact and then scaled.
 constexpr int CHANNELS = 4;
 
-// 16 bytes from p on, of which the first `valid` are there; the others are zero. VEC: p is on a 16-byte boundary. `inner`: there are 4 more bytes on both sides.
-template <bool VEC>
-__device__ __forceinline__ uint4 load16(const int8_t* p, int valid, bool inner) {
-    if (valid >= 16 && VEC) return *reinterpret_cast<const uint4*>(p);
-    uint32_t w[4] = {};
-    if (valid >= 16 && inner) {
-        const uint32_t off = (uint32_t)(uintptr_t)p & 3;
-        const uint32_t* q = reinterpret_cast<const uint32_t*>(p - off);
-        uint32_t v[5];
-#pragma unroll
-        for (int i = 0; i < 5; i++) v[i] = q[i];
-#pragma unroll
-        for (int i = 0; i < 4; i++) w[i] = __funnelshift_r(v[i], v[i + 1], 8 * off);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 16; i++)
-            if (i < valid) w[i / 4] |= (uint32_t)(uint8_t)p[i] << (8 * (i % 4));
-    }
-    return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
 template <bool INT4, int R, bool VEC>
 __global__ void __launch_bounds__(128) product_few_kernel(const __grid_constant__ zkb_step_product_args a) {
     const int lane = threadIdx.x & 31;
@@ -153,6 +132,10 @@ extern "C" int zkb_step_product(zkb_ctx* ctx, const zkb_step_product_args* args)
     ProfScope prof(ctx, "step_product_kernel");
     const int64_t w_row = int4 ? a.w_stride / 2 : a.w_stride;
     const bool vec = aligned_to(a.x, 16) && aligned_to(a.w, 16) && (a.n_rows == 1 || a.x_stride % 16 == 0) && (a.n_out == 1 || w_row % 16 == 0);
+    if (a.n_rows > 8) {
+        ZKB_CUDA(ctx, int4 ? launch_tiles<true>(ctx, a) : launch_tiles<false>(ctx, a));
+        return ZKB_OK;
+    }
     ZKB_CUDA(ctx, int4 ? (vec ? launch_few<true, true>(ctx, a) : launch_few<true, false>(ctx, a)) : (vec ? launch_few<false, true>(ctx, a) : launch_few<false, false>(ctx, a)));
     return ZKB_OK;
 }
