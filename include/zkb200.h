@@ -602,7 +602,7 @@ typedef struct zkb_step_residual_norm_args {
 } zkb_step_residual_norm_args;
 int zkb_step_residual_norm(zkb_ctx* ctx, const zkb_step_residual_norm_args* args);
 
-/* The gate between a feed-forward layer's products: y = gate / (1 + exp(-gate)) * x, or x itself where gate is NULL (which turns rows of
+/* The gate between a feed-forward layer's products: y = gate / (1 + exp(-gate)) * x (0 for gates below -87, where the factor is less than 10^-35), or x itself where gate is NULL (which turns rows of
  * values, an attention's for one, into codes). Values are read as zkb_step_residual_norm reads x, gate with x's type and segments, and y goes to
  * out as there. width is at most 32768. */
 typedef struct zkb_step_gate_args {
@@ -649,7 +649,7 @@ typedef struct zkb_step_logprobs_args {
     uint64_t* off_table;
     int64_t logits_stride;
     uint32_t n_rows, vocab, n_given, n_top, type;
-    float scale; /* above 0: one over the temperature */
+    float scale; /* one over the temperature: 2^-100 to 2^100 */
 } zkb_step_logprobs_args;
 int zkb_step_logprobs(zkb_ctx* ctx, const zkb_step_logprobs_args* args);
 

@@ -61,7 +61,7 @@ def _logprobs_args(zkb, **other):
 
 
 @pytest.mark.parametrize("other,want", [(dict(type=2), "type"), (dict(vocab=0), "vocab"), (dict(vocab=(1 << 19) + 1), "vocab"), (dict(n_rows=(1 << 26) + 1), "n_rows"), (dict(n_top=33), "n_top"),
-                                        (dict(n_given=(1 << 19) + 1), "n_given"), (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"), (dict(scale=math.inf), "scale"), (dict(logits=0), "logits"),
+                                        (dict(n_given=(1 << 19) + 1), "n_given"), (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"), (dict(scale=math.inf), "scale"), (dict(scale=2.0 ** -101), "scale"), (dict(scale=math.nan), "scale"), (dict(logits=0), "logits"),
                                         (dict(logits=65), "logits"), (dict(type=3, logits=66), "logits"), (dict(ids=0), "ids"), (dict(logprobs=0), "logprobs"), (dict(top_ids=0), "top_ids"),
                                         (dict(top_logprobs=66), "top_logprobs"), (dict(entropy=66), "entropy"), (dict(off_table=68), "off_table")])
 def test_logprobs_refuses(zkb, refuse, other, want):  # noqa: F811

@@ -23,67 +23,76 @@ struct RowsArgs {
     uint32_t warps;  // a row's
 };
 
-// This thread's values of a row: VEC eight adjacent ones at a time, on 16-byte boundaries; else a value at a time, adjacent ones in adjacent lanes.
+// This thread's values of a row, in pairs as bf16: VEC eight adjacent ones at a time, on 16-byte boundaries; else a value at a time, adjacent ones in adjacent lanes.
 template <bool VEC>
 __device__ __forceinline__ uint32_t column_of(uint32_t v, uint32_t y, uint32_t threads, uint32_t th) {
     return VEC ? (v * threads + th) * 8 + y : (v * 8 + y) * threads + th;
 }
 template <int V, bool VEC>
-__device__ __forceinline__ void load_row(const void* p, int64_t row, uint32_t segment, int64_t segment_stride, bool word, uint32_t width, uint32_t threads, uint32_t th, float (&x)[V][8]) {
+__device__ __forceinline__ void load_row(const void* p, int64_t row, uint32_t segment, int64_t segment_stride, bool word, uint32_t width, uint32_t threads, uint32_t th, uint32_t (&x)[V][4]) {
     auto place = [&](uint32_t col) { return row + (segment ? (int64_t)(col / segment) * segment_stride + col % segment : (int64_t)col); };
-    if (word) {
+    if constexpr (VEC) {
+        if (word) {
+            uint4 a[V], b[V];
 #pragma unroll
-        for (int v = 0; v < V; v++) {
-            if constexpr (VEC) {
+            for (int v = 0; v < V; v++) {
                 const uint32_t col = column_of<VEC>(v, 0, threads, th);
-                uint4 a = make_uint4(0u, 0u, 0u, 0u), b = a;
+                a[v] = b[v] = make_uint4(0u, 0u, 0u, 0u);
                 if (col < width) {
                     const uint4* w = reinterpret_cast<const uint4*>(static_cast<const uint32_t*>(p) + place(col));
-                    a = w[0], b = w[1];
+                    a[v] = w[0], b[v] = w[1];
                 }
-                x[v][0] = bf16_low(a.x), x[v][1] = bf16_low(a.y), x[v][2] = bf16_low(a.z), x[v][3] = bf16_low(a.w);
-                x[v][4] = bf16_low(b.x), x[v][5] = bf16_low(b.y), x[v][6] = bf16_low(b.z), x[v][7] = bf16_low(b.w);
-            } else {
+            }
 #pragma unroll
-                for (int y = 0; y < 8; y++) {
-                    const uint32_t col = column_of<VEC>(v, y, threads, th);
-                    x[v][y] = col < width ? bf16_low(static_cast<const uint32_t*>(p)[place(col)]) : 0.f;
-                }
+            for (int v = 0; v < V; v++) {
+                x[v][0] = __byte_perm(a[v].x, a[v].y, 0x5410), x[v][1] = __byte_perm(a[v].z, a[v].w, 0x5410);
+                x[v][2] = __byte_perm(b[v].x, b[v].y, 0x5410), x[v][3] = __byte_perm(b[v].z, b[v].w, 0x5410);
+            }
+        } else {
+#pragma unroll
+            for (int v = 0; v < V; v++) {
+                const uint32_t col = column_of<VEC>(v, 0, threads, th);
+                uint4 a = make_uint4(0u, 0u, 0u, 0u);
+                if (col < width) a = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + place(col));
+                x[v][0] = a.x, x[v][1] = a.y, x[v][2] = a.z, x[v][3] = a.w;
             }
         }
     } else {
 #pragma unroll
         for (int v = 0; v < V; v++) {
-            if constexpr (VEC) {
-                const uint32_t col = column_of<VEC>(v, 0, threads, th);
-                uint4 a = make_uint4(0u, 0u, 0u, 0u);
-                if (col < width) a = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + place(col));
-                x[v][0] = bf16_low(a.x), x[v][1] = bf16_high(a.x), x[v][2] = bf16_low(a.y), x[v][3] = bf16_high(a.y);
-                x[v][4] = bf16_low(a.z), x[v][5] = bf16_high(a.z), x[v][6] = bf16_low(a.w), x[v][7] = bf16_high(a.w);
-            } else {
+            uint32_t h[8];
 #pragma unroll
-                for (int y = 0; y < 8; y++) {
-                    const uint32_t col = column_of<VEC>(v, y, threads, th);
-                    x[v][y] = col < width ? bf16_low(static_cast<const uint16_t*>(p)[place(col)]) : 0.f;
-                }
+            for (int y = 0; y < 8; y++) {
+                const uint32_t col = column_of<VEC>(v, y, threads, th);
+                h[y] = 0;
+                if (col < width) h[y] = word ? static_cast<const uint32_t*>(p)[place(col)] : static_cast<const uint16_t*>(p)[place(col)];
             }
+#pragma unroll
+            for (int y = 0; y < 4; y++) x[v][y] = __byte_perm(h[2 * y], h[2 * y + 1], 0x5410);
         }
     }
 }
 template <int V, bool VEC>
-__device__ __forceinline__ void store_row(void* p, int64_t row, bool word, uint32_t width, uint32_t threads, uint32_t th, const float (&x)[V][8]) {
+__device__ __forceinline__ void store_row(void* p, int64_t row, bool word, uint32_t width, uint32_t threads, uint32_t th, const uint32_t (&x)[V][4]) {
 #pragma unroll
     for (int v = 0; v < V; v++) {
         if constexpr (VEC) {
             const uint32_t col = column_of<VEC>(v, 0, threads, th);
-            if (col < width) word ? store8<true>(p, row + col, x[v]) : store8<false>(p, row + col, x[v]);
+            if (col >= width) continue;
+            if (word) {
+                uint4* const to = reinterpret_cast<uint4*>(static_cast<uint32_t*>(p) + row + col);
+                to[0] = make_uint4(x[v][0] & 0xffffu, x[v][0] >> 16, x[v][1] & 0xffffu, x[v][1] >> 16);
+                to[1] = make_uint4(x[v][2] & 0xffffu, x[v][2] >> 16, x[v][3] & 0xffffu, x[v][3] >> 16);
+            } else {
+                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + row + col) = make_uint4(x[v][0], x[v][1], x[v][2], x[v][3]);
+            }
         } else {
 #pragma unroll
             for (int y = 0; y < 8; y++) {
-                const uint32_t col = column_of<VEC>(v, y, threads, th);
+                const uint32_t col = column_of<VEC>(v, y, threads, th), h = y % 2 ? x[v][y / 2] >> 16 : x[v][y / 2] & 0xffffu;
                 if (col >= width) continue;
-                if (word) static_cast<uint32_t*>(p)[row + col] = round_bf16(x[v][y]);
-                else static_cast<uint16_t*>(p)[row + col] = round_bf16(x[v][y]);
+                if (word) static_cast<uint32_t*>(p)[row + col] = h;
+                else static_cast<uint16_t*>(p)[row + col] = (uint16_t)h;
             }
         }
     }
@@ -94,80 +103,102 @@ struct RowRoom {
     float sum[32];
     uint32_t most[32];
 };
-__device__ __forceinline__ void over_row(RowRoom& room, uint32_t warps, float& sum, uint32_t& most) {
+__device__ __forceinline__ void over_row(RowRoom& room, uint32_t warps, float& sum, float& largest) {
+    uint32_t most = __float_as_uint(largest);  // sizes are ordered as their words, NaN above all
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     most = __reduce_max_sync(0xffffffffu, most);
+    largest = __uint_as_float(most);
     if (warps == 1) return;
     if (lane == 0) room.sum[warp] = sum, room.most[warp] = most;
     __syncthreads();
     sum = lane < warps ? room.sum[lane] : 0.f;
-    most = __reduce_max_sync(0xffffffffu, lane < warps ? room.most[lane] : 0u);
+    largest = __uint_as_float(__reduce_max_sync(0xffffffffu, lane < warps ? room.most[lane] : 0u));
 #pragma unroll
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
 }
-__device__ __forceinline__ uint32_t size_word(float x) { return __float_as_uint(x) & 0x7fffffffu; }  // ordered as |x|, NaN above all
+// The larger of a and |b|, NaN where one of them is.
+__device__ __forceinline__ float larger_size(float a, float b) {
+    float r;
+    asm("{\n\t.reg .f32 t;\n\tabs.f32 t, %2;\n\tmax.NaN.f32 %0, %1, t;\n\t}" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+// g / (1 + exp(-g)): two approximations (2^-22 and 2^-23 of their results) and the products.
+__device__ __forceinline__ float gated(float g) {
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.44269504f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+    return g * r;
+}
 
 constexpr int ROW_GROUP = 4;  // rows a thread block has where a row is a warp's
 
 template <int V, bool GATE, bool VEC>
-__global__ void __launch_bounds__(V == 4 ? 512 : 1024) rows_kernel(const __grid_constant__ RowsArgs a, bool x_word) {
+__global__ void __launch_bounds__(V >= 4 ? 512 : 1024, V == 4 ? 2 : 1) rows_kernel(const __grid_constant__ RowsArgs a, bool x_word) {
     __shared__ RowRoom room[2];
     const uint32_t threads = a.warps * 32, th = a.warps == 1 ? threadIdx.x & 31 : threadIdx.x;
     const int64_t t = a.warps == 1 ? (int64_t)blockIdx.x * ROW_GROUP + (threadIdx.x >> 5) : (int64_t)blockIdx.x;
     if (t >= a.n_rows) return;  // (a whole warp)
-    float x[V][8];
-    uint32_t most = 0;
-    float by = 1.f;
-    {
-        float y[V][8];
-        load_row<V, VEC>(a.x, t * a.x_stride, a.segment, a.segment_stride, x_word, a.width, threads, th, x);
-        if (a.other) load_row<V, VEC>(a.other, t * a.other_stride, GATE ? a.segment : 0u, a.segment_stride, GATE ? x_word : a.other_word, a.width, threads, th, y);
+    uint32_t s[V][4];  // what came in: the residual stream's values
+    float y[V][8];     // what goes out, but for the norm's factor
+    float by = 1.f, most = 0.f;
+    load_row<V, VEC>(a.x, t * a.x_stride, a.segment, a.segment_stride, x_word, a.width, threads, th, s);
+    if constexpr (GATE) {
         if (a.other) {
+            uint32_t g[V][4];
+            load_row<V, VEC>(a.other, t * a.other_stride, a.segment, a.segment_stride, x_word, a.width, threads, th, g);
 #pragma unroll
             for (int v = 0; v < V; v++)
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    if constexpr (GATE) {
-                        // 1 / (1 + exp(-g)) by way of e = exp(-|g|), which does not overflow
-                        const float e = __expf(-fabsf(y[v][i])), s = __fdividef(1.f, 1.f + e);
-                        x[v][i] *= y[v][i] * (y[v][i] < 0.f ? e * s : s);
-                    } else {
-                        x[v][i] = bf16_low(round_bf16(x[v][i] + y[v][i]));
-                    }
-                }
+                for (int i = 0; i < 4; i++) y[v][2 * i] = gated(bf16_low(g[v][i])) * bf16_low(s[v][i]), y[v][2 * i + 1] = gated(bf16_high(g[v][i])) * bf16_high(s[v][i]);
+        } else {
+#pragma unroll
+            for (int v = 0; v < V; v++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) y[v][2 * i] = bf16_low(s[v][i]), y[v][2 * i + 1] = bf16_high(s[v][i]);
         }
-    }
-    if constexpr (!GATE) {
-        if (a.sum) store_row<V, VEC>(a.sum, t * a.sum_stride, a.sum_word, a.width, threads, th, x);
+        if (a.out_type == ZKB_VALUE_INT8) {
+#pragma unroll
+            for (int v = 0; v < V; v++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) most = larger_size(most, y[v][i]);
+            float none = 0.f;
+            over_row(room[0], a.warps, none, most);
+        }
+    } else {
+        uint32_t w[V][4];
+        {
+            uint32_t h[V][4];
+            if (a.other) load_row<V, VEC>(a.other, t * a.other_stride, 0, 0, a.other_word, a.width, threads, th, h);
+            if (a.weight) load_row<V, VEC>(a.weight, 0, 0, 0, false, a.width, threads, th, w);
+            if (a.other) {
+#pragma unroll
+                for (int v = 0; v < V; v++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) s[v][i] = pack_bf16(bf16_low(s[v][i]) + bf16_low(h[v][i]), bf16_high(s[v][i]) + bf16_high(h[v][i]));
+            }
+        }
+        if (a.sum) store_row<V, VEC>(a.sum, t * a.sum_stride, a.sum_word, a.width, threads, th, s);
         float ss = 0.f;
-        float w[V][8];
-        if (a.weight) load_row<V, VEC>(a.weight, 0, 0, 0, false, a.width, threads, th, w);
 #pragma unroll
         for (int v = 0; v < V; v++)
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                ss = fmaf(x[v][i], x[v][i], ss);
-                if (a.weight) w[v][i] *= x[v][i];
-                else w[v][i] = x[v][i];
-                most = max(most, size_word(w[v][i]));
+            for (int i = 0; i < 4; i++) {
+                const float lo = bf16_low(s[v][i]), hi = bf16_high(s[v][i]);
+                ss = fmaf(lo, lo, ss), ss = fmaf(hi, hi, ss);
+                y[v][2 * i] = a.weight ? lo * bf16_low(w[v][i]) : lo, y[v][2 * i + 1] = a.weight ? hi * bf16_high(w[v][i]) : hi;
+                most = larger_size(larger_size(most, y[v][2 * i]), y[v][2 * i + 1]);
             }
         over_row(room[0], a.warps, ss, most);
         const float mean = ss / (float)a.width + a.eps;
-        if (mean > 0x1p-90f && mean < 0x1p120f && most < 0x7f800000u) {  // the same for the whole row
-            by = rsqrtf(mean);
-            most = __float_as_uint(__uint_as_float(most) * by);
-#pragma unroll
-            for (int v = 0; v < V; v++)
-#pragma unroll
-                for (int i = 0; i < 8; i++) x[v][i] = w[v][i] * by;
-        } else {  // squares or products that 32 bits do not hold, or values that are no numbers
+        by = rsqrtf(mean);
+        if (!(mean > 0x1p-90f && mean < 0x1p120f && most < INFINITY)) {  // squares or products that 32 bits do not hold, or values that are no numbers: the same for the whole row
             double wide = 0.;
 #pragma unroll
             for (int v = 0; v < V; v++)
 #pragma unroll
-                for (int i = 0; i < 8; i++) wide += (double)x[v][i] * x[v][i];
+                for (int i = 0; i < 4; i++) wide += (double)bf16_low(s[v][i]) * bf16_low(s[v][i]) + (double)bf16_high(s[v][i]) * bf16_high(s[v][i]);
 #pragma unroll
             for (int o = 16; o; o >>= 1) wide += __shfl_xor_sync(0xffffffffu, wide, o);
             __shared__ double wide_sm[32];
@@ -178,48 +209,49 @@ __global__ void __launch_bounds__(V == 4 ? 512 : 1024) rows_kernel(const __grid_
                 for (uint32_t i = 0; i < a.warps; i++) wide += wide_sm[i];
             }
             const double root = rsqrt(wide / a.width + (double)a.eps);
-            most = 0;
-            if (a.weight) load_row<V, VEC>(a.weight, 0, 0, 0, false, a.width, threads, th, w);
+            most = 0.f, by = 1.f;
 #pragma unroll
             for (int v = 0; v < V; v++)
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    x[v][i] = (float)((double)x[v][i] * (a.weight ? (double)w[v][i] : 1.) * root);
-                    if (column_of<VEC>(v, i, threads, th) < a.width) most = max(most, size_word(x[v][i]));
+                    const uint32_t col = column_of<VEC>(v, i, threads, th);
+                    const double by_weight = a.weight && col < a.width ? (double)bf16_low(a.weight[col]) : 1.;
+                    y[v][i] = (float)((double)(i % 2 ? bf16_high(s[v][i / 2]) : bf16_low(s[v][i / 2])) * by_weight * root);
+                    if (col < a.width) most = larger_size(most, y[v][i]);
                 }
             float none = 0.f;
             over_row(room[1], a.warps, none, most);
         }
-    } else if (a.out_type == ZKB_VALUE_INT8) {
+    }
+    if (a.out_type != ZKB_VALUE_INT8) {
 #pragma unroll
         for (int v = 0; v < V; v++)
 #pragma unroll
-            for (int i = 0; i < 8; i++) most = max(most, size_word(x[v][i]));
-        float none = 0.f;
-        over_row(room[0], a.warps, none, most);
-    }
-    if (a.out_type != ZKB_VALUE_INT8) {
-        store_row<V, VEC>(a.out, t * a.out_stride, a.out_type == ZKB_VALUE_WORD, a.width, threads, th, x);
+            for (int i = 0; i < 4; i++) s[v][i] = pack_bf16(y[v][2 * i] * by, y[v][2 * i + 1] * by);
+        store_row<V, VEC>(a.out, t * a.out_stride, a.out_type == ZKB_VALUE_WORD, a.width, threads, th, s);
         return;
     }
-    float top = __uint_as_float(most), up = 1.f;
-    if (th == 0) a.scale[t] = top / 127.f;
-    if (most < 0x1f800000u) top *= 0x1p64f, up = 0x1p64f;  // below 2^-64: 127 over less than 2^-121 is no float
-    const float to_code = top > 0x1.fcp-80f && most < 0x7f800000u ? 127.f / top : 0.f;  // codes are 0 where the scale is (up to 127 x 2^-150), and where it is NaN or infinite
+    // The codes of y * by: by a factor of 127 over the largest of y, which 1.5 * 2^23 added rounds to the last bits of a float.
+    if (th == 0) a.scale[t] = most * by / 127.f;
+    float to_code = 0.f;
+    const bool small = most < 0x1p-64f;  // 127 over less than 2^-121 is no float
+    if (most < INFINITY) to_code = small ? (most * 0x1p64f > 0x1.fcp-80f ? 127.f / (most * 0x1p64f) : 0.f) : 127.f / most;  // codes are 0 where the scale is (up to 127 x 2^-150)
+    const bool numbers = most < INFINITY;  // else codes are 0
+    int8_t* const to = static_cast<int8_t*>(a.out) + t * a.out_stride;
 #pragma unroll
     for (int v = 0; v < V; v++) {
-        uint32_t q[2] = {0, 0};
+        uint32_t q[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) q[i / 4] |= (uint32_t)(max(-127, min(127, __float2int_rn(x[v][i] * up * to_code))) & 255) << (8 * (i % 4));
-        int8_t* to = static_cast<int8_t*>(a.out) + t * a.out_stride;
+        for (int i = 0; i < 8; i++) q[i] = numbers ? __float_as_uint(fmaf(small ? y[v][i] * 0x1p64f : y[v][i], to_code, 12582912.f)) : 0u;
+        const uint32_t lo = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410), hi = __byte_perm(__byte_perm(q[4], q[5], 0x0040), __byte_perm(q[6], q[7], 0x0040), 0x5410);
         if constexpr (VEC) {
             const uint32_t col = column_of<VEC>(v, 0, threads, th);
-            if (col < a.width) *reinterpret_cast<uint2*>(to + col) = make_uint2(q[0], q[1]);
+            if (col < a.width) *reinterpret_cast<uint2*>(to + col) = make_uint2(lo, hi);
         } else {
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 const uint32_t col = column_of<VEC>(v, i, threads, th);
-                if (col < a.width) to[col] = (int8_t)(q[i / 4] >> (8 * (i % 4)));
+                if (col < a.width) to[col] = (int8_t)q[i];
             }
         }
     }
