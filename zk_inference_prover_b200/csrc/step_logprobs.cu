@@ -11,8 +11,8 @@ namespace zk {
 // A row (a piece of it where rows are few: the thread blocks of a cluster have one each, and the first joins) stays in registers, so its logits are read once; longer pieces are
 // taken in parts. With the part's largest value m, a second pass over the registers sums w = exp(z - m) and w (z - m):
 //   lse = m + log(S),  entropy = log(S) - sum(w (z - m)) / S,  S = 1 + what the others leave, so that log1p has all of its bits where one token is nearly certain.
-// The n_top largest: of n_top groups of threads or more each has a value that reaches the smallest of the groups' largest ones, so the n_top largest do. Those that reach
-// it, a few times n_top, are listed, and each one's rank among them is counted; where too many tie for the list, they are found one after the other.
+// The n_top largest: as many values reach the n_top-th largest of the maxima of groups of lanes, so the n_top largest do. Those that reach
+// it, a few more than n_top, are listed, and each one's rank among them is counted; where too many tie for the list, they are found one after the other.
 constexpr int LP_VECTORS = 8, LP_TOP = 32, LP_LIST = 1024, LP_PARTS = 64, LP_RANKS = 16;
 
 // What is left of a part: the largest logit, how many have it, the sums over the others, the largest n_top with their places.
@@ -37,7 +37,7 @@ constexpr uint32_t WORD_NONE = 0x007fffffu;  // -infinity's
 
 struct LogprobArgs {
     zkb_step_logprobs_args a;
-    uint32_t piece, part, lanes, group_warps;  // logits of a thread block, of a part; lanes of a group, or its warps
+    uint32_t piece, part, lanes;  // logits of a thread block, of a part; lanes of a group
     float log2_scale;
 };
 
@@ -77,32 +77,50 @@ __device__ __forceinline__ float logit_at(const char* row, uint32_t i) {
     else return bf16_low(TYPE == ZKB_VALUE_BF16 ? reinterpret_cast<const uint16_t*>(row)[i] : reinterpret_cast<const uint32_t*>(row)[i]);
 }
 
-// The row that comes next: from memory into L2.
-__device__ __forceinline__ void prefetch_row(const char* row, uint32_t bytes) {
+// The whole 16-byte blocks of a row, into shared memory; how many bytes.
+__device__ __forceinline__ uint32_t copy_row(uint32_t to, const char* row, uint32_t bytes, uint32_t bar) {
     const uint32_t ahead = -(uint32_t)(uintptr_t)row & 15, size = bytes > ahead ? (bytes - ahead) & ~15u : 0u;
-    if (size) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(row + ahead), "r"(size) : "memory");
+    mbar_expect(bar, size);
+    if (ahead) to += 16;  // (where the row's first block is)
+    if (size) asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to), "l"(row + ahead), "r"(size), "r"(bar) : "memory");
+    return size;
 }
 
-// TYPE: ZKB_VALUE_*; N: 16-byte vectors a thread.
-template <int TYPE, int N>
-__global__ void __launch_bounds__(512, 2) logprobs_kernel(const __grid_constant__ LogprobArgs p) {
+// TYPE: ZKB_VALUE_*; N: 16-byte vectors a thread. STAGED: a thread block has row after row, and the next one comes to shared memory while this one is summed.
+template <int TYPE, int N, bool STAGED>
+__global__ void __launch_bounds__(512, 2) logprobs_kernel(const __grid_constant__ LogprobArgs p, unsigned* dev_err) {
+    extern __shared__ __align__(16) unsigned char row_sm[];
+    __shared__ __align__(8) unsigned long long row_bar;
     constexpr int PER = TYPE == ZKB_VALUE_BF16 ? 8 : 4, SIZE = 16 / PER;
     __shared__ LpPart parts[LP_PARTS];
     __shared__ uint64_t list[LP_LIST];
-    __shared__ uint32_t groups[64];
+    __shared__ __align__(16) uint32_t groups[64];
     __shared__ float sums[3][16];
     __shared__ uint32_t n_list;
     __shared__ uint64_t best[16];
     const zkb_step_logprobs_args& a = p.a;
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, rank = cluster_rank(), ranks = cluster_ranks(), n_top = a.n_top;
     const uint32_t begin = min(rank * p.piece, a.vocab), end = min(begin + p.piece, a.vocab), n_parts = (p.piece + p.part - 1) / p.part;
+    const bool alone = ranks == 1 && n_parts == 1;
     if (threadIdx.x == 0) n_list = 0;
+    if (threadIdx.x < 64 && threadIdx.x >= warps * (32 / p.lanes)) groups[threadIdx.x] = 0;
     if (ranks > 1) cluster_arrive();
+    const uint32_t stage = (uint32_t)__cvta_generic_to_shared(row_sm);
+    bool failed = false;
+    uint32_t turn = 0;
+    if constexpr (STAGED) {
+        if (threadIdx.x == 0) {
+            mbar_init(bar_of(row_bar), 1);
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            copy_row(stage, static_cast<const char*>(a.logits) + (int64_t)blockIdx.x * a.logits_stride * SIZE, a.vocab * SIZE, bar_of(row_bar));
+        }
+        __syncthreads();
+    }
     for (uint32_t t = blockIdx.x / ranks; t < a.n_rows; t += gridDim.x / ranks) {  // (one row only where a cluster has it)
     const char* const row = static_cast<const char*>(a.logits) + (int64_t)t * a.logits_stride * SIZE;
-    if (threadIdx.x == 0 && t + gridDim.x / ranks < a.n_rows) prefetch_row(row + (int64_t)(gridDim.x / ranks) * a.logits_stride * SIZE, a.vocab * SIZE);
     // what is asked of the row is on its way meanwhile
-    const int32_t id_first = threadIdx.x < a.n_given ? a.ids[(int64_t)t * a.n_given + threadIdx.x] : -1;
+    const int32_t id_first = threadIdx.x < a.n_given && (!alone || warp == 0) ? a.ids[(int64_t)t * a.n_given + threadIdx.x] : -1;
     const float given_first = id_first >= 0 && (uint32_t)id_first < a.vocab ? logit_at<TYPE>(row, (uint32_t)id_first) : 0.f;
     for (uint32_t q = 0; q < n_parts; q++) {
         const uint32_t from = min(begin + q * p.part, end), to = min(from + p.part, end);
@@ -112,15 +130,11 @@ __global__ void __launch_bounds__(512, 2) logprobs_kernel(const __grid_constant_
         auto place = [&](int i, int y) { return ((uint32_t)i * blockDim.x + threadIdx.x) * PER + y - ahead; };  // from `from` on (wraps below it)
         const uint32_t n = to - from;
         uint32_t raw[N][4];
-#pragma unroll
-        for (int i = 0; i < N; i++) {
+        constexpr uint32_t NONE = TYPE == ZKB_VALUE_BF16 ? 0xff80ff80u : TYPE == ZKB_VALUE_WORD ? 0xff80u : 0xff800000u;
+        auto load_some = [&](int i) {  // a vector of which a part, or nothing, is inside
             const uint32_t at = place(i, 0);
-            constexpr uint32_t NONE = TYPE == ZKB_VALUE_BF16 ? 0xff80ff80u : TYPE == ZKB_VALUE_WORD ? 0xff80u : 0xff800000u;
             raw[i][0] = raw[i][1] = raw[i][2] = raw[i][3] = NONE;
-            if (at < n && n - at >= PER) {
-                const uint4 w = __ldcs(reinterpret_cast<const uint4*>(base + (int64_t)at * SIZE));
-                raw[i][0] = w.x, raw[i][1] = w.y, raw[i][2] = w.z, raw[i][3] = w.w;
-            } else if (at + (PER - 1) < n + (PER - 1)) {  // a part of the vector is inside
+            if (at + (PER - 1) < n + (PER - 1)) {
 #pragma unroll
                 for (int y = 0; y < PER; y++)
                     if (at + y < n) {
@@ -131,6 +145,27 @@ __global__ void __launch_bounds__(512, 2) logprobs_kernel(const __grid_constant_
                             raw[i][y] = *reinterpret_cast<const uint32_t*>(base + (int64_t)(int32_t)(at + y) * SIZE);
                         }
                     }
+            }
+        };
+        if constexpr (STAGED) {
+            if (!failed) failed = !mbar_wait(bar_of(row_bar), turn++ & 1);
+            const uint32_t whole = (n + ahead) / PER;  // vectors up to the first that does not end inside
+#pragma unroll
+            for (int i = 0; i < N; i++) ld_shared4(stage + ((uint32_t)i * blockDim.x + threadIdx.x) * 16, raw[i][0], raw[i][1], raw[i][2], raw[i][3]);
+            if (threadIdx.x == 0 && ahead) load_some(0);
+#pragma unroll
+            for (int i = 0; i < N; i++)
+                if ((uint32_t)i * blockDim.x + threadIdx.x >= whole) load_some(i);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const uint32_t at = place(i, 0);
+                if (at < n && n - at >= PER) {
+                    const uint4 w = __ldcs(reinterpret_cast<const uint4*>(base + (int64_t)at * SIZE));
+                    raw[i][0] = w.x, raw[i][1] = w.y, raw[i][2] = w.z, raw[i][3] = w.w;
+                } else {
+                    load_some(i);
+                }
             }
         }
         auto value = [&](int i, int y) {
@@ -147,8 +182,15 @@ __global__ void __launch_bounds__(512, 2) logprobs_kernel(const __grid_constant_
             }
         };
         float mine = -INFINITY;
+        if constexpr (TYPE == ZKB_VALUE_BF16) {
+            uint32_t w = 0xff80ff80u;
 #pragma unroll
-        for (int i = 0; i < N; i++) mine = largest_of(i, mine);
+            for (int i = 0; i < N; i++) w = max_nan_bf16(w, max_nan_bf16(max_nan_bf16(raw[i][0], raw[i][1]), max_nan_bf16(raw[i][2], raw[i][3])));
+            mine = max_nan(bf16_low(w), bf16_high(w));
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; i++) mine = largest_of(i, mine);
+        }
         // NaN and +infinity are the largest word
         const uint32_t mine_word = mine < INFINITY ? value_word(mine) : 0xffffffffu;
         uint32_t group = mine_word;
@@ -158,14 +200,25 @@ __global__ void __launch_bounds__(512, 2) logprobs_kernel(const __grid_constant_
         const uint32_t a_warp = 32 / p.lanes, n_groups = warps * a_warp;
         if (lane % p.lanes == 0) groups[warp * a_warp + lane / p.lanes] = group;
         __syncthreads();
-        // Every warp finds the largest of the groups' maxima, and the smallest one that is a token's: where those are n_top groups at least, as many values reach it.
+        if constexpr (STAGED) {  // all have their logits in registers
+            if (threadIdx.x == blockDim.x - 1 && !failed && t + gridDim.x < a.n_rows) copy_row(stage, row + (int64_t)gridDim.x * a.logits_stride * SIZE, a.vocab * SIZE, bar_of(row_bar));
+        }
+        // Every warp finds the largest of the groups' maxima, and the n_top-th largest, where that is a token's: as many values reach it.
         const uint32_t one = lane < n_groups ? groups[lane] : 0u, two = lane + 32 < n_groups ? groups[lane + 32] : 0u;
         const uint32_t most_word = __reduce_max_sync(0xffffffffu, max(one, two));
-        uint32_t least = one;
-        for (uint32_t o = 1; o < p.group_warps; o <<= 1) least = max(least, __shfl_xor_sync(0xffffffffu, least, o));
-        const bool has_one = lane < n_groups && lane % p.group_warps == 0 && least > WORD_NONE, has_two = lane + 32 < n_groups && two > WORD_NONE;
-        least = __reduce_min_sync(0xffffffffu, min(has_one ? least : 0xffffffffu, has_two ? two : 0xffffffffu));
-        const uint32_t threshold = __popc(__ballot_sync(0xffffffffu, has_one)) + __popc(__ballot_sync(0xffffffffu, has_two)) >= n_top ? least : WORD_NONE + 1;
+        uint32_t threshold = most_word;
+        if (n_top > 1) {
+            uint32_t above_one = 0, above_two = 0;
+            for (uint32_t g = 0; g < n_groups; g += 4) {
+                const uint4 o = *reinterpret_cast<const uint4*>(&groups[g]);
+                above_one += (o.x > one) + (o.y > one) + (o.z > one) + (o.w > one);
+                if (n_groups > 32) above_two += (o.x > two) + (o.y > two) + (o.z > two) + (o.w > two);
+            }
+            // the smallest that fewer than n_top are above: of equal ones any may be the n_top-th
+            threshold = __reduce_min_sync(0xffffffffu, min(lane < n_groups && above_one < n_top ? one : 0xffffffffu, lane + 32 < n_groups && above_two < n_top ? two : 0xffffffffu));
+            if (n_top > n_groups) threshold = 0;
+        }
+        threshold = max(threshold, WORD_NONE + 1);
         const float most = most_word == 0xffffffffu ? __int_as_float(0x7fc00000) : word_value(most_word);
         const float less = most_word <= WORD_NONE || most_word == 0xffffffffu ? 0.f : most;
         // What is further below is taken for that: its weight is zero, and so is its product with a number.
@@ -266,15 +319,19 @@ __global__ void __launch_bounds__(512, 2) logprobs_kernel(const __grid_constant_
         }
         if (threadIdx.x == 0) part.most = most, part.rest = rest, part.lean = lean, part.equal = equal;
         if (listed <= LP_LIST) {
-            for (uint32_t i = threadIdx.x; i < listed; i += blockDim.x) {
+            // a short list is the first warp's, while the others begin with the next row
+            const uint32_t by_threads = alone && listed <= 64 ? 32u : blockDim.x;
+            for (uint32_t i = threadIdx.x; i < listed && threadIdx.x < by_threads; i += by_threads) {
                 const uint64_t key = list[i];
                 uint32_t above = 0;
 #pragma unroll 4
                 for (uint32_t j = 0; j < listed; j++) above += list[j] > key;
                 if (above < n_top) part.top[above] = key;
             }
-            for (uint32_t i = listed + threadIdx.x; i < n_top; i += blockDim.x) part.top[i] = 0;
-            __syncthreads();
+            if (threadIdx.x < by_threads)
+                for (uint32_t i = listed + threadIdx.x; i < n_top; i += by_threads) part.top[i] = 0;
+            if (by_threads > 32) __syncthreads();
+            else __syncwarp();
         } else {
             uint64_t last = ~0ull;
             for (uint32_t k = 0; k < n_top; k++) {
@@ -300,7 +357,9 @@ __global__ void __launch_bounds__(512, 2) logprobs_kernel(const __grid_constant_
             }
         }
         if (threadIdx.x == 0) n_list = 0;
+        __syncwarp();
     }
+    if (alone && warp) continue;  // the first warp has the rest of the row
     // The thread blocks' parts go to the first one's shared memory, behind its own.
     if (ranks > 1) {
         __syncthreads();
@@ -315,7 +374,7 @@ __global__ void __launch_bounds__(512, 2) logprobs_kernel(const __grid_constant_
         cluster_arrive(), cluster_wait();
         if (rank) return;
     }
-    const uint32_t all = ranks * n_parts;
+    const uint32_t all = ranks * n_parts, joiners = alone ? 32u : blockDim.x;
     // every warp joins the sums, a part a lane
     float most = -INFINITY;
     for (uint32_t i = lane; i < all; i += 32) most = max_nan(most, parts[i].most);
@@ -345,19 +404,19 @@ __global__ void __launch_bounds__(512, 2) logprobs_kernel(const __grid_constant_
     const float total = (float)equal + rest;
     const float log_total = none ? 0.f : equal == 1 ? log1pf(rest) : logf(total);
     auto log_probability = [&](float x) { return odd ? nan : none || x == -INFINITY ? -INFINITY : (x - most) * a.scale - log_total; };
-    if (threadIdx.x == blockDim.x - 1 && a.entropy) a.entropy[t] = odd ? nan : none ? 0.f : log_total - lean * LN2 / total;
-    for (uint32_t i = threadIdx.x; i < a.n_given; i += blockDim.x) {
-        const int32_t id = i < blockDim.x ? id_first : a.ids[(int64_t)t * a.n_given + i];
+    if (threadIdx.x == 0 && a.entropy) a.entropy[t] = odd ? nan : none ? 0.f : log_total - lean * LN2 / total;
+    for (uint32_t i = threadIdx.x; i < a.n_given; i += joiners) {
+        const int32_t id = i == threadIdx.x ? id_first : a.ids[(int64_t)t * a.n_given + i];
         float y = 0.f;
         if (id >= 0 && (uint32_t)id < a.vocab) {
-            y = log_probability(i < blockDim.x ? given_first : logit_at<TYPE>(row, (uint32_t)id));
+            y = log_probability(i == threadIdx.x ? given_first : logit_at<TYPE>(row, (uint32_t)id));
         } else if (a.off_table) {
             atomicAdd(reinterpret_cast<unsigned long long*>(a.off_table), 1ull);
         }
         a.logprobs[(int64_t)t * a.n_given + i] = y;
     }
     // (a key's place is how many others are larger: the parts' keys are in order; places without a token lie behind those with one)
-    for (uint32_t i = threadIdx.x; i < all * n_top; i += blockDim.x) {
+    for (uint32_t i = threadIdx.x; i < all * n_top; i += joiners) {
         const uint32_t mine = i / n_top, place = i - mine * n_top;
         const uint64_t key = parts[mine].top[place];
         uint32_t above = place;
@@ -377,8 +436,12 @@ __global__ void __launch_bounds__(512, 2) logprobs_kernel(const __grid_constant_
             found += k;
         }
         found = __reduce_add_sync(0xffffffffu, found);
-        for (uint32_t i = found + threadIdx.x; i < n_top; i += blockDim.x) a.top_ids[(int64_t)t * n_top + i] = -1, a.top_logprobs[(int64_t)t * n_top + i] = odd ? nan : -INFINITY;
+        for (uint32_t i = found + threadIdx.x; i < n_top; i += joiners) a.top_ids[(int64_t)t * n_top + i] = -1, a.top_logprobs[(int64_t)t * n_top + i] = odd ? nan : -INFINITY;
     }
+    }
+    if (STAGED && failed) {  // nothing is on its way to shared memory when the thread block gives it up
+        *dev_err = WAIT_RAN_OUT;
+        mbar_wait(bar_of(row_bar), (turn - 1) & 1);
     }
 }
 
@@ -389,7 +452,7 @@ static cudaError_t launch_logprobs(zkb_ctx* ctx, const zkb_step_logprobs_args& a
     uint32_t ranks = 1;
     while (ranks < LP_RANKS && a.n_rows <= clusters_at_once(2 * ranks) && a.vocab >= ranks * 4096) ranks *= 2;
     return launch_clusters(ranks, [&](uint32_t n) {
-        LogprobArgs p{a, 0, 0, 32, 1, a.scale * 1.44269504f};
+        LogprobArgs p{a, 0, 0, 32, a.scale * 1.44269504f};
         p.piece = ((a.vocab + n - 1) / n + PER - 1) / PER * PER;
         const uint32_t at_most = 512 * LP_VECTORS * PER - PER;  // (less one vector: the first may begin before the piece)
         const uint32_t n_parts = (p.piece + at_most - 1) / at_most;
@@ -399,23 +462,24 @@ static cudaError_t launch_logprobs(zkb_ctx* ctx, const zkb_step_logprobs_args& a
         uint32_t threads = 64, each = 1;
         while (threads < 512 && threads < vectors && (threads * LP_VECTORS < vectors || (uint64_t)threads * n * a.n_rows < 148 * 512)) threads *= 2;
         while (each * threads < vectors) each *= 2;
-        // the groups: at least n_top, of whole warps or of lanes
-        while (a.n_top > std::min(threads, vectors) / p.lanes && threads / p.lanes < 64) p.lanes /= 2;
-        p.group_warps = 1;
-        if (p.lanes == 32)
-            while (threads / 32 / (2 * p.group_warps) >= std::max(a.n_top, 1u)) p.group_warps *= 2;
+        // The groups that look for the n_top largest, by lanes of a warp or by the whole of it: twice as many of those that have logits, where there are so many threads.
+        while (p.lanes > 1 && threads / p.lanes < 64 && 2 * a.n_top > std::min(threads, vectors) / p.lanes) p.lanes /= 2;
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeClusterDimension;
         attr[0].val.clusterDim = {n, 1, 1};
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(n > 1 ? a.n_rows * n : std::min(a.n_rows, 148u * (2048 / threads)));
+        const uint32_t at_once = 148u * (1024 / threads);
+        const bool staged = n == 1 && n_parts == 1 && each == 8 && a.n_rows > at_once;
+        cfg.gridDim = dim3(n > 1 ? a.n_rows * n : std::min(a.n_rows, at_once));
+        cfg.dynamicSmemBytes = staged ? threads * LP_VECTORS * 16 : 0;
         cfg.blockDim = dim3(threads);
         cfg.stream = ctx->stream;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
-        auto kernel = each == 1 ? logprobs_kernel<TYPE, 1> : each == 2 ? logprobs_kernel<TYPE, 2> : each == 4 ? logprobs_kernel<TYPE, 4> : logprobs_kernel<TYPE, 8>;
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-        return e == cudaSuccess ? cudaLaunchKernelEx(&cfg, kernel, p) : e;
+        auto kernel = staged ? logprobs_kernel<TYPE, 8, true> : each == 1 ? logprobs_kernel<TYPE, 1, false> : each == 2 ? logprobs_kernel<TYPE, 2, false> : each == 4 ? logprobs_kernel<TYPE, 4, false> : logprobs_kernel<TYPE, 8, false>;
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e == cudaSuccess && staged) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 512 * LP_VECTORS * 16);
+        return e == cudaSuccess ? cudaLaunchKernelEx(&cfg, kernel, p, ctx->dev_err) : e;
     });
 }
 
