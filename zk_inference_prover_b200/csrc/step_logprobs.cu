@@ -41,25 +41,6 @@ struct LogprobArgs {
     float log2_scale;
 };
 
-// Two 32-bit floats at once.
-__device__ __forceinline__ uint64_t both(float a, float b) { return two_words(__float_as_uint(a), __float_as_uint(b)); }
-__device__ __forceinline__ uint64_t add_both(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t mul_both(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t fma_both(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ float first_of(uint64_t a) { return __uint_as_float((uint32_t)a); }
-__device__ __forceinline__ float second_of(uint64_t a) { return __uint_as_float((uint32_t)(a >> 32)); }
 __device__ __forceinline__ uint32_t max_nan_bf16(uint32_t a, uint32_t b) {
     uint32_t r;
     asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));

@@ -13,63 +13,79 @@ namespace zk {
 // the even and the odd codes of x; 16 bytes are 32 codes of one group, whose sum is exact and then scaled.
 constexpr int CHANNELS = 4;
 
+// VEC: all rows of x and of the weights start on 16-byte boundaries.
 template <bool INT4, int R, bool VEC>
 __global__ void __launch_bounds__(128) product_few_kernel(const __grid_constant__ zkb_step_product_args a) {
     const int lane = threadIdx.x & 31;
     const uint32_t c0 = (blockIdx.x * 4u + (threadIdx.x >> 5)) * CHANNELS, t0 = blockIdx.y * R;
     if (c0 >= a.n_out) return;
-    const int codes = INT4 ? 32 : 16;  // of 16 bytes
+    constexpr int CODES = INT4 ? 32 : 16, XS = CODES / 16, AHEAD = R == 1 ? (INT4 ? 2 : 4) : R == 2 ? 2 : 1;  // codes of 16 bytes; 16s of x to them; rounds whose weights are on their way at a time
     const int bytes = INT4 ? (int)(a.n_in + 1) / 2 : (int)a.n_in;
     const int64_t w_row = INT4 ? a.w_stride / 2 : a.w_stride;
+    const int8_t *const w_lo = static_cast<const int8_t*>(a.w), *const w_hi = w_lo + (a.n_out - 1) * w_row + bytes, *const x_hi = a.x + (int64_t)(a.n_rows - 1) * a.x_stride + a.n_in;
     const int8_t* w[CHANNELS];
     const uint16_t* s[CHANNELS];
     const int8_t* x[R];
 #pragma unroll
     for (int c = 0; c < CHANNELS; c++) {
         const int64_t at = min(c0 + c, a.n_out - 1);
-        w[c] = static_cast<const int8_t*>(a.w) + at * w_row;
+        w[c] = w_lo + at * w_row;
         s[c] = static_cast<const uint16_t*>(a.w_scale) + (INT4 ? at * a.w_scale_stride : 0);
     }
 #pragma unroll
     for (int r = 0; r < R; r++) x[r] = a.x + (int64_t)min(t0 + r, a.n_rows - 1) * a.x_stride;
+    const uint32_t log_group = INT4 ? 31 - __clz(a.group) : 0;
     int sum[CHANNELS][R] = {};
     float part[CHANNELS][R] = {};
-#pragma unroll(INT4 ? 2 : 4)
-    for (int b = lane * 16; b < bytes; b += 512) {
-        const bool inner = b >= 4 && b + 20 <= bytes;
-        uint4 v[CHANNELS];
+#pragma unroll 1
+    for (int b0 = lane * 16; b0 < bytes; b0 += 512 * AHEAD) {
+        Fetched<VEC> v[AHEAD][CHANNELS];
+        uint32_t by[AHEAD][CHANNELS];
 #pragma unroll
-        for (int c = 0; c < CHANNELS; c++) v[c] = load16<VEC>(w[c] + b, bytes - b, inner);
-        const int at = b / 16 * codes, left = (int)a.n_in - at;
-        if constexpr (INT4) {
-            float by[CHANNELS];
+        for (int h = 0; h < AHEAD; h++) {
+            const int b = b0 + h * 512;
 #pragma unroll
-            for (int c = 0; c < CHANNELS; c++) by[c] = bf16_low(s[c][(uint32_t)at / a.group]) * 0.0625f;
-#pragma unroll
-            for (int r = 0; r < R; r++) {
-                const bool x_inner = at >= 4 && left >= 36;
-                const uint4 lo = load16<VEC>(x[r] + at, left, x_inner), hi = load16<VEC>(x[r] + at + 16, left - 16, x_inner);
-                const uint32_t xs[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-#pragma unroll
-                for (int c = 0; c < CHANNELS; c++) {
-                    const uint32_t ws[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
-                    int d = 0;
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        d = __dp4a((int)(ws[i] << 4 & 0xf0f0f0f0u), (int)__byte_perm(xs[2 * i], xs[2 * i + 1], 0x6420), d);
-                        d = __dp4a((int)(ws[i] & 0xf0f0f0f0u), (int)__byte_perm(xs[2 * i], xs[2 * i + 1], 0x7531), d);
-                    }
-                    part[c][r] = fmaf((float)d, by[c], part[c][r]);
-                }
+            for (int c = 0; c < CHANNELS; c++) {
+                if (b < bytes) v[h][c] = fetch16<VEC>(w[c] + b, w_lo, w_hi);
+                if (INT4 && b < bytes) by[h][c] = s[c][(uint32_t)(b * 2) >> log_group];
             }
-        } else {
+        }
+#pragma unroll
+        for (int h = 0; h < AHEAD; h++) {
+            const int b = b0 + h * 512, at = b / 16 * CODES, left = (int)a.n_in - at;
+            if (b >= bytes) break;
+            uint32_t ws[CHANNELS][4];
+#pragma unroll
+            for (int c = 0; c < CHANNELS; c++) {
+                const uint4 u = fetched16<VEC>(v[h][c], w[c] + b, w_lo, w_hi);
+                ws[c][0] = u.x, ws[c][1] = u.y, ws[c][2] = u.z, ws[c][3] = u.w;
+            }
 #pragma unroll
             for (int r = 0; r < R; r++) {
-                const uint4 u = load16<VEC>(x[r] + at, left, inner);
+                uint32_t xs[4 * XS];
 #pragma unroll
-                for (int c = 0; c < CHANNELS; c++) {
-                    sum[c][r] = __dp4a((int)v[c].x, (int)u.x, sum[c][r]), sum[c][r] = __dp4a((int)v[c].y, (int)u.y, sum[c][r]);
-                    sum[c][r] = __dp4a((int)v[c].z, (int)u.z, sum[c][r]), sum[c][r] = __dp4a((int)v[c].w, (int)u.w, sum[c][r]);
+                for (int i = 0; i < XS; i++) {
+                    uint4 u = make_uint4(0u, 0u, 0u, 0u);
+                    const int8_t* const from = x[r] + at + 16 * i;
+                    if (left > 16 * i) u = first_bytes(fetched16<VEC>(fetch16<VEC>(from, a.x, x_hi), from, a.x, x_hi), left - 16 * i);  // what lies behind a row's codes, of x's or of the weights', counts for nothing
+                    xs[4 * i] = u.x, xs[4 * i + 1] = u.y, xs[4 * i + 2] = u.z, xs[4 * i + 3] = u.w;
+                }
+                if constexpr (INT4) {
+                    uint32_t even[4], odd[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) even[i] = __byte_perm(xs[2 * i], xs[2 * i + 1], 0x6420), odd[i] = __byte_perm(xs[2 * i], xs[2 * i + 1], 0x7531);
+#pragma unroll
+                    for (int c = 0; c < CHANNELS; c++) {
+                        int d = 0;
+#pragma unroll
+                        for (int i = 0; i < 4; i++) d = __dp4a((int)(ws[c][i] << 4 & 0xf0f0f0f0u), (int)even[i], d), d = __dp4a((int)(ws[c][i] & 0xf0f0f0f0u), (int)odd[i], d);
+                        part[c][r] = fmaf((float)d, __uint_as_float(by[h][c] << 16) * 0.0625f, part[c][r]);
+                    }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < CHANNELS; c++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) sum[c][r] = __dp4a((int)ws[c][i], (int)xs[i], sum[c][r]);
                 }
             }
         }

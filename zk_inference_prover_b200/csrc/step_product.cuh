@@ -10,25 +10,47 @@ __device__ __forceinline__ void store_value(void* out, int64_t at, uint32_t type
     else static_cast<float*>(out)[at] = y;
 }
 
-// 16 bytes from p on, of which the first `valid` are there; the others are zero. VEC: p is on a 16-byte boundary. `inner`: there are 4 more bytes on both sides.
+// 16 bytes of codes wherever they start. `lo`, `hi`: the array's first byte and the one behind its last. Fetched as the whole 16-byte blocks of memory that they lie in (VEC: the one
+// block that they are), or other blocks of the array where those reach outside of it, so that several can be on their way; then turned into place, or, at the array's ends, read byte by byte.
 template <bool VEC>
-__device__ __forceinline__ uint4 load16(const int8_t* p, int valid, bool inner) {
-    if (valid >= 16 && VEC) return *reinterpret_cast<const uint4*>(p);
-    uint32_t w[4] = {};
-    if (valid >= 16 && inner) {
-        const uint32_t off = (uint32_t)(uintptr_t)p & 3;
-        const uint32_t* q = reinterpret_cast<const uint32_t*>(p - off);
-        uint32_t v[5];
-#pragma unroll
-        for (int i = 0; i < 5; i++) v[i] = q[i];
-#pragma unroll
-        for (int i = 0; i < 4; i++) w[i] = __funnelshift_r(v[i], v[i + 1], 8 * off);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 16; i++)
-            if (i < valid) w[i / 4] |= (uint32_t)(uint8_t)p[i] << (8 * (i % 4));
+struct Fetched {
+    uint4 a, b;
+};
+template <bool VEC>
+__device__ __forceinline__ bool fetch_reaches_out(const int8_t* p, const int8_t* lo, const int8_t* hi) {
+    return VEC ? p + 16 > hi : p - 15 < lo || p + 31 > hi;
+}
+template <bool VEC>
+__device__ __forceinline__ Fetched<VEC> fetch16(const int8_t* p, const int8_t* lo, const int8_t* hi) {
+    Fetched<VEC> r{make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
+    if (!fetch_reaches_out<VEC>(p, lo, hi)) {
+        const uint4* q = reinterpret_cast<const uint4*>(VEC ? p : p - ((uint32_t)(uintptr_t)p & 15));
+        r.a = q[0];
+        if constexpr (!VEC) r.b = q[1];
     }
-    return make_uint4(w[0], w[1], w[2], w[3]);
+    return r;
+}
+template <bool VEC>
+__device__ __forceinline__ uint4 fetched16(const Fetched<VEC>& r, const int8_t* p, const int8_t* lo, const int8_t* hi) {
+    if (fetch_reaches_out<VEC>(p, lo, hi)) {
+        uint32_t w[4] = {};
+#pragma unroll
+        for (int i = 0; i < 16; i++) w[i / 4] |= p + i >= lo && p + i < hi ? (uint32_t)(uint8_t)p[i] << (8 * (i % 4)) : 0u;
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    if constexpr (VEC) return r.a;
+    const uint32_t m = (uint32_t)(uintptr_t)p & 15, v[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+    uint32_t two[6], one[5];
+#pragma unroll
+    for (int i = 0; i < 6; i++) two[i] = m & 8 ? v[i + 2] : v[i];
+#pragma unroll
+    for (int i = 0; i < 5; i++) one[i] = m & 4 ? two[i + 1] : two[i];
+    return make_uint4(__funnelshift_r(one[0], one[1], 8 * (m & 3)), __funnelshift_r(one[1], one[2], 8 * (m & 3)), __funnelshift_r(one[2], one[3], 8 * (m & 3)), __funnelshift_r(one[3], one[4], 8 * (m & 3)));
+}
+// The first n bytes, zeros behind them.
+__device__ __forceinline__ uint4 first_bytes(uint4 v, int n) {
+    auto keep = [&](uint32_t w, int left) { return left >= 4 ? w : left <= 0 ? 0u : w & ((1u << (8 * left)) - 1u); };
+    return n >= 16 ? v : make_uint4(keep(v.x, n), keep(v.y, n - 4), keep(v.z, n - 8), keep(v.w, n - 12));
 }
 
 template <bool INT4>

@@ -18,23 +18,27 @@ struct ProductMaps {
     CUtensorMap w, x;
 };
 
+// RAW: 4-bit weights come to shared memory by the tensor memory unit (their rows start on 16-byte boundaries, and x's); x then has a ring of its own, longer than the codes' one.
 template <bool INT4, int N, bool TMA>
 struct Tile {
-    static constexpr bool FILLED = INT4 || !TMA;                       // the weights' part of a stage is written by warps
-    static constexpr int EPI = N >= 128 ? 8 : 4, FILL = FILLED ? 8 : 0;  // warps that read the sums, and that write codes
-    static constexpr int THREADS = 32 * (EPI + 2 + FILL), FILLERS = 32 * FILL;
-    static constexpr int A = 128 * 128, B = N * 128, STAGE = A + B;
+    static constexpr bool FILLED = INT4 || !TMA, RAW = INT4 && TMA;     // the weights' part of a stage is written by warps; from shared memory
+    static constexpr int EPI = INT4 ? (N <= 32 ? 4 : N / 8) : N >= 128 ? 8 : 4, SETS = RAW ? 1 : 2;  // warps that read the sums; sets of four warps that write codes, in turn
+    static constexpr int FIRST_FILLER = EPI + (INT4 ? 4 : 3), THREADS = 32 * (FILLED ? FIRST_FILLER + 4 * SETS : EPI + 2);
+    static constexpr int A = 128 * 128, B = N * 128, STAGE = RAW ? A : A + B, RAW_BYTES = 128 * 64;
     static constexpr int BLOCKS = N <= 32 || (N == 64 && !FILLED) ? 2 : 1;  // thread blocks an SM
     static constexpr int JOIN = N <= 64 ? N * 512 : 0;                  // a cluster's sums
-    static constexpr int ROOM = BLOCKS == 2 ? 112 * 1024 : 208 * 1024;
-    static constexpr int STAGES = (ROOM - JOIN) / STAGE < 6 ? (ROOM - JOIN) / STAGE : 6;
-    static constexpr int SUMS = INT4 ? 4 : 2;                           // tiles' or groups' sums in tensor memory at a time
-    static constexpr int COLUMNS = SUMS * N < 32 ? 32 : SUMS * N;
+    static constexpr int RAWS = !RAW ? 0 : N <= 32 ? 4 : N == 64 ? 8 : 6, XS = !RAW ? 0 : N <= 32 ? 8 * 16 / N : 4;
+    static constexpr int SCALES = INT4 ? 4 : 0, SCALE_BYTES = 128 * 16; // eight groups' scales of a tile's outputs
+    static constexpr int ROOM = (BLOCKS == 2 ? 112 * 1024 : 216 * 1024) - JOIN - RAWS * RAW_BYTES - XS * B - SCALES * SCALE_BYTES;
+    static constexpr int STAGES = ROOM / STAGE < 6 ? ROOM / STAGE : 6;
+    // The sums of a tile of 8-bit weights, or of 4-bit weights' groups: of a step's all at once where they have room twice.
+    static constexpr bool BY_STEP = INT4 && N <= 64;
+    static constexpr int SUMS = !INT4 ? 2 : N == 16 || N == 128 ? 4 : 2, SUM = BY_STEP ? 4 * N : N, COLUMNS = SUMS * SUM < 32 ? 32 : SUMS * SUM;
     // A thread block never waits for tensor memory: those that fit an SM's shared memory together (this kernel's variants and attention's, which take all columns and 121 KB) fit its
     // 512 columns. Clusters that each hold what another waits for would wait forever.
     static constexpr int LEAST = BLOCKS == 2 ? 108 * 1024 : 121 * 1024;
-    static constexpr int SMEM = 1024 + (STAGES * STAGE + JOIN > LEAST ? STAGES * STAGE + JOIN : LEAST);
-    static_assert(COLUMNS * BLOCKS <= 512 && (COLUMNS & (COLUMNS - 1)) == 0, "");
+    static constexpr int USED = STAGES * STAGE + RAWS * RAW_BYTES + XS * B + SCALES * SCALE_BYTES + JOIN, SMEM = 1024 + (USED > LEAST ? USED : LEAST);
+    static_assert(COLUMNS * BLOCKS <= 512 && (COLUMNS & (COLUMNS - 1)) == 0 && STAGES >= 2 && SMEM <= 226 * 1024, "");
 };
 
 // kind::i8, signed codes, 32-bit sums, 128 outputs.
@@ -49,7 +53,7 @@ __device__ __forceinline__ void tma_load_2d(uint32_t to, const CUtensorMap* map,
 }
 
 struct TileBars {
-    unsigned long long full[6], empty[6], sum_full[4], sum_empty[4], last;
+    unsigned long long full[6], empty[6], x_full[8], x_empty[8], raw_full[8], raw_empty[8], scale_full[4], scale_empty[4], sum_full[4], sum_empty[4], last;
 };
 
 
@@ -68,8 +72,16 @@ __device__ __forceinline__ void by_type(uint32_t type, F f) {
     else f(std::integral_constant<int, ZKB_VALUE_INT32>());
 }
 
-// VEC: 4-bit weights whose rows start on 16-byte boundaries.
-template <bool INT4, int N, bool TMA, bool VEC>
+// A place in a ring that is gone round, and the parity of its barriers' phase.
+template <int SIZE>
+struct Ring {
+    uint32_t at = 0, parity = 0;
+    __device__ __forceinline__ void next() {
+        if (++at == SIZE) at = 0, parity ^= 1;
+    }
+};
+
+template <bool INT4, int N, bool TMA>
 __global__ void __launch_bounds__((Tile<INT4, N, TMA>::THREADS), (Tile<INT4, N, TMA>::BLOCKS))
     product_tiles_kernel(const __grid_constant__ zkb_step_product_args a, const __grid_constant__ ProductMaps maps, uint32_t row_tiles, uint32_t all_tiles, unsigned* dev_err) {
     using T = Tile<INT4, N, TMA>;
@@ -77,16 +89,17 @@ __global__ void __launch_bounds__((Tile<INT4, N, TMA>::THREADS), (Tile<INT4, N, 
     __shared__ __align__(8) TileBars bars;
     __shared__ uint32_t tmem_sm;
     unsigned char* const sm = tiles_sm + (-(uint32_t)__cvta_generic_to_shared(tiles_sm) & 1023);
-    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(sm);
-    uint32_t* const join = reinterpret_cast<uint32_t*>(sm + T::STAGES * T::STAGE);
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(sm), raw_ring = ring + T::STAGES * T::STAGE, x_ring = raw_ring + T::RAWS * T::RAW_BYTES, scale_ring = x_ring + T::XS * T::B;
+    uint32_t* const join = reinterpret_cast<uint32_t*>(sm + T::STAGES * T::STAGE + T::RAWS * T::RAW_BYTES + T::XS * T::B + T::SCALES * T::SCALE_BYTES);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint32_t rank = cluster_rank(), ranks = cluster_ranks();
     if (warp == T::EPI + 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"((uint32_t)__cvta_generic_to_shared(&tmem_sm)), "n"(T::COLUMNS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     } else if (warp == 0 && lane == 0) {
-        for (int i = 0; i < 6; i++) mbar_init(bar_of(bars.full[i]), (TMA ? 1 : 0) + T::FILLERS), mbar_init(bar_of(bars.empty[i]), 1);
-        for (int i = 0; i < 4; i++) mbar_init(bar_of(bars.sum_full[i]), 1), mbar_init(bar_of(bars.sum_empty[i]), 32 * T::EPI);
+        for (int i = 0; i < 6; i++) mbar_init(bar_of(bars.full[i]), (TMA && !T::RAW ? 1 : 0) + (T::FILLED ? 4 : 0)), mbar_init(bar_of(bars.empty[i]), 1);
+        for (int i = 0; i < 8; i++) mbar_init(bar_of(bars.raw_full[i]), 1), mbar_init(bar_of(bars.raw_empty[i]), 4), mbar_init(bar_of(bars.x_full[i]), 1), mbar_init(bar_of(bars.x_empty[i]), 1);
+        for (int i = 0; i < 4; i++) mbar_init(bar_of(bars.sum_full[i]), 1), mbar_init(bar_of(bars.sum_empty[i]), T::EPI), mbar_init(bar_of(bars.scale_full[i]), 1), mbar_init(bar_of(bars.scale_empty[i]), T::EPI);
         mbar_init(bar_of(bars.last), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -96,6 +109,10 @@ __global__ void __launch_bounds__((Tile<INT4, N, TMA>::THREADS), (Tile<INT4, N, 
         if (!failed) failed = !mbar_wait(bar_of(b), parity & 1);
         failed = __any_sync(0xffffffffu, failed);
     };
+    auto arrive = [&](const unsigned long long& b) {  // once for the whole warp: arrivals at one barrier take turns
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_of(b));
+    };
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
@@ -104,76 +121,139 @@ __global__ void __launch_bounds__((Tile<INT4, N, TMA>::THREADS), (Tile<INT4, N, 
     const uint32_t all_steps = (a.n_in + 127) / 128, who = blockIdx.x / ranks, every = gridDim.x / ranks;
     const uint32_t first_step = rank * all_steps / ranks, steps = (rank + 1) * all_steps / ranks - first_step;
     const uint32_t n_tiles = who < all_tiles ? (all_tiles - who + every - 1) / every : 0, items = n_tiles * steps;
-    auto tile_at = [&](uint32_t i, uint32_t& row_tile, uint32_t& out_tile) {
-        const uint32_t tile = who + i * every;
-        row_tile = tile % row_tiles, out_tile = tile / row_tiles;
+    // The steps of all of this thread block's tiles, one after the other.
+    struct Walk {
+        uint32_t tile, step, row_tile, out_tile;
     };
+    auto enter = [&](Walk& w) { w.row_tile = w.tile % row_tiles, w.out_tile = w.tile / row_tiles; };
+    auto first = [&] {
+        Walk w{who, 0, 0, 0};
+        enter(w);
+        return w;
+    };
+    auto next = [&](Walk& w) {
+        if (++w.step == steps) w.step = 0, w.tile += every, enter(w);
+    };
+    const uint32_t log_group = INT4 ? 31 - __clz(a.group) : 7, per_step = 128 >> log_group, groups = (a.n_in + (1u << log_group) - 1) >> log_group;
+    auto groups_in = [&](uint32_t step) { return min(per_step, groups - (first_step + step) * per_step); };
 
     if (warp < T::EPI) {  // ---- the sums: a thread has an output, and half of the rows where two threads share it
-        constexpr int MINE = N / (T::EPI / 4), CHUNK = MINE < 32 ? 8 : 32;
+        constexpr int MINE = N / (T::EPI / 4), CHUNK = MINE < 32 ? 16 : 32;
         const uint32_t c128 = (uint32_t)(warp & 3) * 32 + lane, half = (uint32_t)(warp >> 2) * MINE, at_lanes = tmem + ((uint32_t)(warp & 3) << 21) + half;
-        uint32_t done = 0;  // sums read
-        for (uint32_t i = 0; i < n_tiles; i++) {
-            uint32_t row_tile, out_tile;
-            tile_at(i, row_tile, out_tile);
-            const uint32_t c = out_tile * 128 + c128, t0 = row_tile * N + half;
+        Ring<T::SUMS> sums;
+        Ring<(T::SCALES > 0 ? T::SCALES : 1)> scale;
+        Walk w = first();
+        for (uint32_t i = 0; i < n_tiles; i++, w.tile += every, enter(w)) {
+            const uint32_t c = w.out_tile * 128 + c128, t0 = w.row_tile * N + half;
             const bool live = c < a.n_out;
-            uint32_t x[CHUNK];
-            // the sums of columns `from` on, CHUNK at a time, to `use`
-            auto read = [&](auto use) {
-                const uint32_t buf = done % T::SUMS;
-                wait(bars.sum_full[buf], done / T::SUMS);
-                tmem_fence_after();
+            // CHUNK columns at a time of the sums at `at`, to `use`
+            auto read = [&](uint32_t at, bool last, auto use) {
 #pragma unroll
                 for (int j = 0; j < MINE; j += CHUNK) {
-                    if constexpr (CHUNK == 32) tmem_load32(at_lanes + buf * N + j, x);
-                    else tmem_load8(at_lanes + buf * N + j, x);
+                    uint32_t x[CHUNK];
+                    if constexpr (CHUNK == 32) tmem_load32(at + j, x);
+                    else tmem_load16(at + j, x);
                     tmem_loaded(x);
-                    if (j + CHUNK == MINE) {
+                    if (last && j + CHUNK == MINE) {
                         tmem_fence_before();
-                        mbar_arrive(bar_of(bars.sum_empty[buf]));
+                        arrive(bars.sum_empty[sums.at]);
                     }
-                    use(j);
+                    use(j, x);
                 }
-                done++;
             };
-            auto share = [&](int column, uint32_t word) {  // to the thread block that adds up this row
-                const uint32_t of = N / ranks, to = column / of;
+            auto arrived = [&] {
+                wait(bars.sum_full[sums.at], sums.parity);
+                tmem_fence_after();
+            };
+            auto share = [&](int j, uint32_t word) {  // to the thread block that adds up this row
+                const uint32_t of = N / ranks, column = half + j, to = column / of;
                 peer_store_word(join + (rank * of + column % of) * 128 + c128, (int)to, word);
             };
             if constexpr (INT4) {
-                float acc[MINE];
+                uint64_t acc[MINE / 2];
 #pragma unroll
-                for (int j = 0; j < MINE; j++) acc[j] = 0.f;
-                const uint32_t groups = (a.n_in + a.group - 1) / a.group, per = 128 / a.group;
-                const uint16_t* const scales = static_cast<const uint16_t*>(a.w_scale) + (int64_t)min(c, a.n_out - 1) * a.w_scale_stride;
-                const uint32_t g0 = first_step * per, g1 = min((first_step + steps) * per, groups);
-                uint32_t scale = g0 < g1 ? scales[g0] : 0u;
-#pragma unroll 1
-                for (uint32_t g = g0; g < g1; g++) {
-                    const float by = __uint_as_float(scale << 16) * 0.0625f;  // (the codes are 16 times themselves)
-                    scale = g + 1 < g1 ? scales[g + 1] : 0u;
-                    read([&](int j) {
+                for (int j = 0; j < MINE / 2; j++) acc[j] = 0;
+                uint32_t now[4], k8 = 8;  // eight groups' scales
+                auto next_scale = [&] {
+                    if (k8 == 8) {
+                        k8 = 0;
+                        wait(bars.scale_full[scale.at], scale.parity);
+                        ld_shared4(scale_ring + scale.at * T::SCALE_BYTES + c128 * 16, now[0], now[1], now[2], now[3]);
+                        arrive(bars.scale_empty[scale.at]);
+                        scale.next();
+                    }
+                    const uint32_t two = k8 < 4 ? (k8 < 2 ? now[0] : now[1]) : (k8 < 6 ? now[2] : now[3]);
+                    const float s = __uint_as_float(k8 & 1 ? two & 0xffff0000u : two << 16);
+                    k8++;
+                    return s * 0.0625f;  // (the codes are 16 times themselves)
+                };
+                // the sums of two groups of sixteen rows
+                auto add_two = [&](uint32_t at, bool last) {
+                    const float by0 = next_scale(), by1 = next_scale();
+                    const uint64_t less = both(-12582912.f, -12582912.f);
+                    uint32_t x[32];
+                    tmem_load32(at, x);
+                    tmem_loaded(x);
+                    if (last) {
+                        tmem_fence_before();
+                        arrive(bars.sum_empty[sums.at]);
+                    }
 #pragma unroll
-                        for (int y = 0; y < CHUNK; y++) acc[j + y] = fmaf((float)(int)x[y], by, acc[j + y]);
+                    for (int y = 0; y < 32; y += 2) {
+                        const float by = y < 16 ? by0 : by1;
+                        acc[y % 16 / 2] = fma_both(add_both(two_words(x[y] + 0x4b400000u, x[y + 1] + 0x4b400000u), less), both(by, by), acc[y % 16 / 2]);
+                    }
+                };
+                auto add = [&](uint32_t at, bool last) {
+                    const float by = next_scale();
+                    // A sum below 2^22 added to the pattern of 1.5 * 2^23 is that float plus the sum: a conversion by two additions (the instruction for it has an eighth of their rate).
+                    const uint64_t by_both = both(by, by), less = both(-12582912.f, -12582912.f);
+                    read(at, last, [&](int j, const uint32_t(&x)[CHUNK]) {
+#pragma unroll
+                        for (int y = 0; y < CHUNK; y += 2) acc[(j + y) / 2] = fma_both(add_both(two_words(x[y] + 0x4b400000u, x[y + 1] + 0x4b400000u), less), by_both, acc[(j + y) / 2]);
                     });
+                };
+#pragma unroll 1
+                for (uint32_t s = 0; s < steps; s++) {
+                    const uint32_t n = groups_in(s);
+                    if constexpr (T::BY_STEP) {
+                        arrived();
+#pragma unroll 1
+                        for (uint32_t k = 0; k < n; k++) {
+                            const uint32_t at = at_lanes + sums.at * T::SUM + k * N;
+                            if (N == 16 && k + 1 < n) add_two(at, ++k + 1 == n);
+                            else add(at, k + 1 == n);
+                        }
+                        sums.next();
+                    } else {
+#pragma unroll 1
+                        for (uint32_t k = 0; k < n; k++) {
+                            arrived();
+                            add(at_lanes + sums.at * T::SUM, true);
+                            sums.next();
+                        }
+                    }
                 }
                 if (ranks == 1) {
                     if (live)
                         by_type<INT4>(a.out_type, [&](auto type) {
 #pragma unroll
                             for (int j = 0; j < MINE; j++)
-                                if (t0 + j < a.n_rows) put<decltype(type)::value, INT4>(a, t0 + j, c, __float_as_uint(acc[j]), 1.f);
+                                if (t0 + j < a.n_rows) put<decltype(type)::value, INT4>(a, t0 + j, c, (uint32_t)(acc[j / 2] >> (32 * (j % 2))), 1.f);
                         });
                 } else if constexpr (T::JOIN > 0) {
                     cluster_wait();
 #pragma unroll
-                    for (int j = 0; j < MINE; j++) share(j, __float_as_uint(acc[j]));
+                    for (int j = 0; j < MINE; j++) share(j, (uint32_t)(acc[j / 2] >> (32 * (j % 2))));
                 }
             } else {
                 const float by = live && a.w_scale ? static_cast<const float*>(a.w_scale)[c] : 1.f;
+                if (ranks > 1) {
+                    if constexpr (T::JOIN > 0) cluster_wait();
+                }
+                arrived();
                 if (ranks == 1) {
-                    read([&](int j) {
+                    read(at_lanes + sums.at * T::SUM, true, [&](int j, const uint32_t(&x)[CHUNK]) {
                         if (live)
                             by_type<INT4>(a.out_type, [&](auto type) {
 #pragma unroll
@@ -182,149 +262,226 @@ __global__ void __launch_bounds__((Tile<INT4, N, TMA>::THREADS), (Tile<INT4, N, 
                             });
                     });
                 } else if constexpr (T::JOIN > 0) {
-                    cluster_wait();
-                    read([&](int j) {
+                    read(at_lanes + sums.at * T::SUM, true, [&](int j, const uint32_t(&x)[CHUNK]) {
 #pragma unroll
                         for (int y = 0; y < CHUNK; y++) share(j + y, x[y]);
                     });
                 }
+                sums.next();
             }
         }
     } else if (warp == T::EPI) {  // ---- copies
-        if constexpr (TMA) {
+        if constexpr (TMA) {  // x and 8-bit weights into the stages, or x into its own ring
+            constexpr int SIZE = T::RAW ? T::XS : T::STAGES;
+            auto& full = T::RAW ? bars.x_full : reinterpret_cast<unsigned long long(&)[8]>(bars.full);
+            auto& empty = T::RAW ? bars.x_empty : reinterpret_cast<unsigned long long(&)[8]>(bars.empty);
             uint32_t sent = 0;
-            for (uint32_t i = 0; i < items; i++) {
-                const uint32_t st = i % T::STAGES, step = first_step + i % steps;
-                uint32_t row_tile, out_tile;
-                tile_at(i / steps, row_tile, out_tile);
-                wait(bars.empty[st], i / T::STAGES + 1);
+            Ring<SIZE> st;
+            Walk w = first();
+            for (; sent < items; sent++, st.next(), next(w)) {
+                wait(empty[st.at], st.parity ^ 1);
                 if (failed) break;
-                sent = i + 1;
                 if (lane == 0) {
-                    const uint32_t to = ring + st * T::STAGE, bar = bar_of(bars.full[st]);
-                    mbar_expect(bar, INT4 ? T::B : T::STAGE);
-                    if constexpr (!INT4) tma_load_2d(to, &maps.w, step * 128, out_tile * 128, bar);
-                    tma_load_2d(to + T::A, &maps.x, step * 128, row_tile * N, bar);
+                    const uint32_t to = T::RAW ? x_ring + st.at * T::B : ring + st.at * T::STAGE + T::A, bar = bar_of(full[st.at]);
+                    mbar_expect(bar, T::RAW ? T::B : T::STAGE);
+                    if constexpr (!INT4) tma_load_2d(to - T::A, &maps.w, (first_step + w.step) * 128, w.out_tile * 128, bar);
+                    tma_load_2d(to, &maps.x, (first_step + w.step) * 128, w.row_tile * N, bar);
                 }
                 __syncwarp();
             }
             // Whatever is on its way comes to its place before the thread block ends, though a wait may have run out.
-            for (uint32_t j = sent < T::STAGES ? 0 : sent - T::STAGES; j < sent; j++) mbar_wait(bar_of(bars.full[j % T::STAGES]), (j / T::STAGES) & 1);
+            for (uint32_t j = sent < SIZE ? 0 : sent - SIZE; j < sent; j++) mbar_wait(bar_of(full[j % SIZE]), (j / SIZE) & 1);
         }
     } else if (warp == T::EPI + 1) {  // ---- products
         constexpr uint32_t high = (1024u >> 4) | 1u << 14 | 2u << 29, desc = codes_desc(N);
-        const uint32_t a_low = (ring >> 4 & 0x3fff) | 1u << 16, tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
+        const uint32_t a_low = (ring >> 4 & 0x3fff) | 1u << 16, x_low = (x_ring >> 4 & 0x3fff) | 1u << 16, tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
         const bool one = elect_one();
-        uint32_t done = 0;
+        Ring<T::STAGES> st;
+        Ring<(T::XS > 0 ? T::XS : 1)> xs;
+        Ring<T::SUMS> sums;
+        const uint32_t parts = (1u << log_group) / 32;
+        uint32_t step = 0;
 #pragma unroll 1
-        for (uint32_t i = 0; i < items; i++) {
-            const uint32_t st = i % T::STAGES, in_tile = i % steps;
-            const uint32_t from_a = a_low + st * (T::STAGE >> 4), from_b = from_a + (T::A >> 4);
+        for (uint32_t i = 0; i < items; i++, st.next()) {
+            const uint32_t from_a = a_low + st.at * (T::STAGE >> 4), from_b = T::RAW ? x_low + xs.at * (T::B >> 4) : from_a + (T::A >> 4);
             if constexpr (!INT4) {
-                if (in_tile == 0) wait(bars.sum_empty[done % T::SUMS], done / T::SUMS + 1);
+                if (step == 0) wait(bars.sum_empty[sums.at], sums.parity ^ 1);
             }
-            wait(bars.full[st], i / T::STAGES);
+            if constexpr (T::RAW) wait(bars.x_full[xs.at], xs.parity);
+            wait(bars.full[st.at], st.parity);
             if (failed) break;
             tmem_fence_after();
             if constexpr (INT4) {
-                const uint32_t left = min(128u, a.n_in - (first_step + in_tile) * 128), groups = (left + a.group - 1) / a.group, parts = a.group / 32;
-                for (uint32_t g = 0; g < groups; g++) {
-                    wait(bars.sum_empty[done % T::SUMS], done / T::SUMS + 1);
-                    if (failed) break;
-                    tmem_fence_after();
+                const uint32_t n = groups_in(step);
+                for (uint32_t g = 0; g < n; g++) {
+                    if (!T::BY_STEP || g == 0) {
+                        wait(bars.sum_empty[sums.at], sums.parity ^ 1);
+                        if (failed) break;
+                        tmem_fence_after();
+                    }
                     for (uint32_t k = 0; k < parts; k++) {
                         const uint32_t at = 2 * (g * parts + k);
-                        product_codes(one, tmem_u + done % T::SUMS * N, two_words(from_a + at, high), two_words(from_b + at, high), desc, k > 0);
+                        product_codes(one, tmem_u + sums.at * T::SUM + (T::BY_STEP ? g * N : 0), two_words(from_a + at, high), two_words(from_b + at, high), desc, k > 0);
                     }
-                    if (one) products_done(bar_of(bars.sum_full[done % T::SUMS]));
-                    done++;
+                    if (!T::BY_STEP || g + 1 == n) {
+                        if (one) products_done(bar_of(bars.sum_full[sums.at]));
+                        sums.next();
+                    }
                 }
-                if (one) products_done(bar_of(bars.empty[st]));
+                if (one) {
+                    products_done(bar_of(bars.empty[st.at]));
+                    if constexpr (T::RAW) products_done(bar_of(bars.x_empty[xs.at]));
+                }
+                if constexpr (T::RAW) xs.next();
             } else {
 #pragma unroll
                 for (uint32_t k = 0; k < 4; k++)
-                    product_codes(one, tmem_u + done % T::SUMS * N, two_words(from_a + 2 * k, high), two_words(from_b + 2 * k, high), desc, in_tile > 0 || k > 0);
+                    product_codes(one, tmem_u + sums.at * T::SUM, two_words(from_a + 2 * k, high), two_words(from_b + 2 * k, high), desc, step > 0 || k > 0);
                 if (one) {
-                    products_done(bar_of(bars.empty[st]));
-                    if (in_tile + 1 == steps) products_done(bar_of(bars.sum_full[done % T::SUMS]));
+                    products_done(bar_of(bars.empty[st.at]));
+                    if (step + 1 == steps) products_done(bar_of(bars.sum_full[sums.at]));
                 }
-                if (in_tile + 1 == steps) done++;
+                if (step + 1 == steps) sums.next();
             }
+            if (++step == steps) step = 0;
             __syncwarp();
         }
         // Nothing is at work in tensor memory when the thread block gives it up, though a wait may have run out.
         if (one) products_done(bar_of(bars.last));
         __syncwarp();
         mbar_wait(bar_of(bars.last), 0);
-    } else if constexpr (T::FILLED) {  // ---- codes into shared memory
-        const int f = threadIdx.x - 32 * (T::EPI + 2);
-        const int64_t w_row = INT4 ? a.w_stride / 2 : a.w_stride;
-        const int bytes = INT4 ? (int)(a.n_in + 1) / 2 : (int)a.n_in;
-        constexpr int STEP = INT4 ? 64 : 128, ROW = STEP / 16, MINE = 128 * ROW / T::FILLERS;  // bytes of a row's step, 16s of them, a thread's
-        constexpr int AHEAD = VEC ? 4 : 1;
-        auto load_w = [&](uint32_t i, uint4 (&v)[MINE]) {
-            uint32_t row_tile, out_tile;
-            tile_at(i / steps, row_tile, out_tile);
-            const int step = (int)(first_step + i % steps);
-#pragma unroll
-            for (int j = 0; j < MINE; j++) {
-                const int q = f + j * T::FILLERS, row = q / ROW, b = step * STEP + q % ROW * 16;
-                const int8_t* const from = static_cast<const int8_t*>(a.w) + (int64_t)min(out_tile * 128 + row, a.n_out - 1) * w_row + b;
-                v[j] = b < bytes ? load16<VEC>(from, bytes - b, b >= 4 && b + 20 <= bytes) : make_uint4(0u, 0u, 0u, 0u);
-            }
-        };
-        uint4 v[AHEAD][MINE];
-        if constexpr (VEC) {
-#pragma unroll
-            for (int j = 0; j < AHEAD; j++)
-                if (j < (int)items) load_w(j, v[j]);
-        }
-#pragma unroll 1
-        for (uint32_t i0 = 0; i0 < items; i0 += AHEAD) {
-#pragma unroll
-            for (int k = 0; k < AHEAD; k++) {
-                const uint32_t i = i0 + k, st = i % T::STAGES;
-                if (i >= items) break;
-                if constexpr (!VEC) load_w(i, v[0]);
-                wait(bars.empty[st], i / T::STAGES + 1);
-                if (failed) break;
-                const uint32_t to = ring + st * T::STAGE;
-#pragma unroll
-                for (int j = 0; j < MINE; j++) {
-                    const int q = f + j * T::FILLERS, row = q / ROW, b = q % ROW * 16;
-                    if constexpr (INT4) {
-                        const uint32_t w[4] = {v[k][j].x, v[k][j].y, v[k][j].z, v[k][j].w};
-                        uint32_t u[8];
-#pragma unroll
-                        for (int y = 0; y < 4; y++) {
-                            const uint32_t even = w[y] << 4 & 0xf0f0f0f0u, odd = w[y] & 0xf0f0f0f0u;
-                            u[2 * y] = __byte_perm(even, odd, 0x5140), u[2 * y + 1] = __byte_perm(even, odd, 0x7362);
-                        }
-                        st_shared4(to + box_place<128>(row, 2 * b), u[0], u[1], u[2], u[3]);
-                        st_shared4(to + box_place<128>(row, 2 * b + 16), u[4], u[5], u[6], u[7]);
-                    } else {
-                        st_shared4(to + box_place<128>(row, b), v[k][j].x, v[k][j].y, v[k][j].z, v[k][j].w);
+    } else if constexpr (T::FILLED) {
+        if (warp == T::EPI + 2) {  // ---- copies of 4-bit weights
+            if constexpr (T::RAW) {
+                uint32_t sent = 0;
+                Ring<T::RAWS> rs;
+                Walk w = first();
+                for (; sent < items; sent++, rs.next(), next(w)) {
+                    wait(bars.raw_empty[rs.at], rs.parity ^ 1);
+                    if (failed) break;
+                    if (lane == 0) {
+                        mbar_expect(bar_of(bars.raw_full[rs.at]), T::RAW_BYTES);
+                        tma_load_2d(raw_ring + rs.at * T::RAW_BYTES, &maps.w, (first_step + w.step) * 64, w.out_tile * 128, bar_of(bars.raw_full[rs.at]));
                     }
+                    __syncwarp();
                 }
-                if constexpr (!TMA) {
-                    uint32_t row_tile, out_tile;
-                    tile_at(i / steps, row_tile, out_tile);
-                    const int step = (int)(first_step + i % steps);
-#pragma unroll 4
-                    for (int q = f; q < N * 8; q += T::FILLERS) {
-                        const int row = q / 8, b = q % 8 * 16, at = step * 128 + b;
-                        const int8_t* const from = a.x + (int64_t)min(row_tile * N + row, a.n_rows - 1) * a.x_stride + at;
-                        const uint4 u = at < (int)a.n_in ? load16<false>(from, (int)a.n_in - at, at >= 4 && at + 20 <= (int)a.n_in) : make_uint4(0u, 0u, 0u, 0u);
-                        st_shared4(to + T::A + box_place<128>(row, b), u.x, u.y, u.z, u.w);
+                for (uint32_t j = sent < T::RAWS ? 0 : sent - T::RAWS; j < sent; j++) mbar_wait(bar_of(bars.raw_full[j % T::RAWS]), (j / T::RAWS) & 1);
+            }
+        } else if (INT4 && warp == T::EPI + 3) {  // ---- scales, eight groups of the tile's 128 outputs at a time, four outputs a lane; the next ones on their way
+            Ring<(T::SCALES > 0 ? T::SCALES : 1)> scale;
+            const uint32_t g0 = first_step * per_step, g1 = min((first_step + steps) * per_step, groups), blocks = (g1 - g0 + 7) / 8;
+            const uint16_t* const scales = static_cast<const uint16_t*>(a.w_scale);
+            auto each = [&](auto load) {  // load(first scale, how many are there): eight
+                uint32_t out_tile = who / row_tiles, block = 0, tile = who;
+                uint4 ahead[4];
+                auto fetch = [&] {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) ahead[j] = load(scales + (int64_t)min(out_tile * 128 + j * 32 + lane, a.n_out - 1) * a.w_scale_stride + g0 + block * 8, groups - (g0 + block * 8));
+                    if (++block == blocks) block = 0, tile += every, out_tile = tile / row_tiles;
+                };
+                const uint32_t all = n_tiles * blocks;
+                if (all) fetch();
+                for (uint32_t i = 0; i < all; i++) {
+                    uint4 now[4];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) now[j] = ahead[j];
+                    if (i + 1 < all) fetch();
+                    wait(bars.scale_empty[scale.at], scale.parity ^ 1);
+                    if (failed) break;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) st_shared4(scale_ring + scale.at * T::SCALE_BYTES + (j * 32 + lane) * 16, now[j].x, now[j].y, now[j].z, now[j].w);
+                    arrive(bars.scale_full[scale.at]);
+                    scale.next();
+                }
+            };
+            auto one_by_one = [](const uint16_t* p, uint32_t n) {
+                uint32_t v[8];
+#pragma unroll
+                for (int y = 0; y < 8; y++) v[y] = y < n ? p[y] : 0u;
+                return make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
+            };
+            // 16 bytes at once where all of them are there (a row's last ones may not be)
+            if (aligned16(scales + g0) && (a.n_out == 1 || a.w_scale_stride % 8 == 0) && groups % 8 == 0) each([](const uint16_t* p, uint32_t) { return *reinterpret_cast<const uint4*>(p); });
+            else each(one_by_one);
+        } else {  // ---- codes into shared memory: each set of four warps every SETS-th step
+            const int f = threadIdx.x - 32 * T::FIRST_FILLER, th = f & 127, set = f >> 7;
+            const int64_t w_row = INT4 ? a.w_stride / 2 : a.w_stride;
+            const int bytes = INT4 ? (int)(a.n_in + 1) / 2 : (int)a.n_in;
+            constexpr int STEP = INT4 ? 64 : 128, ROW = STEP / 16, MINE = ROW;  // bytes of a row's step, 16s of them, a thread's
+            auto put_codes = [&](uint32_t to, int row, int b, const uint4& v) {  // 16 bytes from byte b of a row's step on
+                if constexpr (INT4) {
+                    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                    uint32_t u[8];
+#pragma unroll
+                    for (int y = 0; y < 4; y++) {
+                        const uint32_t even = w[y] << 4 & 0xf0f0f0f0u, odd = w[y] & 0xf0f0f0f0u;
+                        u[2 * y] = __byte_perm(even, odd, 0x5140), u[2 * y + 1] = __byte_perm(even, odd, 0x7362);
                     }
+                    st_shared4(to + box_place<128>(row, 2 * b), u[0], u[1], u[2], u[3]);
+                    st_shared4(to + box_place<128>(row, 2 * b + 16), u[4], u[5], u[6], u[7]);
+                } else {
+                    st_shared4(to + box_place<128>(row, b), v.x, v.y, v.z, v.w);
+                }
+            };
+            Ring<T::STAGES> st;
+            Ring<(T::RAWS > 0 ? T::RAWS : 1)> rs;
+            Walk w = first();
+            auto skip = [&] {
+                st.next(), next(w);
+                if constexpr (T::RAW) rs.next();
+            };
+            for (int i = 0; i < set; i++) skip();
+#pragma unroll 1
+            for (uint32_t i = set; i < items; i += T::SETS) {
+                const uint32_t to = ring + st.at * T::STAGE;
+                if constexpr (T::RAW) {
+                    wait(bars.raw_full[rs.at], rs.parity);
+                    uint4 v[MINE];
+#pragma unroll
+                    for (int j = 0; j < MINE; j++) ld_shared4(raw_ring + rs.at * T::RAW_BYTES + (th + j * 128) * 16, v[j].x, v[j].y, v[j].z, v[j].w);
+                    wait(bars.empty[st.at], st.parity ^ 1);
+                    if (failed) break;
+#pragma unroll
+                    for (int j = 0; j < MINE; j++) put_codes(to, (th + j * 128) / ROW, (th + j * 128) % ROW * 16, v[j]);
+                    arrive(bars.raw_empty[rs.at]);
+                } else {
+                    const int step = (int)(first_step + w.step);
+                    const int8_t *const w_lo = static_cast<const int8_t*>(a.w), *const w_hi = w_lo + (a.n_out - 1) * w_row + bytes, *const x_hi = a.x + (int64_t)(a.n_rows - 1) * a.x_stride + a.n_in;
+                    // Four 16s at a time: their loads, and then, into a stage that is free, their codes. What lies behind a row's codes counts for nothing where x is zero there (`cut`).
+                    auto four = [&](int q0, int n, auto from_of, const int8_t* lo, const int8_t* hi, int row_bytes, int at, auto to_place, bool cut) {
+                        Fetched<false> r[4];
+                        const int8_t* p[4];
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            const int q = q0 + j * 128;
+                            p[j] = from_of(q);
+                            if (q < n) r[j] = fetch16<false>(p[j], lo, hi);
+                        }
+                        wait(bars.empty[st.at], st.parity ^ 1);
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            const int q = q0 + j * 128;
+                            if (q < n) {
+                                const uint4 v = fetched16<false>(r[j], p[j], lo, hi);
+                                to_place(q, cut ? first_bytes(v, row_bytes - at - q % 8 * 16) : v);
+                            }
+                        }
+                    };
+#pragma unroll 1
+                    for (int q = th; q < 128 * ROW; q += 512)
+                        four(q, 128 * ROW, [&](int q) { return w_lo + (int64_t)min(w.out_tile * 128 + q / ROW, a.n_out - 1) * w_row + step * STEP + q % ROW * 16; }, w_lo, w_hi, bytes, 0,
+                             [&](int q, const uint4& v) { put_codes(to, q / ROW, q % ROW * 16, v); }, false);
+#pragma unroll 1
+                    for (int q = th; q < N * 8; q += 512)
+                        four(q, N * 8, [&](int q) { return a.x + (int64_t)min(w.row_tile * N + q / 8, a.n_rows - 1) * a.x_stride + step * 128 + q % 8 * 16; }, a.x, x_hi, (int)a.n_in, step * 128,
+                             [&](int q, const uint4& v) { st_shared4(to + T::A + box_place<128>(q / 8, q % 8 * 16), v.x, v.y, v.z, v.w); }, true);
+                    if (failed) break;
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                mbar_arrive(bar_of(bars.full[st]));
-                if constexpr (VEC) {
-                    if (i + AHEAD < items) load_w(i + AHEAD, v[k]);
-                }
+                arrive(bars.full[st.at]);
+#pragma unroll
+                for (int j = 0; j < T::SETS; j++) skip();
             }
-            if (failed) break;
         }
     }
     __syncwarp();
@@ -332,14 +489,13 @@ __global__ void __launch_bounds__((Tile<INT4, N, TMA>::THREADS), (Tile<INT4, N, 
         if (warp >= T::EPI || n_tiles == 0) cluster_wait();
         cluster_arrive(), cluster_wait();
         if constexpr (T::JOIN > 0) {
-            uint32_t row_tile, out_tile;
-            tile_at(0, row_tile, out_tile);
-            const uint32_t c128 = threadIdx.x, c = out_tile * 128 + c128, of = N / ranks;
+            const Walk w = first();
+            const uint32_t c128 = threadIdx.x & 127, c = w.out_tile * 128 + c128, of = N / ranks;
             if (warp < T::EPI && c < a.n_out) {
                 const float by = !INT4 && a.w_scale ? static_cast<const float*>(a.w_scale)[c] : 1.f;
                 by_type<INT4>(a.out_type, [&](auto type) {
-                    for (uint32_t j = 0; j < of; j++) {
-                        const uint32_t t = row_tile * N + rank * of + j;
+                    for (uint32_t j = threadIdx.x >> 7; j < of; j += T::EPI / 4) {
+                        const uint32_t t = w.row_tile * N + rank * of + j;
                         if (t >= a.n_rows) break;
                         uint32_t word = join[j * 128 + c128];
                         for (uint32_t r = 1; r < ranks; r++) {
@@ -361,21 +517,21 @@ __global__ void __launch_bounds__((Tile<INT4, N, TMA>::THREADS), (Tile<INT4, N, 
     }
 }
 
-// A map of rows of codes in boxes of `rows` rows by 128, or false where the layout has none: the unit wants 16-byte boundaries.
-static bool rows_map(CUtensorMap& map, const void* p, uint32_t codes, uint32_t n_rows, int64_t stride, uint32_t rows) {
+// A map of rows of `bytes` bytes in boxes of `rows` rows by `box` bytes, or false where the layout has none: the unit wants 16-byte boundaries.
+static bool rows_map(CUtensorMap& map, const void* p, uint32_t bytes, uint32_t n_rows, int64_t stride, uint32_t rows, uint32_t box) {
     const TensorMapEncode encode = tensor_map_encode();
-    if (n_rows == 1) stride = (codes + 15) / 16 * 16;
+    if (n_rows == 1) stride = (bytes + 15) / 16 * 16;
     if (!encode || !aligned_to(p, 16) || stride % 16 != 0 || stride >= (1ll << 40)) return false;
-    const cuuint64_t dims[2] = {codes, n_rows}, strides[1] = {(cuuint64_t)stride};
-    const cuuint32_t boxes[2] = {128, rows}, ones[2] = {1, 1};
-    return encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(p), dims, strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    const cuuint64_t dims[2] = {bytes, n_rows}, strides[1] = {(cuuint64_t)stride};
+    const cuuint32_t boxes[2] = {box, rows}, ones[2] = {1, 1};
+    return encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(p), dims, strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, box == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <bool INT4, int N, bool TMA, bool VEC>
+template <bool INT4, int N, bool TMA>
 static cudaError_t launch_variant(zkb_ctx* ctx, const zkb_step_product_args& a, const ProductMaps& maps) {
     using T = Tile<INT4, N, TMA>;
-    auto kernel = product_tiles_kernel<INT4, N, TMA, VEC>;
+    auto kernel = product_tiles_kernel<INT4, N, TMA>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM);
     if (e != cudaSuccess) return e;
@@ -402,13 +558,8 @@ static cudaError_t launch_variant(zkb_ctx* ctx, const zkb_step_product_args& a, 
 template <bool INT4, int N>
 static cudaError_t launch_rows_of(zkb_ctx* ctx, const zkb_step_product_args& a) {
     ProductMaps maps{};
-    const bool x = rows_map(maps.x, a.x, a.n_in, a.n_rows, a.x_stride, N);
-    if constexpr (INT4) {
-        const bool vec = aligned_to(a.w, 16) && (a.n_out == 1 || a.w_stride % 32 == 0);
-        return x && vec ? launch_variant<true, N, true, true>(ctx, a, maps) : launch_variant<true, N, false, false>(ctx, a, maps);
-    } else {
-        return x && rows_map(maps.w, a.w, a.n_in, a.n_out, a.w_stride, 128) ? launch_variant<false, N, true, true>(ctx, a, maps) : launch_variant<false, N, false, false>(ctx, a, maps);
-    }
+    const bool tma = rows_map(maps.x, a.x, a.n_in, a.n_rows, a.x_stride, N, 128) && (INT4 ? rows_map(maps.w, a.w, (a.n_in + 1) / 2, a.n_out, a.w_stride / 2, 128, 64) : rows_map(maps.w, a.w, a.n_in, a.n_out, a.w_stride, 128, 128));
+    return tma ? launch_variant<INT4, N, true>(ctx, a, maps) : launch_variant<INT4, N, false>(ctx, a, maps);
 }
 
 template <bool INT4>
