@@ -10,35 +10,36 @@ __device__ __forceinline__ void store_value(void* out, int64_t at, uint32_t type
     else static_cast<float*>(out)[at] = y;
 }
 
-// 16 bytes of codes wherever they start. `lo`, `hi`: the array's first byte and the one behind its last. Fetched as the whole 16-byte blocks of memory that they lie in (VEC: the one
-// block that they are), or other blocks of the array where those reach outside of it, so that several can be on their way; then turned into place, or, at the array's ends, read byte by byte.
-template <bool VEC>
+// The first n (of up to 16) bytes from p on, byte by byte, zeros behind them.
+__device__ __forceinline__ uint4 some_bytes(const int8_t* p, int n) {
+    uint32_t w[4] = {};
+#pragma unroll
+    for (int i = 0; i < 16; i++) w[i / 4] |= i < n ? (uint32_t)(uint8_t)p[i] << (8 * (i % 4)) : 0u;
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// 16 bytes of codes wherever they start. `lo`, `hi`: the array's first byte and the one behind its last. Fetched as the two whole 16-byte blocks of memory that they lie in, where the
+// array has those, so that several fetches can be on their way; then turned into place, or, at the array's ends, read byte by byte (bytes outside of it: zeros).
 struct Fetched {
     uint4 a, b;
 };
-template <bool VEC>
 __device__ __forceinline__ bool fetch_reaches_out(const int8_t* p, const int8_t* lo, const int8_t* hi) {
-    return VEC ? p + 16 > hi : p - 15 < lo || p + 31 > hi;
+    return p - 15 < lo || p + 31 > hi;
 }
-template <bool VEC>
-__device__ __forceinline__ Fetched<VEC> fetch16(const int8_t* p, const int8_t* lo, const int8_t* hi) {
-    Fetched<VEC> r{make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
-    if (!fetch_reaches_out<VEC>(p, lo, hi)) {
-        const uint4* q = reinterpret_cast<const uint4*>(VEC ? p : p - ((uint32_t)(uintptr_t)p & 15));
-        r.a = q[0];
-        if constexpr (!VEC) r.b = q[1];
+__device__ __forceinline__ Fetched fetch16(const int8_t* p, const int8_t* lo, const int8_t* hi) {
+    Fetched r{make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
+    if (!fetch_reaches_out(p, lo, hi)) {
+        const uint4* q = reinterpret_cast<const uint4*>(p - ((uint32_t)(uintptr_t)p & 15));
+        r.a = q[0], r.b = q[1];
     }
     return r;
 }
-template <bool VEC>
-__device__ __forceinline__ uint4 fetched16(const Fetched<VEC>& r, const int8_t* p, const int8_t* lo, const int8_t* hi) {
-    if (fetch_reaches_out<VEC>(p, lo, hi)) {
+__device__ __forceinline__ uint4 fetched16(const Fetched& r, const int8_t* p, const int8_t* lo, const int8_t* hi) {
+    if (fetch_reaches_out(p, lo, hi)) {
         uint32_t w[4] = {};
 #pragma unroll
         for (int i = 0; i < 16; i++) w[i / 4] |= p + i >= lo && p + i < hi ? (uint32_t)(uint8_t)p[i] << (8 * (i % 4)) : 0u;
         return make_uint4(w[0], w[1], w[2], w[3]);
     }
-    if constexpr (VEC) return r.a;
     const uint32_t m = (uint32_t)(uintptr_t)p & 15, v[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
     uint32_t two[6], one[5];
 #pragma unroll

@@ -449,20 +449,20 @@ __global__ void __launch_bounds__((Tile<INT4, N, TMA>::THREADS), (Tile<INT4, N, 
                     const int8_t *const w_lo = static_cast<const int8_t*>(a.w), *const w_hi = w_lo + (a.n_out - 1) * w_row + bytes, *const x_hi = a.x + (int64_t)(a.n_rows - 1) * a.x_stride + a.n_in;
                     // Four 16s at a time: their loads, and then, into a stage that is free, their codes. What lies behind a row's codes counts for nothing where x is zero there (`cut`).
                     auto four = [&](int q0, int n, auto from_of, const int8_t* lo, const int8_t* hi, int row_bytes, int at, auto to_place, bool cut) {
-                        Fetched<false> r[4];
+                        Fetched r[4];
                         const int8_t* p[4];
 #pragma unroll
                         for (int j = 0; j < 4; j++) {
                             const int q = q0 + j * 128;
                             p[j] = from_of(q);
-                            if (q < n) r[j] = fetch16<false>(p[j], lo, hi);
+                            if (q < n) r[j] = fetch16(p[j], lo, hi);
                         }
                         wait(bars.empty[st.at], st.parity ^ 1);
 #pragma unroll
                         for (int j = 0; j < 4; j++) {
                             const int q = q0 + j * 128;
                             if (q < n) {
-                                const uint4 v = fetched16<false>(r[j], p[j], lo, hi);
+                                const uint4 v = fetched16(r[j], p[j], lo, hi);
                                 to_place(q, cut ? first_bytes(v, row_bytes - at - q % 8 * 16) : v);
                             }
                         }
