@@ -22,10 +22,10 @@ struct ProductMaps {
 template <bool INT4, int N, bool TMA>
 struct Tile {
     static constexpr bool FILLED = INT4 || !TMA, RAW = INT4 && TMA;     // the weights' part of a stage is written by warps; from shared memory
-    static constexpr int EPI = INT4 ? (N <= 32 ? 4 : N / 8) : N >= 128 ? 8 : 4, SETS = RAW ? 1 : 2;  // warps that read the sums; sets of four warps that write codes, in turn
+    static constexpr int EPI = INT4 ? (N <= 32 ? 4 : N / 8) : N >= 128 ? 8 : 4, SETS = RAW ? 1 : 4;  // warps that read the sums; sets of four warps that write codes, in turn
     static constexpr int FIRST_FILLER = EPI + (INT4 ? 4 : 3), THREADS = 32 * (FILLED ? FIRST_FILLER + 4 * SETS : EPI + 2);
     static constexpr int A = 128 * 128, B = N * 128, STAGE = RAW ? A : A + B, RAW_BYTES = 128 * 64;
-    static constexpr int BLOCKS = N <= 32 || (N == 64 && !FILLED) ? 2 : 1;  // thread blocks an SM
+    static constexpr int BLOCKS = (N <= 32 && (TMA || !FILLED)) || (N == 64 && !FILLED) ? 2 : 1;  // thread blocks an SM
     static constexpr int JOIN = N <= 64 ? N * 512 : 0;                  // a cluster's sums
     static constexpr int RAWS = !RAW ? 0 : N <= 32 ? 4 : N == 64 ? 8 : 6, XS = !RAW ? 0 : N <= 32 ? 8 * 16 / N : 4;
     static constexpr int SCALES = INT4 ? 4 : 0, SCALE_BYTES = 128 * 16; // eight groups' scales of a tile's outputs
@@ -58,10 +58,14 @@ struct TileBars {
 
 
 template <int TYPE, bool INT4>
-__device__ __forceinline__ void put(const zkb_step_product_args& a, uint32_t t, uint32_t c, uint32_t word, float by) {
+__device__ __forceinline__ void put(const zkb_step_product_args& a, uint32_t t, uint32_t c, uint32_t word, float by, float x_scale) {
     const int64_t at = (int64_t)t * a.out_stride + c;
     if constexpr (TYPE == ZKB_VALUE_INT32) static_cast<uint32_t*>(a.out)[at] = word;
-    else store_value(a.out, at, TYPE, INT4 ? __uint_as_float(word) * a.x_scale[t] : (float)(int)word * (a.x_scale[t] * by));
+    else store_value(a.out, at, TYPE, INT4 ? __uint_as_float(word) * x_scale : (float)(int)word * (x_scale * by));
+}
+template <int TYPE, bool INT4>
+__device__ __forceinline__ void put(const zkb_step_product_args& a, uint32_t t, uint32_t c, uint32_t word, float by) {
+    put<TYPE, INT4>(a, t, c, word, by, TYPE == ZKB_VALUE_INT32 ? 0.f : a.x_scale[t]);
 }
 // f(type as a constant)
 template <bool INT4, class F>
@@ -88,9 +92,11 @@ __global__ void __launch_bounds__((Tile<INT4, N, TMA>::THREADS), (Tile<INT4, N, 
     extern __shared__ unsigned char tiles_sm[];
     __shared__ __align__(8) TileBars bars;
     __shared__ uint32_t tmem_sm;
+    __shared__ float x_scale_sm[T::JOIN > 0 ? N : 1];
     unsigned char* const sm = tiles_sm + (-(uint32_t)__cvta_generic_to_shared(tiles_sm) & 1023);
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(sm), raw_ring = ring + T::STAGES * T::STAGE, x_ring = raw_ring + T::RAWS * T::RAW_BYTES, scale_ring = x_ring + T::XS * T::B;
-    uint32_t* const join = reinterpret_cast<uint32_t*>(sm + T::STAGES * T::STAGE + T::RAWS * T::RAW_BYTES + T::XS * T::B + T::SCALES * T::SCALE_BYTES);
+    const uint32_t join_at = scale_ring + T::SCALES * T::SCALE_BYTES;
+    uint32_t* const join = reinterpret_cast<uint32_t*>(sm + (join_at - ring));
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint32_t rank = cluster_rank(), ranks = cluster_ranks();
     if (warp == T::EPI + 1) {
@@ -113,6 +119,16 @@ __global__ void __launch_bounds__((Tile<INT4, N, TMA>::THREADS), (Tile<INT4, N, 
         __syncwarp();
         if (lane == 0) mbar_arrive(bar_of(b));
     };
+    if constexpr (TMA) {
+        if (warp == T::EPI && lane < 2) asm volatile("prefetch.tensormap [%0];" ::"l"(lane ? &maps.w : &maps.x) : "memory");
+    }
+    // What the last factors are is known now; a cluster has one tile.
+    float out_scale = 1.f;
+    if (T::JOIN > 0 && ranks > 1 && warp < T::EPI) {
+        const uint32_t tile = blockIdx.x / ranks, of = N / ranks, c = tile / row_tiles * 128 + (threadIdx.x & 127), t = tile % row_tiles * N + rank * of + threadIdx.x;
+        if (!INT4 && a.w_scale && c < a.n_out) out_scale = static_cast<const float*>(a.w_scale)[c];
+        if (threadIdx.x < of) x_scale_sm[threadIdx.x] = a.x_scale && t < a.n_rows ? a.x_scale[t] : 0.f;
+    }
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
@@ -165,9 +181,22 @@ __global__ void __launch_bounds__((Tile<INT4, N, TMA>::THREADS), (Tile<INT4, N, 
                 wait(bars.sum_full[sums.at], sums.parity);
                 tmem_fence_after();
             };
-            auto share = [&](int j, uint32_t word) {  // to the thread block that adds up this row
-                const uint32_t of = N / ranks, column = half + j, to = column / of;
-                peer_store_word(join + (rank * of + column % of) * 128 + c128, (int)to, word);
+            // The sums of columns j .. j + COUNT - 1 to the thread blocks that add up those rows, side by side there.
+            auto share = [&](int j, const uint32_t(&x)[CHUNK]) {
+                const uint32_t log_of = 31 - __clz(N / ranks);
+                if (log_of >= 2) {
+#pragma unroll
+                    for (int y = 0; y < CHUNK; y += 4) {
+                        const uint32_t column = half + j + y;
+                        peer_store4(join_at + (((rank * 128 + c128) << log_of) + (column & ((1u << log_of) - 1))) * 4, (int)(column >> log_of), x[y], x[y + 1], x[y + 2], x[y + 3]);
+                    }
+                } else {
+#pragma unroll
+                    for (int y = 0; y < CHUNK; y++) {
+                        const uint32_t column = half + j + y;
+                        peer_store_word(join + (((rank * 128 + c128) << log_of) + (column & ((1u << log_of) - 1))), (int)(column >> log_of), x[y]);
+                    }
+                }
             };
             if constexpr (INT4) {
                 uint64_t acc[MINE / 2];
@@ -244,7 +273,12 @@ __global__ void __launch_bounds__((Tile<INT4, N, TMA>::THREADS), (Tile<INT4, N, 
                 } else if constexpr (T::JOIN > 0) {
                     cluster_wait();
 #pragma unroll
-                    for (int j = 0; j < MINE; j++) share(j, (uint32_t)(acc[j / 2] >> (32 * (j % 2))));
+                    for (int j = 0; j < MINE; j += CHUNK) {
+                        uint32_t x[CHUNK];
+#pragma unroll
+                        for (int y = 0; y < CHUNK; y++) x[y] = (uint32_t)(acc[(j + y) / 2] >> (32 * (y % 2)));
+                        share(j, x);
+                    }
                 }
             } else {
                 const float by = live && a.w_scale ? static_cast<const float*>(a.w_scale)[c] : 1.f;
@@ -262,10 +296,7 @@ __global__ void __launch_bounds__((Tile<INT4, N, TMA>::THREADS), (Tile<INT4, N, 
                             });
                     });
                 } else if constexpr (T::JOIN > 0) {
-                    read(at_lanes + sums.at * T::SUM, true, [&](int j, const uint32_t(&x)[CHUNK]) {
-#pragma unroll
-                        for (int y = 0; y < CHUNK; y++) share(j + y, x[y]);
-                    });
+                    read(at_lanes + sums.at * T::SUM, true, share);
                 }
                 sums.next();
             }
@@ -490,19 +521,18 @@ __global__ void __launch_bounds__((Tile<INT4, N, TMA>::THREADS), (Tile<INT4, N, 
         cluster_arrive(), cluster_wait();
         if constexpr (T::JOIN > 0) {
             const Walk w = first();
-            const uint32_t c128 = threadIdx.x & 127, c = w.out_tile * 128 + c128, of = N / ranks;
+            const uint32_t c128 = threadIdx.x & 127, c = w.out_tile * 128 + c128, of = N / ranks, first_row = w.row_tile * N + rank * of;
             if (warp < T::EPI && c < a.n_out) {
-                const float by = !INT4 && a.w_scale ? static_cast<const float*>(a.w_scale)[c] : 1.f;
                 by_type<INT4>(a.out_type, [&](auto type) {
+#pragma unroll 4
                     for (uint32_t j = threadIdx.x >> 7; j < of; j += T::EPI / 4) {
-                        const uint32_t t = w.row_tile * N + rank * of + j;
-                        if (t >= a.n_rows) break;
-                        uint32_t word = join[j * 128 + c128];
+                        if (first_row + j >= a.n_rows) break;
+                        uint32_t word = join[c128 * of + j];
                         for (uint32_t r = 1; r < ranks; r++) {
-                            const uint32_t more = join[(r * of + j) * 128 + c128];
+                            const uint32_t more = join[(r * 128 + c128) * of + j];
                             word = INT4 ? __float_as_uint(__uint_as_float(word) + __uint_as_float(more)) : word + more;
                         }
-                        put<decltype(type)::value, INT4>(a, t, c, word, by);
+                        put<decltype(type)::value, INT4>(a, first_row + j, c, word, out_scale, x_scale_sm[j]);
                     }
                 });
             }
