@@ -22,18 +22,20 @@ struct ProductMaps {
 template <bool INT4, int N, bool TMA>
 struct Tile {
     static constexpr bool FILLED = INT4 || !TMA, RAW = INT4 && TMA;     // the weights' part of a stage is written by warps; from shared memory
-    static constexpr int EPI = INT4 ? (N <= 32 ? 4 : N / 8) : N >= 128 ? 8 : 4, SETS = RAW ? 1 : 4;  // warps that read the sums; sets of four warps that write codes, in turn
+    static constexpr int EPI = INT4 ? (N <= 32 ? 4 : N / 8) : N >= 128 ? 8 : 4, SETS = RAW ? (N == 128 ? 1 : 2) : 4;  // warps that read the sums; sets of four warps that write codes, in turn
     static constexpr int FIRST_FILLER = EPI + (INT4 ? 4 : 3), THREADS = 32 * (FILLED ? FIRST_FILLER + 4 * SETS : EPI + 2);
-    static constexpr int A = 128 * 128, B = N * 128, STAGE = RAW ? A : A + B, RAW_BYTES = 128 * 64;
-    static constexpr int BLOCKS = (N <= 32 && (TMA || !FILLED)) || (N == 64 && !FILLED) ? 2 : 1;  // thread blocks an SM
+    // A step's codes, in halves of 128 that are a matrix each: what a step costs whatever its codes, waits above all, is some 600 cycles of each of the warps that it goes through.
+    static constexpr int CODES = INT4 ? 256 : 128, HALVES = CODES / 128, A_HALF = 128 * 128, B_HALF = N * 128;
+    static constexpr int A = HALVES * A_HALF, B = HALVES * B_HALF, STAGE = RAW ? A : A + B, RAW_BYTES = 128 * CODES / 2;
+    static constexpr int BLOCKS = N <= 64 && !FILLED ? 2 : 1;           // thread blocks an SM
     static constexpr int JOIN = N <= 64 ? N * 512 : 0;                  // a cluster's sums
-    static constexpr int RAWS = !RAW ? 0 : N <= 32 ? 4 : N == 64 ? 8 : 6, XS = !RAW ? 0 : N <= 32 ? 8 * 16 / N : 4;
+    static constexpr int RAWS = !RAW ? 0 : N <= 32 ? 4 : 3, XS = !RAW ? 0 : N == 16 ? 4 : N == 32 ? 3 : 2;
     static constexpr int SCALES = INT4 ? 4 : 0, SCALE_BYTES = 128 * 16; // eight groups' scales of a tile's outputs
     static constexpr int ROOM = (BLOCKS == 2 ? 112 * 1024 : 216 * 1024) - JOIN - RAWS * RAW_BYTES - XS * B - SCALES * SCALE_BYTES;
     static constexpr int STAGES = ROOM / STAGE < 6 ? ROOM / STAGE : 6;
     // The sums of a tile of 8-bit weights, or of 4-bit weights' groups: of a step's all at once where they have room twice.
-    static constexpr bool BY_STEP = INT4 && N <= 64;
-    static constexpr int SUMS = !INT4 ? 2 : N == 16 || N == 128 ? 4 : 2, SUM = BY_STEP ? 4 * N : N, COLUMNS = SUMS * SUM < 32 ? 32 : SUMS * SUM;
+    static constexpr bool BY_STEP = INT4 && N <= 32;
+    static constexpr int SUMS = !INT4 || BY_STEP ? 2 : 4, SUM = BY_STEP ? 8 * N : N, COLUMNS = SUMS * SUM < 32 ? 32 : SUMS * SUM;
     // A thread block never waits for tensor memory: those that fit an SM's shared memory together (this kernel's variants and attention's, which take all columns and 121 KB) fit its
     // 512 columns. Clusters that each hold what another waits for would wait forever.
     static constexpr int LEAST = BLOCKS == 2 ? 108 * 1024 : 121 * 1024;
@@ -53,7 +55,7 @@ __device__ __forceinline__ void tma_load_2d(uint32_t to, const CUtensorMap* map,
 }
 
 struct TileBars {
-    unsigned long long full[6], empty[6], x_full[8], x_empty[8], raw_full[8], raw_empty[8], scale_full[4], scale_empty[4], sum_full[4], sum_empty[4], last;
+    unsigned long long full[6], empty[6], done[32], x_full[8], raw_full[8], raw_empty[8], scale_full[4], scale_empty[4], sum_full[4], sum_empty[4], last;
 };
 
 
@@ -104,7 +106,8 @@ __global__ void __launch_bounds__((Tile<INT4, N, TMA>::THREADS), (Tile<INT4, N, 
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     } else if (warp == 0 && lane == 0) {
         for (int i = 0; i < 6; i++) mbar_init(bar_of(bars.full[i]), (TMA && !T::RAW ? 1 : 0) + (T::FILLED ? 4 : 0)), mbar_init(bar_of(bars.empty[i]), 1);
-        for (int i = 0; i < 8; i++) mbar_init(bar_of(bars.raw_full[i]), 1), mbar_init(bar_of(bars.raw_empty[i]), 4), mbar_init(bar_of(bars.x_full[i]), 1), mbar_init(bar_of(bars.x_empty[i]), 1);
+        for (int i = 0; i < 8; i++) mbar_init(bar_of(bars.raw_full[i]), 1), mbar_init(bar_of(bars.raw_empty[i]), 4), mbar_init(bar_of(bars.x_full[i]), 1);
+        for (int i = 0; i < 32; i++) mbar_init(bar_of(bars.done[i]), 1);
         for (int i = 0; i < 4; i++) mbar_init(bar_of(bars.sum_full[i]), 1), mbar_init(bar_of(bars.sum_empty[i]), T::EPI), mbar_init(bar_of(bars.scale_full[i]), 1), mbar_init(bar_of(bars.scale_empty[i]), T::EPI);
         mbar_init(bar_of(bars.last), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -134,7 +137,7 @@ __global__ void __launch_bounds__((Tile<INT4, N, TMA>::THREADS), (Tile<INT4, N, 
     tmem_fence_after();
     if (ranks > 1) cluster_arrive();
     const uint32_t tmem = tmem_sm;
-    const uint32_t all_steps = (a.n_in + 127) / 128, who = blockIdx.x / ranks, every = gridDim.x / ranks;
+    const uint32_t all_steps = (a.n_in + T::CODES - 1) / T::CODES, who = blockIdx.x / ranks, every = gridDim.x / ranks;
     const uint32_t first_step = rank * all_steps / ranks, steps = (rank + 1) * all_steps / ranks - first_step;
     const uint32_t n_tiles = who < all_tiles ? (all_tiles - who + every - 1) / every : 0, items = n_tiles * steps;
     // The steps of all of this thread block's tiles, one after the other.
@@ -150,14 +153,19 @@ __global__ void __launch_bounds__((Tile<INT4, N, TMA>::THREADS), (Tile<INT4, N, 
     auto next = [&](Walk& w) {
         if (++w.step == steps) w.step = 0, w.tile += every, enter(w);
     };
-    const uint32_t log_group = INT4 ? 31 - __clz(a.group) : 7, per_step = 128 >> log_group, groups = (a.n_in + (1u << log_group) - 1) >> log_group;
+    const uint32_t log_group = INT4 ? 31 - __clz(a.group) : 7, per_step = T::CODES >> log_group, groups = (a.n_in + (1u << log_group) - 1) >> log_group;
     auto groups_in = [&](uint32_t step) { return min(per_step, groups - (first_step + step) * per_step); };
+    // What the products announce. Of 4-bit weights, each read that ends, a step's or a group's: the sums are there then, and with a step's last one its codes and x are done with. There are more
+    // barriers than reads under way, so none is gone past before all have seen it. Of 8-bit weights: a step's end, and a tile's sums.
+    auto ends_in = [&](uint32_t step) { return !INT4 ? 0u : T::BY_STEP ? 1u : groups_in(step); };
+    auto wait_end = [&](uint32_t n) { wait(bars.done[n % 32], n / 32); };  // of read n
 
     if (warp < T::EPI) {  // ---- the sums: a thread has an output, and half of the rows where two threads share it
         constexpr int MINE = N / (T::EPI / 4), CHUNK = MINE < 32 ? 16 : 32;
         const uint32_t c128 = (uint32_t)(warp & 3) * 32 + lane, half = (uint32_t)(warp >> 2) * MINE, at_lanes = tmem + ((uint32_t)(warp & 3) << 21) + half;
         Ring<T::SUMS> sums;
         Ring<(T::SCALES > 0 ? T::SCALES : 1)> scale;
+        uint32_t read_ends = 0;
         Walk w = first();
         for (uint32_t i = 0; i < n_tiles; i++, w.tile += every, enter(w)) {
             const uint32_t c = w.out_tile * 128 + c128, t0 = w.row_tile * N + half;
@@ -178,7 +186,8 @@ __global__ void __launch_bounds__((Tile<INT4, N, TMA>::THREADS), (Tile<INT4, N, 
                 }
             };
             auto arrived = [&] {
-                wait(bars.sum_full[sums.at], sums.parity);
+                if constexpr (INT4) wait_end(read_ends++);
+                else wait(bars.sum_full[sums.at], sums.parity);
                 tmem_fence_after();
             };
             // The sums of columns j .. j + COUNT - 1 to the thread blocks that add up those rows, side by side there.
@@ -304,19 +313,24 @@ __global__ void __launch_bounds__((Tile<INT4, N, TMA>::THREADS), (Tile<INT4, N, 
     } else if (warp == T::EPI) {  // ---- copies
         if constexpr (TMA) {  // x and 8-bit weights into the stages, or x into its own ring
             constexpr int SIZE = T::RAW ? T::XS : T::STAGES;
-            auto& full = T::RAW ? bars.x_full : reinterpret_cast<unsigned long long(&)[8]>(bars.full);
-            auto& empty = T::RAW ? bars.x_empty : reinterpret_cast<unsigned long long(&)[8]>(bars.empty);
+            const unsigned long long* const full = T::RAW ? bars.x_full : bars.full;
             uint32_t sent = 0;
             Ring<SIZE> st;
-            Walk w = first();
+            Walk w = first(), old = first();  // `old`: the step whose place is taken
+            uint32_t ends = 0;
             for (; sent < items; sent++, st.next(), next(w)) {
-                wait(empty[st.at], st.parity ^ 1);
+                if constexpr (T::RAW) {
+                    if (sent >= SIZE) ends += ends_in(old.step), next(old), wait_end(ends - 1);
+                } else {
+                    wait(bars.empty[st.at], st.parity ^ 1);
+                }
                 if (failed) break;
                 if (lane == 0) {
                     const uint32_t to = T::RAW ? x_ring + st.at * T::B : ring + st.at * T::STAGE + T::A, bar = bar_of(full[st.at]);
                     mbar_expect(bar, T::RAW ? T::B : T::STAGE);
                     if constexpr (!INT4) tma_load_2d(to - T::A, &maps.w, (first_step + w.step) * 128, w.out_tile * 128, bar);
-                    tma_load_2d(to, &maps.x, (first_step + w.step) * 128, w.row_tile * N, bar);
+#pragma unroll
+                    for (int h = 0; h < T::HALVES; h++) tma_load_2d(to + h * T::B_HALF, &maps.x, (first_step + w.step) * T::CODES + h * 128, w.row_tile * N, bar);
                 }
                 __syncwarp();
             }
@@ -331,7 +345,7 @@ __global__ void __launch_bounds__((Tile<INT4, N, TMA>::THREADS), (Tile<INT4, N, 
         Ring<(T::XS > 0 ? T::XS : 1)> xs;
         Ring<T::SUMS> sums;
         const uint32_t parts = (1u << log_group) / 32;
-        uint32_t step = 0;
+        uint32_t step = 0, ends = 0;
 #pragma unroll 1
         for (uint32_t i = 0; i < items; i++, st.next()) {
             const uint32_t from_a = a_low + st.at * (T::STAGE >> 4), from_b = T::RAW ? x_low + xs.at * (T::B >> 4) : from_a + (T::A >> 4);
@@ -350,18 +364,14 @@ __global__ void __launch_bounds__((Tile<INT4, N, TMA>::THREADS), (Tile<INT4, N, 
                         if (failed) break;
                         tmem_fence_after();
                     }
-                    for (uint32_t k = 0; k < parts; k++) {
-                        const uint32_t at = 2 * (g * parts + k);
-                        product_codes(one, tmem_u + sums.at * T::SUM + (T::BY_STEP ? g * N : 0), two_words(from_a + at, high), two_words(from_b + at, high), desc, k > 0);
-                    }
+                    const uint32_t half = g << log_group >> 7, from = 2 * (g * parts & 3), group_a = from_a + half * (T::A_HALF >> 4) + from, group_b = from_b + half * (T::B_HALF >> 4) + from;
+                    for (uint32_t k = 0; k < parts; k++)
+                        product_codes(one, tmem_u + sums.at * T::SUM + (T::BY_STEP ? g * N : 0), two_words(group_a + 2 * k, high), two_words(group_b + 2 * k, high), desc, k > 0);
                     if (!T::BY_STEP || g + 1 == n) {
-                        if (one) products_done(bar_of(bars.sum_full[sums.at]));
+                        if (one) products_done(bar_of(bars.done[ends % 32]));
+                        ends++;
                         sums.next();
                     }
-                }
-                if (one) {
-                    products_done(bar_of(bars.empty[st.at]));
-                    if constexpr (T::RAW) products_done(bar_of(bars.x_empty[xs.at]));
                 }
                 if constexpr (T::RAW) xs.next();
             } else {
@@ -392,7 +402,7 @@ __global__ void __launch_bounds__((Tile<INT4, N, TMA>::THREADS), (Tile<INT4, N, 
                     if (failed) break;
                     if (lane == 0) {
                         mbar_expect(bar_of(bars.raw_full[rs.at]), T::RAW_BYTES);
-                        tma_load_2d(raw_ring + rs.at * T::RAW_BYTES, &maps.w, (first_step + w.step) * 64, w.out_tile * 128, bar_of(bars.raw_full[rs.at]));
+                        tma_load_2d(raw_ring + rs.at * T::RAW_BYTES, &maps.w, (first_step + w.step) * (T::CODES / 2), w.out_tile * 128, bar_of(bars.raw_full[rs.at]));
                     }
                     __syncwarp();
                 }
@@ -438,7 +448,7 @@ __global__ void __launch_bounds__((Tile<INT4, N, TMA>::THREADS), (Tile<INT4, N, 
             const int f = threadIdx.x - 32 * T::FIRST_FILLER, th = f & 127, set = f >> 7;
             const int64_t w_row = INT4 ? a.w_stride / 2 : a.w_stride;
             const int bytes = INT4 ? (int)(a.n_in + 1) / 2 : (int)a.n_in;
-            constexpr int STEP = INT4 ? 64 : 128, ROW = STEP / 16, MINE = ROW;  // bytes of a row's step, 16s of them, a thread's
+            constexpr int STEP = 128, ROW = STEP / 16, MINE = ROW;  // bytes of a row's step, 16s of them, a thread's
             auto put_codes = [&](uint32_t to, int row, int b, const uint4& v) {  // 16 bytes from byte b of a row's step on
                 if constexpr (INT4) {
                     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -448,16 +458,26 @@ __global__ void __launch_bounds__((Tile<INT4, N, TMA>::THREADS), (Tile<INT4, N, 
                         const uint32_t even = w[y] << 4 & 0xf0f0f0f0u, odd = w[y] & 0xf0f0f0f0u;
                         u[2 * y] = __byte_perm(even, odd, 0x5140), u[2 * y + 1] = __byte_perm(even, odd, 0x7362);
                     }
-                    st_shared4(to + box_place<128>(row, 2 * b), u[0], u[1], u[2], u[3]);
-                    st_shared4(to + box_place<128>(row, 2 * b + 16), u[4], u[5], u[6], u[7]);
+                    // (the second half's first: the lanes of a row write to different banks)
+                    const bool second = b >= 64;
+                    const uint32_t place = to + (second ? T::A_HALF : 0), at = 2 * b & 127, x = second ? 16 : 0;
+                    st_shared4(place + box_place<128>(row, at + x), second ? u[4] : u[0], second ? u[5] : u[1], second ? u[6] : u[2], second ? u[7] : u[3]);
+                    st_shared4(place + box_place<128>(row, at + 16 - x), second ? u[0] : u[4], second ? u[1] : u[5], second ? u[2] : u[6], second ? u[3] : u[7]);
                 } else {
                     st_shared4(to + box_place<128>(row, b), v.x, v.y, v.z, v.w);
                 }
             };
             Ring<T::STAGES> st;
             Ring<(T::RAWS > 0 ? T::RAWS : 1)> rs;
-            Walk w = first();
+            Walk w = first(), old = first();
+            uint32_t ends = 0, passed = 0;  // reads that have ended with the step that was in this stage before, steps so far
+            auto stage_free = [&] {
+                if constexpr (!INT4) wait(bars.empty[st.at], st.parity ^ 1);
+                else if (passed >= T::STAGES) wait_end(ends + ends_in(old.step) - 1);
+            };
             auto skip = [&] {
+                if (INT4 && passed >= T::STAGES) ends += ends_in(old.step), next(old);
+                passed++;
                 st.next(), next(w);
                 if constexpr (T::RAW) rs.next();
             };
@@ -467,13 +487,16 @@ __global__ void __launch_bounds__((Tile<INT4, N, TMA>::THREADS), (Tile<INT4, N, 
                 const uint32_t to = ring + st.at * T::STAGE;
                 if constexpr (T::RAW) {
                     wait(bars.raw_full[rs.at], rs.parity);
-                    uint4 v[MINE];
-#pragma unroll
-                    for (int j = 0; j < MINE; j++) ld_shared4(raw_ring + rs.at * T::RAW_BYTES + (th + j * 128) * 16, v[j].x, v[j].y, v[j].z, v[j].w);
-                    wait(bars.empty[st.at], st.parity ^ 1);
+                    stage_free();
                     if (failed) break;
 #pragma unroll
-                    for (int j = 0; j < MINE; j++) put_codes(to, (th + j * 128) / ROW, (th + j * 128) % ROW * 16, v[j]);
+                    for (int j0 = 0; j0 < MINE; j0 += 4) {
+                        uint4 v[4];
+#pragma unroll
+                        for (int j = 0; j < 4; j++) ld_shared4(raw_ring + rs.at * T::RAW_BYTES + (th + (j0 + j) * 128) * 16, v[j].x, v[j].y, v[j].z, v[j].w);
+#pragma unroll
+                        for (int j = 0; j < 4; j++) put_codes(to, (th + (j0 + j) * 128) / ROW, (th + (j0 + j) * 128) % ROW * 16, v[j]);
+                    }
                     arrive(bars.raw_empty[rs.at]);
                 } else {
                     const int step = (int)(first_step + w.step);
@@ -488,7 +511,7 @@ __global__ void __launch_bounds__((Tile<INT4, N, TMA>::THREADS), (Tile<INT4, N, 
                             p[j] = from_of(q);
                             if (q < n) r[j] = fetch16(p[j], lo, hi);
                         }
-                        wait(bars.empty[st.at], st.parity ^ 1);
+                        stage_free();
 #pragma unroll
                         for (int j = 0; j < 4; j++) {
                             const int q = q0 + j * 128;
@@ -503,9 +526,11 @@ __global__ void __launch_bounds__((Tile<INT4, N, TMA>::THREADS), (Tile<INT4, N, 
                         four(q, 128 * ROW, [&](int q) { return w_lo + (int64_t)min(w.out_tile * 128 + q / ROW, a.n_out - 1) * w_row + step * STEP + q % ROW * 16; }, w_lo, w_hi, bytes, 0,
                              [&](int q, const uint4& v) { put_codes(to, q / ROW, q % ROW * 16, v); }, false);
 #pragma unroll 1
-                    for (int q = th; q < N * 8; q += 512)
-                        four(q, N * 8, [&](int q) { return a.x + (int64_t)min(w.row_tile * N + q / 8, a.n_rows - 1) * a.x_stride + step * 128 + q % 8 * 16; }, a.x, x_hi, (int)a.n_in, step * 128,
-                             [&](int q, const uint4& v) { st_shared4(to + T::A + box_place<128>(q / 8, q % 8 * 16), v.x, v.y, v.z, v.w); }, true);
+                    for (int h = 0; h < T::HALVES; h++)
+#pragma unroll 1
+                        for (int q = th; q < N * 8; q += 512)
+                            four(q, N * 8, [&](int q) { return a.x + (int64_t)min(w.row_tile * N + q / 8, a.n_rows - 1) * a.x_stride + step * T::CODES + h * 128 + q % 8 * 16; }, a.x, x_hi, (int)a.n_in,
+                                 step * T::CODES + h * 128, [&](int q, const uint4& v) { st_shared4(to + T::A + h * T::B_HALF + box_place<128>(q / 8, q % 8 * 16), v.x, v.y, v.z, v.w); }, true);
                     if (failed) break;
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -548,13 +573,13 @@ __global__ void __launch_bounds__((Tile<INT4, N, TMA>::THREADS), (Tile<INT4, N, 
 }
 
 // A map of rows of `bytes` bytes in boxes of `rows` rows by `box` bytes, or false where the layout has none: the unit wants 16-byte boundaries.
-static bool rows_map(CUtensorMap& map, const void* p, uint32_t bytes, uint32_t n_rows, int64_t stride, uint32_t rows, uint32_t box) {
+static bool rows_map(CUtensorMap& map, const void* p, uint32_t bytes, uint32_t n_rows, int64_t stride, uint32_t rows, uint32_t box, bool swizzled) {
     const TensorMapEncode encode = tensor_map_encode();
     if (n_rows == 1) stride = (bytes + 15) / 16 * 16;
     if (!encode || !aligned_to(p, 16) || stride % 16 != 0 || stride >= (1ll << 40)) return false;
     const cuuint64_t dims[2] = {bytes, n_rows}, strides[1] = {(cuuint64_t)stride};
     const cuuint32_t boxes[2] = {box, rows}, ones[2] = {1, 1};
-    return encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(p), dims, strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, box == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+    return encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(p), dims, strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzled ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -565,11 +590,11 @@ static cudaError_t launch_variant(zkb_ctx* ctx, const zkb_step_product_args& a, 
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM);
     if (e != cudaSuccess) return e;
-    const uint32_t row_tiles = (a.n_rows + N - 1) / N, tiles = row_tiles * ((a.n_out + 127) / 128), steps = (a.n_in + 127) / 128;
+    const uint32_t row_tiles = (a.n_rows + N - 1) / N, tiles = row_tiles * ((a.n_out + 127) / 128), steps = (a.n_in + T::CODES - 1) / T::CODES;
     // Few tiles are spread over clusters, while all of them are on the GPU at once and each thread block has two steps.
     uint32_t ranks = 1;
     if (T::JOIN > 0)
-        while (ranks < 16 && ranks < N && tiles <= T::BLOCKS * clusters_at_once(2 * ranks) && steps >= 4 * ranks) ranks *= 2;
+        while (ranks < 16 && ranks < N && tiles <= T::BLOCKS * clusters_at_once(2 * ranks) && steps >= (INT4 ? 2 : 4) * ranks) ranks *= 2;
     return launch_clusters(ranks, [&](uint32_t n) {
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -588,7 +613,7 @@ static cudaError_t launch_variant(zkb_ctx* ctx, const zkb_step_product_args& a, 
 template <bool INT4, int N>
 static cudaError_t launch_rows_of(zkb_ctx* ctx, const zkb_step_product_args& a) {
     ProductMaps maps{};
-    const bool tma = rows_map(maps.x, a.x, a.n_in, a.n_rows, a.x_stride, N, 128) && (INT4 ? rows_map(maps.w, a.w, (a.n_in + 1) / 2, a.n_out, a.w_stride / 2, 128, 64) : rows_map(maps.w, a.w, a.n_in, a.n_out, a.w_stride, 128, 128));
+    const bool tma = rows_map(maps.x, a.x, a.n_in, a.n_rows, a.x_stride, N, 128, true) && (INT4 ? rows_map(maps.w, a.w, (a.n_in + 1) / 2, a.n_out, a.w_stride / 2, 128, 128, false) : rows_map(maps.w, a.w, a.n_in, a.n_out, a.w_stride, 128, 128, true));
     return tma ? launch_variant<INT4, N, true>(ctx, a, maps) : launch_variant<INT4, N, false>(ctx, a, maps);
 }
 
