@@ -67,101 +67,69 @@ __device__ __forceinline__ uint32_t copy_row(uint32_t to, const char* row, uint3
     return size;
 }
 
-// TYPE: ZKB_VALUE_*; N: 16-byte vectors a thread. STAGED: a thread block has row after row, and the next one comes to shared memory while this one is summed.
-template <int TYPE, int N, bool STAGED>
-__global__ void __launch_bounds__(512, 2) logprobs_kernel(const __grid_constant__ LogprobArgs p, unsigned* dev_err) {
-    extern __shared__ __align__(16) unsigned char row_sm[];
-    __shared__ __align__(8) unsigned long long row_bar;
-    constexpr int PER = TYPE == ZKB_VALUE_BF16 ? 8 : 4, SIZE = 16 / PER;
-    __shared__ LpPart parts[LP_PARTS];
-    __shared__ uint64_t list[LP_LIST];
-    __shared__ __align__(16) uint32_t groups[64];
-    __shared__ float sums[3][16];
-    __shared__ uint32_t n_list;
-    __shared__ uint64_t best[16];
-    const zkb_step_logprobs_args& a = p.a;
-    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, rank = cluster_rank(), ranks = cluster_ranks(), n_top = a.n_top;
-    const uint32_t begin = min(rank * p.piece, a.vocab), end = min(begin + p.piece, a.vocab), n_parts = (p.piece + p.part - 1) / p.part;
-    const bool alone = ranks == 1 && n_parts == 1;
-    if (threadIdx.x == 0) n_list = 0;
-    if (threadIdx.x < 64 && threadIdx.x >= warps * (32 / p.lanes)) groups[threadIdx.x] = 0;
-    if (ranks > 1) cluster_arrive();
-    const uint32_t stage = (uint32_t)__cvta_generic_to_shared(row_sm);
-    bool failed = false;
-    uint32_t turn = 0;
-    if constexpr (STAGED) {
-        if (threadIdx.x == 0) {
-            mbar_init(bar_of(row_bar), 1);
-            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            copy_row(stage, static_cast<const char*>(a.logits) + (int64_t)blockIdx.x * a.logits_stride * SIZE, a.vocab * SIZE, bar_of(row_bar));
-        }
-        __syncthreads();
-    }
-    for (uint32_t t = blockIdx.x / ranks; t < a.n_rows; t += gridDim.x / ranks) {  // (one row only where a cluster has it)
-    const char* const row = static_cast<const char*>(a.logits) + (int64_t)t * a.logits_stride * SIZE;
-    // what is asked of the row is on its way meanwhile
-    const int32_t id_first = threadIdx.x < a.n_given && (!alone || warp == 0) ? a.ids[(int64_t)t * a.n_given + threadIdx.x] : -1;
-    const float given_first = id_first >= 0 && (uint32_t)id_first < a.vocab ? logit_at<TYPE>(row, (uint32_t)id_first) : 0.f;
-    for (uint32_t q = 0; q < n_parts; q++) {
-        const uint32_t from = min(begin + q * p.part, end), to = min(from + p.part, end);
-        // Vectors lie on 16-byte boundaries: the first one may reach before `from`, and values outside the part are -infinity.
-        const char* const base = row + (int64_t)from * SIZE;
-        const uint32_t ahead = (uint32_t)((uintptr_t)base & 15) / SIZE;
-        auto place = [&](int i, int y) { return ((uint32_t)i * blockDim.x + threadIdx.x) * PER + y - ahead; };  // from `from` on (wraps below it)
-        const uint32_t n = to - from;
-        uint32_t raw[N][4];
-        constexpr uint32_t NONE = TYPE == ZKB_VALUE_BF16 ? 0xff80ff80u : TYPE == ZKB_VALUE_WORD ? 0xff80u : 0xff800000u;
-        auto load_some = [&](int i) {  // a vector of which a part, or nothing, is inside
-            const uint32_t at = place(i, 0);
-            raw[i][0] = raw[i][1] = raw[i][2] = raw[i][3] = NONE;
-            if (at + (PER - 1) < n + (PER - 1)) {
+// A thread's logits of a part: N 16-byte vectors on 16-byte boundaries, `threads` apart. The first one may reach before the part; values outside it are -infinity.
+template <int TYPE, int N>
+struct Logits {
+    static constexpr int PER = TYPE == ZKB_VALUE_BF16 ? 8 : 4, SIZE = 16 / PER;
+    static constexpr uint32_t NONE = TYPE == ZKB_VALUE_BF16 ? 0xff80ff80u : TYPE == ZKB_VALUE_WORD ? 0xff80u : 0xff800000u;
+    uint32_t raw[N][4];
+    const char* base;  // the part's first logit
+    uint32_t n, ahead, threads, thread;
+    __device__ __forceinline__ Logits(const char* first, uint32_t count, uint32_t all, uint32_t mine) : base(first), n(count), ahead((uint32_t)((uintptr_t)first & 15) / SIZE), threads(all), thread(mine) {}
+    __device__ __forceinline__ uint32_t place(int i, int y) const { return ((uint32_t)i * threads + thread) * PER + y - ahead; }  // in the part (wraps before it)
+    __device__ __forceinline__ void load_some(int i) {  // a vector of which a part, or nothing, is inside
+        const uint32_t at = place(i, 0);
+        raw[i][0] = raw[i][1] = raw[i][2] = raw[i][3] = NONE;
+        if (at + (PER - 1) < n + (PER - 1)) {
 #pragma unroll
-                for (int y = 0; y < PER; y++)
-                    if (at + y < n) {
-                        if constexpr (TYPE == ZKB_VALUE_BF16) {
-                            const uint32_t h = *reinterpret_cast<const uint16_t*>(base + (int64_t)(int32_t)(at + y) * SIZE);
-                            raw[i][y / 2] = y % 2 ? (raw[i][y / 2] & 0xffffu) | h << 16 : (raw[i][y / 2] & 0xffff0000u) | h;
-                        } else {
-                            raw[i][y] = *reinterpret_cast<const uint32_t*>(base + (int64_t)(int32_t)(at + y) * SIZE);
-                        }
+            for (int y = 0; y < PER; y++)
+                if (at + y < n) {
+                    if constexpr (TYPE == ZKB_VALUE_BF16) {
+                        const uint32_t h = *reinterpret_cast<const uint16_t*>(base + (int64_t)(int32_t)(at + y) * SIZE);
+                        raw[i][y / 2] = y % 2 ? (raw[i][y / 2] & 0xffffu) | h << 16 : (raw[i][y / 2] & 0xffff0000u) | h;
+                    } else {
+                        raw[i][y] = *reinterpret_cast<const uint32_t*>(base + (int64_t)(int32_t)(at + y) * SIZE);
                     }
-            }
-        };
-        if constexpr (STAGED) {
-            if (!failed) failed = !mbar_wait(bar_of(row_bar), turn++ & 1);
-            const uint32_t whole = (n + ahead) / PER;  // vectors up to the first that does not end inside
-#pragma unroll
-            for (int i = 0; i < N; i++) ld_shared4(stage + ((uint32_t)i * blockDim.x + threadIdx.x) * 16, raw[i][0], raw[i][1], raw[i][2], raw[i][3]);
-            if (threadIdx.x == 0 && ahead) load_some(0);
-#pragma unroll
-            for (int i = 0; i < N; i++)
-                if ((uint32_t)i * blockDim.x + threadIdx.x >= whole) load_some(i);
-        } else {
-#pragma unroll
-            for (int i = 0; i < N; i++) {
-                const uint32_t at = place(i, 0);
-                if (at < n && n - at >= PER) {
-                    const uint4 w = __ldcs(reinterpret_cast<const uint4*>(base + (int64_t)at * SIZE));
-                    raw[i][0] = w.x, raw[i][1] = w.y, raw[i][2] = w.z, raw[i][3] = w.w;
-                } else {
-                    load_some(i);
                 }
+        }
+    }
+    __device__ __forceinline__ void load() {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const uint32_t at = place(i, 0);
+            if (at < n && n - at >= PER) {
+                const uint4 w = __ldcs(reinterpret_cast<const uint4*>(base + (int64_t)at * SIZE));
+                raw[i][0] = w.x, raw[i][1] = w.y, raw[i][2] = w.z, raw[i][3] = w.w;
+            } else {
+                load_some(i);
             }
         }
-        auto value = [&](int i, int y) {
-            if constexpr (TYPE == ZKB_VALUE_BF16) return y % 2 ? bf16_high(raw[i][y / 2]) : bf16_low(raw[i][y / 2]);
-            else if constexpr (TYPE == ZKB_VALUE_WORD) return bf16_low(raw[i][y]);
-            else return __uint_as_float(raw[i][y]);
-        };
-        auto largest_of = [&](int i, float m) {
-            if constexpr (TYPE == ZKB_VALUE_BF16) {
-                const uint32_t w = max_nan_bf16(max_nan_bf16(raw[i][0], raw[i][1]), max_nan_bf16(raw[i][2], raw[i][3]));
-                return max_nan(m, max_nan(bf16_low(w), bf16_high(w)));
-            } else {
-                return max_nan(m, max_nan(max_nan(value(i, 0), value(i, 1)), max_nan(value(i, 2), value(i, 3))));
-            }
-        };
+    }
+    // From shared memory, where copy_row has put the whole ones.
+    __device__ __forceinline__ void load_copied(uint32_t stage) {
+        const uint32_t whole = (n + ahead) / PER;  // vectors up to the first that does not end inside
+#pragma unroll
+        for (int i = 0; i < N; i++) ld_shared4(stage + ((uint32_t)i * threads + thread) * 16, raw[i][0], raw[i][1], raw[i][2], raw[i][3]);
+        if (thread == 0 && ahead) load_some(0);
+#pragma unroll
+        for (int i = 0; i < N; i++)
+            if ((uint32_t)i * threads + thread >= whole) load_some(i);
+    }
+    __device__ __forceinline__ float value(int i, int y) const {
+        if constexpr (TYPE == ZKB_VALUE_BF16) return y % 2 ? bf16_high(raw[i][y / 2]) : bf16_low(raw[i][y / 2]);
+        else if constexpr (TYPE == ZKB_VALUE_WORD) return bf16_low(raw[i][y]);
+        else return __uint_as_float(raw[i][y]);
+    }
+    __device__ __forceinline__ float largest_of(int i, float m) const {
+        if constexpr (TYPE == ZKB_VALUE_BF16) {
+            const uint32_t w = max_nan_bf16(max_nan_bf16(raw[i][0], raw[i][1]), max_nan_bf16(raw[i][2], raw[i][3]));
+            return max_nan(m, max_nan(bf16_low(w), bf16_high(w)));
+        } else {
+            return max_nan(m, max_nan(max_nan(value(i, 0), value(i, 1)), max_nan(value(i, 2), value(i, 3))));
+        }
+    }
+    // The largest one's word; NaN and +infinity are the largest word.
+    __device__ __forceinline__ uint32_t largest() const {
         float mine = -INFINITY;
         if constexpr (TYPE == ZKB_VALUE_BF16) {
             uint32_t w = 0xff80ff80u;
@@ -172,40 +140,12 @@ __global__ void __launch_bounds__(512, 2) logprobs_kernel(const __grid_constant_
 #pragma unroll
             for (int i = 0; i < N; i++) mine = largest_of(i, mine);
         }
-        // NaN and +infinity are the largest word
-        const uint32_t mine_word = mine < INFINITY ? value_word(mine) : 0xffffffffu;
-        uint32_t group = mine_word;
-        if (p.lanes == 32) group = __reduce_max_sync(0xffffffffu, group);
-        else
-            for (uint32_t o = 1; o < p.lanes; o <<= 1) group = max(group, __shfl_xor_sync(0xffffffffu, group, o));
-        const uint32_t a_warp = 32 / p.lanes, n_groups = warps * a_warp;
-        if (lane % p.lanes == 0) groups[warp * a_warp + lane / p.lanes] = group;
-        __syncthreads();
-        if constexpr (STAGED) {  // all have their logits in registers
-            if (threadIdx.x == blockDim.x - 1 && !failed && t + gridDim.x < a.n_rows) copy_row(stage, row + (int64_t)gridDim.x * a.logits_stride * SIZE, a.vocab * SIZE, bar_of(row_bar));
-        }
-        // Every warp finds the largest of the groups' maxima, and the n_top-th largest, where that is a token's: as many values reach it.
-        const uint32_t one = lane < n_groups ? groups[lane] : 0u, two = lane + 32 < n_groups ? groups[lane + 32] : 0u;
-        const uint32_t most_word = __reduce_max_sync(0xffffffffu, max(one, two));
-        uint32_t threshold = most_word;
-        if (n_top > 1) {
-            uint32_t above_one = 0, above_two = 0;
-            for (uint32_t g = 0; g < n_groups; g += 4) {
-                const uint4 o = *reinterpret_cast<const uint4*>(&groups[g]);
-                above_one += (o.x > one) + (o.y > one) + (o.z > one) + (o.w > one);
-                if (n_groups > 32) above_two += (o.x > two) + (o.y > two) + (o.z > two) + (o.w > two);
-            }
-            // the smallest that fewer than n_top are above: of equal ones any may be the n_top-th
-            threshold = __reduce_min_sync(0xffffffffu, min(lane < n_groups && above_one < n_top ? one : 0xffffffffu, lane + 32 < n_groups && above_two < n_top ? two : 0xffffffffu));
-            if (n_top > n_groups) threshold = 0;
-        }
-        threshold = max(threshold, WORD_NONE + 1);
-        const float most = most_word == 0xffffffffu ? __int_as_float(0x7fc00000) : word_value(most_word);
-        const float less = most_word <= WORD_NONE || most_word == 0xffffffffu ? 0.f : most;
-        // What is further below is taken for that: its weight is zero, and so is its product with a number.
-        const float low = fminf(less, fmaxf(less - 300.f / p.log2_scale, -3.38953139e38f));  // (bf16 has none below)
+        return mine < INFINITY ? value_word(mine) : 0xffffffffu;
+    }
+    // Sums of w = exp2(d) and of w d over this thread's logits x, d = (x - less) * log2_scale. What is below `low` is taken for that: its weight is zero, and so is its product with a number.
+    __device__ __forceinline__ void weigh(float less, float low, float log2_scale, bool tokens, float& rest, float& lean) const {
         const uint32_t low_bf16 = (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rd(low)) * 0x10001u;
-        const uint64_t minus = both(-less, -less), by = both(p.log2_scale, p.log2_scale);
+        const uint64_t minus = both(-less, -less), by = both(log2_scale, log2_scale);
         uint64_t rests = 0, leans = 0;  // (zero is a pair of zeros)
 #pragma unroll
         for (int i = 0; i < N; i++)
@@ -222,106 +162,202 @@ __global__ void __launch_bounds__(512, 2) logprobs_kernel(const __grid_constant_
                 rests = add_both(rests, w);
                 leans = fma_both(w, d, leans);
             }
-        float rest = first_of(rests) + second_of(rests), lean = first_of(leans) + second_of(leans);
-        if (most_word > WORD_NONE && (less - low) * p.log2_scale < 200.f) {  // there is no number that far below: -infinity is told from the lowest one
+        rest = first_of(rests) + second_of(rests), lean = first_of(leans) + second_of(leans);
+        if (tokens && (less - low) * log2_scale < 200.f) {  // there is no number that far below: -infinity is told from the lowest one
             rest = lean = 0.f;
 #pragma unroll
             for (int i = 0; i < N; i++)
 #pragma unroll
                 for (int y = 0; y < PER; y++) {
-                    const float x = value(i, y), d = (fmaxf(x, low) - less) * p.log2_scale, w = x > -INFINITY ? exp2_fast(d) : 0.f;
+                    const float x = value(i, y), d = (fmaxf(x, low) - less) * log2_scale, w = x > -INFINITY ? exp2_fast(d) : 0.f;
                     rest += w, lean = fmaf(w, d, lean);
                 }
         }
+    }
+    // The sum of w without the largest one's.
+    __device__ __forceinline__ float weigh_others(float less, float low, float log2_scale) const {
+        float rest = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; i++)
+#pragma unroll
+            for (int y = 0; y < PER; y++) {
+                const float x = value(i, y), d = (fmaxf(x, low) - less) * log2_scale;
+                rest += x > -INFINITY && x != less ? exp2_fast(d) : 0.f;
+            }
+        return rest;
+    }
+    // Those that reach the threshold, to a list shared by the warps (by a whole warp; mine: this thread's largest). `from`: the part's place in the row.
+    __device__ __forceinline__ void list_reaching(uint32_t threshold, uint32_t mine, uint32_t from, uint64_t* list, uint32_t* n_list) const {
+        uint64_t found = 0;
+        float first = 0.f;  // the last one's value: the one that is written first
+        if (mine >= threshold) {
+            const float reach = word_value(threshold);
+#pragma unroll
+            for (int i = 0; i < N; i++)
+                if (largest_of(i, -INFINITY) >= reach) {  // (few do)
+#pragma unroll
+                    for (int y = 0; y < PER; y++)
+                        if (value(i, y) >= reach) found |= 1ull << (i * PER + y), first = value(i, y);
+                }
+        }
+        if (!__any_sync(0xffffffffu, found != 0)) return;
+        const uint32_t lane = threadIdx.x & 31, n_mine = __popcll(found);
+        uint32_t before = n_mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t x = __shfl_up_sync(0xffffffffu, before, o);
+            if (lane >= o) before += x;
+        }
+        uint32_t at = 0;
+        if (lane == 31) at = atomicAdd(n_list, before);
+        at = __shfl_sync(0xffffffffu, at, 31) + before - n_mine;
+        if (found) {
+            const uint32_t last_bit = 63 - __clzll(found);
+            for (bool again = false; found && at < LP_LIST; at++, again = true) {  // the others are fetched once more
+                const uint32_t bit = again ? __ffsll(found) - 1 : last_bit, where = place((int)(bit / PER), (int)(bit % PER));
+                list[at] = (uint64_t)value_word(again ? logit_at<TYPE>(base, where) : first) << 32 | (0xffffffffu - (from + where));
+                found &= ~(1ull << bit);
+            }
+        }
+    }
+};
+
+// What a part's sums are relative to, from its largest word.
+struct LpScale {
+    float most, less, low;
+    bool tokens;  // there is one at least, and no NaN or +infinity
+    __device__ __forceinline__ LpScale(uint32_t word, float log2_scale) {
+        tokens = word > WORD_NONE && word != 0xffffffffu;
+        most = word == 0xffffffffu ? __int_as_float(0x7fc00000) : word_value(word);
+        less = tokens ? most : 0.f;
+        low = fminf(less, fmaxf(less - 300.f / log2_scale, -3.38953139e38f));  // (bf16 has none below)
+    }
+};
+
+// Groups of `lanes` lanes: their largest words, and the n_top-th largest of those where that is a token's: as many values reach it. By every warp for itself, behind a barrier.
+__device__ __forceinline__ void store_group(uint32_t* groups, uint32_t lanes, uint32_t warp, uint32_t lane, uint32_t word) {
+    if (lanes == 32) word = __reduce_max_sync(0xffffffffu, word);
+    else
+        for (uint32_t o = 1; o < lanes; o <<= 1) word = max(word, __shfl_xor_sync(0xffffffffu, word, o));
+    if (lane % lanes == 0) groups[warp * (32 / lanes) + lane / lanes] = word;
+}
+__device__ __forceinline__ uint32_t threshold_of(const uint32_t* groups, uint32_t n_groups, uint32_t lane, uint32_t n_top, uint32_t& most_word) {
+    const uint32_t one = lane < n_groups ? groups[lane] : 0u, two = lane + 32 < n_groups ? groups[lane + 32] : 0u;
+    most_word = __reduce_max_sync(0xffffffffu, max(one, two));
+    uint32_t threshold = most_word;
+    if (n_top > 1) {
+        uint32_t above_one = 0, above_two = 0;
+        for (uint32_t g = 0; g < n_groups; g += 4) {
+            const uint4 o = *reinterpret_cast<const uint4*>(&groups[g]);
+            above_one += (o.x > one) + (o.y > one) + (o.z > one) + (o.w > one);
+            if (n_groups > 32) above_two += (o.x > two) + (o.y > two) + (o.z > two) + (o.w > two);
+        }
+        // the smallest that fewer than n_top are above: of equal ones any may be the n_top-th
+        threshold = __reduce_min_sync(0xffffffffu, min(lane < n_groups && above_one < n_top ? one : 0xffffffffu, lane + 32 < n_groups && above_two < n_top ? two : 0xffffffffu));
+        if (n_top > n_groups) threshold = 0;
+    }
+    return max(threshold, WORD_NONE + 1);
+}
+__device__ __forceinline__ float over_warps(const float* x, uint32_t warps, uint32_t lane) {
+    float y = lane < warps ? x[lane] : 0.f;
+#pragma unroll
+    for (int o = 8; o; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
+    return __shfl_sync(0xffffffffu, y, 0);
+}
+
+// What a row's outputs are made of.
+struct LpResult {
+    float most, scale, log_total, total, lean;
+    bool odd, none;
+    __device__ __forceinline__ LpResult(float largest, uint32_t equal, float rest, float lean_sum, float by) : most(largest), scale(by), total((float)equal + rest), lean(lean_sum) {
+        odd = most != most, none = most == -INFINITY;
+        log_total = none ? 0.f : equal == 1 ? log1pf(rest) : logf(total);
+    }
+    __device__ __forceinline__ float log_probability(float x) const { return odd ? __int_as_float(0x7fc00000) : none || x == -INFINITY ? -INFINITY : (x - most) * scale - log_total; }
+    __device__ __forceinline__ float entropy() const { return odd ? __int_as_float(0x7fc00000) : none ? 0.f : log_total - lean * 0.693147181f / total; }
+    __device__ __forceinline__ void give(const zkb_step_logprobs_args& a, uint32_t t, uint32_t i, int32_t id, float x) const {
+        float y = 0.f;
+        if (id >= 0 && (uint32_t)id < a.vocab) y = log_probability(x);
+        else if (a.off_table) atomicAdd(reinterpret_cast<unsigned long long*>(a.off_table), 1ull);
+        a.logprobs[(int64_t)t * a.n_given + i] = y;
+    }
+    __device__ __forceinline__ void give_top(const zkb_step_logprobs_args& a, uint32_t t, uint32_t place, uint64_t key) const {
+        a.top_ids[(int64_t)t * a.n_top + place] = odd || !key ? -1 : (int32_t)(0xffffffffu - (uint32_t)key);
+        a.top_logprobs[(int64_t)t * a.n_top + place] = odd ? __int_as_float(0x7fc00000) : !key ? -INFINITY : log_probability(word_value((uint32_t)(key >> 32)));
+    }
+};
+
+// Few rows, or long ones: a thread block has a row, or a piece of it. TYPE: ZKB_VALUE_*; N: 16-byte vectors a thread.
+template <int TYPE, int N>
+__global__ void __launch_bounds__(512, 2) logprobs_kernel(const __grid_constant__ LogprobArgs p) {
+    constexpr int SIZE = Logits<TYPE, N>::SIZE;
+    __shared__ LpPart parts[LP_PARTS];
+    __shared__ uint64_t list[LP_LIST];
+    __shared__ __align__(16) uint32_t groups[64];
+    __shared__ float sums[3][16];
+    __shared__ uint32_t n_list;
+    __shared__ uint64_t best[16];
+    const zkb_step_logprobs_args& a = p.a;
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, rank = cluster_rank(), ranks = cluster_ranks(), n_top = a.n_top, n_groups = warps * (32 / p.lanes);
+    const uint32_t begin = min(rank * p.piece, a.vocab), end = min(begin + p.piece, a.vocab), n_parts = (p.piece + p.part - 1) / p.part, t = blockIdx.x / ranks;
+    if (threadIdx.x == 0) n_list = 0;
+    if (threadIdx.x < 64 && threadIdx.x >= n_groups) groups[threadIdx.x] = 0;
+    if (ranks > 1) cluster_arrive();
+    const char* const row = static_cast<const char*>(a.logits) + (int64_t)t * a.logits_stride * SIZE;
+    // what is asked of the row is on its way meanwhile
+    const int32_t id_first = threadIdx.x < a.n_given && rank == 0 ? a.ids[(int64_t)t * a.n_given + threadIdx.x] : -1;
+    const float given_first = id_first >= 0 && (uint32_t)id_first < a.vocab ? logit_at<TYPE>(row, (uint32_t)id_first) : 0.f;
+    for (uint32_t q = 0; q < n_parts; q++) {
+        const uint32_t from = min(begin + q * p.part, end), to = min(from + p.part, end), n = to - from;
+        Logits<TYPE, N> x(row + (int64_t)from * SIZE, n, blockDim.x, threadIdx.x);
+        x.load();
+        const uint32_t mine = x.largest();
+        store_group(groups, p.lanes, warp, lane, mine);
+        __syncthreads();
+        uint32_t most_word;
+        const uint32_t threshold = threshold_of(groups, n_groups, lane, n_top, most_word);
+        const LpScale s(most_word, p.log2_scale);
+        float rest, lean;
+        x.weigh(s.less, s.low, p.log2_scale, s.tokens, rest, lean);
 #pragma unroll
         for (int o = 16; o; o >>= 1) rest += __shfl_xor_sync(0xffffffffu, rest, o), lean += __shfl_xor_sync(0xffffffffu, lean, o);
         if (lane == 0) sums[0][warp] = rest, sums[1][warp] = lean;
-        if (n_top) {
-            uint64_t found = 0;  // which of this thread's values reach the threshold
-            float first = 0.f;   // the last one of those, first written
-            if (mine_word >= threshold) {
-                const float reach = word_value(threshold);
-#pragma unroll
-                for (int i = 0; i < N; i++)
-                    if (largest_of(i, -INFINITY) >= reach) {  // (few do)
-#pragma unroll
-                        for (int y = 0; y < PER; y++)
-                            if (value(i, y) >= reach) found |= 1ull << (i * PER + y), first = value(i, y);
-                    }
-            }
-            if (__any_sync(0xffffffffu, found != 0)) {
-                const uint32_t n_mine = __popcll(found);
-                uint32_t before = n_mine;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const uint32_t x = __shfl_up_sync(0xffffffffu, before, o);
-                    if (lane >= o) before += x;
-                }
-                uint32_t at = 0;
-                if (lane == 31) at = atomicAdd(&n_list, before);
-                at = __shfl_sync(0xffffffffu, at, 31) + before - n_mine;
-                if (found) {
-                    const uint32_t top_bit = 63 - __clzll(found);
-                    for (bool again = false; found && at < LP_LIST; at++, again = true) {  // the others are fetched once more
-                        const uint32_t bit = again ? __ffsll(found) - 1 : top_bit, where = place((int)(bit / PER), (int)(bit % PER));
-                        list[at] = (uint64_t)value_word(again ? logit_at<TYPE>(base, where) : first) << 32 | (0xffffffffu - (from + where));
-                        found &= ~(1ull << bit);
-                    }
-                }
-            }
-        }
+        if (n_top) x.list_reaching(threshold, mine, from, list, &n_list);
         __syncthreads();
         LpPart& part = parts[q];
         const uint32_t listed = n_list;
-        auto over_warps = [&](const float* x) {
-            float y = lane < warps ? x[lane] : 0.f;
-#pragma unroll
-            for (int o = 8; o; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
-            return __shfl_sync(0xffffffffu, y, 0);
-        };
-        rest = over_warps(sums[0]);
-        lean = over_warps(sums[1]);
+        rest = over_warps(sums[0], warps, lane);
+        lean = over_warps(sums[1], warps, lane);
         uint32_t equal = 0;
-        if (rest < 1.25f && most_word > WORD_NONE && most_word != 0xffffffffu) {  // one token is likely: the sum without it, for all of its bits
+        if (rest < 1.25f && s.tokens) {  // one token is likely: the sum without it, for all of its bits
             equal = 1;
-            rest = 0.f;
-#pragma unroll
-            for (int i = 0; i < N; i++)
-#pragma unroll
-                for (int y = 0; y < PER; y++) {
-                    const float x = value(i, y), d = (fmaxf(x, low) - less) * p.log2_scale;
-                    rest += x > -INFINITY && x != less ? exp2_fast(d) : 0.f;
-                }
+            rest = x.weigh_others(s.less, s.low, p.log2_scale);
 #pragma unroll
             for (int o = 16; o; o >>= 1) rest += __shfl_xor_sync(0xffffffffu, rest, o);
             if (lane == 0) sums[2][warp] = rest;
             __syncthreads();
-            rest = over_warps(sums[2]);
+            rest = over_warps(sums[2], warps, lane);
         }
-        if (threadIdx.x == 0) part.most = most, part.rest = rest, part.lean = lean, part.equal = equal;
+        if (threadIdx.x == 0) part.most = s.most, part.rest = rest, part.lean = lean, part.equal = equal;
         if (listed <= LP_LIST) {
-            // a short list is the first warp's, while the others begin with the next row
-            const uint32_t by_threads = alone && listed <= 64 ? 32u : blockDim.x;
-            for (uint32_t i = threadIdx.x; i < listed && threadIdx.x < by_threads; i += by_threads) {
+            for (uint32_t i = threadIdx.x; i < listed; i += blockDim.x) {
                 const uint64_t key = list[i];
                 uint32_t above = 0;
 #pragma unroll 4
                 for (uint32_t j = 0; j < listed; j++) above += list[j] > key;
                 if (above < n_top) part.top[above] = key;
             }
-            if (threadIdx.x < by_threads)
-                for (uint32_t i = listed + threadIdx.x; i < n_top; i += by_threads) part.top[i] = 0;
-            if (by_threads > 32) __syncthreads();
-            else __syncwarp();
+            for (uint32_t i = listed + threadIdx.x; i < n_top; i += blockDim.x) part.top[i] = 0;
+            __syncthreads();
         } else {
             uint64_t last = ~0ull;
             for (uint32_t k = 0; k < n_top; k++) {
                 uint64_t key = 0;
 #pragma unroll 4
                 for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {  // (from memory: registers for this would be missed above)
-                    const uint32_t w = value_word(logit_at<TYPE>(base, i));
-                    const uint64_t x = (uint64_t)w << 32 | (0xffffffffu - (from + i));
-                    if (w > WORD_NONE && x < last && x > key) key = x;
+                    const uint32_t w = value_word(logit_at<TYPE>(x.base, i));
+                    const uint64_t y = (uint64_t)w << 32 | (0xffffffffu - (from + i));
+                    if (w > WORD_NONE && y < last && y > key) key = y;
                 }
 #pragma unroll
                 for (int o = 16; o; o >>= 1) {
@@ -338,9 +374,7 @@ __global__ void __launch_bounds__(512, 2) logprobs_kernel(const __grid_constant_
             }
         }
         if (threadIdx.x == 0) n_list = 0;
-        __syncwarp();
     }
-    if (alone && warp) continue;  // the first warp has the rest of the row
     // The thread blocks' parts go to the first one's shared memory, behind its own.
     if (ranks > 1) {
         __syncthreads();
@@ -355,7 +389,7 @@ __global__ void __launch_bounds__(512, 2) logprobs_kernel(const __grid_constant_
         cluster_arrive(), cluster_wait();
         if (rank) return;
     }
-    const uint32_t all = ranks * n_parts, joiners = alone ? 32u : blockDim.x;
+    const uint32_t all = ranks * n_parts;
     // every warp joins the sums, a part a lane
     float most = -INFINITY;
     for (uint32_t i = lane; i < all; i += 32) most = max_nan(most, parts[i].most);
@@ -379,35 +413,21 @@ __global__ void __launch_bounds__(512, 2) logprobs_kernel(const __grid_constant_
     } else {
         rest = __shfl_sync(0xffffffffu, rest, 0), lean = __shfl_sync(0xffffffffu, lean, 0), equal = __shfl_sync(0xffffffffu, equal, 0);
     }
-    constexpr float LN2 = 0.693147181f;
-    const bool odd = most != most, none = most == -INFINITY;
-    const float nan = __int_as_float(0x7fc00000);
-    const float total = (float)equal + rest;
-    const float log_total = none ? 0.f : equal == 1 ? log1pf(rest) : logf(total);
-    auto log_probability = [&](float x) { return odd ? nan : none || x == -INFINITY ? -INFINITY : (x - most) * a.scale - log_total; };
-    if (threadIdx.x == 0 && a.entropy) a.entropy[t] = odd ? nan : none ? 0.f : log_total - lean * LN2 / total;
-    for (uint32_t i = threadIdx.x; i < a.n_given; i += joiners) {
+    const LpResult r(most, equal, rest, lean, a.scale);
+    if (threadIdx.x == 0 && a.entropy) a.entropy[t] = r.entropy();
+    for (uint32_t i = threadIdx.x; i < a.n_given; i += blockDim.x) {
         const int32_t id = i == threadIdx.x ? id_first : a.ids[(int64_t)t * a.n_given + i];
-        float y = 0.f;
-        if (id >= 0 && (uint32_t)id < a.vocab) {
-            y = log_probability(i == threadIdx.x ? given_first : logit_at<TYPE>(row, (uint32_t)id));
-        } else if (a.off_table) {
-            atomicAdd(reinterpret_cast<unsigned long long*>(a.off_table), 1ull);
-        }
-        a.logprobs[(int64_t)t * a.n_given + i] = y;
+        r.give(a, t, i, id, i == threadIdx.x ? given_first : id >= 0 && (uint32_t)id < a.vocab ? logit_at<TYPE>(row, (uint32_t)id) : 0.f);
     }
     // (a key's place is how many others are larger: the parts' keys are in order; places without a token lie behind those with one)
-    for (uint32_t i = threadIdx.x; i < all * n_top; i += joiners) {
+    for (uint32_t i = threadIdx.x; i < all * n_top; i += blockDim.x) {
         const uint32_t mine = i / n_top, place = i - mine * n_top;
         const uint64_t key = parts[mine].top[place];
         uint32_t above = place;
-        if (key || place == 0)
+        if (key)
             for (uint32_t j = 0; j < all && above < n_top; j++)
                 for (uint32_t k = 0; j != mine && k < n_top && parts[j].top[k] > key; k++) above++;
-        if (key && above < n_top) {
-            a.top_ids[(int64_t)t * n_top + above] = odd ? -1 : (int32_t)(0xffffffffu - (uint32_t)key);
-            a.top_logprobs[(int64_t)t * n_top + above] = log_probability(word_value((uint32_t)(key >> 32)));
-        }
+        if (key && above < n_top) r.give_top(a, t, above, key);
     }
     if (n_top) {  // what is left without a token
         uint32_t found = 0;
@@ -417,10 +437,139 @@ __global__ void __launch_bounds__(512, 2) logprobs_kernel(const __grid_constant_
             found += k;
         }
         found = __reduce_add_sync(0xffffffffu, found);
-        for (uint32_t i = found + threadIdx.x; i < n_top; i += joiners) a.top_ids[(int64_t)t * n_top + i] = -1, a.top_logprobs[(int64_t)t * n_top + i] = odd ? nan : -INFINITY;
+        for (uint32_t i = found + threadIdx.x; i < n_top; i += blockDim.x) r.give_top(a, t, i, 0);
     }
+}
+
+// Many rows: a thread block has row after row. The next one comes to shared memory while this one is summed, and a warp of its own writes a row's outputs while the others are at the next:
+// the chain from the last sum to the last store, some 2000 cycles, is hidden.
+constexpr int LP_ROWS_N = 8;
+template <int TYPE>
+__global__ void __launch_bounds__(544, 2) logprobs_rows_kernel(const __grid_constant__ LogprobArgs p, unsigned* dev_err) {
+    constexpr int SIZE = Logits<TYPE, LP_ROWS_N>::SIZE;
+    extern __shared__ __align__(16) unsigned char row_sm[];
+    __shared__ __align__(8) unsigned long long row_bar;
+    __shared__ uint64_t list[2][LP_LIST];
+    __shared__ __align__(16) uint32_t groups[64];
+    __shared__ float sums[3][16], part_sm[2][3];  // most, rest, lean
+    __shared__ uint32_t n_list[2], equal_sm[2];
+    const zkb_step_logprobs_args& a = p.a;
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = (blockDim.x >> 5) - 1, threads = 32 * warps, n_top = a.n_top, n_groups = warps * (32 / p.lanes);
+    const uint32_t stage = (uint32_t)__cvta_generic_to_shared(row_sm);
+    auto row_of = [&](uint32_t t) { return static_cast<const char*>(a.logits) + (int64_t)t * a.logits_stride * SIZE; };
+    // Barriers: 1 the summing warps', 2 and 3 a row's results are there, 4 and 5 they have been written.
+    enum { SUMMING = 1, THERE = 2, WRITTEN = 4 };
+    auto arrive = [&](int id) {
+        __syncwarp();
+        asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads + 32) : "memory");
+    };
+    if (threadIdx.x == 0) {
+        mbar_init(bar_of(row_bar), 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        copy_row(stage, row_of(blockIdx.x), a.vocab * SIZE, bar_of(row_bar));
+        n_list[0] = n_list[1] = 0;
     }
-    if (STAGED && failed) {  // nothing is on its way to shared memory when the thread block gives it up
+    if (threadIdx.x < 64 && threadIdx.x >= n_groups) groups[threadIdx.x] = 0;
+    __syncthreads();
+    uint32_t turn = 0;
+    if (warp == warps) {  // ---- outputs
+        for (uint32_t t = blockIdx.x; t < a.n_rows; t += gridDim.x, turn++) {
+            const uint32_t buf = turn & 1;
+            const char* const row = row_of(t);
+            const int32_t id_first = lane < a.n_given ? a.ids[(int64_t)t * a.n_given + lane] : -1;
+            const float given_first = id_first >= 0 && (uint32_t)id_first < a.vocab ? logit_at<TYPE>(row, (uint32_t)id_first) : 0.f;
+            named_sync(THERE + buf, threads + 32);
+            const uint32_t listed = n_list[buf];
+            const LpResult r(part_sm[buf][0], equal_sm[buf], part_sm[buf][1], part_sm[buf][2], a.scale);
+            if (lane == 0 && a.entropy) a.entropy[t] = r.entropy();
+            for (uint32_t i = lane; i < a.n_given; i += 32) {
+                const int32_t id = i == lane ? id_first : a.ids[(int64_t)t * a.n_given + i];
+                r.give(a, t, i, id, i == lane ? given_first : id >= 0 && (uint32_t)id < a.vocab ? logit_at<TYPE>(row, (uint32_t)id) : 0.f);
+            }
+            __syncwarp();
+            if (n_top) {
+                // Lane k holds the k-th largest key so far: a larger one than the n_top-th takes its place and moves those behind it on. (Of equal logits the keys of lower indexes are larger.)
+                uint64_t mine = 0, least = 0;
+                auto take = [&](uint64_t key) {
+                    uint32_t who = __ballot_sync(0xffffffffu, key > least);
+                    while (who) {
+                        const uint64_t k = __shfl_sync(0xffffffffu, key, __ffs(who) - 1);
+                        const uint32_t smaller = __ballot_sync(0xffffffffu, mine < k), at = __ffs(smaller) - 1;  // (some lane's is: the n_top-th)
+                        const uint64_t before = __shfl_up_sync(0xffffffffu, mine, 1);
+                        if (lane == at) mine = k;
+                        else if (lane > at) mine = before;
+                        least = __shfl_sync(0xffffffffu, mine, n_top - 1);
+                        who &= who - 1;
+                        who &= __ballot_sync(0xffffffffu, key > least);
+                    }
+                };
+                if (listed <= LP_LIST) {
+                    for (uint32_t i = 0; i < listed; i += 32) take(i + lane < listed ? list[buf][i + lane] : 0);
+                } else {
+                    for (uint32_t i = 0; i < a.vocab; i += 256) {  // too many tie: from the row itself
+                        uint64_t key[8];
+#pragma unroll
+                        for (int y = 0; y < 8; y++) {
+                            const uint32_t at = i + y * 32 + lane, w = at < a.vocab ? value_word(logit_at<TYPE>(row, at)) : 0u;
+                            key[y] = w > WORD_NONE ? (uint64_t)w << 32 | (0xffffffffu - at) : 0;
+                        }
+#pragma unroll
+                        for (int y = 0; y < 8; y++) take(key[y]);
+                    }
+                }
+                if (lane < n_top) r.give_top(a, t, lane, mine);
+            }
+            __syncwarp();
+            if (lane == 0) n_list[buf] = 0;
+            arrive(WRITTEN + buf);
+        }
+        return;
+    }
+    bool failed = false;
+    for (uint32_t t = blockIdx.x; t < a.n_rows; t += gridDim.x, turn++) {
+        const uint32_t buf = turn & 1;
+        if (!failed) failed = !mbar_wait(bar_of(row_bar), turn & 1);
+        Logits<TYPE, LP_ROWS_N> x(row_of(t), a.vocab, threads, threadIdx.x);
+        x.load_copied(stage);
+        const uint32_t mine = x.largest();
+        __syncwarp();
+        store_group(groups, p.lanes, warp, lane, mine);
+        named_sync(SUMMING, threads);
+        // all have their logits in registers
+        if (threadIdx.x == threads - 1 && !failed && t + gridDim.x < a.n_rows) copy_row(stage, row_of(t + gridDim.x), a.vocab * SIZE, bar_of(row_bar));
+        __syncwarp();
+        uint32_t most_word;
+        const uint32_t threshold = threshold_of(groups, n_groups, lane, n_top, most_word);
+        const LpScale s(most_word, p.log2_scale);
+        float rest, lean;
+        x.weigh(s.less, s.low, p.log2_scale, s.tokens, rest, lean);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) rest += __shfl_xor_sync(0xffffffffu, rest, o), lean += __shfl_xor_sync(0xffffffffu, lean, o);
+        if (lane == 0) sums[0][warp] = rest, sums[1][warp] = lean;
+        if (turn >= 2) named_sync(WRITTEN + buf, threads + 32);  // the list is free
+        if (n_top) x.list_reaching(threshold, mine, 0, list[buf], &n_list[buf]);
+        named_sync(SUMMING, threads);
+        rest = over_warps(sums[0], warps, lane);
+        uint32_t equal = 0;
+        if (rest < 1.25f && s.tokens) {  // one token is likely: the sum without it, for all of its bits
+            equal = 1;
+            rest = x.weigh_others(s.less, s.low, p.log2_scale);
+#pragma unroll
+            for (int o = 16; o; o >>= 1) rest += __shfl_xor_sync(0xffffffffu, rest, o);
+            if (lane == 0) sums[2][warp] = rest;
+            named_sync(SUMMING, threads);
+            rest = over_warps(sums[2], warps, lane);
+        }
+        if (warp == 0) {
+            lean = over_warps(sums[1], warps, lane);
+            if (lane == 0) part_sm[buf][0] = s.most, part_sm[buf][1] = rest, part_sm[buf][2] = lean, equal_sm[buf] = equal;
+        }
+        arrive(THERE + buf);
+    }
+    // (every arrival is waited for: the last rows' results have been written)
+    for (uint32_t last = turn < 2 ? 0 : turn - 2; last < turn; last++) named_sync(WRITTEN + (last & 1), threads + 32);
+    if (failed) {  // nothing is on its way to shared memory when the thread block gives it up
         *dev_err = WAIT_RAN_OUT;
         mbar_wait(bar_of(row_bar), (turn - 1) & 1);
     }
@@ -449,18 +598,21 @@ static cudaError_t launch_logprobs(zkb_ctx* ctx, const zkb_step_logprobs_args& a
         attr[0].id = cudaLaunchAttributeClusterDimension;
         attr[0].val.clusterDim = {n, 1, 1};
         cudaLaunchConfig_t cfg = {};
-        const uint32_t at_once = 148u * (1024 / threads);
-        const bool staged = n == 1 && n_parts == 1 && each == 8 && a.n_rows > at_once;
-        cfg.gridDim = dim3(n > 1 ? a.n_rows * n : std::min(a.n_rows, at_once));
-        cfg.dynamicSmemBytes = staged ? threads * LP_VECTORS * 16 : 0;
-        cfg.blockDim = dim3(threads);
+        const uint32_t at_once = 148u * std::min(1024 / threads, 216 * 1024 / (threads * LP_ROWS_N * 16 + 18 * 1024));  // of the kernel for many rows
+        const bool rows = n == 1 && n_parts == 1 && each == LP_ROWS_N && a.n_rows > at_once;
+        cfg.gridDim = dim3(rows ? at_once : a.n_rows * n);
+        cfg.blockDim = dim3(rows ? threads + 32 : threads);
         cfg.stream = ctx->stream;
+        if (rows) {
+            cfg.dynamicSmemBytes = threads * LP_ROWS_N * 16;
+            const cudaError_t e = cudaFuncSetAttribute(logprobs_rows_kernel<TYPE>, cudaFuncAttributeMaxDynamicSharedMemorySize, 512 * LP_ROWS_N * 16);
+            return e == cudaSuccess ? cudaLaunchKernelEx(&cfg, logprobs_rows_kernel<TYPE>, p, ctx->dev_err) : e;
+        }
         cfg.attrs = attr;
         cfg.numAttrs = 1;
-        auto kernel = staged ? logprobs_kernel<TYPE, 8, true> : each == 1 ? logprobs_kernel<TYPE, 1, false> : each == 2 ? logprobs_kernel<TYPE, 2, false> : each == 4 ? logprobs_kernel<TYPE, 4, false> : logprobs_kernel<TYPE, 8, false>;
-        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-        if (e == cudaSuccess && staged) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 512 * LP_VECTORS * 16);
-        return e == cudaSuccess ? cudaLaunchKernelEx(&cfg, kernel, p, ctx->dev_err) : e;
+        auto kernel = each == 1 ? logprobs_kernel<TYPE, 1> : each == 2 ? logprobs_kernel<TYPE, 2> : each == 4 ? logprobs_kernel<TYPE, 4> : logprobs_kernel<TYPE, 8>;
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        return e == cudaSuccess ? cudaLaunchKernelEx(&cfg, kernel, p) : e;
     });
 }
 
