@@ -22,7 +22,7 @@ struct ProductMaps {
 template <bool INT4, int N, bool TMA>
 struct Tile {
     static constexpr bool FILLED = INT4 || !TMA, RAW = INT4 && TMA;     // the weights' part of a stage is written by warps; from shared memory
-    static constexpr int EPI = INT4 ? (N <= 32 ? 4 : N / 8) : N >= 128 ? 8 : 4, SETS = RAW ? (N == 128 ? 1 : 2) : 4;  // warps that read the sums; sets of four warps that write codes, in turn
+    static constexpr int EPI = N == 64 ? (INT4 ? 8 : 4) : N >= 128 ? 8 : 4, SETS = RAW ? (N == 128 ? 1 : 2) : 4;  // warps that read the sums; sets of four warps that write codes, in turn
     static constexpr int FIRST_FILLER = EPI + (INT4 ? 4 : 3), THREADS = 32 * (FILLED ? FIRST_FILLER + 4 * SETS : EPI + 2);
     // A step's codes, in halves of 128 that are a matrix each: what a step costs whatever its codes, waits above all, is some 600 cycles of each of the warps that it goes through.
     static constexpr int CODES = INT4 ? 256 : 128, HALVES = CODES / 128, A_HALF = 128 * 128, B_HALF = N * 128;
@@ -53,6 +53,10 @@ __device__ __forceinline__ void product_codes(bool one, uint32_t d, uint64_t a, 
 __device__ __forceinline__ void tma_load_2d(uint32_t to, const CUtensorMap* map, int code, int row, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(to), "l"(map), "r"(code), "r"(row), "r"(bar) : "memory");
 }
+
+// Sums of 4-bit weights' groups, below 2^22, begin with the pattern of 1.5 * 2^23: what is read is that float plus the sum, and a subtraction is the whole conversion (the instruction for it
+// has an eighth of the rate of additions). Tensor memory is filled with it again as it is read.
+constexpr uint32_t SUM_ZERO = 0x4b400000u;
 
 struct TileBars {
     unsigned long long full[6], empty[6], done[32], x_full[8], raw_full[8], raw_empty[8], scale_full[4], scale_empty[4], sum_full[4], sum_empty[4], last;
@@ -166,6 +170,18 @@ __global__ void __launch_bounds__((Tile<INT4, N, TMA>::THREADS), (Tile<INT4, N, 
         Ring<T::SUMS> sums;
         Ring<(T::SCALES > 0 ? T::SCALES : 1)> scale;
         uint32_t read_ends = 0;
+        if constexpr (INT4) {
+#pragma unroll 1
+            for (int b = 0; b < T::SUMS; b++) {
+#pragma unroll 1
+                for (int k = 0; k < T::SUM; k += N)
+#pragma unroll
+                    for (int j = 0; j < MINE; j += 16) tmem_fill16(at_lanes + b * T::SUM + k + j, SUM_ZERO);
+                tmem_stored();
+                tmem_fence_before();
+                arrive(bars.sum_empty[b]);
+            }
+        }
         Walk w = first();
         for (uint32_t i = 0; i < n_tiles; i++, w.tile += every, enter(w)) {
             const uint32_t c = w.out_tile * 128 + c128, t0 = w.row_tile * N + half;
@@ -178,7 +194,12 @@ __global__ void __launch_bounds__((Tile<INT4, N, TMA>::THREADS), (Tile<INT4, N, 
                     if constexpr (CHUNK == 32) tmem_load32(at + j, x);
                     else tmem_load16(at + j, x);
                     tmem_loaded(x);
+                    if constexpr (INT4) {
+#pragma unroll
+                        for (int y = 0; y < CHUNK; y += 16) tmem_fill16(at + j + y, SUM_ZERO);
+                    }
                     if (last && j + CHUNK == MINE) {
+                        if constexpr (INT4) tmem_stored();
                         tmem_fence_before();
                         arrive(bars.sum_empty[sums.at]);
                     }
@@ -232,27 +253,54 @@ __global__ void __launch_bounds__((Tile<INT4, N, TMA>::THREADS), (Tile<INT4, N, 
                     uint32_t x[32];
                     tmem_load32(at, x);
                     tmem_loaded(x);
+                    tmem_fill16(at, SUM_ZERO), tmem_fill16(at + 16, SUM_ZERO);
                     if (last) {
+                        tmem_stored();
                         tmem_fence_before();
                         arrive(bars.sum_empty[sums.at]);
                     }
 #pragma unroll
                     for (int y = 0; y < 32; y += 2) {
                         const float by = y < 16 ? by0 : by1;
-                        acc[y % 16 / 2] = fma_both(add_both(two_words(x[y] + 0x4b400000u, x[y + 1] + 0x4b400000u), less), both(by, by), acc[y % 16 / 2]);
+                        acc[y % 16 / 2] = fma_both(add_both(two_words(x[y], x[y + 1]), less), both(by, by), acc[y % 16 / 2]);
                     }
                 };
                 auto add = [&](uint32_t at, bool last) {
                     const float by = next_scale();
-                    // A sum below 2^22 added to the pattern of 1.5 * 2^23 is that float plus the sum: a conversion by two additions (the instruction for it has an eighth of their rate).
                     const uint64_t by_both = both(by, by), less = both(-12582912.f, -12582912.f);
                     read(at, last, [&](int j, const uint32_t(&x)[CHUNK]) {
 #pragma unroll
-                        for (int y = 0; y < CHUNK; y += 2) acc[(j + y) / 2] = fma_both(add_both(two_words(x[y] + 0x4b400000u, x[y + 1] + 0x4b400000u), less), by_both, acc[(j + y) / 2]);
+                        for (int y = 0; y < CHUNK; y += 2) acc[(j + y) / 2] = fma_both(add_both(two_words(x[y], x[y + 1]), less), by_both, acc[(j + y) / 2]);
                     });
                 };
+                if constexpr (!T::BY_STEP) {
+                    const uint32_t all = min((first_step + steps) * per_step, groups) - first_step * per_step;
+                    const uint64_t less = both(-12582912.f, -12582912.f);
 #pragma unroll 1
-                for (uint32_t s = 0; s < steps; s++) {
+                    for (uint32_t g = 0; g < all; g++) {
+                        const float by = next_scale();
+                        arrived();
+                        const uint32_t at = at_lanes + sums.at * T::SUM;
+#pragma unroll
+                        for (int j = 0; j < MINE; j += 16) {
+                            uint32_t x[16];
+                            tmem_load16(at + j, x);
+                            tmem_loaded(x);
+                            tmem_fill16(at + j, SUM_ZERO);
+                            if (j + 16 == MINE) {
+                                tmem_stored();
+                                tmem_fence_before();
+                                arrive(bars.sum_empty[sums.at]);
+                            }
+#pragma unroll
+                            for (int y = 0; y < 16; y += 2)
+                                acc[(j + y) / 2] = fma_both(add_both(two_words(x[y], x[y + 1]), less), both(by, by), acc[(j + y) / 2]);
+                        }
+                        sums.next();
+                    }
+                }
+#pragma unroll 1
+                for (uint32_t s = 0; T::BY_STEP && s < steps; s++) {
                     const uint32_t n = groups_in(s);
                     if constexpr (T::BY_STEP) {
                         arrived();
@@ -263,13 +311,6 @@ __global__ void __launch_bounds__((Tile<INT4, N, TMA>::THREADS), (Tile<INT4, N, 
                             else add(at, k + 1 == n);
                         }
                         sums.next();
-                    } else {
-#pragma unroll 1
-                        for (uint32_t k = 0; k < n; k++) {
-                            arrived();
-                            add(at_lanes + sums.at * T::SUM, true);
-                            sums.next();
-                        }
                     }
                 }
                 if (ranks == 1) {
@@ -360,13 +401,13 @@ __global__ void __launch_bounds__((Tile<INT4, N, TMA>::THREADS), (Tile<INT4, N, 
                 const uint32_t n = groups_in(step);
                 for (uint32_t g = 0; g < n; g++) {
                     if (!T::BY_STEP || g == 0) {
-                        wait(bars.sum_empty[sums.at], sums.parity ^ 1);
+                        wait(bars.sum_empty[sums.at], sums.parity);  // (filled to begin with: its first arrivals)
                         if (failed) break;
                         tmem_fence_after();
                     }
                     const uint32_t half = g << log_group >> 7, from = 2 * (g * parts & 3), group_a = from_a + half * (T::A_HALF >> 4) + from, group_b = from_b + half * (T::B_HALF >> 4) + from;
                     for (uint32_t k = 0; k < parts; k++)
-                        product_codes(one, tmem_u + sums.at * T::SUM + (T::BY_STEP ? g * N : 0), two_words(group_a + 2 * k, high), two_words(group_b + 2 * k, high), desc, k > 0);
+                        product_codes(one, tmem_u + sums.at * T::SUM + (T::BY_STEP ? g * N : 0), two_words(group_a + 2 * k, high), two_words(group_b + 2 * k, high), desc, true);
                     if (!T::BY_STEP || g + 1 == n) {
                         if (one) products_done(bar_of(bars.done[ends % 32]));
                         ends++;

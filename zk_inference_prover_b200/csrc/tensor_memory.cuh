@@ -35,6 +35,10 @@ __device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t* x) {
                  W8(x, 0), W8(x, 8), W8(x, 16), W8(x, 24) : "memory");
 }
 __device__ __forceinline__ void tmem_store8(uint32_t at, const uint32_t* x) { asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(at), W8(x, 0) : "memory"); }
+// The same word to sixteen columns of this thread's row.
+__device__ __forceinline__ void tmem_fill16(uint32_t at, uint32_t w) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %1, %1, %1, %1, %1, %1, %1, %1, %1, %1, %1, %1, %1, %1, %1};" ::"r"(at), "r"(w) : "memory");
+}
 #undef R8
 #undef W8
 
