@@ -22,7 +22,7 @@ struct ProductMaps {
 template <bool INT4, int N, bool TMA>
 struct Tile {
     static constexpr bool FILLED = INT4 || !TMA, RAW = INT4 && TMA;     // the weights' part of a stage is written by warps; from shared memory
-    static constexpr int EPI = N == 64 ? (INT4 ? 8 : 4) : N >= 128 ? 8 : 4, SETS = RAW ? (N == 128 ? 1 : 2) : 4;  // warps that read the sums; sets of four warps that write codes, in turn
+    static constexpr int EPI = N == 64 ? (INT4 ? 8 : 4) : N >= 128 ? 8 : 4, SETS = RAW ? (N == 128 ? 1 : 2) : INT4 ? 2 : 4;  // warps that read the sums; sets of four warps that write codes, in turn
     static constexpr int FIRST_FILLER = EPI + (INT4 ? 4 : 3), THREADS = 32 * (FILLED ? FIRST_FILLER + 4 * SETS : EPI + 2);
     // A step's codes, in halves of 128 that are a matrix each: what a step costs whatever its codes, waits above all, is some 600 cycles of each of the warps that it goes through.
     static constexpr int CODES = INT4 ? 256 : 128, HALVES = CODES / 128, A_HALF = 128 * 128, B_HALF = N * 128;
