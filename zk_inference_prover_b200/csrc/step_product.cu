@@ -15,7 +15,7 @@ constexpr int CHANNELS = 4, FEW_WARPS = 4;
 
 // VEC: all rows of x and of the weights start on 16-byte boundaries.
 template <bool INT4, int R, bool VEC>
-__global__ void __launch_bounds__(32 * FEW_WARPS, R == 1 ? 8 : R == 2 ? 6 : 4) product_few_kernel(const __grid_constant__ zkb_step_product_args a) {
+__global__ void __launch_bounds__(32 * FEW_WARPS, R == 1 ? 8 : 6) product_few_kernel(const __grid_constant__ zkb_step_product_args a) {
     __shared__ uint32_t joined[FEW_WARPS][R][CHANNELS];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint32_t c0 = blockIdx.x * CHANNELS, t0 = blockIdx.y * R;
