@@ -192,3 +192,28 @@ def test_rows_of_outputs_that_descend(ctx, zkb):
     ctx.step_gate(zkb.StepGate(x=xs.ptr, x_stride=xs.stride, out=out.data_ptr() + 49 * 128, out_type=INT8, out_scale=scale.data_ptr(), out_stride=-128, n_rows=50, width=128))
     done(ctx)
     check_out(out.flip(0), scale, "codes", x.double(), 0.0)
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "words", "f32"])
+@pytest.mark.parametrize("rows,vocab", [(3, 4097), (1, 100003), (400, 20011), (2, 50)])
+def test_logprobs_of_temperatures_near_zero(ctx, zkb, kind, rows, vocab):
+    """Scales so large that a step of the largest logit decides, up to the largest that is taken: the likeliest token, or those that tie, have everything."""
+    g = gen(rows + vocab)
+    x = 10 + 30 * torch.randn(rows, vocab, generator=g, device="cuda")
+    x[0, vocab // 3] = x[0, vocab // 2] = 200.0
+    x[:, vocab - 7] = -math.inf
+    ids = torch.tensor([[vocab // 3, vocab // 2, 0, vocab - 7]], device="cuda", dtype=torch.int32).expand(rows, -1).contiguous()
+    held, values = held_logits(x, kind, 1, 0)
+    few = slice(0, rows, -(-rows // 20))
+    for scale in (3e5, 3e7, 1e9, 2.0 ** 100):
+        got = answer(ctx, zkb, held, kind, ids, 4, scale)
+        check_answer(tuple(y[few] for y in got), values[few], ids[few], 4, scale)
+    # products that no float holds: what is below the largest logit has nothing
+    held, values = held_logits(torch.where(x > 0, x * 1e35, x), kind, 1, 0)
+    for scale in (1e6, 2.0 ** 100):
+        lp, entropy, top, top_lp = answer(ctx, zkb, held, kind, ids, 4, scale)
+        ties = (values == values.amax(-1, keepdim=True)).sum(-1).double()
+        assert bool(((entropy - ties.log()).abs() <= 2.0 ** -15 * ties.log()).all()) and bool(((top_lp[:, 0] + ties.log()).abs() <= 2.0 ** -15 * ties.log()).all())
+        assert bool((values.gather(1, top[:, :1].long()) == values.amax(-1, keepdim=True)).all())
+        assert not bool(torch.isnan(lp).any()) and bool((lp[1:] == -math.inf).sum() >= rows - 1)

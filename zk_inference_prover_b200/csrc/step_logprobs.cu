@@ -163,26 +163,29 @@ struct Logits {
                 leans = fma_both(w, d, leans);
             }
         rest = first_of(rests) + second_of(rests), lean = first_of(leans) + second_of(leans);
-        if (tokens && (less - low) * log2_scale < 200.f) {  // there is no number that far below: -infinity is told from the lowest one
+        // `low` leaves nothing where it is 200 or more below; it is not where there is no number that far below, where its step from `less` was rounded away, or where the product leaves 32
+        // bits. -infinity is then told from the lowest number, and a weight of zero has no product.
+        const float below = (less - (TYPE == ZKB_VALUE_BF16 ? bf16_low(low_bf16) : low)) * log2_scale;
+        if (tokens && !(below >= 200.f && below < INFINITY)) {
             rest = lean = 0.f;
 #pragma unroll
             for (int i = 0; i < N; i++)
 #pragma unroll
                 for (int y = 0; y < PER; y++) {
-                    const float x = value(i, y), d = (fmaxf(x, low) - less) * log2_scale, w = x > -INFINITY ? exp2_fast(d) : 0.f;
-                    rest += w, lean = fmaf(w, d, lean);
+                    const float d = (value(i, y) - less) * log2_scale, w = exp2_fast(d);
+                    rest += w, lean += w > 0.f ? w * d : 0.f;
                 }
         }
     }
     // The sum of w without the largest one's.
-    __device__ __forceinline__ float weigh_others(float less, float low, float log2_scale) const {
+    __device__ __forceinline__ float weigh_others(float less, float log2_scale) const {
         float rest = 0.f;
 #pragma unroll
         for (int i = 0; i < N; i++)
 #pragma unroll
             for (int y = 0; y < PER; y++) {
-                const float x = value(i, y), d = (fmaxf(x, low) - less) * log2_scale;
-                rest += x > -INFINITY && x != less ? exp2_fast(d) : 0.f;
+                const float x = value(i, y);
+                rest += x != less ? exp2_fast((x - less) * log2_scale) : 0.f;
             }
         return rest;
     }
@@ -331,7 +334,7 @@ __global__ void __launch_bounds__(512, 2) logprobs_kernel(const __grid_constant_
         uint32_t equal = 0;
         if (rest < 1.25f && s.tokens) {  // one token is likely: the sum without it, for all of its bits
             equal = 1;
-            rest = x.weigh_others(s.less, s.low, p.log2_scale);
+            rest = x.weigh_others(s.less, p.log2_scale);
 #pragma unroll
             for (int o = 16; o; o >>= 1) rest += __shfl_xor_sync(0xffffffffu, rest, o);
             if (lane == 0) sums[2][warp] = rest;
@@ -554,7 +557,7 @@ __global__ void __launch_bounds__(544, 2) logprobs_rows_kernel(const __grid_cons
         uint32_t equal = 0;
         if (rest < 1.25f && s.tokens) {  // one token is likely: the sum without it, for all of its bits
             equal = 1;
-            rest = x.weigh_others(s.less, s.low, p.log2_scale);
+            rest = x.weigh_others(s.less, p.log2_scale);
 #pragma unroll
             for (int o = 16; o; o >>= 1) rest += __shfl_xor_sync(0xffffffffu, rest, o);
             if (lane == 0) sums[2][warp] = rest;
