@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from test_step_layer import (INT8, TYPES, Rows, Weights, answer, check_answer, check_out, check_product, codes_of, held_logits, norm_reference, room, run_product, untouched)
+from test_step_layer import (INT8, TYPES, Rows, Weights, answer, check_answer, check_out, check_product, codes_of, held_logits, norm_reference, room, run_product, untouched, values_of)
 from test_step_values import done, gen
 
 gpu = pytest.mark.gpu
@@ -217,3 +217,25 @@ def test_logprobs_of_temperatures_near_zero(ctx, zkb, kind, rows, vocab):
         assert bool(((entropy - ties.log()).abs() <= 2.0 ** -15 * ties.log()).all()) and bool(((top_lp[:, 0] + ties.log()).abs() <= 2.0 ** -15 * ties.log()).all())
         assert bool((values.gather(1, top[:, :1].long()) == values.amax(-1, keepdim=True)).all())
         assert not bool(torch.isnan(lp).any()) and bool((lp[1:] == -math.inf).sum() >= rows - 1)
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["codes", "bf16", "words"])
+@pytest.mark.parametrize("width", [64, 777, 4096])
+def test_norms_whose_products_with_the_weights_are_tiny(ctx, zkb, kind, width):
+    """Small rows and small weights, with a norm that is a number all the same. (x^2 has a mean of 2^-80 about, and weights of 2^-100: products of 2^-140, norms of 2^-100.)"""
+    g = gen(width)
+    x = (torch.randn(5, width, generator=g, device="cuda") * 2.0 ** -40).bfloat16()
+    w = ((1 + torch.rand(width, generator=g, device="cuda")) * 2.0 ** -100).bfloat16()
+    full, got = room(kind, 5, width)
+    scale = torch.zeros(5, device="cuda")
+    torch.cuda.synchronize()
+    ctx.step_residual_norm(zkb.StepResidualNorm(x=x.data_ptr(), x_stride=width, weight=w.data_ptr(), out=got.data_ptr(), out_type=TYPES[kind], out_scale=scale.data_ptr() if kind == "codes" else 0,
+                                                out_stride=width, n_rows=5, width=width, eps=0.0))
+    done(ctx)
+    y = norm_reference(x, w, 0.0)
+    if kind == "codes":  # (in units of 2^-100: what is compared has absolute terms)
+        scale, y = scale.double() * 2.0 ** 100, y * 2.0 ** 100
+        check_out(got, scale, kind, y, 2.0 ** -18)
+    else:
+        assert bool(((values_of(got) - y).abs() <= (2.0 ** -8 + 2.0 ** -17) * y.abs()).all())

@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(V >= 4 ? 512 : 1024, V == 4 ? 2 : 1) rows_kern
         over_row(room[0], a.warps, ss, most);
         const float mean = ss / (float)a.width + a.eps;
         by = rsqrtf(mean);
-        if (!(mean > 0x1p-90f && mean < 0x1p120f && most < INFINITY)) {  // squares or products that 32 bits do not hold, or values that are no numbers: the same for the whole row
+        if (!(mean > 0x1p-90f && mean < 0x1p120f && most > 0x1p-80f && most < INFINITY)) {  // squares or products that 32 bits do not hold, or values that are no numbers: the same for the whole row
             double wide = 0.;
 #pragma unroll
             for (int v = 0; v < V; v++)
@@ -208,19 +208,21 @@ __global__ void __launch_bounds__(V >= 4 ? 512 : 1024, V == 4 ? 2 : 1) rows_kern
                 wide = 0.;
                 for (uint32_t i = 0; i < a.warps; i++) wide += wide_sm[i];
             }
-            const double root = rsqrt(wide / a.width + (double)a.eps);
-            most = 0.f, by = 1.f;
+            if (wide != 0.) {  // (a row of zeros is as it was)
+                const double root = rsqrt(wide / a.width + (double)a.eps);
+                most = 0.f, by = 1.f;
 #pragma unroll
-            for (int v = 0; v < V; v++)
+                for (int v = 0; v < V; v++)
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const uint32_t col = column_of<VEC>(v, i, threads, th);
-                    const double by_weight = a.weight && col < a.width ? (double)bf16_low(a.weight[col]) : 1.;
-                    y[v][i] = (float)((double)(i % 2 ? bf16_high(s[v][i / 2]) : bf16_low(s[v][i / 2])) * by_weight * root);
-                    if (col < a.width) most = larger_size(most, y[v][i]);
-                }
-            float none = 0.f;
-            over_row(room[1], a.warps, none, most);
+                    for (int i = 0; i < 8; i++) {
+                        const uint32_t col = column_of<VEC>(v, i, threads, th);
+                        const double by_weight = a.weight && col < a.width ? (double)bf16_low(a.weight[col]) : 1.;
+                        y[v][i] = (float)((double)(i % 2 ? bf16_high(s[v][i / 2]) : bf16_low(s[v][i / 2])) * by_weight * root);
+                        if (col < a.width) most = larger_size(most, y[v][i]);
+                    }
+                float none = 0.f;
+                over_row(room[1], a.warps, none, most);
+            }
         }
     }
     if (a.out_type != ZKB_VALUE_INT8) {
