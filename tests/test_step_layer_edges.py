@@ -239,3 +239,35 @@ def test_norms_whose_products_with_the_weights_are_tiny(ctx, zkb, kind, width):
         check_out(got, scale, kind, y, 2.0 ** -18)
     else:
         assert bool(((values_of(got) - y).abs() <= (2.0 ** -8 + 2.0 ** -17) * y.abs()).all())
+
+
+@gpu
+@pytest.mark.parametrize("kind,group,rows,n_out", [
+    # as many tiles as the GPU holds at once, and one more: of 32, 64 and 128 rows
+    ("int8", 0, 33, 18944), ("int8", 0, 64, 18945), ("int8", 0, 63, 19100), ("int8", 0, 65, 12673), ("int8", 0, 128, 12640), ("int8", 0, 256, 18944), ("int8", 0, 250, 18945), ("int8", 0, 513, 7681),
+    ("int4", 128, 33, 18945), ("int4", 32, 64, 9472), ("int4", 64, 65, 9473), ("int4", 128, 128, 9472), ("int4", 32, 129, 6273), ("int4", 64, 192, 6272)])
+@pytest.mark.parametrize("n_in,pad", [(256, 0), (208, 0), (163, 1)])
+def test_products_at_the_borders_between_tiles(ctx, zkb, kind, group, rows, n_out, n_in, pad):
+    g = gen(rows + n_out)
+    x, w, x_scale = codes_of(g, rows, n_in, pad), Weights(g, kind, n_out, n_in, group, pad), torch.rand(rows, generator=g, device="cuda") + 0.1
+    full, y = room("f32", rows, n_out, 1)
+    torch.cuda.synchronize()
+    run_product(ctx, zkb, x, x_scale, w, ("f32", y))
+    done(ctx)
+    check_product("f32", y, x, x_scale, w)
+    untouched(full, y, 0)
+
+
+@gpu
+@pytest.mark.parametrize("kind,group", [("int8", 0), ("int4", 32), ("int4", 128)])
+@pytest.mark.parametrize("n_in", [1024, 2816, 3000, 4096, 4224, 9000])
+def test_products_of_few_tiles_and_more_steps(ctx, zkb, kind, group, n_in):
+    """One row tile and a few outputs' tiles, with as many codes as are, and are not, spread over several thread blocks."""
+    g = gen(n_in)
+    for rows, n_out in ((17, 200), (40, 1000), (33, 4300), (128, 600)):
+        x, w, x_scale = codes_of(g, rows, n_in), Weights(g, kind, n_out, n_in, group), torch.rand(rows, generator=g, device="cuda") + 0.1
+        y = torch.zeros(rows, n_out, device="cuda")
+        torch.cuda.synchronize()
+        run_product(ctx, zkb, x, x_scale, w, ("f32", y))
+        done(ctx)
+        check_product("f32", y, x, x_scale, w)

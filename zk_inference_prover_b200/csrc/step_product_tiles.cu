@@ -14,6 +14,9 @@ namespace zk {
 //   Rows on other boundaries by the same warps.
 // Few rows leave the tensor cores idle and are bound by the weights' bytes: N is as small as the rows allow, two thread blocks share an SM, and the steps are spread over the thread
 // blocks of a cluster, which add up through each other's shared memory, each a share of the rows.
+// Measured: 4096 rows of 4096 x 14336 8-bit weights 174 to 182 us, 2.7 PFLOP/s (a tile's sums are read while the next tile's products run); 32 rows of 4096 x 28672 24 us, 5.0 TB/s; 2001 rows
+// of 4096 x 6144 4-bit weights with groups of 128 118 us, 850 TFLOP/s: there each group's 128 x 128 sums pass through registers, some 2700 warp instructions an SM and group of a tile,
+// codes and sums, against 256 cycles of the tensor cores, so the rate of instructions bounds it (59 % of all cycles issue one).
 struct ProductMaps {
     CUtensorMap w, x;
 };
@@ -23,12 +26,14 @@ template <bool INT4, int N, bool TMA>
 struct Tile {
     static constexpr bool FILLED = INT4 || !TMA, RAW = INT4 && TMA;     // the weights' part of a stage is written by warps; from shared memory
     static constexpr int EPI = N == 64 ? (INT4 ? 8 : 4) : N >= 128 ? 8 : 4, SETS = RAW ? (N == 128 ? 1 : 2) : INT4 ? 2 : 4;  // warps that read the sums; sets of four warps that write codes, in turn
+    // (as many sets as leave the registers in place: 1193 rows of 6744 x 1342 8-bit codes on odd boundaries 122 us by 4 sets and 167 by 2; 2001 of 4097 x 6145 4-bit ones 527 by 2 and 1532 by 4)
     static constexpr int FIRST_FILLER = EPI + (INT4 ? 4 : 3), THREADS = 32 * (FILLED ? FIRST_FILLER + 4 * SETS : EPI + 2);
     // A step's codes, in halves of 128 that are a matrix each: what a step costs whatever its codes, waits above all, is some 600 cycles of each of the warps that it goes through.
     static constexpr int CODES = INT4 ? 256 : 128, HALVES = CODES / 128, A_HALF = 128 * 128, B_HALF = N * 128;
     static constexpr int A = HALVES * A_HALF, B = HALVES * B_HALF, STAGE = RAW ? A : A + B, RAW_BYTES = 128 * CODES / 2;
-    static constexpr int BLOCKS = N <= 64 && !FILLED ? 2 : 1;           // thread blocks an SM
-    static constexpr int JOIN = N <= 64 ? N * 512 : 0;                  // a cluster's sums
+    // thread blocks an SM (4-bit weights: sixteen rows of 4096 x 32000 29 us by one and 45 by two, whose registers go to memory)
+    static constexpr int BLOCKS = N <= 64 && !FILLED ? 2 : 1;
+    static constexpr int JOIN = N <= (INT4 ? 64 : 32) ? N * 512 : 0;                 // a cluster's sums
     static constexpr int RAWS = !RAW ? 0 : N <= 32 ? 4 : 3, XS = !RAW ? 0 : N == 16 ? 4 : N == 32 ? 3 : 2;
     static constexpr int SCALES = INT4 ? 4 : 0, SCALE_BYTES = 128 * 16; // eight groups' scales of a tile's outputs
     static constexpr int ROOM = (BLOCKS == 2 ? 112 * 1024 : 216 * 1024) - JOIN - RAWS * RAW_BYTES - XS * B - SCALES * SCALE_BYTES;
@@ -632,10 +637,12 @@ static cudaError_t launch_variant(zkb_ctx* ctx, const zkb_step_product_args& a, 
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM);
     if (e != cudaSuccess) return e;
     const uint32_t row_tiles = (a.n_rows + N - 1) / N, tiles = row_tiles * ((a.n_out + 127) / 128), steps = (a.n_in + T::CODES - 1) / T::CODES;
-    // Few tiles are spread over clusters, while all of them are on the GPU at once and each thread block has two steps.
+    // Few tiles are spread over clusters, while all of them are on the GPU at once, with an SM for each thread block where a share is short: a cluster costs some 4 us, as much as 6 steps of 4-bit
+    // weights or 12 of 8-bit ones. By 1, 2, 4 and 8 thread blocks a tile, in us: 20 rows of 8192 x 1024 8-bit (4-bit) weights 22, 16, 12, 9 (29, 21, 15, 11.5), 17 of 4096 x 4096 14.1, 13.1, 10.8
+    // (18.6, 15.9, 13.0); by 1 and 2, 128 rows of 14336 x 4096 35 and 27, of 4096 x 4096 14.3 and 14.9; 64 rows of 1024 x 4096 8.2 by 1 and 10.2 by 4.
     uint32_t ranks = 1;
-    if (T::JOIN > 0)
-        while (ranks < 16 && ranks < N && tiles <= T::BLOCKS * clusters_at_once(2 * ranks) && steps >= (INT4 ? 2 : 4) * ranks) ranks *= 2;
+    if (T::JOIN > 0 && steps >= (INT4 ? 12 : 24))
+        while (ranks < 16 && ranks < N && tiles <= (!INT4 && steps > 32 * ranks ? 2 : 1) * clusters_at_once(2 * ranks) && steps >= (INT4 ? 2 : 4) * ranks) ranks *= 2;
     return launch_clusters(ranks, [&](uint32_t n) {
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -660,10 +667,23 @@ static cudaError_t launch_rows_of(zkb_ctx* ctx, const zkb_step_product_args& a) 
 
 template <bool INT4>
 cudaError_t launch_tiles(zkb_ctx* ctx, const zkb_step_product_args& a) {
-    // As many rows a tile as there are, up to 256 (4-bit weights 128: a group's sums are kept in registers); fewer while that leaves SMs without a tile.
-    uint32_t n = 16;
-    while (n < (INT4 ? 128u : 256u) && n < a.n_rows) n *= 2;
-    while (n > 32 && (uint64_t)((a.n_rows + n - 1) / n) * ((a.n_out + 127) / 128) < 120) n /= 2;
+    // Rows a tile: the fewest that leave no more tiles than are on the GPU at once, of those that the rows need and the kernels have (a group's sums of 4-bit weights are kept in registers: up to
+    // 128). Of 8-bit weights that is two tiles an SM: they share it up to 64 rows, and of 128 rows two take less than one of 256. In us:
+    //   8-bit, n_in 4096, rows x n_out       32     64    128    256       4-bit, groups of 128     32     64    128
+    //      256 x 4096                      16.3   18.3   16.5   23.2          33 x 14336          31.8   21.0
+    //      128 x 14336                     25.1   21.5   18.8                128 x 8192           31.6   20.8   24.4
+    //      256 x 14336                     39.9   30.9   25.2   27.5         128 x 14336          56.7   34.4   25.1
+    //      512 x 14336                     63.7   49.5   40.3   35.6         160 x 8192           44.4   34.4   24.7
+    // 32 rows of more than 32 are not taken of 4-bit weights: the best by a tenth at 128 x 1024 (12.4 and 14.1), the worst by a fifth at 64 x 4096 with groups of 32 (25.3 and 20.1). 64 of 8-bit
+    // weights are for up to 64 rows only (64 x 28672: 29.0, 26.2 and 28.3 by 32, 64 and 128). On odd boundaries an SM has one tile of each size (700 x 4097 x 4095: 104 by 128, 84 by 256).
+    const uint64_t out_tiles = (a.n_out + 127) / 128;
+    const bool pairs = !INT4 && aligned_to(a.x, 16) && aligned_to(a.w, 16) && a.x_stride % 16 == 0 && a.w_stride % 16 == 0;
+    auto at_once = [&](uint32_t n) { return (a.n_rows + n - 1) / n * out_tiles <= (pairs ? 296 : 148); };
+    uint32_t n = INT4 ? 128 : 256;
+    if (a.n_rows <= 16) n = 16;
+    else if (a.n_rows <= 32 || (!INT4 && at_once(32))) n = 32;
+    else if (a.n_rows <= 64 || (INT4 && at_once(64))) n = 64;
+    else if (a.n_rows <= 128 || at_once(128)) n = 128;
     if (n == 16) return launch_rows_of<INT4, 16>(ctx, a);
     if (n == 32) return launch_rows_of<INT4, 32>(ctx, a);
     if (n == 64) return launch_rows_of<INT4, 64>(ctx, a);
