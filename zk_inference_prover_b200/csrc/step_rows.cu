@@ -8,7 +8,9 @@
 namespace zk {
 
 // Both calls are a pass over rows: values in, one number of the whole row (the mean of squares, the largest value), values out. A row stays in registers between
-// its reading and its writing, V times eight values a thread, so nothing is read twice: bound by the bytes.
+// its reading and its writing, V times eight values a thread, so nothing is read twice: bound by the bytes, and by a row's one barrier, which two thread blocks an SM cover for one another.
+// Measured: the norm of 8191 rows of 4096 with the residual's sum and codes 38 us, 6.15 TB/s; of one row 2.9, a launch and two trips to memory; the gate of 4096 rows of 14336 to codes 58 us,
+// 5.0 TB/s (two sixteens of bytes of each input and thread are as much as its registers hold under way).
 struct RowsArgs {
     const void* x;
     const void* other;  // the residual stream, or the gate
@@ -261,6 +263,9 @@ __global__ void __launch_bounds__(V >= 4 ? 512 : 1024, V == 4 ? 2 : 1) rows_kern
 
 template <bool GATE>
 static cudaError_t launch_rows(zkb_ctx* ctx, RowsArgs a, bool x_word, bool vec) {
+    // Few rows: a row over many warps, for the time of one; many: four times eight values a thread, for the bytes under way; a row of up to 512 values to each warp. In us by 1, 2, 4 and 8 times
+    // eight values a thread: norms of 1 x 4096 2.9, 2.8, 3.4; of 592 x 4096 7.3, 5.8, 6.3; of 8191 x 4096 63, 45, 38; of 8191 x 512 10, 8.5, 9.9; gates of 32 x 14336 -, 4.1, 4.3, 4.7, of
+    // 4096 x 14336 -, 83, 58, 67, of 4096 x 16384 -, 93, 63, 68.
     const uint32_t eights = (a.width + 7) / 8;
     uint32_t v = 4;
     if (eights <= 32 || (a.n_rows < 148 * 4 && eights <= 1024)) v = 1;
