@@ -19,13 +19,13 @@ template <bool INT4, int R, bool VEC>
 __global__ void __launch_bounds__(32 * FEW_WARPS, R == 1 ? 8 : 6) product_few_kernel(const __grid_constant__ zkb_step_product_args a) {
     __shared__ uint32_t joined[FEW_WARPS][R][CHANNELS];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const uint32_t c0 = blockIdx.x * CHANNELS, t0 = blockIdx.y * R;
+    const uint32_t c0 = blockIdx.x * CHANNELS;
     constexpr int CODES = INT4 ? 32 : 16, XS = CODES / 16;  // codes of 16 bytes; 16s of x to them
     const int n_in = (int)a.n_in, bytes = INT4 ? (n_in + 1) / 2 : n_in;
     const int64_t w_row = INT4 ? a.w_stride / 2 : a.w_stride;
     const int8_t *const w_lo = static_cast<const int8_t*>(a.w), *const w_hi = w_lo + (a.n_out - 1) * w_row + bytes, *const x_hi = a.x + (int64_t)(a.n_rows - 1) * a.x_stride + n_in;
     auto w_of = [&](int c) { return w_lo + (int64_t)min(c0 + c, a.n_out - 1) * w_row; };
-    auto x_of = [&](int r) { return a.x + (int64_t)min(t0 + r, a.n_rows - 1) * a.x_stride; };
+    auto x_of = [&](int r) { return a.x + (int64_t)min((uint32_t)r, a.n_rows - 1) * a.x_stride; };
     const uint32_t log_group = INT4 ? 31 - __clz(a.group) : 0;
     int sum[CHANNELS][R] = {};
     float part[CHANNELS][R] = {};
@@ -113,77 +113,73 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, R == 1 ? 8 : 6) product_few_ke
         }
     __syncthreads();
     const uint32_t c = threadIdx.x % CHANNELS, r = threadIdx.x / CHANNELS;
-    if (r < R && c0 + c < a.n_out && t0 + r < a.n_rows) {
+    if (r < R && c0 + c < a.n_out && r < a.n_rows) {
         uint32_t y = joined[0][r][c];
 #pragma unroll
         for (int w = 1; w < FEW_WARPS; w++) y = INT4 ? __float_as_uint(__uint_as_float(y) + __uint_as_float(joined[w][r][c])) : y + joined[w][r][c];
-        const int64_t at = (int64_t)(t0 + r) * a.out_stride + c0 + c;
+        const int64_t at = (int64_t)r * a.out_stride + c0 + c;
         if (a.out_type == ZKB_VALUE_INT32) static_cast<uint32_t*>(a.out)[at] = y;
-        else store_value(a.out, at, a.out_type, INT4 ? __uint_as_float(y) * a.x_scale[t0 + r] : (float)(int)y * (a.x_scale[t0 + r] * static_cast<const float*>(a.w_scale)[c0 + c]));
+        else store_value(a.out, at, a.out_type, INT4 ? __uint_as_float(y) * a.x_scale[r] : (float)(int)y * (a.x_scale[r] * static_cast<const float*>(a.w_scale)[c0 + c]));
     }
 }
 
-template <bool INT4, bool VEC>
-static cudaError_t launch_few(zkb_ctx* ctx, const zkb_step_product_args& a) {
+template <bool INT4>
+static cudaError_t launch_few(zkb_ctx* ctx, const zkb_step_product_args& a, bool vec) {
     const uint32_t grid = (a.n_out + CHANNELS - 1) / CHANNELS;
-    auto launch = [&](auto kernel, uint32_t r) { kernel<<<dim3(grid, (a.n_rows + r - 1) / r), 32 * FEW_WARPS, 0, ctx->stream>>>(a); };
-    if (a.n_rows == 1) launch(product_few_kernel<INT4, 1, VEC>, 1);
-    else launch(product_few_kernel<INT4, 2, VEC>, 2);
+    if (a.n_rows == 2) product_few_kernel<INT4, 2, true><<<grid, 32 * FEW_WARPS, 0, ctx->stream>>>(a);  // (on other boundaries: below)
+    else if (vec) product_few_kernel<INT4, 1, true><<<grid, 32 * FEW_WARPS, 0, ctx->stream>>>(a);
+    else product_few_kernel<INT4, 1, false><<<grid, 32 * FEW_WARPS, 0, ctx->stream>>>(a);
     return cudaGetLastError();
 }
 
 // ---- up to sixteen rows ----------------------------------------------------------------------------------------------------------------
 // Codes from memory into the registers that multiply them: m16n8k32 with 16 outputs of the weights as its long side and eight rows of x as the short one. Which code is which k of a product
-// is free as long as both sides agree, so a lane takes the codes that it loads side by side: of 8-bit weights 16 of an output's 64, of 4-bit ones a quarter of a group, whose low and high
-// halves of bytes are 16 times the even and the odd codes. A warp has 32 outputs and every so manieth run of codes; a thread block's warps add up through shared memory. Nothing waits
-// for anything but its own loads, three runs of which are under way. Sixteen rows of 14336 x 4096 4-bit (8-bit) codes: 17.5 (16.1) us, 1.8 (3.7) TB/s: loads of 8 bytes, x's among them, by a lane
-// take turns in the first cache (62 % of its rate). Sixteen-byte loads of 4-bit weights leave no registers for the runs under way: 21 to 23 us.
+// is free as long as both sides agree, so a lane takes the 16 bytes that it loads side by side; low and high halves of 4-bit codes' bytes are 16 times the even and the odd codes. A warp has 32
+// outputs and every so manieth run of codes; a thread block's warps add up through shared memory. Nothing waits for anything but its own loads, two or three runs of which are under way.
+// Sixteen rows of 14336 x 4096 codes: 4-bit in groups of 128 (64, 32) 13.6 us (15.0, 19.7), 8-bit 16.1, 3.7 TB/s: what bounds it is the first cache, whose lines the eight rows of a load take one
+// after the other, x's among them in every thread block (with 8 bytes of 4-bit weights a lane 17.6), and registers: more runs under way go to memory.
 __device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 constexpr int SOME_OUTPUTS = 32;  // of a warp
 
-// T: eights of rows. PARTS: groups in a run of 4-bit codes: each is a product of its own, with zeros for the codes of the lanes that have the others.
-template <bool INT4, int T, int PARTS, bool VEC>
+// T: eights of rows. GROUP: of 4-bit codes; 0: 8-bit ones. The groups of a run are products of their own. Of 64 codes: lanes exchange halves of their codes, so that each has a quarter
+// of either group. Of 32: each lane's codes are one group's, and the others' are zeros in its product.
+template <int GROUP, int T, bool VEC>
 __global__ void __launch_bounds__(512, 1) product_some_kernel(const __grid_constant__ zkb_step_product_args a) {
     extern __shared__ uint32_t some_sm[];  // [warp][row][output]
-    constexpr int RUN = 64, W = INT4 ? 2 : 4, D = 3;  // codes of a run, of which a lane has W words of weights and four of x; runs on their way
+    constexpr bool INT4 = GROUP > 0, LONG = GROUP >= 64;
+    constexpr int RUN = LONG ? 128 : 64, W = INT4 ? RUN / 32 : 4, XS = RUN / 64, PARTS = !INT4 || GROUP == 128 ? 1 : 2;  // codes of a run, of which a lane has W words of weights and XS sixteens of x
+    constexpr int D = LONG ? 2 : 3;  // runs on their way
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, g = lane >> 2, q = lane & 3;
     const uint32_t c0 = blockIdx.x * SOME_OUTPUTS, n_in = a.n_in, whole = n_in / RUN;
     const int64_t w_row = INT4 ? a.w_stride / 2 : a.w_stride;
     const int8_t* w[2][2];
     const int8_t* x[T];
-    const uint16_t* s[2][2];
 #pragma unroll
     for (int m = 0; m < 2; m++)
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             const int64_t c = min(c0 + m * 16 + h * 8 + g, a.n_out - 1);
             w[m][h] = static_cast<const int8_t*>(a.w) + c * w_row + q * (4 * W);
-            s[m][h] = static_cast<const uint16_t*>(a.w_scale) + (INT4 ? c * a.w_scale_stride : 0);
         }
+    constexpr int X_NEXT = GROUP == 128 ? 16 : 64;  // from a lane's first sixteen of x to its second
+    const int x_first = GROUP == 128 ? q * 32 : GROUP == 64 ? (q & 1) * 32 + (q >> 1) * 16 : q * 16;
 #pragma unroll
-    for (int n = 0; n < T; n++) x[n] = a.x + (int64_t)min((uint32_t)(n * 8 + g), a.n_rows - 1) * a.x_stride + q * 16;
-    const uint32_t log_group = INT4 ? 31 - __clz(a.group) : 0;
+    for (int n = 0; n < T; n++) x[n] = a.x + (int64_t)min((uint32_t)(n * 8 + g), a.n_rows - 1) * a.x_stride + x_first;
     struct Run {
-        uint32_t w[2][2][W], x[T][4], s[2][2];
+        uint32_t w[2][2][W], x[T][4 * XS], s;
     };
-    auto scales = [&](uint32_t run, Run& r) {
-        if constexpr (INT4) {
-#pragma unroll
-            for (int m = 0; m < 2; m++)
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-#pragma unroll
-                    for (int p = 0; p < PARTS; p++) {
-                        const uint32_t v = run * RUN + p * (RUN / PARTS) < n_in ? s[m][h][(run * RUN >> log_group) + p] : 0u;
-                        r.s[m][h] = p ? r.s[m][h] | v << 16 : v;
-                    }
-                }
-        }
+    // A lane has the scales of a run of one output, and asks the others for those that it needs.
+    const uint16_t* const s = static_cast<const uint16_t*>(a.w_scale) + (INT4 ? (int64_t)min(c0 + lane, a.n_out - 1) * a.w_scale_stride : 0);
+    const bool pairs = PARTS == 2 && (reinterpret_cast<uintptr_t>(a.w_scale) & 3) == 0 && (a.n_out == 1 || a.w_scale_stride % 2 == 0);
+    auto scales = [&](uint32_t run) {
+        if (PARTS == 1) return (uint32_t)s[run];
+        if (pairs && run * RUN + RUN <= n_in) return *reinterpret_cast<const uint32_t*>(s + run * 2);
+        return (uint32_t)s[run * 2] | (run * RUN + RUN / 2 < n_in ? (uint32_t)s[run * 2 + 1] << 16 : 0u);
     };
-    auto put4 = [](uint32_t (&to)[4], const uint4& v) { to[0] = v.x, to[1] = v.y, to[2] = v.z, to[3] = v.w; };
+    auto put4 = [](uint32_t* to, const uint4& v) { to[0] = v.x, to[1] = v.y, to[2] = v.z, to[3] = v.w; };
     auto put_w = [&](uint32_t (&to)[W], const uint4& v) {
         to[0] = v.x, to[1] = v.y;
         if constexpr (W == 4) to[2] = v.z, to[3] = v.w;
@@ -205,20 +201,42 @@ __global__ void __launch_bounds__(512, 1) product_some_kernel(const __grid_const
                 }
             }
 #pragma unroll
-        for (int n = 0; n < T; n++) {
-            const int8_t *const p = x[n] + run * RUN, *const hi = a.x + (int64_t)(a.n_rows - 1) * a.x_stride + n_in;
-            put4(r.x[n], VEC ? __ldg(reinterpret_cast<const uint4*>(p)) : fetched16(fetch16(p, a.x, hi), p, a.x, hi));
-        }
-        scales(run, r);
+        for (int n = 0; n < T; n++)
+#pragma unroll
+            for (int k = 0; k < XS; k++) {
+                const int8_t *const p = x[n] + run * RUN + k * X_NEXT, *const hi = a.x + (int64_t)(a.n_rows - 1) * a.x_stride + n_in;
+                put4(&r.x[n][4 * k], VEC ? __ldg(reinterpret_cast<const uint4*>(p)) : fetched16(fetch16(p, a.x, hi), p, a.x, hi));
+            }
+        if constexpr (INT4) r.s = scales(run);
     };
     float acc[2][T][4] = {};
     int sum[2][T][4] = {};
-    auto multiply = [&](const Run& r) {
+    auto multiply = [&](Run& r) {
+        uint32_t by[2][2];
+        if constexpr (INT4) {
+#pragma unroll
+            for (int m = 0; m < 2; m++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) by[m][h] = __shfl_sync(0xffffffffu, r.s, m * 16 + h * 8 + g);
+        }
+        if constexpr (GROUP == 64) {  // lanes 0 and 1 have the first group's codes, 2 and 3 the second's
+#pragma unroll
+            for (int m = 0; m < 2; m++)
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int y = 0; y < 2; y++) {
+                        uint32_t &lo = r.w[m][h][y], &hi = r.w[m][h][2 + y];
+                        const uint32_t got = __shfl_xor_sync(0xffffffffu, q < 2 ? hi : lo, 2);
+                        if (q < 2) hi = got;
+                        else lo = got;
+                    }
+        }
 #pragma unroll
         for (int n = 0; n < T; n++) {
-            uint32_t b[4];
+            uint32_t b[4 * XS];
 #pragma unroll
-            for (int i = 0; i < 4; i += 2) {
+            for (int i = 0; i < 4 * XS; i += 2) {
                 b[i] = INT4 ? __byte_perm(r.x[n][i], r.x[n][i + 1], 0x6420) : r.x[n][i];
                 b[i + 1] = INT4 ? __byte_perm(r.x[n][i], r.x[n][i + 1], 0x7531) : r.x[n][i + 1];
             }
@@ -227,12 +245,15 @@ __global__ void __launch_bounds__(512, 1) product_some_kernel(const __grid_const
                 if constexpr (INT4) {
 #pragma unroll
                     for (int p = 0; p < PARTS; p++) {
-                        const uint32_t mine = PARTS == 1 || q / (4 / PARTS) == p ? 0xffffffffu : 0u;
+                        const uint32_t mine = GROUP != 32 || q / 2 == p ? 0xffffffffu : 0u;
+                        constexpr int WORDS = GROUP == 64 ? 2 : W;  // of a part
                         int c[4] = {};
 #pragma unroll
-                        for (int i = 0; i < W; i++)
+                        for (int y = 0; y < WORDS; y++) {
+                            const int i = (GROUP == 64 ? 2 * p : 0) + y;
                             mma_s8(c, r.w[m][0][i] << 4 & 0xf0f0f0f0u, r.w[m][1][i] << 4 & 0xf0f0f0f0u, r.w[m][0][i] & 0xf0f0f0f0u, r.w[m][1][i] & 0xf0f0f0f0u, b[2 * i] & mine, b[2 * i + 1] & mine);
-                        const float lo = (p ? bf16_high(r.s[m][0]) : bf16_low(r.s[m][0])) * 0.0625f, hi = (p ? bf16_high(r.s[m][1]) : bf16_low(r.s[m][1])) * 0.0625f;
+                        }
+                        const float lo = (p ? bf16_high(by[m][0]) : bf16_low(by[m][0])) * 0.0625f, hi = (p ? bf16_high(by[m][1]) : bf16_low(by[m][1])) * 0.0625f;
 #pragma unroll
                         for (int i = 0; i < 4; i++) acc[m][n][i] = fmaf((float)c[i], i < 2 ? lo : hi, acc[m][n][i]);
                     }
@@ -262,8 +283,10 @@ __global__ void __launch_bounds__(512, 1) product_some_kernel(const __grid_const
 #pragma unroll
             for (int h = 0; h < 2; h++) put_w(r[0].w[m][h], some_bytes(w[m][h] + whole * (16 * W), (INT4 ? (left + 1) / 2 : left) - q * (4 * W)));
 #pragma unroll
-        for (int n = 0; n < T; n++) put4(r[0].x[n], some_bytes(x[n] + whole * RUN, left - q * 16));
-        scales(whole, r[0]);
+        for (int n = 0; n < T; n++)
+#pragma unroll
+            for (int k = 0; k < XS; k++) put4(&r[0].x[n][4 * k], some_bytes(x[n] + whole * RUN + k * X_NEXT, left - x_first - k * X_NEXT));
+        if constexpr (INT4) r[0].s = scales(whole);
         multiply(r[0]);
     }
 #pragma unroll
@@ -288,18 +311,18 @@ __global__ void __launch_bounds__(512, 1) product_some_kernel(const __grid_const
     }
 }
 
-template <bool INT4, int T, int PARTS>
+template <int GROUP, int T>
 static cudaError_t launch_some(zkb_ctx* ctx, const zkb_step_product_args& a, bool vec) {
     // Eight warps let two thread blocks share an SM; where there is one for each, it has sixteen. Eight rows of 4096 x 4096 codes: 8.7 us by 8 and 6.7 by 16; of 4096 x 6144 9.7 and 10.7.
     const uint32_t grid = (a.n_out + SOME_OUTPUTS - 1) / SOME_OUTPUTS, warps = grid <= 148 ? 16 : 8;
     const size_t room = (size_t)warps * 8 * T * SOME_OUTPUTS * 4;
-    if (vec) product_some_kernel<INT4, T, PARTS, true><<<grid, 32 * warps, room, ctx->stream>>>(a);
-    else product_some_kernel<INT4, T, PARTS, false><<<grid, 32 * warps, room, ctx->stream>>>(a);
+    if (vec) product_some_kernel<GROUP, T, true><<<grid, 32 * warps, room, ctx->stream>>>(a);
+    else product_some_kernel<GROUP, T, false><<<grid, 32 * warps, room, ctx->stream>>>(a);
     return cudaGetLastError();
 }
-template <bool INT4, int PARTS>
+template <int GROUP>
 static cudaError_t launch_some(zkb_ctx* ctx, const zkb_step_product_args& a, bool vec) {
-    return a.n_rows <= 8 ? launch_some<INT4, 1, PARTS>(ctx, a, vec) : launch_some<INT4, 2, PARTS>(ctx, a, vec);
+    return a.n_rows <= 8 ? launch_some<GROUP, 1>(ctx, a, vec) : launch_some<GROUP, 2>(ctx, a, vec);
 }
 
 }  // namespace zk
@@ -325,18 +348,26 @@ extern "C" int zkb_step_product(zkb_ctx* ctx, const zkb_step_product_args* args)
     ProfScope prof(ctx, "step_product_kernel");
     const int64_t w_row = int4 ? a.w_stride / 2 : a.w_stride;
     const bool vec = aligned_to(a.x, 16) && aligned_to(a.w, 16) && (a.n_rows == 1 || a.x_stride % 16 == 0) && (a.n_out == 1 || w_row % 16 == 0);
-    // By what each was measured to take, in us: one row of 4096 x 4096 4-bit (8-bit) codes 4.4 (5.3) by dp4a and 6.4 (6.8) by a warp's products, two rows 6.2 (6.6) and 6.4 (6.9), four 6.9 (7.2) and
-    // 6.5 (6.8). Eight of 4096 x 4096 5 to 7 by a warp's products and 11 (9) by tiles, sixteen of 14336 x 4096 17 (18) and 18 to 22 (16), of 4096 x 32000 35 (37) and 29 (25): tiles are
-    // better at more than 32 MB of weights. Rows on odd boundaries: 7 of 1637 x 9144 13 (14) and 14 (15), 12 of 10344 x 6512 69 (70) and 37 (46).
-    const uint64_t bytes = (uint64_t)a.n_out * (int4 ? a.n_in / 2 : a.n_in);
-    if (a.n_rows > 2 && a.n_rows <= 16 && bytes <= (32u << 20)) {
-        ZKB_CUDA(ctx, (!int4 ? launch_some<false, 1>(ctx, a, vec) : a.group > 32 ? launch_some<true, 1>(ctx, a, vec) : launch_some<true, 2>(ctx, a, vec)));
+    // By what each was measured to take, in us (4-bit codes in groups of 128, of 64, of 32; 8-bit ones):
+    //                                   dp4a                     a warp's products          tiles
+    //   1 row of 4096 x 4096            4.4  4.3  4.4  5.5       5.4  6.1  7.3  6.9
+    //   2 rows of 4096 x 4096           6.2  6.1  6.2  6.7       5.4  6.2  7.3  6.9
+    //   2 rows of 14336 x 4096          14   14   14   15        11.2 11.9 17.5 16.9
+    //   1 of 1637 x 9144, odd rows      12.2 12.3 12.3 12.2      9.9  10.0 13.3 13.8   (of 10344 x 6512: 25 and 38)
+    //   2 of 1637 x 9144, odd rows      19.8 19.9 19.9 16.3      9.9  10.2 13.3 13.9
+    //   8 rows of 4096 x 4096                                    5.6  6.2  7.4  6.9         11.2 12.1 14.1 9.0
+    //   16 rows of 4096 x 14336                                  15.6 18.1 22.8 19.6        18.1 21.6 27.7 15.3
+    //   16 rows of 4096 x 32000                                  28.8 33.2 43.2 36.9        29.4 36.1 48.2 25.4
+    const uint64_t bytes = (uint64_t)a.n_out * a.n_in;
+    const bool some = a.n_rows > 2 ? a.n_rows <= 16 && (int4 || bytes <= (32u << 20)) : a.n_rows == 2 && (!vec || a.group == 128);
+    if (some) {
+        ZKB_CUDA(ctx, (!int4 ? launch_some<0>(ctx, a, vec) : a.group == 32 ? launch_some<32>(ctx, a, vec) : a.group == 64 ? launch_some<64>(ctx, a, vec) : launch_some<128>(ctx, a, vec)));
         return ZKB_OK;
     }
     if (a.n_rows > 2) {
         ZKB_CUDA(ctx, int4 ? launch_tiles<true>(ctx, a) : launch_tiles<false>(ctx, a));
         return ZKB_OK;
     }
-    ZKB_CUDA(ctx, int4 ? (vec ? launch_few<true, true>(ctx, a) : launch_few<true, false>(ctx, a)) : (vec ? launch_few<false, true>(ctx, a) : launch_few<false, false>(ctx, a)));
+    ZKB_CUDA(ctx, int4 ? launch_few<true>(ctx, a, vec) : launch_few<false>(ctx, a, vec));
     return ZKB_OK;
 }

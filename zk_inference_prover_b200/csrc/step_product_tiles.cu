@@ -31,15 +31,15 @@ struct Tile {
     // A step's codes, in halves of 128 that are a matrix each: what a step costs whatever its codes, waits above all, is some 600 cycles of each of the warps that it goes through.
     static constexpr int CODES = INT4 ? 256 : 128, HALVES = CODES / 128, A_HALF = 128 * 128, B_HALF = N * 128;
     static constexpr int A = HALVES * A_HALF, B = HALVES * B_HALF, STAGE = RAW ? A : A + B, RAW_BYTES = 128 * CODES / 2;
-    // thread blocks an SM (4-bit weights: sixteen rows of 4096 x 32000 29 us by one and 45 by two, whose registers go to memory)
+    // thread blocks an SM (one where codes are written by warps: two leave too few registers, sixteen rows of 4096 x 32000 4-bit codes 45 us and 29 by one)
     static constexpr int BLOCKS = N <= 64 && !FILLED ? 2 : 1;
     static constexpr int JOIN = N <= (INT4 ? 64 : 32) ? N * 512 : 0;                 // a cluster's sums
-    static constexpr int RAWS = !RAW ? 0 : N <= 32 ? 4 : 3, XS = !RAW ? 0 : N == 16 ? 4 : N == 32 ? 3 : 2;
+    static constexpr int RAWS = !RAW ? 0 : N == 32 ? 4 : 3, XS = !RAW ? 0 : N == 32 ? 3 : 2;
     static constexpr int SCALES = INT4 ? 4 : 0, SCALE_BYTES = 128 * 16; // eight groups' scales of a tile's outputs
     static constexpr int ROOM = (BLOCKS == 2 ? 112 * 1024 : 216 * 1024) - JOIN - RAWS * RAW_BYTES - XS * B - SCALES * SCALE_BYTES;
     static constexpr int STAGES = ROOM / STAGE < 6 ? ROOM / STAGE : 6;
     // The sums of a tile of 8-bit weights, or of 4-bit weights' groups: of a step's all at once where they have room twice.
-    static constexpr bool BY_STEP = INT4 && N <= 32;
+    static constexpr bool BY_STEP = INT4 && N == 32;
     static constexpr int SUMS = !INT4 || BY_STEP ? 2 : 4, SUM = BY_STEP ? 8 * N : N, COLUMNS = SUMS * SUM < 32 ? 32 : SUMS * SUM;
     // A thread block never waits for tensor memory: those that fit an SM's shared memory together (this kernel's variants and attention's, which take all columns and 121 KB) fit its
     // 512 columns. Clusters that each hold what another waits for would wait forever.
@@ -251,25 +251,6 @@ __global__ void __launch_bounds__((Tile<INT4, N, TMA>::THREADS), (Tile<INT4, N, 
                     k8++;
                     return s * 0.0625f;  // (the codes are 16 times themselves)
                 };
-                // the sums of two groups of sixteen rows
-                auto add_two = [&](uint32_t at, bool last) {
-                    const float by0 = next_scale(), by1 = next_scale();
-                    const uint64_t less = both(-12582912.f, -12582912.f);
-                    uint32_t x[32];
-                    tmem_load32(at, x);
-                    tmem_loaded(x);
-                    tmem_fill16(at, SUM_ZERO), tmem_fill16(at + 16, SUM_ZERO);
-                    if (last) {
-                        tmem_stored();
-                        tmem_fence_before();
-                        arrive(bars.sum_empty[sums.at]);
-                    }
-#pragma unroll
-                    for (int y = 0; y < 32; y += 2) {
-                        const float by = y < 16 ? by0 : by1;
-                        acc[y % 16 / 2] = fma_both(add_both(two_words(x[y], x[y + 1]), less), both(by, by), acc[y % 16 / 2]);
-                    }
-                };
                 auto add = [&](uint32_t at, bool last) {
                     const float by = next_scale();
                     const uint64_t by_both = both(by, by), less = both(-12582912.f, -12582912.f);
@@ -312,8 +293,7 @@ __global__ void __launch_bounds__((Tile<INT4, N, TMA>::THREADS), (Tile<INT4, N, 
 #pragma unroll 1
                         for (uint32_t k = 0; k < n; k++) {
                             const uint32_t at = at_lanes + sums.at * T::SUM + k * N;
-                            if (N == 16 && k + 1 < n) add_two(at, ++k + 1 == n);
-                            else add(at, k + 1 == n);
+                            add(at, k + 1 == n);
                         }
                         sums.next();
                     }
@@ -680,11 +660,12 @@ cudaError_t launch_tiles(zkb_ctx* ctx, const zkb_step_product_args& a) {
     const bool pairs = !INT4 && aligned_to(a.x, 16) && aligned_to(a.w, 16) && a.x_stride % 16 == 0 && a.w_stride % 16 == 0;
     auto at_once = [&](uint32_t n) { return (a.n_rows + n - 1) / n * out_tiles <= (pairs ? 296 : 148); };
     uint32_t n = INT4 ? 128 : 256;
-    if (a.n_rows <= 16) n = 16;
+    if (!INT4 && a.n_rows <= 16) n = 16;  // (4-bit weights of up to sixteen rows come another way)
     else if (a.n_rows <= 32 || (!INT4 && at_once(32))) n = 32;
     else if (a.n_rows <= 64 || (INT4 && at_once(64))) n = 64;
     else if (a.n_rows <= 128 || at_once(128)) n = 128;
-    if (n == 16) return launch_rows_of<INT4, 16>(ctx, a);
+    if constexpr (!INT4)
+        if (n == 16) return launch_rows_of<INT4, 16>(ctx, a);
     if (n == 32) return launch_rows_of<INT4, 32>(ctx, a);
     if (n == 64) return launch_rows_of<INT4, 64>(ctx, a);
     if constexpr (!INT4)
