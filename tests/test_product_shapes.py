@@ -1,0 +1,58 @@
+"""Products of codes on the host (csrc/product_shapes.hpp): what a set of warps knows when it waits for a tile's 4-bit weights."""
+import ctypes
+import os
+import subprocess
+
+import pytest
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "zk_inference_prover_b200", "csrc")
+
+SOURCE = """
+#include "product_shapes.hpp"
+#include <set>
+#include <vector>
+// The first step whose wait for its weights is over before they are there, -1 if none is. Sets of warps take the steps in turn. A copy into a place of the ring is one phase of its barrier, and a wait
+// names the parity of its phase alone: it is over at once while the copy before the last is still on its way, which is what a set may not know to be done. It knows of the copies that it has waited
+// for, and, where a step's products have ended, of those of all steps up to that one. `swapped`: the two waits the other way round.
+template <class T>
+int first_early(bool swapped) {
+    std::vector<std::set<int>> known(T::SETS);
+    for (int i = 0; i < 400; i++) {
+        std::set<int>& mine = known[i % T::SETS];
+        bool early = false;
+        auto stage_free = [&] {
+            for (int k = 0; k <= i - T::STAGES; k++) mine.insert(k);
+        };
+        auto weights_there = [&] {
+            early = i >= T::RAWS && !mine.count(i - T::RAWS);
+            mine.insert(i);
+        };
+        if (swapped) weights_there(), stage_free();
+        else zk::before_codes(stage_free, weights_there);
+        if (early) return i;
+    }
+    return -1;
+}
+extern "C" int early(int n, int swapped) {
+    return n == 32 ? first_early<zk::Tile<true, 32, true>>(swapped) : n == 64 ? first_early<zk::Tile<true, 64, true>>(swapped) : first_early<zk::Tile<true, 128, true>>(swapped);
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def shapes(tmp_path_factory):
+    d = tmp_path_factory.mktemp("shapes")
+    src, so = d / "s.cpp", d / "s.so"
+    src.write_text(SOURCE)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-shared", "-fPIC", "-I", CSRC, "-o", str(so), str(src)], check=True)
+    return ctypes.CDLL(str(so))
+
+
+@pytest.mark.parametrize("rows", [32, 64, 128])
+def test_weights_are_waited_for_in_their_own_phase(shapes, rows):
+    assert shapes.early(rows, 0) == -1
+
+
+def test_the_other_order_of_waits_is_seen(shapes):
+    """Two sets over three places: the fourth step's place was read by the other set."""
+    assert shapes.early(64, 1) == 3

@@ -1,6 +1,7 @@
 // Products of codes, many rows: tiles on the tensor cores' own memory.
 #include <algorithm>
 
+#include "product_shapes.hpp"
 #include "step_product.cuh"
 #include "tensor_memory.cuh"
 
@@ -19,33 +20,6 @@ namespace zk {
 // codes and sums, against 256 cycles of the tensor cores, so the rate of instructions bounds it (59 % of all cycles issue one).
 struct ProductMaps {
     CUtensorMap w, x;
-};
-
-// RAW: 4-bit weights come to shared memory by the tensor memory unit (their rows start on 16-byte boundaries, and x's); x then has a ring of its own, longer than the codes' one.
-template <bool INT4, int N, bool TMA>
-struct Tile {
-    static constexpr bool FILLED = INT4 || !TMA, RAW = INT4 && TMA;     // the weights' part of a stage is written by warps; from shared memory
-    static constexpr int EPI = N == 64 ? (INT4 ? 8 : 4) : N >= 128 ? 8 : 4, SETS = RAW ? (N == 128 ? 1 : 2) : INT4 ? 2 : 4;  // warps that read the sums; sets of four warps that write codes, in turn
-    // (as many sets as leave the registers in place: 1193 rows of 6744 x 1342 8-bit codes on odd boundaries 122 us by 4 sets and 167 by 2; 2001 of 4097 x 6145 4-bit ones 527 by 2 and 1532 by 4)
-    static constexpr int FIRST_FILLER = EPI + (INT4 ? 4 : 3), THREADS = 32 * (FILLED ? FIRST_FILLER + 4 * SETS : EPI + 2);
-    // A step's codes, in halves of 128 that are a matrix each: what a step costs whatever its codes, waits above all, is some 600 cycles of each of the warps that it goes through.
-    static constexpr int CODES = INT4 ? 256 : 128, HALVES = CODES / 128, A_HALF = 128 * 128, B_HALF = N * 128;
-    static constexpr int A = HALVES * A_HALF, B = HALVES * B_HALF, STAGE = RAW ? A : A + B, RAW_BYTES = 128 * CODES / 2;
-    // thread blocks an SM (one where codes are written by warps: two leave too few registers, sixteen rows of 4096 x 32000 4-bit codes 45 us and 29 by one)
-    static constexpr int BLOCKS = N <= 64 && !FILLED ? 2 : 1;
-    static constexpr int JOIN = N <= (INT4 ? 64 : 32) ? N * 512 : 0;                 // a cluster's sums
-    static constexpr int RAWS = !RAW ? 0 : N == 32 ? 4 : 3, XS = !RAW ? 0 : N == 32 ? 3 : 2;
-    static constexpr int SCALES = INT4 ? 4 : 0, SCALE_BYTES = 128 * 16; // eight groups' scales of a tile's outputs
-    static constexpr int ROOM = (BLOCKS == 2 ? 112 * 1024 : 216 * 1024) - JOIN - RAWS * RAW_BYTES - XS * B - SCALES * SCALE_BYTES;
-    static constexpr int STAGES = ROOM / STAGE < 6 ? ROOM / STAGE : 6;
-    // The sums of a tile of 8-bit weights, or of 4-bit weights' groups: of a step's all at once where they have room twice.
-    static constexpr bool BY_STEP = INT4 && N == 32;
-    static constexpr int SUMS = !INT4 || BY_STEP ? 2 : 4, SUM = BY_STEP ? 8 * N : N, COLUMNS = SUMS * SUM < 32 ? 32 : SUMS * SUM;
-    // A thread block never waits for tensor memory: those that fit an SM's shared memory together (this kernel's variants and attention's, which take all columns and 121 KB) fit its
-    // 512 columns. Clusters that each hold what another waits for would wait forever.
-    static constexpr int LEAST = BLOCKS == 2 ? 108 * 1024 : 121 * 1024;
-    static constexpr int USED = STAGES * STAGE + RAWS * RAW_BYTES + XS * B + SCALES * SCALE_BYTES + JOIN, SMEM = 1024 + (USED > LEAST ? USED : LEAST);
-    static_assert(COLUMNS * BLOCKS <= 512 && (COLUMNS & (COLUMNS - 1)) == 0 && STAGES >= 2 && SMEM <= 226 * 1024, "");
 };
 
 // kind::i8, signed codes, 32-bit sums, 128 outputs.
@@ -512,8 +486,7 @@ __global__ void __launch_bounds__((Tile<INT4, N, TMA>::THREADS), (Tile<INT4, N, 
             for (uint32_t i = set; i < items; i += T::SETS) {
                 const uint32_t to = ring + st.at * T::STAGE;
                 if constexpr (T::RAW) {
-                    wait(bars.raw_full[rs.at], rs.parity);
-                    stage_free();
+                    before_codes(stage_free, [&] { wait(bars.raw_full[rs.at], rs.parity); });
                     if (failed) break;
 #pragma unroll
                     for (int j0 = 0; j0 < MINE; j0 += 4) {
