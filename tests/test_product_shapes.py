@@ -1,4 +1,4 @@
-"""Products of codes on the host (csrc/product_shapes.hpp): what a set of warps knows when it waits for a tile's 4-bit weights."""
+"""Products of codes on the host (csrc/product_shapes.hpp): what a set of warps knows when it waits for a tile's 4-bit weights, and which bytes are read."""
 import ctypes
 import os
 import subprocess
@@ -36,6 +36,7 @@ int first_early(bool swapped) {
 extern "C" int early(int n, int swapped) {
     return n == 32 ? first_early<zk::Tile<true, 32, true>>(swapped) : n == 64 ? first_early<zk::Tile<true, 64, true>>(swapped) : first_early<zk::Tile<true, 128, true>>(swapped);
 }
+extern "C" int reaches_out(uint64_t p, uint64_t lo, uint64_t hi) { return zk::blocks_reach_out(p, lo, hi); }
 """
 
 
@@ -56,3 +57,15 @@ def test_weights_are_waited_for_in_their_own_phase(shapes, rows):
 def test_the_other_order_of_waits_is_seen(shapes):
     """Two sets over three places: the fourth step's place was read by the other set."""
     assert shapes.early(64, 1) == 3
+
+
+def test_blocks_of_memory_that_a_fetch_takes_lie_in_the_array(shapes):
+    """Every start and end of a short array, by the byte: blocks that the fetch takes are inside, and those that are inside are taken."""
+    call = shapes.reaches_out
+    call.argtypes = [ctypes.c_uint64] * 3
+    base = 1 << 20
+    for lo in range(base, base + 16):
+        for hi in range(lo + 1, lo + 70):
+            for p in range(lo, hi):
+                first = p // 16 * 16
+                assert bool(call(p, lo, hi)) == (not (lo <= first and first + 32 <= hi)), (p - base, lo - base, hi - base)

@@ -26,3 +26,21 @@ def test_weights_that_arrive_in_any_order(ctx, zkb, group, rows, n_in, n_out):
     other.synchronize()
     check_product("f32", ys[0], x, x_scale, w)
     assert all(torch.equal(ys[0], y) for y in ys[1:])
+
+
+@gpu
+@pytest.mark.parametrize("kind,group", [("int8", 0), ("int4", 32), ("int4", 128)])
+@pytest.mark.parametrize("rows", [1, 2, 5, 13, 40, 300])
+@pytest.mark.parametrize("short", [1, 15, 16, 17, 31])
+def test_arrays_that_end_inside_a_block_of_memory(ctx, zkb, kind, group, rows, short):
+    """Rows and weights on odd boundaries whose last bytes lie `short` before a multiple of 32 bytes; what is behind them is no part of the sums."""
+    g, n_out = gen(rows + short), 37
+    n_in = 1024 + 33 if kind == "int8" else 1024 + 2 * 33
+    bytes_ = n_in if kind == "int8" else n_in // 2
+    x, w = codes_of(g, rows, n_in, 0, -(rows * n_in + short) % 32), Weights(g, kind, n_out, n_in, group, 0, -(n_out * bytes_ + short) % 32)
+    assert (x.data_ptr() + rows * n_in) % 32 == 32 - short and (w.w.data_ptr() + n_out * bytes_) % 32 == 32 - short
+    x_scale, y = torch.rand(rows, generator=g, device="cuda") + 0.1, torch.zeros(rows, n_out, device="cuda")
+    torch.cuda.synchronize()
+    run_product(ctx, zkb, x, x_scale, w, ("f32", y))
+    done(ctx)
+    check_product("f32", y, x, x_scale, w)

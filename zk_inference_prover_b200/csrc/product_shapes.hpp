@@ -51,4 +51,10 @@ ZK_ON_DEVICE void before_codes(StageFree stage_free, WeightsThere weights_there)
     weights_there();
 }
 
+// Whether the two whole 16-byte blocks of memory that 16 bytes from p on lie in (the second one is taken with p on a boundary, too) reach out of the array [lo, hi).
+ZK_ON_DEVICE bool blocks_reach_out(uintptr_t p, uintptr_t lo, uintptr_t hi) {
+    const uintptr_t first = p - (p & 15);
+    return first < lo || first + 32 > hi;
+}
+
 }  // namespace zk

@@ -1,5 +1,6 @@
 // Products of codes: what their kernels share.
 #pragma once
+#include "product_shapes.hpp"
 #include "step_attention.cuh"
 
 namespace zk {
@@ -22,9 +23,7 @@ __device__ __forceinline__ uint4 some_bytes(const int8_t* p, int n) {
 struct Fetched {
     uint4 a, b;
 };
-__device__ __forceinline__ bool fetch_reaches_out(const int8_t* p, const int8_t* lo, const int8_t* hi) {
-    return p - 15 < lo || p + 31 > hi;
-}
+__device__ __forceinline__ bool fetch_reaches_out(const int8_t* p, const int8_t* lo, const int8_t* hi) { return blocks_reach_out((uintptr_t)p, (uintptr_t)lo, (uintptr_t)hi); }
 __device__ __forceinline__ Fetched fetch16(const int8_t* p, const int8_t* lo, const int8_t* hi) {
     Fetched r{make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
     if (!fetch_reaches_out(p, lo, hi)) {

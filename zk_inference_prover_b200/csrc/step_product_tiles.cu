@@ -1,7 +1,6 @@
 // Products of codes, many rows: tiles on the tensor cores' own memory.
 #include <algorithm>
 
-#include "product_shapes.hpp"
 #include "step_product.cuh"
 #include "tensor_memory.cuh"
 
