@@ -36,6 +36,7 @@ int first_early(bool swapped) {
 extern "C" int early(int n, int swapped) {
     return n == 32 ? first_early<zk::Tile<true, 32, true>>(swapped) : n == 64 ? first_early<zk::Tile<true, 64, true>>(swapped) : first_early<zk::Tile<true, 128, true>>(swapped);
 }
+extern "C" int by_eights(uint64_t at, unsigned first, unsigned groups, int64_t stride, unsigned n_out) { return zk::scales_by_eights(at, first, groups, stride, n_out); }
 extern "C" int reaches_out(uint64_t p, uint64_t lo, uint64_t hi) { return zk::blocks_reach_out(p, lo, hi); }
 """
 
@@ -69,3 +70,21 @@ def test_blocks_of_memory_that_a_fetch_takes_lie_in_the_array(shapes):
             for p in range(lo, hi):
                 first = p // 16 * 16
                 assert bool(call(p, lo, hi)) == (not (lo <= first and first + 32 <= hi)), (p - base, lo - base, hi - base)
+
+
+def test_scales_that_come_eight_at_a_time_are_there(shapes):
+    """Every base by the byte pair, group that a thread block begins with, and number of groups and of scales a row: eights on 16-byte boundaries that no row's end cuts."""
+    call = shapes.by_eights
+    call.argtypes = [ctypes.c_uint64, ctypes.c_uint32, ctypes.c_uint32, ctypes.c_int64, ctypes.c_uint32]
+    taken = 0
+    for base in range(1 << 20, (1 << 20) + 16, 2):
+        for groups in range(1, 34):
+            for stride in range(groups, groups + 9):
+                for first in range(groups):
+                    if call(base + 2 * first, first, groups, stride, 3):
+                        taken += 1
+                        for row in range(3):
+                            for block in range(first, groups, 8):
+                                assert (base + 2 * (row * stride + block)) % 16 == 0 and block + 8 <= groups
+    assert taken > 0
+    assert call(1 << 20, 0, 32, 32, 3) and call(1 << 20, 0, 32, 33, 1) and not call((1 << 20) + 8 + 56, 28, 32, 32, 3)

@@ -1,4 +1,6 @@
 """Products of codes (zkb_step_product): the ways that their sizes and layouts lead to, beside those of test_step_layer.py and test_step_layer_edges.py."""
+import math
+
 import pytest
 import torch
 
@@ -44,3 +46,30 @@ def test_arrays_that_end_inside_a_block_of_memory(ctx, zkb, kind, group, rows, s
     run_product(ctx, zkb, x, x_scale, w, ("f32", y))
     done(ctx)
     check_product("f32", y, x, x_scale, w)
+
+
+def with_scales(w, pad, off):
+    """w's scales laid out with `pad` more behind each output's, from `off` scales behind a multiple of 16 bytes on, NaN in between and behind."""
+    groups = -(-w.n_in // w.group)
+    keep = torch.full((w.scale.shape[0] * (groups + pad) + off,), math.nan, device="cuda", dtype=torch.bfloat16)
+    scale = keep[off:].view(-1, groups + pad)
+    scale[:, :groups] = w.scale[:, :groups]
+    assert keep.data_ptr() % 16 == 0
+    w.scale = scale
+    return w
+
+
+@gpu
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("pad,off", [(0, 0), (8, 0), (0, 1), (0, 2), (0, 4), (1, 0), (3, 2), (8, 4), (4, 8)])
+@pytest.mark.parametrize("rows,n_out", [(1, 200), (2, 130), (5, 300), (16, 260), (20, 256), (40, 300), (64, 1), (150, 257), (300, 700)])
+def test_scales_wherever_they_lie(ctx, zkb, group, pad, off, rows, n_out):
+    """Groups by eights and not, in rows that follow one another and that do not, on every boundary that is taken; codes spread over clusters where they are many."""
+    g = gen(rows + group)
+    for n_in in (group * 8, 4096, 4096 + group, 14336):
+        x, w, x_scale = codes_of(g, rows, n_in), with_scales(Weights(g, "int4", n_out, n_in, group), pad, off), torch.rand(rows, generator=g, device="cuda") + 0.1
+        y = torch.zeros(rows, n_out, device="cuda")
+        torch.cuda.synchronize()
+        run_product(ctx, zkb, x, x_scale, w, ("f32", y))
+        done(ctx)
+        check_product("f32", y, x, x_scale, w)

@@ -51,6 +51,12 @@ ZK_ON_DEVICE void before_codes(StageFree stage_free, WeightsThere weights_there)
     weights_there();
 }
 
+// Whether the scales of groups from `first` on, at address `at`, come eight at a time by 16 bytes: on their boundaries for every output (`stride` scales apart), and with nothing behind a row's last
+// group, which of an array's last row is behind the array.
+ZK_ON_DEVICE bool scales_by_eights(uintptr_t at, uint32_t first, uint32_t groups, int64_t stride, uint32_t n_out) {
+    return at % 16 == 0 && (n_out == 1 || stride % 8 == 0) && first % 8 == 0 && groups % 8 == 0;
+}
+
 // Whether the two whole 16-byte blocks of memory that 16 bytes from p on lie in (the second one is taken with p on a boundary, too) reach out of the array [lo, hi).
 ZK_ON_DEVICE bool blocks_reach_out(uintptr_t p, uintptr_t lo, uintptr_t hi) {
     const uintptr_t first = p - (p & 15);

@@ -440,8 +440,7 @@ __global__ void __launch_bounds__((Tile<INT4, N, TMA>::THREADS), (Tile<INT4, N, 
                 for (int y = 0; y < 8; y++) v[y] = y < n ? p[y] : 0u;
                 return make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
             };
-            // 16 bytes at once where all of them are there (a row's last ones may not be)
-            if (aligned16(scales + g0) && (a.n_out == 1 || a.w_scale_stride % 8 == 0) && groups % 8 == 0) each([](const uint16_t* p, uint32_t) { return *reinterpret_cast<const uint4*>(p); });
+            if (scales_by_eights((uintptr_t)(scales + g0), g0, groups, a.w_scale_stride, a.n_out)) each([](const uint16_t* p, uint32_t) { return *reinterpret_cast<const uint4*>(p); });
             else each(one_by_one);
         } else {  // ---- codes into shared memory: each set of four warps every SETS-th step
             const int f = threadIdx.x - 32 * T::FIRST_FILLER, th = f & 127, set = f >> 7;
