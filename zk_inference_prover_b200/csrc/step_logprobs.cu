@@ -278,7 +278,12 @@ struct LpResult {
         odd = most != most, none = most == -INFINITY;
         log_total = none ? 0.f : equal == 1 ? log1pf(rest) : logf(total);
     }
-    __device__ __forceinline__ float log_probability(float x) const { return odd ? __int_as_float(0x7fc00000) : none || x == -INFINITY ? -INFINITY : (x - most) * scale - log_total; }
+    __device__ __forceinline__ float log_probability(float x) const {
+        if (odd) return __int_as_float(0x7fc00000);
+        if (none || x == -INFINITY) return -INFINITY;
+        const float d = x - most;  // (of two numbers that no float holds it is -infinity: scaled, it may be one)
+        return (d > -INFINITY ? d * scale : x * scale - most * scale) - log_total;
+    }
     __device__ __forceinline__ float entropy() const { return odd ? __int_as_float(0x7fc00000) : none ? 0.f : log_total - lean * 0.693147181f / total; }
     __device__ __forceinline__ void give(const zkb_step_logprobs_args& a, uint32_t t, uint32_t i, int32_t id, float x) const {
         float y = 0.f;
