@@ -1,0 +1,43 @@
+"""Norms and gates (zkb_step_residual_norm, zkb_step_gate) of values at the ends of the 32-bit floats."""
+import math
+
+import pytest
+import torch
+
+from test_step_layer import HALF, INT8, TYPES, check_out, norm_reference, room
+from test_step_layer import values_of
+from test_step_values import done, gen
+
+gpu = pytest.mark.gpu
+
+
+def norms(ctx, zkb, x, w, kind, eps):
+    rows, width = x.shape
+    full, got = room(kind, rows, width)
+    scale = torch.zeros(rows, device="cuda") if kind == "codes" else None
+    torch.cuda.synchronize()
+    ctx.step_residual_norm(zkb.StepResidualNorm(x=x.data_ptr(), x_stride=width, weight=w.data_ptr(), out=got.data_ptr(), out_type=TYPES[kind], out_scale=scale.data_ptr() if scale is not None else 0,
+                                                out_stride=width, n_rows=rows, width=width, eps=eps))
+    done(ctx)
+    return got, scale
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["codes", "bf16", "words"])
+@pytest.mark.parametrize("width", [64, 777, 4096, 20000])
+@pytest.mark.parametrize("small", [-7, -9, -12, -20, -44, -60])
+@pytest.mark.parametrize("eps", [0.0, 2.0 ** -60])
+def test_weights_of_unlike_sizes(ctx, zkb, kind, width, small, eps):
+    """Small rows with weights of which one is near 1 and others are so small that values times them have few bits in 32, or none, though the norm has all. A norm in 32 bits is off by
+    2^-18 (test_residual_norm); where products were taken at up to 2^10 times less than the norm they are off by 2^-150 each, of the least bf16 steps, 2^-133, by 2^-7."""
+    g = gen(width)
+    x = (torch.randn(7, width, generator=g, device="cuda") * 2.0 ** small).bfloat16()
+    x[0] = 2.0 ** small
+    w = ((1 + torch.rand(width, generator=g, device="cuda")) * torch.exp2(-140.0 * torch.rand(width, generator=g, device="cuda").double())).bfloat16()
+    w[0], w[1], w[2] = 1.0, 1.297 * 2.0 ** -101, 1.3 * 2.0 ** -126
+    got, scale = norms(ctx, zkb, x, w, kind, eps)
+    y = norm_reference(x, w, eps)
+    if kind == "codes":
+        check_out(got, scale, kind, y, 2.0 ** -18)
+    else:
+        assert bool(((values_of(got) - y).abs() <= (HALF + 2.0 ** -17) * y.abs() + (0.5 + 2.0 ** -7) * 2.0 ** -133).all())

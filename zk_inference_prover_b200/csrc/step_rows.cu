@@ -195,7 +195,10 @@ __global__ void __launch_bounds__(V >= 4 ? 512 : 1024, V == 4 ? 2 : 1) rows_kern
         over_row(room[0], a.warps, ss, most);
         const float mean = ss / (float)a.width + a.eps;
         by = rsqrtf(mean);
-        if (!(mean > 0x1p-90f && mean < 0x1p120f && most > 0x1p-80f && most < INFINITY)) {  // squares or products that 32 bits do not hold, or values that are no numbers: the same for the whole row
+        // Squares or products that 32 bits do not hold, or values that are no numbers: the same for the whole row. A product, y before the norm's factor, is off by up to 2^-150, whatever its size. To codes
+        // that is nothing beside the largest one; of values it is 2^-7 of bf16's least step, 2^-133, where the factor is less than 2^10 (with an eps of 10^-6 it always is).
+        const float least = a.out_type == ZKB_VALUE_INT8 ? 0x1p-90f : 0x1p-20f;
+        if (!(mean > least && mean < 0x1p120f && most > 0x1p-80f && most < INFINITY)) {
             double wide = 0.;
 #pragma unroll
             for (int v = 0; v < V; v++)
