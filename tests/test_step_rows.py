@@ -41,3 +41,31 @@ def test_weights_of_unlike_sizes(ctx, zkb, kind, width, small, eps):
         check_out(got, scale, kind, y, 2.0 ** -18)
     else:
         assert bool(((values_of(got) - y).abs() <= (HALF + 2.0 ** -17) * y.abs() + (0.5 + 2.0 ** -7) * 2.0 ** -133).all())
+
+
+@gpu
+@pytest.mark.parametrize("source,width", [("bf16", 64), ("bf16", 333), ("words", 4096), ("words", 77)])
+@pytest.mark.parametrize("kind", ["codes", "bf16", "words"])
+def test_gates_of_minus_infinity_are_closed(ctx, zkb, source, width, kind):
+    """0 below -87, down to -infinity; x that are no numbers and gates that are NaN stay what they are."""
+    from step_cases import words
+
+    g = gen(width)
+    x, a = (torch.randn(4, width, generator=g, device="cuda").bfloat16() for _ in range(2))
+    a[0, ::3], a[1], a[2, 5], a[3, 7] = -math.inf, -math.inf, math.nan, -math.inf
+    x[3, 7] = math.inf
+    out, scale = room(kind, 4, width)[1], torch.full((4,), -1.0, device="cuda")
+    xs, gs = (words(v) if source == "words" else v for v in (x, a))
+    torch.cuda.synchronize()
+    ctx.step_gate(zkb.StepGate(gate=gs.data_ptr(), gate_stride=width, x=xs.data_ptr(), x_stride=width, x_type=TYPES[source], out=out.data_ptr(), out_type=TYPES[kind],
+                               out_scale=scale.data_ptr() if kind == "codes" else 0, out_stride=width, n_rows=4, width=width))
+    done(ctx)
+    d = a.double()
+    y = x.double() * torch.where(d == -math.inf, 0.0, d / (1 + torch.exp(-d)))
+    rel = (6 + 1.2 * d.abs().clamp(max=87)) * 2.0 ** -23
+    rows = slice(0, 2)
+    check_out(out[rows], scale[rows] if kind == "codes" else None, kind, y[rows], rel[rows])
+    if kind == "codes":
+        assert bool(torch.isnan(scale[2:]).all()) and not bool(out[2:].any()) and scale[1] == 0
+    else:
+        assert bool(torch.equal(torch.isnan(values_of(out)), torch.isnan(y)))

@@ -126,6 +126,12 @@ __device__ __forceinline__ float larger_size(float a, float b) {
     asm("{\n\t.reg .f32 t;\n\tabs.f32 t, %2;\n\tmax.NaN.f32 %0, %1, t;\n\t}" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
+// Two bf16 values, -infinity as the lowest number: its factor, zero, then has a product.
+__device__ __forceinline__ uint32_t numbers_from_below(uint32_t w) {
+    uint32_t r;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(w), "r"(0xff7fff7fu));
+    return r;
+}
 // g / (1 + exp(-g)): two approximations (2^-22 and 2^-23 of their results) and the products.
 __device__ __forceinline__ float gated(float g) {
     float e, r;
@@ -153,7 +159,10 @@ __global__ void __launch_bounds__(V >= 4 ? 512 : 1024, V == 4 ? 2 : 1) rows_kern
 #pragma unroll
             for (int v = 0; v < V; v++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) y[v][2 * i] = gated(bf16_low(g[v][i])) * bf16_low(s[v][i]), y[v][2 * i + 1] = gated(bf16_high(g[v][i])) * bf16_high(s[v][i]);
+                for (int i = 0; i < 4; i++) {
+                    const uint32_t two = numbers_from_below(g[v][i]);
+                    y[v][2 * i] = gated(bf16_low(two)) * bf16_low(s[v][i]), y[v][2 * i + 1] = gated(bf16_high(two)) * bf16_high(s[v][i]);
+                }
         } else {
 #pragma unroll
             for (int v = 0; v < V; v++)
