@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from test_step_layer import Weights, check_product, codes_of, run_product
+from test_step_layer import INT8, TYPES, Weights, check_product, codes_of, room, run_product, untouched
 from test_step_values import done, gen
 
 gpu = pytest.mark.gpu
@@ -73,3 +73,77 @@ def test_scales_wherever_they_lie(ctx, zkb, group, pad, off, rows, n_out):
         run_product(ctx, zkb, x, x_scale, w, ("f32", y))
         done(ctx)
         check_product("f32", y, x, x_scale, w)
+
+
+@gpu
+@pytest.mark.parametrize("rows", [3, 8, 9, 16])
+@pytest.mark.parametrize("n_in,n_out", [(4096, 9000), (14336, 2400), (131071, 300), (1024, 40001), (4100, 8200), (2049, 17000)])
+@pytest.mark.parametrize("pad,off", [(0, 0), (16, 0), (1, 3)])
+@pytest.mark.parametrize("kind", ["int32", "bf16"])
+def test_few_rows_and_many_8_bit_weights(ctx, zkb, rows, n_in, n_out, pad, off, kind):
+    """More than 2^25 weights: tiles of sixteen rows, spread over clusters or one after the other in a thread block, on 16-byte boundaries and others."""
+    assert n_in * n_out > 1 << 25
+    g = gen(rows + n_in)
+    pad += -n_in % 16 if pad == 16 else 0
+    x, w, x_scale = codes_of(g, rows, n_in, pad, off), Weights(g, "int8", n_out, n_in, 0, pad, off), torch.rand(rows, generator=g, device="cuda") + 0.1
+    full, y = room(kind, rows, n_out, pad, off)
+    torch.cuda.synchronize()
+    run_product(ctx, zkb, x, x_scale, w, (kind, y))
+    done(ctx)
+    check_product(kind, y, x, x_scale, w)
+    untouched(full, y, off)
+
+
+@gpu
+@pytest.mark.parametrize("most", [1, 2, 4])
+@pytest.mark.parametrize("n_in,n_out", [(4096, 9000), (14336, 2400), (131071, 300)])
+def test_few_rows_and_many_8_bit_weights_whose_clusters_are_refused(ctx, zkb, monkeypatch, most, n_in, n_out):
+    monkeypatch.setenv("ZKB_STEP_CLUSTERS", str(most))
+    g = gen(most)
+    x, w = codes_of(g, 11, n_in, -n_in % 16), Weights(g, "int8", n_out, n_in, 0, -n_in % 16)
+    y = torch.zeros(11, n_out, device="cuda", dtype=torch.int32)
+    torch.cuda.synchronize()
+    run_product(ctx, zkb, x, None, w, ("int32", y))
+    done(ctx)
+    check_product("int32", y, x, None, w)
+
+
+@gpu
+@pytest.mark.parametrize("rows", [33, 50, 64])
+@pytest.mark.parametrize("kind,group", [("int8", 0), ("int4", 32), ("int4", 128)])
+@pytest.mark.parametrize("n_in,n_out,pad", [(256, 128256, 0), (1024, 40000, 0), (272, 37889, 0), (300, 40000, 1)])
+def test_tiles_of_64_rows_one_after_the_other(ctx, zkb, rows, kind, group, n_in, n_out, pad):
+    """More outputs' tiles of 33 to 64 rows than the GPU holds at once: an output head."""
+    g = gen(rows + n_out)
+    x, w, x_scale = codes_of(g, rows, n_in, pad), Weights(g, kind, n_out, n_in, group, pad), torch.rand(rows, generator=g, device="cuda") + 0.1
+    full, y = room("f32", rows, n_out, 3)
+    torch.cuda.synchronize()
+    run_product(ctx, zkb, x, x_scale, w, ("f32", y))
+    done(ctx)
+    check_product("f32", y, x, x_scale, w)
+    untouched(full, y, 0)
+
+
+@gpu
+@pytest.mark.parametrize("rows", [1, 2, 7, 40, 200])
+@pytest.mark.parametrize("kind,group", [("int8", 0), ("int4", 64)])
+def test_rows_and_weights_of_one_buffer(ctx, zkb, rows, kind, group):
+    """Rows of x that lie behind each output's weights, and that are the weights themselves."""
+    g, n_in, n_out = gen(rows), 256, 130
+    w = Weights(g, kind, n_out, n_in, group, n_in)
+    lines = w.w  # [output][weights, and 256 codes behind them]
+    x = lines[:, -n_in:][:rows] if rows <= n_out else torch.cat([lines, lines])[:rows, -n_in:]
+    x_scale = torch.rand(rows, generator=g, device="cuda") + 0.1
+    y = torch.zeros(rows, n_out, device="cuda")
+    torch.cuda.synchronize()
+    run_product(ctx, zkb, x, x_scale, w, ("f32", y))
+    done(ctx)
+    check_product("f32", y, x, x_scale, w)
+    if kind == "int8":  # rows as the weights, too
+        rows = min(rows, n_out)
+        y = torch.zeros(rows, rows, device="cuda", dtype=torch.int32)
+        torch.cuda.synchronize()
+        ctx.step_product(zkb.StepProduct(x=x.data_ptr(), x_stride=x.stride(0), w=x.data_ptr(), w_stride=x.stride(0), w_type=INT8, out=y.data_ptr(), out_type=TYPES["int32"], out_stride=rows, n_rows=rows,
+                                         n_in=n_in, n_out=rows))
+        done(ctx)
+        assert torch.equal(y.double(), x[:rows].double() @ x[:rows].double().T)
