@@ -224,17 +224,24 @@ __global__ void __launch_bounds__((Tile<INT4, N, TMA>::THREADS), (Tile<INT4, N, 
                     k8++;
                     return s * 0.0625f;  // (the codes are 16 times themselves)
                 };
-                auto add = [&](uint32_t at, bool last) {
-                    const float by = next_scale();
-                    const uint64_t by_both = both(by, by), less = both(-12582912.f, -12582912.f);
-                    read(at, last, [&](int j, const uint32_t(&x)[CHUNK]) {
+                const uint64_t less = both(-12582912.f, -12582912.f);
+                if constexpr (T::BY_STEP) {
+#pragma unroll 1
+                    for (uint32_t s = 0; s < steps; s++) {
+                        const uint32_t n = groups_in(s);
+                        arrived();
+#pragma unroll 1
+                        for (uint32_t k = 0; k < n; k++) {
+                            const float by = next_scale();
+                            read(at_lanes + sums.at * T::SUM + k * N, k + 1 == n, [&](int j, const uint32_t(&x)[CHUNK]) {
 #pragma unroll
-                        for (int y = 0; y < CHUNK; y += 2) acc[(j + y) / 2] = fma_both(add_both(two_words(x[y], x[y + 1]), less), by_both, acc[(j + y) / 2]);
-                    });
-                };
-                if constexpr (!T::BY_STEP) {
+                                for (int y = 0; y < CHUNK; y += 2) acc[(j + y) / 2] = fma_both(add_both(two_words(x[y], x[y + 1]), less), both(by, by), acc[(j + y) / 2]);
+                            });
+                        }
+                        sums.next();
+                    }
+                } else {  // (sixteen columns at a time: more wait in registers)
                     const uint32_t all = min((first_step + steps) * per_step, groups) - first_step * per_step;
-                    const uint64_t less = both(-12582912.f, -12582912.f);
 #pragma unroll 1
                     for (uint32_t g = 0; g < all; g++) {
                         const float by = next_scale();
@@ -252,21 +259,7 @@ __global__ void __launch_bounds__((Tile<INT4, N, TMA>::THREADS), (Tile<INT4, N, 
                                 arrive(bars.sum_empty[sums.at]);
                             }
 #pragma unroll
-                            for (int y = 0; y < 16; y += 2)
-                                acc[(j + y) / 2] = fma_both(add_both(two_words(x[y], x[y + 1]), less), both(by, by), acc[(j + y) / 2]);
-                        }
-                        sums.next();
-                    }
-                }
-#pragma unroll 1
-                for (uint32_t s = 0; T::BY_STEP && s < steps; s++) {
-                    const uint32_t n = groups_in(s);
-                    if constexpr (T::BY_STEP) {
-                        arrived();
-#pragma unroll 1
-                        for (uint32_t k = 0; k < n; k++) {
-                            const uint32_t at = at_lanes + sums.at * T::SUM + k * N;
-                            add(at, k + 1 == n);
+                            for (int y = 0; y < 16; y += 2) acc[(j + y) / 2] = fma_both(add_both(two_words(x[y], x[y + 1]), less), both(by, by), acc[(j + y) / 2]);
                         }
                         sums.next();
                     }

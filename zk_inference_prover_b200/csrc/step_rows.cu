@@ -282,7 +282,6 @@ static cudaError_t launch_rows(zkb_ctx* ctx, RowsArgs a, bool x_word, bool vec) 
     uint32_t v = 4;
     if (eights <= 32 || (a.n_rows < 148 * 4 && eights <= 1024)) v = 1;
     else if (eights <= 64 || (a.n_rows < 148 * 4 && eights <= 2048)) v = 2;
-    while (v < 4 && (eights + 32 * v - 1) / (32 * v) > 32) v *= 2;
     a.warps = (eights + 32 * v - 1) / (32 * v);
     if (v == 4 && a.warps > 16) v = 8, a.warps = (eights + 255) / 256;
     const uint32_t block = a.warps == 1 ? 32 * ROW_GROUP : 32 * a.warps, grid = a.warps == 1 ? (a.n_rows + ROW_GROUP - 1) / ROW_GROUP : a.n_rows;
