@@ -348,18 +348,21 @@ extern "C" int zkb_step_product(zkb_ctx* ctx, const zkb_step_product_args* args)
     ProfScope prof(ctx, "step_product_kernel");
     const int64_t w_row = int4 ? a.w_stride / 2 : a.w_stride;
     const bool vec = aligned_to(a.x, 16) && aligned_to(a.w, 16) && (a.n_rows == 1 || a.x_stride % 16 == 0) && (a.n_out == 1 || w_row % 16 == 0);
-    // By what each was measured to take, in us (4-bit codes in groups of 128, of 64, of 32; 8-bit ones):
+    // By what each was measured to take, in us, calls of a graph on inputs in turn that the L2 does not hold (4-bit codes in groups of 128, of 64, of 32; 8-bit ones):
     //                                   dp4a                     a warp's products          tiles
-    //   1 row of 4096 x 4096            4.4  4.3  4.4  5.5       5.4  6.1  7.3  6.9
-    //   2 rows of 4096 x 4096           6.2  6.1  6.2  6.7       5.4  6.2  7.3  6.9
-    //   2 rows of 14336 x 4096          14   14   14   15        11.2 11.9 17.5 16.9
-    //   1 of 1637 x 9144, odd rows      12.2 12.3 12.3 12.2      9.9  10.0 13.3 13.8   (of 10344 x 6512: 25 and 38)
-    //   2 of 1637 x 9144, odd rows      19.8 19.9 19.9 16.3      9.9  10.2 13.3 13.9
-    //   8 rows of 4096 x 4096                                    5.6  6.2  7.4  6.9         11.2 12.1 14.1 9.0
-    //   16 rows of 4096 x 14336                                  15.6 18.1 22.8 19.6        18.1 21.6 27.7 15.3
-    //   16 rows of 4096 x 32000                                  28.8 33.2 43.2 36.9        29.4 36.1 48.2 25.4
+    //   1 row of 4096 x 4096            3.5  3.9  4.0  5.0       4.6  5.7  6.9  6.5
+    //   1 row of 14336 x 4096           7.3  7.5  7.6  11.0      10.7 11.2 16.8 16.3
+    //   2 rows of 4096 x 4096           5.0  5.0  5.0  6.3       5.0  5.7  6.9  6.5
+    //   2 rows of 14336 x 4096          10.4 10.6 10.7 14.2      10.6 11.3 16.9 16.3
+    //   1 of 1637 x 9144, odd rows      11.8 11.8 11.9 11.1      9.3  9.8  12.9 13.4
+    //   1 of 10344 x 6512, odd rows     19.3 19.7 20.0 25.0      38.4 41.4 68.4 61.5
+    //   8 rows of 4096 x 4096                                    5.1  5.7  7.0  6.6         12.1 13.6 17.0 8.6
+    //   16 rows of 14336 x 4096                                  12.9 14.4 19.2 17.6        19.7 24.4 35.1 15.5
+    //   16 rows of 4096 x 14336                                  15.0 17.5 22.3 19.1        18.7 24.7 36.6 14.9
+    //   16 rows of 4096 x 32000                                  28.2 32.3 42.4 36.2        31.5 43.3 67.1 24.5
+    // (One short row on odd boundaries with long groups would take a fifth less the other way, a long one twice as much. Two rows on odd boundaries have no dp4a: it took twice as long at 1637 x 9144.)
     const uint64_t bytes = (uint64_t)a.n_out * a.n_in;
-    const bool some = a.n_rows > 2 ? a.n_rows <= 16 && (int4 || bytes <= (32u << 20)) : a.n_rows == 2 && (!vec || a.group == 128);
+    const bool some = a.n_rows > 2 ? a.n_rows <= 16 && (int4 || bytes <= (32u << 20)) : a.n_rows == 2 && !vec;
     if (some) {
         ZKB_CUDA(ctx, (!int4 ? launch_some<0>(ctx, a, vec) : a.group == 32 ? launch_some<32>(ctx, a, vec) : a.group == 64 ? launch_some<64>(ctx, a, vec) : launch_some<128>(ctx, a, vec)));
         return ZKB_OK;
