@@ -582,7 +582,8 @@ int zkb_step_attention(zkb_ctx* ctx, const zkb_step_attention_args* args);
 /* What lies between those calls and behind them, with the same conventions. zkb_step_residual_norm and zkb_step_gate leave rows of 8-bit
  * codes with a scale a row, zkb_step_product multiplies them with weights held as codes (as INT32 its results are the accumulators that
  * zkb_witness_dequant proves), and zkb_step_logprobs reads the output head's. Rows of codes: scale = max|y| / 127 and code =
- * y * (127 / max|y|), rounded to nearest even (a scale of zero, NaN or infinity: codes 0), y the values before any rounding. */
+ * y * (127 / max|y|), rounded to nearest even (a scale of zero, NaN or infinity: codes 0), y the values before any rounding, the factor
+ * a 32-bit float: a value halfway between two codes may go to either. */
 
 /* The residual stream's next rows and their norms: s = bf16(residual + x), or x itself where residual is NULL, and
  * y = s * rsqrt(mean(s^2) + eps) * weight over a row's `width` values (weight: bf16, NULL: ones). s goes to sum_out where that is given; it
@@ -619,7 +620,7 @@ int zkb_step_gate(zkb_ctx* ctx, const zkb_step_gate_args* args);
  * for INT4 an even number) from one output's weights to the next. With INT8 weights, out is INT32: acc itself (x_scale and w_scale NULL), or BF16, WORD
  * or F32: acc * (x_scale[t] * w_scale[c]), w_scale n_out floats. With INT4 weights each `group` (32, 64 or 128) of a row's codes has a bf16 scale,
  * the scales of output c from w_scale + c * w_scale_stride on, and out is BF16, WORD or F32: x_scale[t] times the sum, in
- * 32-bit floats, of scale * the exact sum of 32 or more codes of a group. out[t][c] is at t * out_stride + c. n_in is at most 131071, so that no sum leaves 32 bits; n_out at most 2^24, n_rows 2^18. Which
+ * 32-bit floats, of scale * the exact sum of 32 or more codes of a group. out[t][c] is at t * out_stride + c. Strides are no shorter than what they lead past. n_in is at most 131071, so that no sum leaves 32 bits; n_out at most 2^24, n_rows 2^18. Which
  * kernel computes a sum of groups, and so its order, is decided by the sizes and the alignment alone. */
 typedef struct zkb_step_product_args {
     const int8_t* x;

@@ -13,8 +13,9 @@ namespace zk {
 //   lse = m + log(S),  entropy = log(S) - sum(w (z - m)) / S,  S = 1 + what the others leave, so that log1p has all of its bits where one token is nearly certain.
 // The n_top largest: as many values reach the n_top-th largest of the maxima of groups of lanes, so the n_top largest do. Those that reach
 // it, a few more than n_top, are listed, and each one's rank among them is counted; where too many tie for the list, they are found one after the other.
-// Measured: 4096 rows of 32003 bf16 logits 74 us without and 94 with the likeliest 5 (40 is the bytes' time): a logit costs some 2.3 instructions, an exp2 among them, and 60 % of all cycles issue
-// one; one row of 32000 floats 4.7 us without and 8.0 with the likeliest 8: trips to memory, barriers and a cluster's joining, one after the other.
+// Measured: 4096 rows of 32003 bf16 logits 70 to 74 us without and 90 to 94 with the likeliest 5 (40 is the bytes' time): 14.7 warp instructions for 32 logits, and 60 % of all cycles issue one. By the
+// source the sums are five of them, an exp2 and a half of every packed operation; the others have not been told apart. One row of 32000 floats 4.3 us without and 9 to 10 with the likeliest 8: trips to
+// memory, barriers and a cluster's joining, one after the other.
 constexpr int LP_VECTORS = 8, LP_TOP = 32, LP_LIST = 1024, LP_PARTS = 64, LP_RANKS = 16;
 
 // What is left of a part: the largest logit, how many have it, the sums over the others, the largest n_top with their places.

@@ -10,8 +10,8 @@ namespace zk {
 // ---- few rows ------------------------------------------------------------------------------------------------------------------------
 // The weights are read once and everything else is small, so this is bound by the weights' bytes. A thread block has CHANNELS outputs of R rows; its warps' lanes take turns in
 // the weights, 16 bytes each, and multiply four codes an instruction (dp4a). Of 4-bit codes the two halves of the bytes are taken apart in place, as 16 times the code, against
-// the even and the odd codes of x; 16 bytes are 32 codes of one group, whose sum is exact and then scaled. One row of 4096 x 32000 8-bit codes: 23.3 us, 5.6 TB/s, its loads' latency
-// between a thread block's start and its end is what is left; of 4096 x 4096 4-bit codes 4.4 us, where a launch and three trips to memory are most of it.
+// the even and the odd codes of x; 16 bytes are 32 codes of one group, whose sum is exact and then scaled. One row of 4096 x 32000 8-bit codes: 22.7 to 24.6 us, 5.3 to 5.8 TB/s, its loads' latency
+// between a thread block's start and its end is what is left; of 4096 x 4096 4-bit codes 3.5 to 4.1 us, where a launch and three trips to memory are most of it.
 constexpr int CHANNELS = 4, FEW_WARPS = 4;
 
 // VEC: all rows of x and of the weights start on 16-byte boundaries.
@@ -136,7 +136,7 @@ static cudaError_t launch_few(zkb_ctx* ctx, const zkb_step_product_args& a, bool
 // Codes from memory into the registers that multiply them: m16n8k32 with 16 outputs of the weights as its long side and eight rows of x as the short one. Which code is which k of a product
 // is free as long as both sides agree, so a lane takes the 16 bytes that it loads side by side; low and high halves of 4-bit codes' bytes are 16 times the even and the odd codes. A warp has 32
 // outputs and every so manieth run of codes; a thread block's warps add up through shared memory. Nothing waits for anything but its own loads, two or three runs of which are under way.
-// Sixteen rows of 14336 x 4096 codes: 4-bit in groups of 128 (64, 32) 13.6 us (15.0, 19.7), 8-bit 16.1, 3.7 TB/s: what bounds it is the first cache, whose lines the eight rows of a load take one
+// Sixteen rows of 14336 x 4096 4-bit codes in groups of 128 (64, 32): 12.9 us (14.4, 19.2), of 4096 x 4096 8-bit ones, eight rows, 6.6 (more weights go to the tiles: 17.6 and 15.5): what bounds it is the first cache, whose lines the eight rows of a load take one
 // after the other, x's among them in every thread block (with 8 bytes of 4-bit weights a lane 17.6), and registers: more runs under way go to memory.
 __device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"

@@ -14,9 +14,10 @@ namespace zk {
 //   Rows on other boundaries by the same warps.
 // Few rows leave the tensor cores idle and are bound by the weights' bytes: N is as small as the rows allow, two thread blocks share an SM, and the steps are spread over the thread
 // blocks of a cluster, which add up through each other's shared memory, each a share of the rows.
-// Measured: 4096 rows of 4096 x 14336 8-bit weights 174 to 182 us, 2.7 PFLOP/s (a tile's sums are read while the next tile's products run); 32 rows of 4096 x 28672 24 us, 5.0 TB/s; 2001 rows
-// of 4096 x 6144 4-bit weights with groups of 128 118 us, 850 TFLOP/s: there each group's 128 x 128 sums pass through registers, some 2700 warp instructions an SM and group of a tile,
-// codes and sums, against 256 cycles of the tensor cores, so the rate of instructions bounds it (59 % of all cycles issue one).
+// Measured: 4096 rows of 4096 x 14336 8-bit weights 174 to 213 us on different GPUs, 2.7 to 2.3 PFLOP/s (a tile's sums are read while the next tile's products run); 32 rows of 4096 x 28672 24 to 25 us, 4.8 TB/s; 2001 rows
+// of 4096 x 6144 4-bit weights with groups of 128 118 us, 850 TFLOP/s: there each group's 128 x 128 sums pass through registers, some 2700 warp instructions an SM and group of a tile
+// against 256 cycles of the tensor cores, so the rate of instructions bounds it (59 % of all cycles issue one). By the source the sums are some 750 of them and the codes 480; the others, among them
+// waits that try again and moves into pairs of registers, have not been told apart.
 struct ProductMaps {
     CUtensorMap w, x;
 };

@@ -9,7 +9,7 @@ namespace zk {
 
 // Both calls are a pass over rows: values in, one number of the whole row (the mean of squares, the largest value), values out. A row stays in registers between
 // its reading and its writing, V times eight values a thread, so nothing is read twice: bound by the bytes, and by a row's one barrier, which two thread blocks an SM cover for one another.
-// Measured: the norm of 8191 rows of 4096 with the residual's sum and codes 38 us, 6.15 TB/s; of one row 2.9, a launch and two trips to memory; the gate of 4096 rows of 14336 to codes 58 us,
+// Measured: the norm of 8191 rows of 4096 with the residual's sum and codes 38 us, 6.15 TB/s; of one row 2.1 to 2.9, a launch and two trips to memory; the gate of 4096 rows of 14336 to codes 58 us,
 // 5.0 TB/s (two sixteens of bytes of each input and thread are as much as its registers hold under way).
 struct RowsArgs {
     const void* x;
@@ -132,7 +132,7 @@ __device__ __forceinline__ uint32_t numbers_from_below(uint32_t w) {
     asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(w), "r"(0xff7fff7fu));
     return r;
 }
-// g / (1 + exp(-g)): two approximations (2^-22 and 2^-23 of their results) and the products.
+// g / (1 + exp(-g)): the exponent's rounding, which is 2^-17 of the result at |g| near 87 and less in proportion, two approximations (2^-22 and 2^-23 of their results), and the products.
 __device__ __forceinline__ float gated(float g) {
     float e, r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.44269504f));
