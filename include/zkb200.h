@@ -582,8 +582,8 @@ int zkb_step_attention(zkb_ctx* ctx, const zkb_step_attention_args* args);
 /* What lies between those calls and behind them, with the same conventions. zkb_step_residual_norm and zkb_step_gate leave rows of 8-bit
  * codes with a scale a row, zkb_step_product multiplies them with weights held as codes (as INT32 its results are the accumulators that
  * zkb_witness_dequant proves), and zkb_step_logprobs reads the output head's. Rows of codes: scale = max|y| / 127 and code =
- * y * (127 / max|y|), rounded to nearest even (a scale of zero, NaN or infinity: codes 0), y the values before any rounding, the factor
- * a 32-bit float: a value halfway between two codes may go to either. */
+ * y * (127 / max|y|), rounded to nearest even (a scale of zero, NaN or infinity: codes 0), y the values before any rounding, in 32-bit floats:
+ * what lies within 2^-23 of itself beside the middle between two codes may go to either. */
 
 /* The residual stream's next rows and their norms: s = bf16(residual + x), or x itself where residual is NULL, and
  * y = s * rsqrt(mean(s^2) + eps) * weight over a row's `width` values (weight: bf16, NULL: ones). s goes to sum_out where that is given; it

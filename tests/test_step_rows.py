@@ -69,3 +69,56 @@ def test_gates_of_minus_infinity_are_closed(ctx, zkb, source, width, kind):
         assert bool(torch.isnan(scale[2:]).all()) and not bool(out[2:].any()) and scale[1] == 0
     else:
         assert bool(torch.equal(torch.isnan(values_of(out)), torch.isnan(y)))
+
+
+def codes_to_even(y):
+    """y * 127 / max|y| of rows in 64 bits that hold 127 y exactly, rounded to nearest even without a rounding on the way, and how far from halfway between two codes (a quotient of
+    exact numbers) each one is."""
+    size, most = 127 * y.abs(), y.abs().amax(-1, keepdim=True)
+    k = torch.floor(size / most)
+    k = k - (k * most > size).double()
+    k = k + ((k + 1) * most <= size).double()
+    twice = 2 * (size - k * most) - most  # exact: of 24 bits each
+    up = (twice > 0) | ((twice == 0) & (k % 2 == 1))
+    return torch.sign(y) * (k + up.double()), (twice / most).abs()
+
+
+@gpu
+@pytest.mark.parametrize("rows,width,source", [(700, 64, "bf16"), (33, 4096, "bf16"), (9, 777, "words"), (650, 1000, "words"), (64, 14336, "bf16")])
+def test_values_halfway_between_two_codes_go_to_the_even_one(ctx, zkb, rows, width, source):
+    """Rows of bf16 values whose largest has few bits hold many. A value of c codes that is not halfway is 2^-17 c and more from it (eight bits over eight), and the kernel's error is 2^-23 c at most: all
+    codes are those of the definition."""
+    from step_cases import words
+
+    g = gen(width)
+    x = torch.randn(rows, width, generator=g, device="cuda").bfloat16()
+    top = torch.tensor([1, 3, 5, 7, 96, 127, 255, 129], device="cuda").float()[torch.arange(rows, device="cuda") % 8] * torch.exp2(torch.arange(rows, device="cuda") % 40 - 20.0)
+    x = (x.float() / x.float().abs().amax(-1, keepdim=True) * top[:, None]).bfloat16()
+    x[:, 5] = -top.bfloat16()
+    held = words(x) if source == "words" else x
+    out, scale = room("codes", rows, width)[1], torch.zeros(rows, device="cuda")
+    torch.cuda.synchronize()
+    ctx.step_gate(zkb.StepGate(x=held.data_ptr(), x_stride=width, x_type=TYPES[source], out=out.data_ptr(), out_type=INT8, out_scale=scale.data_ptr(), out_stride=width, n_rows=rows, width=width))
+    done(ctx)
+    want, far = codes_to_even(x.double())
+    assert int((far == 0).sum()) > 10
+    assert torch.equal(out.double(), want)
+
+
+@gpu
+@pytest.mark.parametrize("rows,width", [(700, 64), (33, 4096), (9, 777), (64, 14336), (2000, 4096)])
+def test_norms_halfway_between_two_codes_go_to_the_even_one(ctx, zkb, rows, width):
+    """Products of bf16 values and weights, sixteen bits over sixteen: what is not halfway may be as near to it as the kernel's error, 2^-23 of 127 codes."""
+    g = gen(width)
+    x, w = torch.randn(rows, width, generator=g, device="cuda").clamp(-3, 3), 1 + 0.2 * torch.randn(width, generator=g, device="cuda")
+    w[::2] = 3.0
+    x[:, 0], x[:, 2], x[:, 4], x[:, 6] = 8.0, 4.0, -4.0, -2.0  # the largest is 24; 12 is half of it
+    x[1::2] = torch.randint(-200, 200, (rows // 2, width), generator=g, device="cuda").float()  # the largest is 762, six times 127: odd ones times 3 are halfway
+    x[1::2, 0] = 254.0
+    x[1::2, 1::2] *= 0.125
+    x, w = x.bfloat16(), w.bfloat16()
+    got, scale = norms(ctx, zkb, x, w, "codes", 1e-5)
+    want, far = codes_to_even(x.double() * w.double())
+    assert int((far == 0).sum()) >= 2 * rows
+    off = got.double() != want
+    assert not bool((off & ((far == 0) | (far > 2.0 ** -15))).any()), (int(off.sum()), int((off & (far == 0)).sum()))

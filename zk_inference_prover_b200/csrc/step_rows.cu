@@ -247,18 +247,35 @@ __global__ void __launch_bounds__(V >= 4 ? 512 : 1024, V == 4 ? 2 : 1) rows_kern
         store_row<V, VEC>(a.out, t * a.out_stride, a.out_type == ZKB_VALUE_WORD, a.width, threads, th, s);
         return;
     }
-    // The codes of y * by: by a factor of 127 over the largest of y, which 1.5 * 2^23 added rounds to the last bits of a float.
+    // The codes of y * by: y times 127 over the largest of y, which 1.5 * 2^23 added rounds to the last bits of a float. Halfway between two codes, exactly, lies half the largest value, at 63.5, whose even code is
+    // the upper one: the factor is the float not below 127 over the largest. Others, y / most = odd / 254, are there only where 127 divides the largest one's bits (then the factor, of eight bits, is exact;
+    // of sixteen, a product's, the code by the float below is another one, and the even one of both is it).
     if (th == 0) a.scale[t] = most * by / 127.f;
-    float to_code = 0.f;
-    const bool small = most < 0x1p-64f;  // 127 over less than 2^-121 is no float
-    if (most < INFINITY) to_code = small ? (most * 0x1p64f > 0x1.fcp-80f ? 127.f / (most * 0x1p64f) : 0.f) : 127.f / most;  // codes are 0 where the scale is (up to 127 x 2^-150)
     const bool numbers = most < INFINITY;  // else codes are 0
+    if (most < 0x1p-64f) {                 // 127 over less than 2^-121 is no float
+        most *= 0x1p64f;
+#pragma unroll
+        for (int v = 0; v < V; v++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) y[v][i] *= 0x1p64f;
+    }
+    float to_code = 0.f, below = 0.f;
+    if (numbers && most > 0x1.fcp-80f) {  // codes are 0 where the scale is (up to 127 x 2^-150)
+        const float near = 127.f / most, left = fmaf(-near, most, 127.f);
+        to_code = __uint_as_float(__float_as_uint(near) + (left > 0.f)), below = __uint_as_float(__float_as_uint(near) - (left < 0.f));
+    }
+    const bool halves = !GATE && ((__float_as_uint(most) & 0x7fffffu) | 0x800000u) % 127 == 0;
     int8_t* const to = static_cast<int8_t*>(a.out) + t * a.out_stride;
 #pragma unroll
     for (int v = 0; v < V; v++) {
         uint32_t q[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) q[i] = numbers ? __float_as_uint(fmaf(small ? y[v][i] * 0x1p64f : y[v][i], to_code, 12582912.f)) : 0u;
+        for (int i = 0; i < 8; i++) q[i] = numbers ? __float_as_uint(fmaf(y[v][i], to_code, 12582912.f)) : 0u;
+        if (halves) {
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (q[i] & 1) q[i] = __float_as_uint(fmaf(y[v][i], below, 12582912.f));
+        }
         const uint32_t lo = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410), hi = __byte_perm(__byte_perm(q[4], q[5], 0x0040), __byte_perm(q[6], q[7], 0x0040), 0x5410);
         if constexpr (VEC) {
             const uint32_t col = column_of<VEC>(v, 0, threads, th);
